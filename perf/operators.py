@@ -1,0 +1,779 @@
+"""Performance cases of windowed attention and of the block pool it reads.
+
+A sequence's token at position i sees the tokens j <= i with j > i - window,
+and the first ``sinks`` tokens whatever their distance.  Kinds of cases:
+
+* ``decode``   one new token per sequence over its cached context
+               (``WindowAttention.forward``);
+* ``prefill``  several new tokens per sequence, their keys and values already
+               in cache blocks (``WindowAttention.prefill``);
+* ``train``    packed sequences, forward and gradients
+               (``WindowAttention.dense``);
+* ``copy``     cache blocks copied to other blocks, in every layer of a stage
+               (``BlockPool.copy``);
+* ``fork``     the rows of a running batch replaced by copies of chosen rows,
+               as a beam step or parallel sampling does: full blocks shared, a
+               half-filled last block copied (``BlockPool.fork``);
+* ``extend``   blocks given to rows that grow (``BlockPool.extend``);
+* ``free``     the blocks that no later token sees and those of finished rows
+               given back (``BlockPool.free``);
+* ``compact``  the live blocks moved to the front of the pool, tables rewritten
+               (``BlockPool.compact``).
+
+Head counts and sizes are those of the repository's benchmark layers (32 or 40
+heads of 128) and its grouped forms; block sizes 16 and 32.  With ``own`` false
+the operators run in their plain form, elementary torch operations in float32.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PKG = os.path.join(REPO, "drofell-for-revision_amd")
+
+
+def listed():
+    return [
+        # one request in a chat whose old turns have left the window: the
+        # smallest decode call, where the call itself counts
+        dict(name="decode-1seq", kind="decode", seqs=1, ctx=700, least=700, window=512, sinks=4,
+             heads=32, kv_heads=8, head_dim=128, block=32, dtype="fp16"),
+        # a serving batch far into long streams, blocks behind the window freed
+        dict(name="decode-streams", kind="decode", seqs=48, ctx=70001, least=1500, window=4096,
+             sinks=4, heads=32, kv_heads=8, head_dim=128, block=32, dtype="bf16"),
+        # a draft's few tokens checked against whole contexts (no window)
+        dict(name="prefill-7tokens", kind="prefill", seqs=12, new=7, least_new=1, ctx=3500, window=0,
+             sinks=0, heads=32, kv_heads=8, head_dim=128, block=16, dtype="fp16"),
+        # a chunk of two prompts behind cached tokens, one query head per kv head
+        dict(name="prefill-chunk", kind="prefill", seqs=2, new=600, least_new=413, ctx=2300,
+             window=1024, sinks=4, heads=40, kv_heads=40, head_dim=128, block=32, dtype="fp16"),
+        # whole prompts of a batch, ragged, the longest past the window
+        dict(name="prefill-prompts", kind="prefill", seqs=4, new=12000, least_new=900, ctx=12000,
+             window=4096, sinks=4, heads=32, kv_heads=8, head_dim=128, block=32, dtype="bf16"),
+        # adapter training on short packed sequences of an odd head size
+        dict(name="train-short", kind="train", seqs=5, tokens=333, least=1, window=128, sinks=2,
+             heads=16, kv_heads=4, head_dim=80, dtype="fp16"),
+        # adapter training on long sequences
+        dict(name="train-long", kind="train", seqs=2, tokens=6000, least=4100, window=2048, sinks=4,
+             heads=32, kv_heads=32, head_dim=128, dtype="bf16"),
+        # a shared prompt's blocks duplicated in the layers of a stage
+        dict(name="copy-150blocks", kind="copy", layers=3, blocks=400, pairs=150, kv_heads=32,
+             head_dim=128, block=32, dtype="fp16"),
+        # eight requests of four beams each, one beam step
+        dict(name="fork-beams", kind="fork", layers=8, blocks=1200, groups=8, beams=4, ctx=1500,
+             kv_heads=8, head_dim=128, block=16, dtype="bf16"),
+        # a batch's tables before the next chunk of every prompt
+        dict(name="extend-chunk", kind="extend", blocks=30000, rows=48, ctx=4000, add=512, block=16),
+        # long streams after a chunk: blocks behind the window and finished rows
+        dict(name="free-window", kind="free", blocks=20000, rows=64, ctx=30000, window=4096, sinks=4,
+             block=32),
+        # a pool half emptied by finished requests, before its tail is given back
+        dict(name="compact-half", kind="compact", layers=4, blocks=2000, rows=40, ctx=1200,
+             kv_heads=8, head_dim=128, block=32, dtype="fp16"),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(lo * (hi / lo) ** rng.random()))))
+
+
+# a drawn case moves and computes no more than the largest listed ones
+_MOST_BYTES, _MOST_FLOPS = 7.9e8, 1.7e12
+_SHRINKS = ("seqs", "new", "tokens", "ctx", "pairs", "layers")
+
+
+def draw(rng):
+    case = _drawn(rng)
+    names = [n for n in _SHRINKS if case.get(n, 0) > 1]
+    while any(a > b for a, b in zip(work(case).values(), (_MOST_BYTES, _MOST_FLOPS))):
+        name = rng.choice(names)
+        case[name] = max(1, case[name] // 2)
+        case["ctx"] = max(case.get("ctx", 1), case.get("new", 1))
+        for least, most in (("least", "ctx" if case["kind"] == "decode" else "tokens"),
+                            ("least_new", "new")):
+            if least in case:
+                case[least] = min(case[least], case[most])
+        if case["kind"] in ("copy", "train"):
+            case.pop("ctx")
+    return case
+
+
+def _drawn(rng):
+    kind = rng.choice(["decode", "decode", "prefill", "prefill", "train", "train", "copy", "fork",
+                       "extend", "free", "compact"])
+    heads, kv_heads = rng.choice([(32, 32), (40, 40), (32, 8), (64, 8), (8, 2), (24, 2), (16, 16)])
+    shape = dict(head_dim=rng.choice([64, 80, 96, 112, 128, 128, 128, 256]), block=rng.choice([16, 32]),
+                 dtype=rng.choice(["fp16", "bf16"]))
+    band = dict(window=rng.choice([0, 1, _log_int(rng, 16, 4096), _log_int(rng, 16, 4096)]),
+                sinks=rng.choice([0, 1, 4, rng.randint(5, 70)]))
+    if kind == "decode":
+        ctx = _log_int(rng, 1, 20000 if band["window"] else 4000)
+        return dict(kind=kind, seqs=_log_int(rng, 1, 48), ctx=ctx, least=rng.randint(1, ctx),
+                    heads=heads, kv_heads=kv_heads, **band, **shape)
+    if kind == "prefill":
+        new = _log_int(rng, 2, 4000)
+        return dict(kind=kind, seqs=rng.randint(1, 4), new=new, least_new=rng.randint(1, new),
+                    ctx=new + rng.choice([0, _log_int(rng, 1, 3000)]), heads=heads,
+                    kv_heads=kv_heads, **band, **shape)
+    if kind == "train":
+        tokens = _log_int(rng, 2, 2500)
+        shape.pop("block")
+        return dict(kind=kind, seqs=rng.randint(1, 4), tokens=tokens, least=rng.randint(1, tokens),
+                    heads=heads, kv_heads=kv_heads, **band, **shape)
+    blocks = _log_int(rng, 100, 400)
+    if kind == "copy":
+        return dict(kind=kind, layers=rng.randint(1, 4), blocks=blocks,
+                    pairs=rng.randint(1, blocks // 2), kv_heads=min(kv_heads, 32), **shape)
+    if kind == "fork":
+        groups, beams = rng.randint(1, 12), rng.randint(2, 8)
+        ctx = _log_int(rng, 1, 1500)
+        need = groups * ((ctx + shape["block"] - 1) // shape["block"]) + 2 * groups * beams
+        return dict(kind=kind, layers=rng.randint(1, 3), blocks=need + rng.randint(0, 100),
+                    groups=groups, beams=beams, ctx=ctx, kv_heads=min(kv_heads, 8), **shape)
+    if kind == "extend":
+        rows, ctx, add = _log_int(rng, 1, 100), _log_int(rng, 1, 4000), _log_int(rng, 1, 600)
+        need = rows * ((ctx + add) // shape["block"] + 2)
+        return dict(kind=kind, blocks=need + rng.randint(0, 1000), rows=rows, ctx=ctx, add=add,
+                    block=shape["block"])
+    if kind == "free":
+        rows, ctx = _log_int(rng, 1, 100), _log_int(rng, 1, 20000)
+        return dict(kind=kind, blocks=rows * (ctx // shape["block"] + 1) + rng.randint(0, 1000),
+                    rows=rows, ctx=ctx, block=shape["block"], **band)
+    rows, ctx = rng.randint(1, 30), _log_int(rng, 1, 500)
+    need = rows * (ctx // shape["block"] + 1)
+    return dict(kind=kind, layers=rng.randint(1, 3), blocks=need + rng.randint(1, 300), rows=rows,
+                ctx=ctx, kv_heads=min(kv_heads, 8), **shape)
+
+
+# ---------------------------------------------------------------------------
+# Inputs
+# ---------------------------------------------------------------------------
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _dtype(case):
+    return torch.bfloat16 if case["dtype"] == "bf16" else torch.float16
+
+
+def _spread(n, most, least):
+    """n lengths from least to most, the first the longest, the others spread over the range."""
+    return [most if i == 0 else least + int((most - least) * ((i * 0.6180339887) % 1.0))
+            for i in range(n)]
+
+
+def _up(a, b):
+    return (a + b - 1) // b
+
+
+def _first_visible(pos, window):
+    """The first token that the query at pos sees, sinks aside."""
+    return max(0, pos - window + 1) if window else 0
+
+
+def _ints(values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype).to("cuda")
+
+
+def _contexts(case):
+    """(new tokens, context length) of each sequence of a decode or prefill case."""
+    if case["kind"] == "decode":
+        return [1] * case["seqs"], _spread(case["seqs"], case["ctx"], case["least"])
+    new = _spread(case["seqs"], case["new"], case["least_new"])
+    past = case["ctx"] - case["new"]
+    return new, [n + (past if i % 2 == 0 else past // 2) for i, n in enumerate(new)]
+
+
+def _kept_tables(gen, case, new, ctxs):
+    """Block tables whose blocks lie anywhere in the pool; -1 where a block has
+    left the window of every new token."""
+    bs = case["block"]
+    width = max(_up(c, bs) for c in ctxs)
+    b = torch.arange(width, device="cuda")
+    ctx = _ints(ctxs, torch.int64)[:, None]
+    first = _ints([_first_visible(c - n, case["window"]) for n, c in zip(new, ctxs)],
+                  torch.int64)[:, None]
+    live = (b * bs < ctx) & (((b + 1) * bs > first) | (b * bs < case["sinks"]))
+    total = sum(sum(1 for x in range(_up(c, bs)) if (x + 1) * bs > _first_visible(c - n, case["window"])
+                    or x * bs < case["sinks"]) for n, c in zip(new, ctxs))
+    order = torch.randperm(total, device="cuda", generator=gen)
+    rank = (live.flatten().cumsum(0) - 1).clamp_(min=0)
+    tables = torch.where(live, order[rank].view_as(live), -1)
+    return tables.to(torch.int32), total
+
+
+def _pages(gen, case, blocks):
+    """One layer's blocks: keys [blocks, kv heads, dims / 8, slots, 8], values
+    [blocks, kv heads, dims, slots]."""
+    kvh, hd, bs = case["kv_heads"], case["head_dim"], case["block"]
+    k = torch.empty(blocks, kvh, hd // 8, bs, 8, dtype=_dtype(case), device="cuda")
+    v = torch.empty(blocks, kvh, hd, bs, dtype=_dtype(case), device="cuda")
+    k.normal_(generator=gen)
+    v.normal_(generator=gen)
+    return k, v
+
+
+def _queries(gen, case, rows):
+    """Queries with a part in common, towards which the first tokens' keys lean."""
+    q = torch.randn(rows, case["heads"], case["head_dim"], device="cuda", generator=gen)
+    return (q + 0.5).to(_dtype(case))
+
+
+def _lean(k, case, tables=None):
+    """The sink tokens' keys: larger logits than other tokens get."""
+    n = case["sinks"]
+    if tables is None:
+        k[:, :n] += 0.6
+    elif n:
+        bs = case["block"]
+        for b in range(min(tables.shape[1], _up(n, bs))):
+            slots = min(bs, n - b * bs)
+            rows = tables[:, b].long().clamp_(min=0)
+            k[rows, :, :, :slots] += 0.6
+
+
+def _package():
+    for p in (PKG, REPO):
+        if p not in sys.path:
+            sys.path.insert(0, p)
+
+
+def _holder(k, v, case):
+    """The framework's handle of one layer's blocks."""
+    _package()
+    from operators import flags
+    from operators.core.block.common import BlockInfo
+    from operators.core.block.real import LayerBlocksHolder
+    flags.BLOCK_SIZE = case["block"]
+    info = BlockInfo(head_dim=case["head_dim"], num_key_value_heads=case["kv_heads"], dtype=k.dtype)
+    step = [t.stride(0) * t.element_size() for t in (k, v)]
+    kp = [k.data_ptr() + step[0] * i for i in range(k.shape[0])]
+    vp = [v.data_ptr() + step[1] * i for i in range(v.shape[0])]
+    kc, vc = torch.tensor(kp, dtype=torch.int64), torch.tensor(vp, dtype=torch.int64)
+    return LayerBlocksHolder(info, kc.to(k.device), vc.to(v.device), kc, vc, kp, vp,
+                             contigious_kv_tensor=(k, v))
+
+
+def _attention(case):
+    _package()
+    from operators.core.attention.common import AttentionConfig
+    from operators.core.attention.real_window import WindowAttention
+    h, kvh, hd = case["heads"], case["kv_heads"], case["head_dim"]
+    return WindowAttention(AttentionConfig(h * hd, hd, h, kvh, h // kvh),
+                           window=case["window"] or None, sinks=case["sinks"])
+
+
+def prepare(case, seed):
+    gen = _gen(seed)
+    state = {"case": case, "own": own}
+    kind = case["kind"]
+    if kind in ("decode", "prefill"):
+        new, ctxs = _contexts(case)
+        tables, total = _kept_tables(gen, case, new, ctxs)
+        k, v = _pages(gen, case, total)
+        _lean(k, case, tables)
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        state.update(k=k, v=v, tables=tables, lens=_ints(ctxs), new=new, ctxs=ctxs, most=max(ctxs),
+                     starts=_ints(starts), q=_queries(gen, case, starts[-1]))
+        if own:
+            state.update(att=_attention(case), holder=_holder(k, v, case))
+    elif kind == "train":
+        lens = _spread(case["seqs"], case["tokens"], case["least"])
+        starts = [0]
+        for n in lens:
+            starts.append(starts[-1] + n)
+        kv = (starts[-1], case["kv_heads"], case["head_dim"])
+        q = _queries(gen, case, starts[-1])
+        k = torch.randn(kv, device="cuda", generator=gen)
+        v = torch.randn(kv, device="cuda", generator=gen)
+        for a in starts[:-1]:
+            _lean(k[a:].unsqueeze(0), case)
+        dout = torch.randn(q.shape, device="cuda", generator=gen)
+        state.update(q=q, k=k.to(q.dtype), v=v.to(q.dtype), dout=dout.to(q.dtype), lens=lens,
+                     starts=_ints(starts))
+        if own:
+            for name in ("q", "k", "v"):
+                state[name].requires_grad_(True)
+            state["att"] = _attention(case)
+    else:
+        state.update(_pool_state(gen, case))
+    return state
+
+
+def _pool_state(gen, case):
+    """Tables, lengths and reference counts of a running batch, and the layers' blocks."""
+    kind, bs, nb = case["kind"], case["block"], case["blocks"]
+    order = torch.randperm(nb, device="cuda", generator=gen).to(torch.int32)
+    out = {}
+    if kind == "copy":
+        n = case["pairs"]
+        out["pairs"] = order[:2 * n].view(n, 2).contiguous()
+    elif kind == "fork":
+        # the beams of a request share its full blocks and own a half-filled one
+        groups, beams = case["groups"], case["beams"]
+        lens = _spread(groups, case["ctx"], max(1, case["ctx"] // 2))
+        width = _up(case["ctx"], bs) + 1
+        full, used, rows, refs = [c // bs for c in lens], 0, [], torch.zeros(nb, dtype=torch.int32)
+        flat = order.tolist()
+        for g in range(groups):
+            shared = flat[used:used + full[g]]
+            used += full[g]
+            for p in shared:
+                refs[p] = beams
+            for _ in range(beams):
+                row = list(shared)
+                if lens[g] % bs:
+                    row.append(flat[used])
+                    refs[flat[used]] = 1
+                    used += 1
+                rows.append(row + [-1] * (width - len(row)))
+        pick = torch.randint(0, beams, (groups, beams), device="cuda", generator=gen)
+        pick += torch.arange(groups, device="cuda")[:, None] * beams
+        out.update(tables=_ints(rows), lens=_ints([c for c in lens for _ in range(beams)]),
+                   refs=refs.to("cuda"), parents=pick.flatten().to(torch.int32))
+    else:
+        rows, ctx = case["rows"], case["ctx"]
+        lens = _spread(rows, ctx, max(1, ctx // 2))
+        width = _up(ctx + case.get("add", 0), bs) + 1
+        lens_t = _ints(lens)
+        count = torch.div(lens_t + bs - 1, bs, rounding_mode="floor").long()
+        if kind == "free":  # already without the blocks that left the window long ago
+            gone = [max(0, c - case["window"] - 700) // bs if case["window"] else 0 for c in lens]
+        else:
+            gone = [0] * rows
+        b = torch.arange(width, device="cuda")
+        has = (b < count[:, None]) & ((b >= _ints(gone, torch.int64)[:, None]) |
+                                      (b * bs < case.get("sinks", 0)))
+        if kind == "free":  # as many blocks as the pool holds
+            has &= (has.flatten().cumsum(0) <= nb).view_as(has)
+        rank = (has.flatten().cumsum(0) - 1).clamp_(min=0)
+        tables = torch.where(has, order[rank].view_as(has), -1).to(torch.int32)
+        refs = torch.zeros(nb + 1, dtype=torch.int32, device="cuda")
+        refs[torch.where(has, tables, nb).flatten().long()] = 1
+        out.update(tables=tables, lens=lens_t, refs=refs[:nb].contiguous())
+        if kind == "extend":
+            out["add"] = torch.randint(0, case["add"] + 1, (rows,), device="cuda",
+                                       generator=gen).to(torch.int32)
+            out["add"][0] = case["add"]
+        if kind == "free":
+            out["finished"] = torch.rand(rows, device="cuda", generator=gen) < 0.1
+    layers = case.get("layers", 0)
+    pages = [_pages(gen, case, nb) for _ in range(layers)]
+    out["pages"] = pages
+    if own:
+        _package()
+        from operators import flags
+        from operators.core.block.pool import BlockPool, BlockState
+        flags.BLOCK_SIZE = bs
+        out["pool"] = BlockPool([_holder(k, v, case) for k, v in pages], nb, torch.device("cuda"))
+        if kind != "copy":
+            out["state"] = BlockState(out["tables"], out["lens"], out["refs"])
+    return out
+
+
+# ---------------------------------------------------------------------------
+# run
+# ---------------------------------------------------------------------------
+def run(state):
+    return (_own if state["own"] else _plain)[state["case"]["kind"]](state)
+
+
+def _own_decode(s):
+    return s["att"].forward(s["q"], s["most"], s["lens"], s["tables"], s["holder"])
+
+
+def _own_prefill(s):
+    return s["att"].prefill(s["q"], s["starts"], max(s["new"]), s["most"], s["lens"], s["tables"],
+                            s["holder"])
+
+
+def _own_train(s):
+    out = s["att"].dense(s["q"], s["k"], s["v"], s["starts"], max(s["lens"]))
+    return (out.detach(), *torch.autograd.grad(out, (s["q"], s["k"], s["v"]), s["dout"]))
+
+
+def _own_copy(s):
+    s["pool"].copy(s["pairs"])
+    return s["pages"]
+
+
+def _state_out(new, s):
+    return new.block_tables, new.context_lens, new.refs, new.shortage, s["pages"]
+
+
+def _own_fork(s):
+    return _state_out(s["pool"].fork(s["state"], s["parents"]), s)
+
+
+def _own_extend(s):
+    return _state_out(s["pool"].extend(s["state"], s["add"]), s)
+
+
+def _own_free(s):
+    c = s["case"]
+    return _state_out(s["pool"].free(s["state"], c["window"] or None, c["sinks"], s["finished"]), s)
+
+
+def _own_compact(s):
+    new, live = s["pool"].compact(s["state"])
+    return (*_state_out(new, s), live)
+
+
+def _gather(s, blk, off):
+    """Keys and values [..., kv heads, dims] of cache slots, in float32."""
+    k = s["k"][blk, :, :, off].float()
+    return k.reshape(*k.shape[:-2], -1), s["v"][blk, :, :, off].float()
+
+
+def _softmax(x):
+    """exp(x - max) / sum over the last axis; rows without a finite logit are zero."""
+    m = x.amax(-1, keepdim=True)
+    p = torch.exp(x - torch.where(m == -math.inf, 0.0, m))
+    total = p.sum(-1, keepdim=True)
+    return p / torch.where(total == 0, 1.0, total)
+
+
+def _plain_decode(s):
+    c = s["case"]
+    bs, kvh, hd = c["block"], c["kv_heads"], c["head_dim"]
+    g = c["heads"] // kvh
+    lens = s["lens"].long()
+    span = min(c["window"] or s["most"], s["most"])
+    start = (lens - span).clamp(min=0)
+    pos = start[:, None] + torch.arange(span, device="cuda")
+    valid = pos < lens[:, None]
+    if c["sinks"]:
+        sink = torch.arange(min(c["sinks"], s["most"]), device="cuda").expand(len(lens), -1)
+        pos = torch.cat([sink, pos], 1)
+        valid = torch.cat([sink < start[:, None], valid], 1)
+    blk = s["tables"].long().gather(1, (pos // bs).clamp(max=s["tables"].shape[1] - 1))
+    valid &= blk >= 0
+    blk, off = blk.clamp(min=0), pos % bs
+    out = torch.empty_like(s["q"])
+    step = max(1, 2 ** 28 // (pos.shape[1] * kvh * hd))  # sequences at once
+    for a in range(0, len(lens), step):
+        r = slice(a, a + step)
+        k, v = _gather(s, blk[r], off[r])
+        q = s["q"][r].float().view(-1, kvh, g, hd)
+        logits = torch.matmul(q, k.permute(0, 2, 3, 1).contiguous()) * hd ** -0.5
+        p = _softmax(logits.masked_fill(~valid[r, None, None], -math.inf))
+        o = torch.matmul(p, v.permute(0, 2, 1, 3).contiguous())
+        out[r] = o.reshape(-1, c["heads"], hd).to(out.dtype)
+    return out
+
+
+def _visible(i, j, case):
+    """Whether positions i (rows) see positions j (columns)."""
+    m = j <= i
+    if case["window"]:
+        m &= (j > i - case["window"]) | (j < case["sinks"])
+    return m
+
+
+def _plain_prefill(s):
+    c = s["case"]
+    bs, kvh, hd = c["block"], c["kv_heads"], c["head_dim"]
+    g = c["heads"] // kvh
+    out = torch.empty_like(s["q"])
+    at = 0
+    for i, (n, ctx) in enumerate(zip(s["new"], s["ctxs"])):
+        for a in range(0, n, 1024):
+            rows = min(1024, n - a)
+            first, end = ctx - n + a, ctx - n + a + rows
+            lo = _first_visible(first, c["window"])
+            j = torch.cat([torch.arange(min(c["sinks"], lo), device="cuda"),
+                           torch.arange(lo, end, device="cuda")])
+            blk = s["tables"][i].long()[j // bs]
+            k, v = _gather(s, blk.clamp(min=0), j % bs)
+            q = s["q"][at + a:at + a + rows].float().view(rows, kvh, g, hd).permute(1, 2, 0, 3)
+            q = q.reshape(kvh, g * rows, hd)
+            seen = _visible(torch.arange(first, end, device="cuda")[:, None], j, c) & (blk >= 0)
+            logits = torch.matmul(q, k.permute(1, 2, 0).contiguous()) * hd ** -0.5
+            p = _softmax(logits.masked_fill_(~seen.repeat(g, 1), -math.inf))
+            o = torch.matmul(p, v.permute(1, 0, 2).contiguous())
+            o = o.view(kvh, g, rows, hd).permute(2, 0, 1, 3).reshape(rows, c["heads"], hd)
+            out[at + a:at + a + rows] = o.to(out.dtype)
+        at += n
+    return out
+
+
+def _plain_train(s):
+    c = s["case"]
+    h, kvh, hd = c["heads"], c["kv_heads"], c["head_dim"]
+    g, scale = h // kvh, hd ** -0.5
+    res = [torch.empty_like(s[n]) for n in ("q", "q", "k", "v")]
+    at = 0
+    for n in s["lens"]:
+        i = torch.arange(n, device="cuda")
+        hide = ~_visible(i[:, None], i, c)
+        r = slice(at, at + n)
+        step = max(1, 2 ** 28 // (n * n * g))  # kv heads at once
+        for a in range(0, kvh, step):
+            z = min(kvh, a + step)
+            hs = slice(a * g, z * g)
+
+            def heads_of(x, sl):
+                return x[r, sl].float().transpose(0, 1).contiguous()
+
+            q, do = heads_of(s["q"], hs), heads_of(s["dout"], hs)
+            k, v = heads_of(s["k"], slice(a, z)), heads_of(s["v"], slice(a, z))
+            kr, vr = k.repeat_interleave(g, 0), v.repeat_interleave(g, 0)
+            p = torch.matmul(q, kr.transpose(1, 2).contiguous()).mul_(scale)
+            p = _softmax(p.masked_fill_(hide, -math.inf))
+            out = torch.matmul(p, vr)
+            dv = torch.matmul(p.transpose(1, 2).contiguous(), do)
+            ds = torch.matmul(do, vr.transpose(1, 2).contiguous())
+            ds = (ds - (ds * p).sum(-1, keepdim=True)).mul_(p).mul_(scale)
+            del p
+            dq = torch.matmul(ds, kr)
+            dk = torch.matmul(ds.transpose(1, 2).contiguous(), q)
+            del ds
+            for t, x, sl in zip(res, (out, dq, dk.view(z - a, g, n, hd).sum(1),
+                                      dv.view(z - a, g, n, hd).sum(1)),
+                                (hs, hs, slice(a, z), slice(a, z))):
+                t[r, sl] = x.transpose(0, 1).to(t.dtype)
+        at += n
+    return tuple(res)
+
+
+def _plain_copy(s):
+    src, dst = s["pairs"].long().unbind(1)
+    for pair in s["pages"]:
+        for t in pair:
+            t[dst] = t[src]
+    return s["pages"]
+
+
+def _free_list(refs):
+    """Free blocks in ascending order (then the pool's size), and their count."""
+    nb = refs.shape[0]
+    idx = torch.arange(nb, device=refs.device)
+    free = refs == 0
+    return torch.where(free, idx, nb).sort().values, free.sum()
+
+
+def _add_refs(refs, pages, amount):
+    """refs plus amount at every page of the list that is one (0 <= page)."""
+    wide = torch.cat([refs, refs.new_zeros(1)])
+    flat = pages.flatten().long()
+    flat = torch.where(flat < 0, refs.shape[0], flat)
+    wide.index_add_(0, flat, torch.full_like(flat, amount, dtype=refs.dtype))
+    return wide[:-1]
+
+
+def _plain_fork(s):
+    bs = s["case"]["block"]
+    tables, lens, refs, parents = s["tables"], s["lens"], s["refs"], s["parents"].long()
+    rows = torch.arange(len(lens), device="cuda")
+    alive = parents >= 0
+    src = parents.clamp(min=0)
+    new = torch.where(alive[:, None], tables[src], -1)
+    new_lens = torch.where(alive, lens[src], 0)
+    last = (new_lens // bs).long().clamp(max=tables.shape[1] - 1)
+    page = new.gather(1, last[:, None])[:, 0].long()
+    partial = alive & (new_lens % bs != 0) & (page >= 0)
+    earlier = ((parents[:, None] == parents) & (rows < rows[:, None])).any(1)
+    need = partial & (earlier | (refs[page.clamp(min=0)] > 1))
+    listed_free, count = _free_list(refs)
+    short = (need.sum() - count).clamp(min=0)
+    ok = short == 0
+    fresh = listed_free[(need.cumsum(0) - 1).clamp(min=0)].clamp(max=len(refs) - 1)
+    new.scatter_(1, last[:, None], torch.where(need, fresh, page)[:, None].to(torch.int32))
+    new_refs = _add_refs(_add_refs(refs, tables, -1), new, 1)
+    dst = torch.where(need & ok, fresh, page.clamp(min=0))
+    for pair in s["pages"]:
+        for t in pair:
+            t[dst] = t[page.clamp(min=0)]
+    return (torch.where(ok, new, tables), torch.where(ok, new_lens, lens),
+            torch.where(ok, new_refs, refs), short.to(torch.int32).view(1), s["pages"])
+
+
+def _plain_extend(s):
+    bs = s["case"]["block"]
+    tables, lens, refs = s["tables"], s["lens"], s["refs"]
+    new_lens = lens + s["add"].clamp(min=0)
+    have, want = (torch.div(x + bs - 1, bs, rounding_mode="floor").long() for x in (lens, new_lens))
+    wide = (want - tables.shape[1]).clamp(min=0).sum()
+    listed_free, count = _free_list(refs)
+    need = want - have
+    short = (need.sum() - count).clamp(min=0) + wide
+    ok = short == 0
+    b = torch.arange(tables.shape[1], device="cuda")
+    give = (b >= have[:, None]) & (b < want[:, None])
+    k = (need.cumsum(0) - need)[:, None] + b - have[:, None]
+    got = listed_free[k.clamp(0, len(refs) - 1)].to(torch.int32)
+    new = torch.where(give, got, tables)
+    new_refs = _add_refs(refs, torch.where(give & (got < len(refs)), got, -1), 1)
+    return (torch.where(ok, new, tables), torch.where(ok, new_lens, lens),
+            torch.where(ok, new_refs, refs), short.to(torch.int32).view(1), s["pages"])
+
+
+def _plain_free(s):
+    c = s["case"]
+    bs, tables, lens = c["block"], s["tables"], s["lens"]
+    b = torch.arange(tables.shape[1], device="cuda")
+    drop = s["finished"][:, None].expand_as(tables)
+    if c["window"]:
+        drop = drop | (((b + 1) * bs <= lens[:, None] - c["window"] + 1) & (b * bs >= c["sinks"]))
+    new = torch.where(drop, -1, tables)
+    refs = _add_refs(s["refs"], torch.where(drop, tables, -1), -1)
+    return (new, torch.where(s["finished"], 0, lens), refs,
+            torch.zeros(1, dtype=torch.int32, device="cuda"), s["pages"])
+
+
+def _plain_compact(s):
+    tables, refs = s["tables"], s["refs"]
+    nb = refs.shape[0]
+    idx = torch.arange(nb, device="cuda")
+    alive = refs > 0
+    live = alive.sum()
+    src = (alive & (idx >= live)).nonzero()[:, 0]
+    dst = (~alive & (idx < live)).nonzero()[:, 0]
+    remap = idx.to(torch.int32)
+    remap[src] = dst.to(torch.int32)
+    new_refs = refs.clone()
+    new_refs[dst] = refs[src]
+    new_refs[src] = 0
+    new = torch.where(tables >= 0, remap[tables.long().clamp(min=0)], tables)
+    for pair in s["pages"]:
+        for t in pair:
+            t[dst] = t[src]
+    return (new, s["lens"], new_refs, torch.zeros(1, dtype=torch.int32, device="cuda"), s["pages"],
+            live.to(torch.int32).view(1))
+
+
+_KINDS = ("decode", "prefill", "train", "copy", "fork", "extend", "free", "compact")
+_plain = {k: globals()["_plain_" + k] for k in _KINDS}
+_own = {k: globals()["_own_" + k] for k in _KINDS}
+
+
+# ---------------------------------------------------------------------------
+# exact: the definition in float64, one sequence and kv head at a time
+# ---------------------------------------------------------------------------
+def _band(i, j, case):
+    """Logit offsets: 0 where position i sees position j, minus infinity elsewhere."""
+    gap = i[:, None] - j[None, :]
+    near = (gap >= 0) if not case["window"] else (gap >= 0) & (gap < case["window"])
+    far = (gap >= 0) & (j[None, :] < case["sinks"])
+    return torch.zeros(gap.shape, dtype=torch.float64, device="cuda").masked_fill(~(near | far), -math.inf)
+
+
+def _attend(q, k, v, offsets):
+    """softmax(q . k / sqrt(dims) + offsets) . v of one head, rows that see nothing zero."""
+    w = torch.softmax((q @ k.T) / math.sqrt(q.shape[1]) + offsets, dim=1)
+    return torch.nan_to_num(w, nan=0.0) @ v
+
+
+def exact(case, seed):
+    global own
+    kind = case["kind"]
+    if kind not in ("decode", "prefill", "train"):
+        return None  # copies and whole numbers
+    was, own = own, False
+    try:
+        s = prepare(case, seed)
+    finally:
+        own = was
+    g = case["heads"] // case["kv_heads"]
+    if kind == "train":
+        return _exact_train(case, s, g)
+    bs = case["block"]
+    out = torch.zeros(s["q"].shape, dtype=torch.float64, device="cuda")
+    at = 0
+    for n, ctx, table in zip(s["new"], s["ctxs"], s["tables"]):
+        t = torch.arange(ctx, device="cuda")
+        held = table.long()[t // bs]
+        t = t[held >= 0]
+        held = held[held >= 0]
+        for h in range(case["kv_heads"]):
+            kh, vh = s["k"][:, h], s["v"][:, h]
+            k = kh[held, :, t % bs].reshape(len(t), -1).double()
+            v = vh[held, :, t % bs].double()
+            for a in range(0, n, 2048):
+                m = min(2048, n - a)
+                i = torch.arange(ctx - n + a, ctx - n + a + m, device="cuda")
+                offsets = _band(i, t, case)
+                for x in range(h * g, h * g + g):
+                    out[at + a:at + a + m, x] = _attend(s["q"][at + a:at + a + m, x].double(), k, v, offsets)
+        at += n
+    return out
+
+
+def _exact_train(case, s, g):
+    q, k, v, dout = (s[n].double() for n in ("q", "k", "v", "dout"))
+    out, dq, dk, dv = (torch.zeros_like(t) for t in (q, q, k, v))
+    at = 0
+    for n in s["lens"]:
+        r = slice(at, at + n)
+        i = torch.arange(n, device="cuda")
+        offsets = _band(i, i, case)
+        for h in range(case["heads"]):
+            with torch.enable_grad():
+                parts = [t[r, x].clone().requires_grad_(True) for t, x in ((q, h), (k, h // g), (v, h // g))]
+                o = _attend(*parts, offsets)
+                grads = torch.autograd.grad(o, parts, dout[r, h])
+            out[r, h] = o.detach()
+            dq[r, h] = grads[0]
+            dk[r, h // g] += grads[1]
+            dv[r, h // g] += grads[2]
+        at += n
+    return out, dq, dk, dv
+
+
+# ---------------------------------------------------------------------------
+# work
+# ---------------------------------------------------------------------------
+def _seen(first, n, case):
+    """(token pairs, distinct tokens) that the n queries from position first see."""
+    w, sinks = case["window"], case["sinks"]
+    if not w:
+        return n * first + n * (n + 1) // 2, first + n
+    pairs = 0
+    for i in range(first, first + n):
+        lo = max(0, i - w + 1)
+        pairs += i + 1 - lo + min(sinks, lo)
+    lo = _first_visible(first, w)
+    return pairs, first + n - lo + min(sinks, lo)
+
+
+def work(case):
+    kind = case["kind"]
+    if kind in ("decode", "prefill"):
+        h, kvh, hd = case["heads"], case["kv_heads"], case["head_dim"]
+        pairs = tokens = rows = 0
+        for n, ctx in zip(*_contexts(case)):
+            p, t = _seen(ctx - n, n, case)
+            pairs, tokens, rows = pairs + p, tokens + t, rows + n
+        return {"bytes": 4 * tokens * kvh * hd + 4 * rows * h * hd, "flops": 4 * pairs * h * hd}
+    if kind == "train":
+        h, kvh, hd = case["heads"], case["kv_heads"], case["head_dim"]
+        lens = _spread(case["seqs"], case["tokens"], case["least"])
+        pairs = sum(_seen(0, n, case)[0] for n in lens)
+        return {"bytes": 2 * sum(lens) * hd * 4 * (h + kvh), "flops": 14 * pairs * h * hd}
+    bs, nb = case["block"], case["blocks"]
+    page = 4 * case.get("layers", 0) * case.get("kv_heads", 0) * case.get("head_dim", 0) * bs
+    if kind == "copy":
+        return {"bytes": 2 * case["pairs"] * page + 8 * case["pairs"], "flops": 0}
+    if kind == "fork":
+        rows = case["groups"] * case["beams"]
+        lens = _spread(case["groups"], case["ctx"], max(1, case["ctx"] // 2))
+        # a beam that is picked keeps its half-filled block; of b picks among b
+        # beams b (1 - 1/b)^b beams stay unpicked, and as many picks are copies
+        b = case["beams"]
+        copies = sum(1 for c in lens if c % bs) * b * (1 - 1 / b) ** b
+        return {"bytes": int(2 * copies * page) + 8 * rows * _up(case["ctx"], bs) + 8 * nb, "flops": 0}
+    rows, width = case["rows"], _up(case["ctx"] + case.get("add", 0), bs) + 1
+    meta = 8 * rows * width + 8 * nb
+    if kind == "compact":
+        lens = _spread(rows, case["ctx"], max(1, case["ctx"] // 2))
+        live = sum(_up(c, bs) for c in lens)
+        return {"bytes": int(2 * live * (1 - live / nb) * page) + meta, "flops": 0}
+    return {"bytes": meta, "flops": 0}

@@ -20,13 +20,16 @@
 
 namespace {
 
+using dw4::cu_count;
 using dw4::kChunkK;
 using dw4::kStripN;
 
 constexpr int kMaxDevices = 64;
 std::atomic<int> g_cu_count[kMaxDevices];  // per-device property cache (0 = unknown)
 
-int cu_count() {
+}  // namespace
+
+int dw4::cu_count() {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) return 256;
   int v = g_cu_count[dev].load(std::memory_order_relaxed);
@@ -37,8 +40,6 @@ int cu_count() {
   }
   return v;
 }
-
-}  // namespace
 
 hipError_t dw4::allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
   int dev = 0;

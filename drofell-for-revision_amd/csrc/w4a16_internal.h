@@ -236,6 +236,9 @@ inline bool auto_decode(int m, int n, int cus, int k = 0) {
           (strips <= cus || (k > 0 && k <= 8192 && 4 * strips <= 5 * cus)));
 }
 
+// Compute units of the current device.
+int cu_count();
+
 // A kernel launched with more than 64 KiB of dynamic LDS needs that size
 // allowed once per device (hipFuncSetAttribute).  `done` is the kernel's own
 // per-device record (bit d: device d allowed); concurrent first calls only

@@ -1,0 +1,204 @@
+// Device helpers of the windowed-attention kernels.
+//
+// All of them work on 32 x 32 x 16 matrix instructions, with the scores'
+// columns one row of the softmax each: lane l holds column l % 32, and register
+// i the token (of 32) 16 (i / 8) + 8 (l / 32) + i % 8.  The instruction itself
+// puts row 8 (i / 4) + 4 (l / 32) + i % 4 there; the A operand's rows are
+// loaded in the order row_token() for it, and then a lane's eight scores
+// i / 8 == s are those of the eight consecutive tokens that the B operand of the
+// next product wants of it (reduction step s): probabilities go from one
+// product to the next without leaving their lane.
+#pragma once
+
+#include "w4a16_device.h"
+
+namespace dw4 {
+
+constexpr float kNoMax = -3.4028234663852886e38f;  // running maximum of a row that saw no token
+// exp2 offset of fp16 probabilities: those down to 2^-24 of the largest keep
+// all of fp16's bits (a running maximum may lag kLag behind: 2^10 * 2^4 < 65504)
+template <bool BF>
+__device__ __forceinline__ constexpr float p_shift() { return BF ? 0.f : 10.f; }
+constexpr float kLag = 4.f;
+
+__device__ __forceinline__ int row_token(int r) {  // token (of 32) of the A operand's row r
+  return (r & 16) | ((r & 4) << 1) | ((r & 8) >> 1) | (r & 3);
+}
+
+// max / sum over the two lanes of a column
+__device__ __forceinline__ float both_max(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)x[0]), __builtin_bit_cast(float, (uint32_t)x[1]));
+}
+__device__ __forceinline__ float both_sum(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (uint32_t)x[0]) + __builtin_bit_cast(float, (uint32_t)x[1]);
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (BF) return pack_bf16(lo, hi);
+  else return __builtin_bit_cast(uint32_t, h2{(_Float16)lo, (_Float16)hi});
+}
+template <bool BF>
+__device__ __forceinline__ float unpack(uint32_t u, int hi) {
+  if constexpr (BF) return __builtin_bit_cast(float, hi ? u & 0xFFFF0000u : u << 16);
+  else return (float)as_h2(u)[hi];
+}
+template <bool BF>
+__device__ __forceinline__ float value_of(uint16_t b) {
+  if constexpr (BF) return bf16_f32(b);
+  else return (float)as_h(b);
+}
+
+// Which tokens a tile of rows at positions first..last sees, in steps of BK
+// tokens that start at multiples of BK: the steps over the sinks that lie
+// before the window, then those of the window.
+struct Span {
+  int lo, sink_steps, steps;
+  template <int BK>
+  __device__ __forceinline__ static Span of(int first, int last, int cap, int window, int sinks) {
+    Span s;
+    const int hi = min(last + 1, cap);
+    s.lo = (window == 0 ? 0 : max(0, first - window + 1)) & ~(BK - 1);
+    s.sink_steps = hi > 0 ? (min(sinks, s.lo) + BK - 1) / BK : 0;
+    s.steps = s.sink_steps + (hi > s.lo ? (hi - s.lo + BK - 1) / BK : 0);
+    return s;
+  }
+  template <int BK>
+  __device__ __forceinline__ int token(int step) const {
+    return step < sink_steps ? step * BK : lo + (step - sink_steps) * BK;
+  }
+};
+
+// Row range of a sequence, kept within the tensor whatever the starts hold.
+__device__ __forceinline__ void seq_rows(const int32_t* starts, int seq, int total, int& q0, int& q1) {
+  q0 = seq;
+  q1 = seq + 1;
+  if (starts != nullptr) {
+    q0 = min(max(starts[seq], 0), total);
+    q1 = min(max(starts[seq + 1], q0), total);
+  }
+}
+
+// Rows of a result that belong to no sequence (before the first, behind the
+// last) become zeros, spread over the workgroups of the launch; usually none.
+__device__ __forceinline__ void zero_outside(uint16_t* x, int64_t stride, int width, const int32_t* starts,
+                                             int num_seqs, int total, int wg, int wgs) {
+  const int head = min(max(starts[0], 0), total), tail = min(max(starts[num_seqs], head), total);
+  const int n = head + total - tail;
+  for (int i = wg; i < n; i += wgs) {
+    const int64_t row = i < head ? i : tail + i - head;
+    for (int d = threadIdx.x * 8; d < width; d += blockDim.x * 8) *(u4*)(x + row * stride + d) = u4{};
+  }
+}
+
+// Workgroups go round-robin to the eight XCDs, each with an L2 of its own:
+// neighbours in `order` (row tiles of one kv head, which read the same keys
+// and values) get the same XCD.
+__device__ __forceinline__ int xcd_order(int b, int padded) { return (b & 7) * (padded >> 3) + (b >> 3); }
+
+// Non-finite elements of a 16-byte operand (eight 16-bit values).
+template <bool BF>
+__device__ __forceinline__ bool any_nonfinite(h8 x) {
+  constexpr uint32_t kExp = BF ? 0x7F80u : 0x7C00u;
+  const u4 v = __builtin_bit_cast(u4, x);
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    bad |= (v[e] & kExp) == kExp;
+    bad |= (v[e] & (kExp << 16)) == kExp << 16;
+  }
+  return bad;
+}
+
+// x without its non-finite elements; pos (neg): 1 where x is +inf (-inf) or NaN.
+template <bool BF>
+__device__ __forceinline__ void split_nonfinite(h8& x, h8& pos, h8& neg) {
+  constexpr uint32_t kExp = BF ? 0x7F80u : 0x7C00u, kOne = BF ? 0x3F80u : 0x3C00u;
+  u4 v = __builtin_bit_cast(u4, x), p, n;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t vo = 0, po = 0, no = 0;
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      const uint32_t b = (v[e] >> h) & 0xFFFFu;
+      const bool bad = (b & kExp) == kExp;
+      vo |= (bad ? 0u : b) << h;
+      po |= (bad && b != (0x8000u | kExp) ? kOne : 0u) << h;
+      no |= (bad && b != kExp ? kOne : 0u) << h;
+    }
+    v[e] = vo;
+    p[e] = po;
+    n[e] = no;
+  }
+  x = __builtin_bit_cast(h8, v);
+  pos = __builtin_bit_cast(h8, p);
+  neg = __builtin_bit_cast(h8, n);
+}
+
+// The lane's eight scores of reduction step s: bit e set where token
+// t0 + 16 s + 8 (lane / 32) + e is visible from a row: not after `last` (and
+// within the cache), after `before`, or a sink.
+__device__ __forceinline__ bool sees(int j, int last, int before, int sinks) {
+  return j <= last && (j > before || j < sinks);
+}
+
+// global -> LDS copy of 16 / 4 bytes per active lane, to lds + lane * 16 / 4 (a
+// wave-uniform base).  In assembly, so that the compiler does not make every
+// later LDS read wait for it; the kernels wait themselves (wait_copies()).
+typedef __attribute__((address_space(3))) const void lds_cvoid;
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return (uint32_t)(uintptr_t)(lds_cvoid*)p;
+}
+__device__ __forceinline__ void copy16(const void* g, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void copy4(const void* g, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory");
+}
+// Every copy of this workgroup has landed and every wave has left the stage before.
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Row-major tiles in LDS ([row][HS], as the tensors have them): 16-byte unit u
+// of row r stands at unit u ^ swizzle<HS>(r), so that both reads, a unit of 32
+// rows (row_unit) and four rows by 32 dims (column_unit), spread over the banks.
+template <int HS>
+__device__ __forceinline__ int swizzle(int r) {
+  if constexpr (HS == 64) return ((r & 2) << 1) | ((r >> 2) & 3);
+  else if constexpr (HS % 128 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else return 0;  // 80, 96 and 112: the rows' own stride does it
+}
+// A operand: row r, units 2 kk + lane / 32.
+template <int HS>
+__device__ __forceinline__ h8 row_unit(const unsigned char* tile, int r, int unit) {
+  return *(const h8*)(tile + r * (HS * 2) + ((unit ^ swizzle<HS>(r)) << 4));
+}
+// A operand of the transposed tile: dims 32 dt + lane % 32 (below HS), rows
+// r0 + 8 (lane / 32) .. + 7, by two transposing reads.  Lane l of 16 gives the
+// address of four dims of row l / 4 and receives dim l of the four rows.
+template <int HS>
+__device__ __forceinline__ h8 column_unit(const unsigned char* tile, int r0, int dt) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s4 lds_s4;
+  const int lane = threadIdx.x & 63;
+  int d = dt * 32 + (lane & 16);
+  if (HS % 32 != 0) d = min(d, HS - 16);
+  d += 4 * (lane & 3);
+  const int r = r0 + ((lane >> 5) << 3) + ((lane >> 2) & 3);
+  s4 x[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const unsigned char* at = tile + (r + 4 * h) * (HS * 2) +
+                              ((((d >> 3) ^ swizzle<HS>(r + 4 * h)) << 4) | ((d & 7) << 1));
+    x[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
+  }
+  typedef short s8 __attribute__((ext_vector_type(8)));
+  return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+}  // namespace dw4

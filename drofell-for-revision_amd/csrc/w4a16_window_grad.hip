@@ -1,0 +1,377 @@
+// Gradients of windowed attention over packed sequences (training).
+//
+// With P the probabilities, dO the output's gradient and c the scale:
+//   delta_i = dO_i . O_i          dV_j = sum_i P_ij dO_i
+//   dS_ij   = P_ij (dO_i . V_j - delta_i)
+//   dQ_i = c sum_j dS_ij K_j      dK_j = c sum_i dS_ij Q_i
+// P is formed again from the forward's log-sums.  Two kernels, seven products
+// where one pass with atomic sums would need five, so that every sum has one
+// order and results repeat bit for bit:
+//   * window_dq_kernel: as the forward, 128 rows (tokens x query heads of a kv
+//     head) of a workgroup, steps of 64 tokens through LDS; it writes delta too;
+//   * window_dkv_kernel: 128 tokens of a workgroup, a wave's 32 as the columns
+//     of its products, steps of 64 rows through LDS; the heads of a group are
+//     rows like any others, so that shared heads' gradients add up in registers.
+// Both read a tile from LDS in both directions, rows in plain and columns in
+// transposing reads.  Matrix-core and LDS-read bound.
+//
+// Roundings: P and dS enter the products in 16 bits, as the matrix cores take
+// them, with independent errors.  fp16 holds neither small probabilities nor
+// small gradients, so P goes in as 2^10 P and dS times a power of two that
+// brings the largest |dO| of the rows it is summed with to 1/16 .. 1/8; bf16
+// needs neither.  delta comes from the rounded output: its error is half a
+// step of O, one part in some thousands of |dO| |O|, beside dS's own rounding.
+// A sequence's non-finite values may reach any gradient of that sequence.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+
+#include "w4a16_device.h"
+#include "w4a16_window.h"
+#include "w4a16_window_device.h"
+
+namespace dw4 {
+
+namespace {
+
+constexpr int kBk = kWinTileTokens;
+constexpr int kGradTile = 128;  // rows of a dq workgroup, tokens of a dkv workgroup
+
+// The power of two that brings a largest |dO| to 1/16 .. 1/8 (1 for 0, inf and NaN, and for bf16).
+template <bool BF>
+__device__ __forceinline__ float grad_scale(float most) {
+  if (BF || !(most > 0.f) || !(most < INFINITY)) return 1.f;
+  return __builtin_amdgcn_ldexpf(1.f, -3 - __builtin_amdgcn_frexp_expf(most));
+}
+
+template <bool BF>
+__device__ __forceinline__ void dot8(u4 x, u4 y, float& sum, float& most) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float a = unpack<BF>(x[e], h);
+      sum = fmaf(a, unpack<BF>(y[e], h), sum);
+      most = fmaxf(most, fabsf(a));
+    }
+}
+
+template <int HS, bool BF>
+__global__ void __launch_bounds__(256, HS <= 128 ? 2 : 1)
+window_dq_kernel(WindowGradArgs g, int tiles, int padded, float* __restrict__ delta, float* __restrict__ most) {
+  constexpr int KD = HS / 16, ND = (HS + 31) / 32;
+  constexpr bool VTAIL = HS % 32 != 0;
+  constexpr int TILE = kBk * HS * 2, STAGE = 2 * TILE;  // keys, values
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const WindowArgs& a = g.f;
+  zero_outside(g.dq, g.dq_stride, a.num_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, padded);
+  const int id = xcd_order(blockIdx.x, padded);
+  if (id >= a.num_seqs * a.num_kv_heads * tiles) return;
+  const int tile = tiles - 1 - id % tiles;
+  const int pair = id / tiles;
+  const int seq = pair / a.num_kv_heads, kvh = pair % a.num_kv_heads;
+  const int G = a.num_heads / a.num_kv_heads;
+  int q0, q1;
+  seq_rows(a.starts, seq, a.total_rows, q0, q1);
+  const int n = min(q1 - q0, a.max_query);
+  const int rows = n * G, base = tile * kGradTile;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (base >= rows) return;
+  const int c = lane & 31, half = lane >> 5;
+  const Span span = Span::of<kBk>(base / G, (min(base + kGradTile, rows) - 1) / G, n, a.window, a.sinks);
+  const int wbase = base + 32 * wave;
+  const int nrows = min(32, rows - wbase);
+  const int row = min(wbase + c, rows - 1);
+  const int pos = row / G, before = a.window == 0 ? INT32_MIN : pos - a.window;
+  const int wfirst = min(wbase, rows - 1) / G, wlast = min(wbase + 31, rows - 1) / G;
+  const int token = q0 + pos, head = kvh * G + row % G;
+
+  const uint32_t lds0 = lds_offset(lds);
+  auto issue = [&](int s, int stage) {
+    const uint32_t dst = lds0 + stage * STAGE;
+    const int t = span.token<kBk>(s);
+    constexpr int UNITS = HS / 8, CHUNKS = kBk * UNITS / 64;
+    for (int ch = wave; ch < CHUNKS; ch += 4) {
+      const int u = ch * 64 + lane;
+      const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
+      const int64_t tok = q0 + min(t + r, n - 1);
+      const size_t col = (size_t)kvh * HS + at * 8;
+      copy16(a.k + tok * a.k_stride + col, dst + ch * 1024);
+      copy16(a.v + tok * a.v_stride + col, dst + TILE + ch * 1024);
+    }
+  };
+  if (span.steps > 0) issue(0, 0);
+  h8 qreg[KD], oreg[KD];  // B operands: this row of Q and of dO
+  float dl = 0.f, mo = 0.f;
+  {
+    const size_t col = (size_t)head * HS + 8 * half;
+    const uint16_t* qp = a.q + (size_t)token * a.q_stride + col;
+    const uint16_t* dp = g.dout + (size_t)token * g.do_stride + col;
+    const uint16_t* op = a.out + (size_t)token * a.o_stride + col;
+#pragma unroll
+    for (int j = 0; j < KD; ++j) {
+      qreg[j] = *(const h8*)(qp + 16 * j);
+      oreg[j] = *(const h8*)(dp + 16 * j);
+      dot8<BF>(__builtin_bit_cast(u4, oreg[j]), *(const u4*)(op + 16 * j), dl, mo);
+    }
+  }
+  dl = both_sum(dl);
+  mo = both_max(mo);
+  const float lse = a.lse[(size_t)token * a.num_heads + head];
+  if (c < nrows && half == 0) delta[(size_t)token * a.num_heads + head] = dl;
+  const float gs = grad_scale<BF>(mo);
+  if constexpr (!BF) {  // the largest |dO| of the tile, for the dkv kernel
+    __shared__ float top[4];
+    float w = mo;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) w = fmaxf(w, __shfl_xor(w, off));
+    if (lane == 0) top[wave] = w;
+    __syncthreads();
+    if (threadIdx.x == 0) most[(size_t)pair * tiles + tile] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  }
+
+  f16v dq[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dq[d] = f16v{};
+  for (int step = 0; step < span.steps; ++step) {
+    wait_copies();
+    if (step + 1 < span.steps) issue(step + 1, (step + 1) & 1);
+    const int t = span.token<kBk>(step);
+    if (nrows <= 0) continue;
+    const unsigned char* st = lds + (step & 1) * STAGE;
+    for (int b = 0; b < 2; ++b) {
+      const int tb = t + 32 * b;
+      if (tb > wlast || (a.window != 0 && tb + 31 <= wfirst - a.window && tb >= a.sinks)) continue;
+      const bool full = tb + 31 <= wfirst && (a.window == 0 || tb > wlast - a.window || tb + 31 < a.sinks);
+      f16v s = {}, p = {};
+#pragma unroll
+      for (int j = 0; j < KD; ++j) s = mfma32_of<BF>(row_unit<HS>(st, 32 * b + row_token(c), 2 * j + half), qreg[j], s);
+#pragma unroll
+      for (int j = 0; j < KD; ++j) p = mfma32_of<BF>(row_unit<HS>(st + TILE, 32 * b + row_token(c), 2 * j + half), oreg[j], p);
+      float ds[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * ((p[e] - dl) * gs);
+      if (!full) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          ds[e] = sees(tb + 16 * (e >> 3) + 8 * half + (e & 7), pos, before, a.sinks) ? ds[e] : 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const h8 w = __builtin_bit_cast(h8, u4{pack2<BF>(ds[8 * x], ds[8 * x + 1]), pack2<BF>(ds[8 * x + 2], ds[8 * x + 3]),
+                                               pack2<BF>(ds[8 * x + 4], ds[8 * x + 5]), pack2<BF>(ds[8 * x + 6], ds[8 * x + 7])});
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dq[d] = mfma32_of<BF>(column_unit<HS>(st, 32 * b + 16 * x, d), w, dq[d]);
+      }
+    }
+  }
+  if (c >= nrows) return;
+  const float f = g.scale / gs;
+  uint16_t* out = g.dq + (size_t)token * g.dq_stride + (size_t)head * HS;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int dim = d * 32 + 2 * e + 4 * half;
+      if (!VTAIL || dim < HS)
+        *(uint2*)(out + dim) = make_uint2(pack2<BF>(dq[d][e] * f, dq[d][e + 1] * f),
+                                          pack2<BF>(dq[d][e + 2] * f, dq[d][e + 3] * f));
+    }
+}
+
+template <int HS, bool BF>
+__global__ void __launch_bounds__(256, 1)
+window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, int padded, uint32_t magic,
+                  const float* __restrict__ delta, const float* __restrict__ most) {
+  constexpr int KD = HS / 16, ND = (HS + 31) / 32;
+  constexpr bool VTAIL = HS % 32 != 0;
+  constexpr int TILE = kBk * HS * 2;
+  constexpr int STAGE = 2 * TILE + 3 * kBk * 4;  // rows of Q and of dO, log-sums, deltas, positions
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const WindowArgs& a = g.f;
+  zero_outside(g.dk, g.dk_stride, a.num_kv_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, padded);
+  zero_outside(g.dv, g.dv_stride, a.num_kv_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, padded);
+  const int id = xcd_order(blockIdx.x, padded);
+  if (id >= a.num_seqs * a.num_kv_heads * tiles) return;
+  const int tile = id % tiles;  // the longest row ranges first
+  const int pair = id / tiles;
+  const int seq = pair / a.num_kv_heads, kvh = pair % a.num_kv_heads;
+  const int G = a.num_heads / a.num_kv_heads;
+  int q0, q1;
+  seq_rows(a.starts, seq, a.total_rows, q0, q1);
+  const int n = min(q1 - q0, a.max_query);
+  const int t0 = tile * kGradTile;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (t0 >= n) return;
+  const int c = lane & 31, half = lane >> 5;
+  // rows that see a token of the tile
+  const int64_t reach = a.window == 0 || t0 < a.sinks ? n : (int64_t)t0 + kGradTile - 1 + a.window;
+  const int r0 = t0 * G, r1 = (int)min<int64_t>(n, reach) * G;
+  const int steps = (r1 - r0 + kBk - 1) / kBk;
+  const int wa = t0 + 32 * wave, wb = min(wa + 31, n - 1);  // this wave's tokens
+  const int tk = min(wa + c, n - 1);
+
+  const uint32_t lds0 = lds_offset(lds);
+  auto issue = [&](int s, int stage) {
+    const uint32_t dst = lds0 + stage * STAGE;
+    constexpr int UNITS = HS / 8, CHUNKS = kBk * UNITS / 64;
+    for (int ch = wave; ch < CHUNKS; ch += 4) {
+      const int u = ch * 64 + lane;
+      const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
+      const int row = min(r0 + s * kBk + r, r1 - 1), i = div_by_magic(row, magic);
+      const size_t col = (size_t)(kvh * G + row - i * G) * HS + at * 8;
+      copy16(a.q + (size_t)(q0 + i) * a.q_stride + col, dst + ch * 1024);
+      copy16(g.dout + (size_t)(q0 + i) * g.do_stride + col, dst + TILE + ch * 1024);
+    }
+    if (wave < 3) {
+      const int row = r0 + s * kBk + lane, in = min(row, r1 - 1), i = div_by_magic(in, magic);
+      const size_t at = (size_t)(q0 + i) * a.num_heads + kvh * G + in - i * G;
+      if (wave == 0) copy4(a.lse + at, dst + 2 * TILE);
+      else if (wave == 1) copy4(delta + at, dst + 2 * TILE + kBk * 4);
+      else *(int*)(lds + stage * STAGE + 2 * TILE + 2 * kBk * 4 + lane * 4) = row < r1 ? i : -1;
+    }
+  };
+  issue(0, 0);
+  h8 kreg[KD], vreg[KD];  // B operands: this token's key and value
+  {
+    const size_t col = (size_t)kvh * HS + 8 * half;
+    const uint16_t* kp = a.k + (size_t)(q0 + tk) * a.k_stride + col;
+    const uint16_t* vp = a.v + (size_t)(q0 + tk) * a.v_stride + col;
+#pragma unroll
+    for (int j = 0; j < KD; ++j) {
+      kreg[j] = *(const h8*)(kp + 16 * j);
+      vreg[j] = *(const h8*)(vp + 16 * j);
+    }
+  }
+  float gs = 1.f;
+  if constexpr (!BF) {
+    float w = 0.f;
+    for (int i = lane; i < (n * G + kGradTile - 1) / kGradTile; i += 64) w = fmaxf(w, most[(size_t)pair * row_tiles + i]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) w = fmaxf(w, __shfl_xor(w, off));
+    gs = grad_scale<BF>(w);
+  }
+  const float ps = p_shift<BF>(), gp = gs * __builtin_amdgcn_exp2f(-ps);
+
+  f16v dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f16v{};
+  for (int step = 0; step < steps; ++step) {
+    wait_copies();
+    if (step + 1 < steps) issue(step + 1, (step + 1) & 1);
+    if (wa >= n) continue;
+    const unsigned char* st = lds + (step & 1) * STAGE;
+    const float* ls = (const float*)(st + 2 * TILE);
+    const int* at = (const int*)(st + 2 * TILE + 2 * kBk * 4);
+    for (int b = 0; b < 2; ++b) {
+      const int ra = r0 + step * kBk + 32 * b;
+      if (ra >= r1) continue;
+      const int ia = div_by_magic(ra, magic), ib = div_by_magic(min(ra + 31, r1 - 1), magic);
+      if (ib < wa || (a.window != 0 && ia - a.window >= wb && wa >= a.sinks)) continue;
+      const bool full = ra + 31 < r1 && ia >= wb && (a.window == 0 || ib < wa + a.window || wb < a.sinks);
+      f16v s = {}, p = {};
+#pragma unroll
+      for (int j = 0; j < KD; ++j) s = mfma32_of<BF>(row_unit<HS>(st, 32 * b + row_token(c), 2 * j + half), kreg[j], s);
+#pragma unroll
+      for (int j = 0; j < KD; ++j) p = mfma32_of<BF>(row_unit<HS>(st + TILE, 32 * b + row_token(c), 2 * j + half), vreg[j], p);
+      h8 pw[2], dw[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = 32 * b + 16 * x + 8 * half;  // the lane's eight rows
+        float pr[8], ds[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          pr[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * x + e], a.scale_log2, ps - ls[r + e]));
+          ds[e] = pr[e] * ((p[8 * x + e] - ls[kBk + r + e]) * gp);
+        }
+        if (!full) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int i = at[r + e];
+            const bool seen = sees(wa + c, i, a.window == 0 ? INT32_MIN : i - a.window, i < 0 ? 0 : a.sinks);
+            pr[e] = seen ? pr[e] : 0.f;
+            ds[e] = seen ? ds[e] : 0.f;
+          }
+        }
+        pw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(pr[0], pr[1]), pack2<BF>(pr[2], pr[3]), pack2<BF>(pr[4], pr[5]), pack2<BF>(pr[6], pr[7])});
+        dw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(ds[0], ds[1]), pack2<BF>(ds[2], ds[3]), pack2<BF>(ds[4], ds[5]), pack2<BF>(ds[6], ds[7])});
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          dv[d] = mfma32_of<BF>(column_unit<HS>(st + TILE, 32 * b + 16 * x, d), pw[x], dv[d]);
+          dk[d] = mfma32_of<BF>(column_unit<HS>(st, 32 * b + 16 * x, d), dw[x], dk[d]);
+        }
+    }
+  }
+  if (wa + c >= n) return;
+  const float fk = g.scale / gs, fv = __builtin_amdgcn_exp2f(-ps);
+  uint16_t* ok = g.dk + (size_t)(q0 + tk) * g.dk_stride + (size_t)kvh * HS;
+  uint16_t* ov = g.dv + (size_t)(q0 + tk) * g.dv_stride + (size_t)kvh * HS;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int dim = d * 32 + 2 * e + 4 * half;
+      if (!VTAIL || dim < HS) {
+        *(uint2*)(ok + dim) = make_uint2(pack2<BF>(dk[d][e] * fk, dk[d][e + 1] * fk), pack2<BF>(dk[d][e + 2] * fk, dk[d][e + 3] * fk));
+        *(uint2*)(ov + dim) = make_uint2(pack2<BF>(dv[d][e] * fv, dv[d][e + 1] * fv), pack2<BF>(dv[d][e + 2] * fv, dv[d][e + 3] * fv));
+      }
+    }
+}
+
+template <int HS, bool BF>
+hipError_t launch_grad_hs(const WindowGradArgs& g, float* ws, hipStream_t stream) {
+  static std::atomic<uint64_t> done_q{0}, done_kv{0};
+  const WindowArgs& a = g.f;
+  const int G = a.num_heads / a.num_kv_heads;
+  const size_t smem = win_tile_smem(HS), smem_kv = smem + 2 * 3 * kBk * 4;
+  auto dq = &window_dq_kernel<HS, BF>;
+  auto dkv = &window_dkv_kernel<HS, BF>;
+  hipError_t e = allow_lds(reinterpret_cast<const void*>(dq), smem, done_q);
+  if (e == hipSuccess) e = allow_lds(reinterpret_cast<const void*>(dkv), smem_kv, done_kv);
+  if (e != hipSuccess) return e;
+  const int pairs = a.num_seqs * a.num_kv_heads;
+  const int row_tiles = (int)(((int64_t)a.max_query * G + kGradTile - 1) / kGradTile);
+  const int tiles = (a.max_query + kGradTile - 1) / kGradTile;
+  float* delta = ws;
+  float* most = ws + (size_t)a.total_rows * a.num_heads;
+  const int pq = (pairs * row_tiles + 7) / 8 * 8, pk = (pairs * tiles + 7) / 8 * 8;
+  dq<<<(unsigned)pq, 256, smem, stream>>>(g, row_tiles, pq, delta, most);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const uint32_t magic = G == 1 ? 0u : (uint32_t)((0x100000000ull + G - 1) / G);
+  dkv<<<(unsigned)pk, 256, smem_kv, stream>>>(g, tiles, row_tiles, pk, magic, delta, most);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+template <bool BF>
+hipError_t launch_window_grad(const WindowGradArgs& g, float* ws, hipStream_t stream) {
+  switch (g.f.head_size) {
+    case 64: return launch_grad_hs<64, BF>(g, ws, stream);
+    case 80: return launch_grad_hs<80, BF>(g, ws, stream);
+    case 96: return launch_grad_hs<96, BF>(g, ws, stream);
+    case 112: return launch_grad_hs<112, BF>(g, ws, stream);
+    case 128: return launch_grad_hs<128, BF>(g, ws, stream);
+    case 256: return launch_grad_hs<256, BF>(g, ws, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+template hipError_t launch_window_grad<WINDOW_BF16>(const WindowGradArgs&, float*, hipStream_t);
+
+#if !WINDOW_BF16
+size_t window_grad_ws_bytes(int num_seqs, int total_rows, int num_heads, int num_kv_heads, int max_query) {
+  const int64_t row_tiles = ((int64_t)max_query * (num_heads / num_kv_heads) + kGradTile - 1) / kGradTile;
+  return sizeof(float) * ((size_t)total_rows * num_heads + (size_t)num_seqs * num_kv_heads * row_tiles);
+}
+#endif
+
+}  // namespace dw4

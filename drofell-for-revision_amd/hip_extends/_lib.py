@@ -26,6 +26,9 @@ DW4_ERR_DEVICE = 7
 DW4_ERR_SCRATCH = 8
 NOALLOC_SCRATCH_BYTES = 64 << 20
 
+DW4_F16 = 0
+DW4_BF16 = 1
+
 DW4_PATH_AUTO = 0
 DW4_PATH_DECODE = 1
 DW4_PATH_PREFILL = 2
@@ -123,6 +126,19 @@ SIGNATURES = {
     "dw4_rope_and_cache": (_c.c_int, [_c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _P,
                                       _c.c_int64, _P, _c.c_int64, _P, _c.c_int64, _P, _P,
                                       _c.c_int, _P, _P, _c.c_int, _P, _P, _c.c_int, _P, _P]),
+    "dw4_window_attention": (_c.c_int, [_c.c_int] * 7 + [_P, _c.c_int64, _P, _c.c_int64, _P,
+                                        _c.c_int, _c.c_int, _P, _P, _c.c_int, _c.c_float,
+                                        _c.c_int, _c.c_int, _P, _c.c_int, _P, _c.c_int, _P,
+                                        _c.c_size_t, _P]),
+    "dw4_window_attention_workspace_size": (_c.c_int, [_c.c_int] * 10 + [_SZ]),
+    "dw4_window_attention_dense": (_c.c_int, [_c.c_int] * 5 + [_P, _c.c_int64] * 4
+                                   + [_P, _P, _c.c_int, _c.c_int, _c.c_float, _c.c_int,
+                                      _c.c_int, _P]),
+    "dw4_window_attention_dense_backward": (_c.c_int, [_c.c_int] * 5 + [_P, _c.c_int64] * 4 + [_P]
+                                            + [_P, _c.c_int64] * 4
+                                            + [_P, _c.c_int, _c.c_int, _c.c_float, _c.c_int,
+                                               _c.c_int, _P, _c.c_size_t, _P]),
+    "dw4_window_attention_dense_backward_workspace_size": (_c.c_int, [_c.c_int] * 5 + [_SZ]),
     "dw4_gemm_group": (_c.c_int, [_c.c_int, _IP, _c.c_int, _P, _c.c_int64, _P, _c.c_size_t, _P]),
     "dw4_gemm_silu_mul": (_c.c_int, [_c.c_int, _P, _c.c_int64, _IP, _IP, _P, _c.c_int64,
                                      _P, _c.c_size_t, _P]),
@@ -274,4 +290,27 @@ def paged_attention_workspace_size(num_seqs: int, num_heads: int, num_kv_heads: 
     check("dw4_paged_attention_workspace_size", lib.dw4_paged_attention_workspace_size(
         num_seqs, num_heads, num_kv_heads, head_size, block_size, max_context_len,
         ctypes.byref(out)))
+    return out.value
+
+
+@functools.lru_cache(maxsize=4096)
+def window_attention_workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int,
+                                    head_size: int, block_size: int, total_rows: int,
+                                    max_query_len: int, window: int, sinks: int,
+                                    max_context_len: int, device: Optional[int] = None) -> int:
+    """Bytes of one such dw4_window_attention call on the current device
+    (``device``, its index, only tells several devices' sizes apart)."""
+    out = ctypes.c_size_t(0)
+    check("dw4_window_attention_workspace_size", load().dw4_window_attention_workspace_size(
+        num_seqs, num_heads, num_kv_heads, head_size, block_size, total_rows, max_query_len, window,
+        sinks, max_context_len, ctypes.byref(out)))
+    return out.value
+
+
+def window_attention_backward_workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int,
+                                             total_rows: int, max_seq_len: int) -> int:
+    out = ctypes.c_size_t(0)
+    fn = "dw4_window_attention_dense_backward_workspace_size"
+    check(fn, getattr(load(), fn)(num_seqs, num_heads, num_kv_heads, total_rows, max_seq_len,
+                                  ctypes.byref(out)))
     return out.value

@@ -50,6 +50,11 @@ class LayerBlocksHolder:
         self.device = layer_key_ptr_table_device.device
 
     @property
+    def dtype(self) -> torch.dtype:
+        """Type of the cached keys and values: bf16 for a bf16 geometry, else fp16."""
+        return torch.bfloat16 if self.block_info.dtype == torch.bfloat16 else torch.float16
+
+    @property
     def is_contigious(self) -> bool:
         return self._contigious_kv_tensor is not None
 
@@ -63,8 +68,8 @@ class LayerBlocksHolder:
               slot_mapping: torch.Tensor) -> None:
         if key_states.shape[0] != slot_mapping.shape[0] or key_states.shape != val_states.shape:
             raise AssertionError("key/value rows must match slot_mapping")
-        if key_states.dtype != torch.float16 or val_states.dtype != torch.float16:
-            raise TypeError("the KV cache holds fp16")
+        if key_states.dtype != self.dtype or val_states.dtype != self.dtype:
+            raise TypeError(f"the KV cache holds {self.dtype}")
         n, heads, hs = key_states.shape
         if heads != self.block_info.num_key_value_heads or hs != self.block_info.head_dim:
             raise AssertionError("key/value shape does not match the block geometry")
@@ -91,8 +96,8 @@ class LayerBlocksHolder:
             self, slot_mapping: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         n = slot_mapping.shape[0]
         shape = (n, self.block_info.num_key_value_heads, self.block_info.head_dim)
-        k = torch.empty(shape, dtype=torch.float16, device=self.device)
-        v = torch.empty(shape, dtype=torch.float16, device=self.device)
+        k = torch.empty(shape, dtype=self.dtype, device=self.device)
+        v = torch.empty(shape, dtype=self.dtype, device=self.device)
         self.kv_tensor_from_slots_with_convert(k, v, slot_mapping)
         return k, v
 

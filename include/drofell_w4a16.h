@@ -482,6 +482,73 @@ int dw4_rope_and_cache(int num_seqs, int num_heads, int num_kv_heads, int head_d
                        const int64_t* value_block_ptrs, int kv_head_stride,
                        int32_t* context_lens_out, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Windowed attention: the token at position i of a sequence sees the tokens
+ * j <= i with j > i - window (window 0: all of them), and the first `sinks`
+ * tokens whatever their distance.  No counterpart in the reference.  Softmax
+ * and both products are summed in fp32; results are deterministic.  A row that
+ * sees nothing is zero.  dtype: DW4_F16 or DW4_BF16, of queries, keys, values and
+ * outputs; head_size as in dw4_paged_attention, any number of query heads per
+ * kv head; scale > 0.
+ * ------------------------------------------------------------------------- */
+#define DW4_F16 0
+#define DW4_BF16 1
+
+/* New tokens of each sequence over its cached context (their own keys and
+ * values are in the cache already).  Rows of query and out: [total_rows]
+ * [num_heads][head_size], sequence s having the rows query_starts[s] ..
+ * query_starts[s + 1] - 1 (int32 device [num_seqs + 1], ascending; NULL: one row
+ * each), at most max_query_len of them, the last at position
+ * context_lens[s] - 1.  Sequences may have no row, and contexts no token.  Rows
+ * of no sequence are left as they are.  Block tables, cache layout and
+ * pointer tables (num_blocks entries) as in dw4_paged_attention, block
+ * addresses 16-byte aligned; a table entry outside 0 .. num_blocks - 1 means
+ * that the block is not there (freed behind the window): its tokens are not
+ * seen, and nothing is read.  Keys and values of tokens that a row does not see
+ * do not reach it, whatever they hold.  context_lens at most max_context_len.
+ * workspace: dw4_window_attention_workspace_size bytes (0 for most calls). */
+int dw4_window_attention(int dtype, int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                         int block_size, int num_blocks, const uint16_t* query, int64_t q_stride,
+                         uint16_t* out, int64_t o_stride, const int32_t* query_starts, int total_rows,
+                         int max_query_len, const int64_t* key_block_ptrs,
+                         const int64_t* value_block_ptrs, int kv_head_stride, float scale, int window,
+                         int sinks, const int32_t* block_tables, int max_blocks_per_seq,
+                         const int32_t* context_lens, int max_context_len, void* workspace,
+                         size_t workspace_bytes, void* stream);
+int dw4_window_attention_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                                        int block_size, int total_rows, int max_query_len, int window,
+                                        int sinks, int max_context_len, size_t* workspace_bytes);
+
+/* Packed sequences: q, out [total_rows][num_heads][head_size], k, v
+ * [total_rows][num_kv_heads][head_size] with row strides, sequence s in the rows
+ * seq_starts[s] .. seq_starts[s + 1] - 1 (int32 device, ascending), each at most
+ * max_seq_len long.  Output rows of no sequence become zeros.  lse: float
+ * [total_rows][num_heads], the base-2 logarithm of each row's softmax sum, for
+ * the backward pass, or NULL. */
+int dw4_window_attention_dense(int dtype, int num_seqs, int num_heads, int num_kv_heads,
+                               int head_size, const uint16_t* q, int64_t q_stride, const uint16_t* k,
+                               int64_t k_stride, const uint16_t* v, int64_t v_stride, uint16_t* out,
+                               int64_t o_stride, float* lse, const int32_t* seq_starts, int total_rows,
+                               int max_seq_len, float scale, int window, int sinks, void* stream);
+
+/* Its gradients dq, dk, dv (shapes of q, k, v; rows of no sequence become
+ * zeros) for the output gradient dout, from the forward's inputs, out and lse.
+ * Deterministic, also where query heads share a kv head.  workspace:
+ * dw4_window_attention_dense_backward_workspace_size bytes. */
+int dw4_window_attention_dense_backward(int dtype, int num_seqs, int num_heads, int num_kv_heads,
+                                        int head_size, const uint16_t* q, int64_t q_stride,
+                                        const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                                        int64_t v_stride, const uint16_t* out, int64_t o_stride,
+                                        const float* lse, const uint16_t* dout, int64_t do_stride,
+                                        uint16_t* dq, int64_t dq_stride, uint16_t* dk,
+                                        int64_t dk_stride, uint16_t* dv, int64_t dv_stride,
+                                        const int32_t* seq_starts, int total_rows, int max_seq_len,
+                                        float scale, int window, int sinks, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+int dw4_window_attention_dense_backward_workspace_size(int num_seqs, int num_heads, int num_kv_heads,
+                                                       int total_rows, int max_seq_len,
+                                                       size_t* workspace_bytes);
+
 /* ------------------------------------------------------------------------
  * Decode chain: one launch over a list of projections at m <= 4 (no single
  * reference call: it runs the per-projection q4_matmul_cuda_v2 calls,

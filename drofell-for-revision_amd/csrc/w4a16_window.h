@@ -47,6 +47,13 @@ constexpr int kWinRowsTile = 32;    // rows of a wave's MFMA columns
 constexpr int kWinRowsTokens = 32;  // tokens of a step of the rows kernel
 constexpr int kWinTileTokens = 64;  // tokens of a step of the tile kernels
 constexpr int kWinMaxWindow = 1 << 30;
+// Workgroups that share an XCD (work_of in w4a16_window_device.h), and the grid for them.
+constexpr int kWinUnit = 8;
+inline unsigned win_grid(int pairs, int items) {
+  const int64_t unit = items < kWinUnit ? items : kWinUnit;
+  const int64_t units = (items + unit - 1) / unit * pairs;
+  return (unsigned)((units + 7) / 8 * 8 * unit);
+}
 
 inline size_t win_rows_smem(int hs, int cols, int waves) {
   return sizeof(float) * (size_t)waves * cols * (hs + 2);

@@ -35,7 +35,7 @@ namespace {
 
 template <int HS, int BS, bool BF, int W>
 __global__ void __launch_bounds__(W * 64, W == 8 || HS <= 128 ? 2 : 1)
-window_rows_kernel(WindowArgs a, int tiles, int splits, int padded, int cols, float* __restrict__ ws_ml,
+window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restrict__ ws_ml,
                    float* __restrict__ ws_out) {
   constexpr int KD = HS / 16;         // 16-dim reduction steps of q . k
   constexpr int ND = (HS + 31) / 32;  // 32-dim tiles of p . v (the last may be half empty)
@@ -43,11 +43,10 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int padded, int cols, fl
   constexpr bool VTAIL = HS % 32 != 0;
   extern __shared__ __attribute__((aligned(16))) float sm[];
 
-  const int id = xcd_order(blockIdx.x, padded);
-  if (id >= a.num_seqs * a.num_kv_heads * tiles * splits) return;
-  const int split = id % splits;
-  const int tile = id / splits % tiles;
-  const int pair = id / (splits * tiles);
+  int pair, item;
+  if (!work_of(blockIdx.x, a.num_seqs * a.num_kv_heads, tiles * splits, pair, item)) return;
+  const int split = item % splits;
+  const int tile = item / splits;
   const int seq = pair / a.num_kv_heads, kvh = pair % a.num_kv_heads;
   const int G = a.num_heads / a.num_kv_heads;
   int q0, q1;
@@ -199,36 +198,26 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int padded, int cols, fl
       odd = __any(odd);
     }
     if (odd) {
-      h8 vis[2];
+      uint32_t seen = 0;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        u4 b;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          b[e] = 0;
-          for (int k = 0; k < 2; ++k) {
-            const bool there = (held_now >> (NB == 2 ? g : 0)) & 1;
-            if (there && sees(t + 16 * g + 8 * half + 2 * e + k, last, before, a.sinks))
-              b[e] |= (BF ? 0x3F80u : 0x3C00u) << (16 * k);
-          }
-        }
-        vis[g] = __builtin_bit_cast(h8, b);
+      for (int e = 0; e < 16; ++e) {
+        const bool there = (held_now >> (NB == 2 ? e >> 3 : 0)) & 1;
+        seen |= (uint32_t)(there && sees(t + 16 * (e >> 3) + 8 * half + (e & 7), last, before, a.sinks)) << e;
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        f16v up = {}, down = {};
+        for (uint32_t sign = 0; sign <= 0x8000u; sign += 0x8000u) {
+          const float inf = sign ? -INFINITY : INFINITY;
+          f16v count = {};
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          h8 pn, nn;
-          split_nonfinite<BF>(vreg[d][g], pn, nn);
-          up = mfma32_of<BF>(pn, vis[g], up);
-          down = mfma32_of<BF>(nn, vis[g], down);
-        }
+          for (int g = 0; g < 2; ++g)
+            count = mfma32_of<BF>(infinite_part<BF>(vreg[d][g], sign), ones_of<BF>(seen >> (8 * g)), count);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (up[e] > 0.f) o[d][e] += INFINITY;
-          if (down[e] > 0.f) o[d][e] -= INFINITY;
+          for (int e = 0; e < 16; ++e)
+            if (count[e] > 0.f) o[d][e] += inf;
         }
+        vreg[d][0] = finite_part<BF>(vreg[d][0]);
+        vreg[d][1] = finite_part<BF>(vreg[d][1]);
       }
     }
 #pragma unroll
@@ -347,8 +336,8 @@ hipError_t launch_rows_w(const WindowArgs& a, const WindowPlan& p, float* ws_ml,
   auto kern = &window_rows_kernel<HS, BS, BF, W>;
   const hipError_t e = allow_lds(reinterpret_cast<const void*>(kern), win_rows_smem(HS, kWinRowsTile, W), done);
   if (e != hipSuccess) return e;
-  const int total = a.num_seqs * a.num_kv_heads * p.tiles * p.splits, padded = (total + 7) / 8 * 8;
-  kern<<<(unsigned)padded, W * 64, smem, stream>>>(a, p.tiles, p.splits, padded, cols, ws_ml, ws_out);
+  kern<<<win_grid(a.num_seqs * a.num_kv_heads, p.tiles * p.splits), W * 64, smem, stream>>>(a, p.tiles, p.splits, cols, ws_ml,
+                                                                                         ws_out);
   return hipGetLastError();
 }
 

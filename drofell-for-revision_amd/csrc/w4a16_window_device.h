@@ -47,10 +47,15 @@ __device__ __forceinline__ float unpack(uint32_t u, int hi) {
   if constexpr (BF) return __builtin_bit_cast(float, hi ? u & 0xFFFF0000u : u << 16);
   else return (float)as_h2(u)[hi];
 }
+// sum + both halves of a packed pair (v_dot2 with ones: exact products, fp32 sum)
 template <bool BF>
-__device__ __forceinline__ float value_of(uint16_t b) {
-  if constexpr (BF) return bf16_f32(b);
-  else return (float)as_h(b);
+__device__ __forceinline__ float add_pair(uint32_t u, float sum) {
+  if constexpr (BF) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, u), __builtin_bit_cast(bf2, kOnesBf16), sum, false);
+  } else {
+    return __builtin_amdgcn_fdot2(as_h2(u), h2{(_Float16)1.f, (_Float16)1.f}, sum, false);
+  }
 }
 
 // Which tokens a tile of rows at positions first..last sees, in steps of BK
@@ -95,10 +100,20 @@ __device__ __forceinline__ void zero_outside(uint16_t* x, int64_t stride, int wi
   }
 }
 
-// Workgroups go round-robin to the eight XCDs, each with an L2 of its own:
-// neighbours in `order` (row tiles of one kv head, which read the same keys
-// and values) get the same XCD.
-__device__ __forceinline__ int xcd_order(int b, int padded) { return (b & 7) * (padded >> 3) + (b >> 3); }
+// Workgroup b's (sequence, kv head) pair and its item of `items` (row tiles,
+// longest spans first, x splits), false where there is none.  Workgroups go
+// round-robin to the eight XCDs, each with an L2 of its own: kWinUnit
+// neighbouring items, which read the same keys and values, go to one XCD, and
+// the units of all pairs in turn over the XCDs, so that long and short
+// sequences spread evenly.  (Pairs in one run per XCD: four prompts of 3500 to
+// 12000 tokens took 1.4 times as long, the longest one's XCDs being last.)
+__device__ __forceinline__ bool work_of(int b, int pairs, int items, int& pair, int& item) {
+  const int unit = min(items, kWinUnit), slot = b >> 3;
+  const int u = (b & 7) + 8 * (slot / unit);
+  pair = u % pairs;
+  item = u / pairs * unit + slot % unit;
+  return item < items;
+}
 
 // Non-finite elements of a 16-byte operand (eight 16-bit values).
 template <bool BF>
@@ -114,34 +129,43 @@ __device__ __forceinline__ bool any_nonfinite(h8 x) {
   return bad;
 }
 
-// x without its non-finite elements; pos (neg): 1 where x is +inf (-inf) or NaN.
+// x without its non-finite elements.
 template <bool BF>
-__device__ __forceinline__ void split_nonfinite(h8& x, h8& pos, h8& neg) {
-  constexpr uint32_t kExp = BF ? 0x7F80u : 0x7C00u, kOne = BF ? 0x3F80u : 0x3C00u;
-  u4 v = __builtin_bit_cast(u4, x), p, n;
+__device__ __forceinline__ h8 finite_part(h8 x) {
+  constexpr uint32_t kExp = BF ? 0x7F80u : 0x7C00u;
+  u4 v = __builtin_bit_cast(u4, x);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    uint32_t vo = 0, po = 0, no = 0;
-#pragma unroll
-    for (int h = 0; h < 32; h += 16) {
-      const uint32_t b = (v[e] >> h) & 0xFFFFu;
-      const bool bad = (b & kExp) == kExp;
-      vo |= (bad ? 0u : b) << h;
-      po |= (bad && b != (0x8000u | kExp) ? kOne : 0u) << h;
-      no |= (bad && b != kExp ? kOne : 0u) << h;
-    }
-    v[e] = vo;
-    p[e] = po;
-    n[e] = no;
+    const uint32_t lo = (v[e] & kExp) == kExp ? 0u : v[e] & 0xFFFFu;
+    const uint32_t hi = (v[e] & (kExp << 16)) == kExp << 16 ? 0u : v[e] & 0xFFFF0000u;
+    v[e] = lo | hi;
   }
-  x = __builtin_bit_cast(h8, v);
-  pos = __builtin_bit_cast(h8, p);
-  neg = __builtin_bit_cast(h8, n);
+  return __builtin_bit_cast(h8, v);
+}
+// 1 where x is NaN or the infinity of this sign bit, else 0.
+template <bool BF>
+__device__ __forceinline__ h8 infinite_part(h8 x, uint32_t sign) {
+  constexpr uint32_t kExp = BF ? 0x7F80u : 0x7C00u, kOne = BF ? 0x3F80u : 0x3C00u;
+  u4 v = __builtin_bit_cast(u4, x);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t lo = v[e] & 0xFFFFu, hi = v[e] >> 16, other = kExp | (sign ^ 0x8000u);
+    v[e] = ((lo & kExp) == kExp && lo != other ? kOne : 0u) | ((hi & kExp) == kExp && hi != other ? kOne << 16 : 0u);
+  }
+  return __builtin_bit_cast(h8, v);
+}
+// Eight ones and zeros as an operand, from the bits of a mask.
+template <bool BF>
+__device__ __forceinline__ h8 ones_of(uint32_t bits) {
+  constexpr uint32_t kOne = BF ? 0x3F80u : 0x3C00u;
+  u4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (bits >> (2 * e) & 1 ? kOne : 0u) | (bits >> (2 * e + 1) & 1 ? kOne << 16 : 0u);
+  return __builtin_bit_cast(h8, v);
 }
 
-// The lane's eight scores of reduction step s: bit e set where token
-// t0 + 16 s + 8 (lane / 32) + e is visible from a row: not after `last` (and
-// within the cache), after `before`, or a sink.
+// Whether a row sees token j: not after `last` (the row's position, and within
+// the cache), and after `before` or a sink.
 __device__ __forceinline__ bool sees(int j, int last, int before, int sinks) {
   return j <= last && (j > before || j < sinks);
 }
@@ -162,6 +186,28 @@ __device__ __forceinline__ void copy4(const void* g, uint32_t lds) {
 // Every copy of this workgroup has landed and every wave has left the stage before.
 __device__ __forceinline__ void wait_copies() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Every load of this wave has landed, to the compiler's knowledge too (a load
+// into registers used in a loop would make it wait in every round of it).
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }
+
+// N operands, each loaded (from LDS) AHEAD uses before its use.  The loads and
+// the matrix instructions keep this order; vector-ALU work may move among them.
+template <int N, int AHEAD, typename Load, typename Use>
+__device__ __forceinline__ void feed(Load&& load, Use&& use) {
+  constexpr int kMoves = 0x2 | 0x4 | 0x400;  // vector ALU, scalar ALU, transcendental
+  h8 f[N];
+#pragma unroll
+  for (int i = 0; i < (AHEAD < N ? AHEAD : N); ++i) f[i] = load(i);
+  __builtin_amdgcn_sched_barrier(kMoves);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i + AHEAD < N) f[i + AHEAD] = load(i + AHEAD);
+    __builtin_amdgcn_sched_barrier(kMoves);
+    use(i, f[i]);
+    __builtin_amdgcn_sched_barrier(kMoves);
+  }
 }
 
 // Row-major tiles in LDS ([row][HS], as the tensors have them): 16-byte unit u

@@ -61,17 +61,16 @@ __device__ __forceinline__ void dot8(u4 x, u4 y, float& sum, float& most) {
 
 template <int HS, bool BF>
 __global__ void __launch_bounds__(256, HS <= 128 ? 2 : 1)
-window_dq_kernel(WindowGradArgs g, int tiles, int padded, float* __restrict__ delta, float* __restrict__ most) {
+window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* __restrict__ most) {
   constexpr int KD = HS / 16, ND = (HS + 31) / 32;
   constexpr bool VTAIL = HS % 32 != 0;
   constexpr int TILE = kBk * HS * 2, STAGE = 2 * TILE;  // keys, values
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const WindowArgs& a = g.f;
-  zero_outside(g.dq, g.dq_stride, a.num_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, padded);
-  const int id = xcd_order(blockIdx.x, padded);
-  if (id >= a.num_seqs * a.num_kv_heads * tiles) return;
-  const int tile = tiles - 1 - id % tiles;
-  const int pair = id / tiles;
+  zero_outside(g.dq, g.dq_stride, a.num_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, gridDim.x);
+  int pair, tile;
+  if (!work_of(blockIdx.x, a.num_seqs * a.num_kv_heads, tiles, pair, tile)) return;
+  tile = tiles - 1 - tile;
   const int seq = pair / a.num_kv_heads, kvh = pair % a.num_kv_heads;
   const int G = a.num_heads / a.num_kv_heads;
   int q0, q1;
@@ -134,6 +133,7 @@ window_dq_kernel(WindowGradArgs g, int tiles, int padded, float* __restrict__ de
     if (threadIdx.x == 0) most[(size_t)pair * tiles + tile] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   }
 
+  wait_loads();
   f16v dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = f16v{};
@@ -148,10 +148,12 @@ window_dq_kernel(WindowGradArgs g, int tiles, int padded, float* __restrict__ de
       if (tb > wlast || (a.window != 0 && tb + 31 <= wfirst - a.window && tb >= a.sinks)) continue;
       const bool full = tb + 31 <= wfirst && (a.window == 0 || tb > wlast - a.window || tb + 31 < a.sinks);
       f16v s = {}, p = {};
-#pragma unroll
-      for (int j = 0; j < KD; ++j) s = mfma32_of<BF>(row_unit<HS>(st, 32 * b + row_token(c), 2 * j + half), qreg[j], s);
-#pragma unroll
-      for (int j = 0; j < KD; ++j) p = mfma32_of<BF>(row_unit<HS>(st + TILE, 32 * b + row_token(c), 2 * j + half), oreg[j], p);
+      feed<2 * KD, 8>(
+          [&](int i) { return row_unit<HS>(st + (i & 1) * TILE, 32 * b + row_token(c), (i & ~1) + half); },
+          [&](int i, h8 f) {
+            if (i & 1) p = mfma32_of<BF>(f, oreg[i >> 1], p);
+            else s = mfma32_of<BF>(f, qreg[i >> 1], s);
+          });
       float ds[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * ((p[e] - dl) * gs);
@@ -160,13 +162,13 @@ window_dq_kernel(WindowGradArgs g, int tiles, int padded, float* __restrict__ de
         for (int e = 0; e < 16; ++e)
           ds[e] = sees(tb + 16 * (e >> 3) + 8 * half + (e & 7), pos, before, a.sinks) ? ds[e] : 0.f;
       }
+      h8 w[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const h8 w = __builtin_bit_cast(h8, u4{pack2<BF>(ds[8 * x], ds[8 * x + 1]), pack2<BF>(ds[8 * x + 2], ds[8 * x + 3]),
-                                               pack2<BF>(ds[8 * x + 4], ds[8 * x + 5]), pack2<BF>(ds[8 * x + 6], ds[8 * x + 7])});
-#pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] = mfma32_of<BF>(column_unit<HS>(st, 32 * b + 16 * x, d), w, dq[d]);
-      }
+      for (int x = 0; x < 2; ++x)
+        w[x] = __builtin_bit_cast(h8, u4{pack2<BF>(ds[8 * x], ds[8 * x + 1]), pack2<BF>(ds[8 * x + 2], ds[8 * x + 3]),
+                                         pack2<BF>(ds[8 * x + 4], ds[8 * x + 5]), pack2<BF>(ds[8 * x + 6], ds[8 * x + 7])});
+      feed<2 * ND, 6>([&](int i) { return column_unit<HS>(st, 32 * b + 16 * (i / ND), i % ND); },
+                      [&](int i, h8 f) { dq[i % ND] = mfma32_of<BF>(f, w[i / ND], dq[i % ND]); });
     }
   }
   if (c >= nrows) return;
@@ -185,7 +187,7 @@ window_dq_kernel(WindowGradArgs g, int tiles, int padded, float* __restrict__ de
 
 template <int HS, bool BF>
 __global__ void __launch_bounds__(256, 1)
-window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, int padded, uint32_t magic,
+window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, uint32_t magic,
                   const float* __restrict__ delta, const float* __restrict__ most) {
   constexpr int KD = HS / 16, ND = (HS + 31) / 32;
   constexpr bool VTAIL = HS % 32 != 0;
@@ -193,12 +195,10 @@ window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, int padded, uint32
   constexpr int STAGE = 2 * TILE + 3 * kBk * 4;  // rows of Q and of dO, log-sums, deltas, positions
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const WindowArgs& a = g.f;
-  zero_outside(g.dk, g.dk_stride, a.num_kv_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, padded);
-  zero_outside(g.dv, g.dv_stride, a.num_kv_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, padded);
-  const int id = xcd_order(blockIdx.x, padded);
-  if (id >= a.num_seqs * a.num_kv_heads * tiles) return;
-  const int tile = id % tiles;  // the longest row ranges first
-  const int pair = id / tiles;
+  zero_outside(g.dk, g.dk_stride, a.num_kv_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, gridDim.x);
+  zero_outside(g.dv, g.dv_stride, a.num_kv_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, gridDim.x);
+  int pair, tile;
+  if (!work_of(blockIdx.x, a.num_seqs * a.num_kv_heads, tiles, pair, tile)) return;
   const int seq = pair / a.num_kv_heads, kvh = pair % a.num_kv_heads;
   const int G = a.num_heads / a.num_kv_heads;
   int q0, q1;
@@ -258,6 +258,7 @@ window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, int padded, uint32
   }
   const float ps = p_shift<BF>(), gp = gs * __builtin_amdgcn_exp2f(-ps);
 
+  wait_loads();
   f16v dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f16v{};
@@ -275,10 +276,12 @@ window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, int padded, uint32
       if (ib < wa || (a.window != 0 && ia - a.window >= wb && wa >= a.sinks)) continue;
       const bool full = ra + 31 < r1 && ia >= wb && (a.window == 0 || ib < wa + a.window || wb < a.sinks);
       f16v s = {}, p = {};
-#pragma unroll
-      for (int j = 0; j < KD; ++j) s = mfma32_of<BF>(row_unit<HS>(st, 32 * b + row_token(c), 2 * j + half), kreg[j], s);
-#pragma unroll
-      for (int j = 0; j < KD; ++j) p = mfma32_of<BF>(row_unit<HS>(st + TILE, 32 * b + row_token(c), 2 * j + half), vreg[j], p);
+      feed<2 * KD, 8>(
+          [&](int i) { return row_unit<HS>(st + (i & 1) * TILE, 32 * b + row_token(c), (i & ~1) + half); },
+          [&](int i, h8 f) {
+            if (i & 1) p = mfma32_of<BF>(f, vreg[i >> 1], p);
+            else s = mfma32_of<BF>(f, kreg[i >> 1], s);
+          });
       h8 pw[2], dw[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -301,13 +304,13 @@ window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, int padded, uint32
         pw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(pr[0], pr[1]), pack2<BF>(pr[2], pr[3]), pack2<BF>(pr[4], pr[5]), pack2<BF>(pr[6], pr[7])});
         dw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(ds[0], ds[1]), pack2<BF>(ds[2], ds[3]), pack2<BF>(ds[4], ds[5]), pack2<BF>(ds[6], ds[7])});
       }
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          dv[d] = mfma32_of<BF>(column_unit<HS>(st + TILE, 32 * b + 16 * x, d), pw[x], dv[d]);
-          dk[d] = mfma32_of<BF>(column_unit<HS>(st, 32 * b + 16 * x, d), dw[x], dk[d]);
-        }
+      feed<4 * ND, 6>(  // of each 16 rows and 32 dims: dO, then Q
+          [&](int i) { return column_unit<HS>(st + (1 - (i & 1)) * TILE, 32 * b + 16 * (i / (2 * ND)), i / 2 % ND); },
+          [&](int i, h8 f) {
+            const int x = i / (2 * ND), d = i / 2 % ND;
+            if (i & 1) dk[d] = mfma32_of<BF>(f, dw[x], dk[d]);
+            else dv[d] = mfma32_of<BF>(f, pw[x], dv[d]);
+          });
     }
   }
   if (wa + c >= n) return;
@@ -342,12 +345,11 @@ hipError_t launch_grad_hs(const WindowGradArgs& g, float* ws, hipStream_t stream
   const int tiles = (a.max_query + kGradTile - 1) / kGradTile;
   float* delta = ws;
   float* most = ws + (size_t)a.total_rows * a.num_heads;
-  const int pq = (pairs * row_tiles + 7) / 8 * 8, pk = (pairs * tiles + 7) / 8 * 8;
-  dq<<<(unsigned)pq, 256, smem, stream>>>(g, row_tiles, pq, delta, most);
+  dq<<<win_grid(pairs, row_tiles), 256, smem, stream>>>(g, row_tiles, delta, most);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   const uint32_t magic = G == 1 ? 0u : (uint32_t)((0x100000000ull + G - 1) / G);
-  dkv<<<(unsigned)pk, 256, smem_kv, stream>>>(g, tiles, row_tiles, pk, magic, delta, most);
+  dkv<<<win_grid(pairs, tiles), 256, smem_kv, stream>>>(g, tiles, row_tiles, magic, delta, most);
   return hipGetLastError();
 }
 

@@ -17,7 +17,7 @@
 // Matrix-core and vector-ALU bound.  Probabilities enter p . v rounded to the
 // value type (fp16: of 2^10 p), as the matrix cores take it: their errors are
 // independent of each other, and add to the output's own rounding about as much
-// again; the sum of the denominator is of the unrounded ones.
+// again; the denominator sums the rounded ones, so that the weights add up to 1.
 
 #include <hip/hip_runtime.h>
 
@@ -38,7 +38,7 @@ constexpr int kBk = kWinTileTokens;
 // BS: block size of the cache, 0 for token rows.
 template <int HS, int BS, bool BF>
 __global__ void __launch_bounds__(256, HS <= 128 ? 2 : 1)
-window_tile_kernel(WindowArgs a, int tiles, int splits, int padded, float* __restrict__ ws_ml,
+window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_ml,
                    float* __restrict__ ws_out) {
   constexpr int KD = HS / 16;
   constexpr int ND = (HS + 31) / 32;
@@ -50,12 +50,11 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, int padded, float* __res
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
 
   if constexpr (BS == 0)
-    zero_outside(a.out, a.o_stride, a.num_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, padded);
-  const int id = xcd_order(blockIdx.x, padded);
-  if (id >= a.num_seqs * a.num_kv_heads * tiles * splits) return;
-  const int split = id % splits;
-  const int tile = tiles - 1 - id / splits % tiles;  // the longest spans first
-  const int pair = id / (splits * tiles);
+    zero_outside(a.out, a.o_stride, a.num_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, gridDim.x);
+  int pair, item;
+  if (!work_of(blockIdx.x, a.num_seqs * a.num_kv_heads, tiles * splits, pair, item)) return;
+  const int split = item % splits;
+  const int tile = tiles - 1 - item / splits;
   const int seq = pair / a.num_kv_heads, kvh = pair % a.num_kv_heads;
   const int G = a.num_heads / a.num_kv_heads;
   int q0, q1;
@@ -163,51 +162,43 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, int padded, float* __res
 #pragma unroll
     for (int j = 0; j < KD; ++j) qreg[j] = *(const h8*)(qp + 16 * j);
   }
-  float m = kNoMax, l = 0.f;  // of the row (l: this lane's tokens)
+  wait_loads();
+  float m = kNoMax, l[2] = {0.f, 0.f};  // of the row (l: this lane's tokens, in two parts)
   f16v o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f16v{};
 
-  for (int step = s0; step < s1; ++step) {
-    const int stage = (step - s0) & 1;
-    wait_copies();
-    if (step + 1 < s1) issue(step + 1, stage ^ 1);
-    const int t = span.token<kBk>(step);
-    // does the wave see any of it, and all its rows all of it?
-    if (nrows <= 0 || t > wlast || (a.window != 0 && t + kBk - 1 <= wfirst - a.window && t >= a.sinks)) continue;
-    const bool full = held[stage] == (1u << NB) - 1 && t + kBk - 1 <= min(wfirst, cap - 1) &&
-                      (a.window == 0 || t > wlast - a.window || t + kBk - 1 < a.sinks);
-    const unsigned char* st = lds + stage * STAGE;
-    f16v s[2] = {f16v{}, f16v{}};
-#pragma unroll
-    for (int j = 0; j < KD; ++j)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) s[b] = mfma32_of<BF>(key(st, b, j), qreg[j], s[b]);
-    auto visible = [&](int b, int e) {  // of score e of the 32 tokens b
-      const int in = 32 * b + 16 * (e >> 3) + 8 * half + (e & 7);
-      const bool there = BS == 0 || ((held[stage] >> (BS == 32 ? b : 2 * b + (e >> 3))) & 1);
-      return there && sees(t + in, last, before, a.sinks);
-    };
-    if (!full) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[b][e] = visible(b, e) ? s[b][e] : -INFINITY;
+  // the steps of which every row of the workgroup sees every token
+  int f0 = s1, f1 = s0;
+  {
+    const int first = p0 + base / G, last_row = p0 + (min(base + 128, rows) - 1) / G;
+    const int most = min(first, cap - 1) - (kBk - 1) - span.lo;  // of token(step) - lo
+    const int least = a.window == 0 ? 0 : last_row - a.window + 1 - span.lo;
+    if (most >= 0) {
+      f0 = span.sink_steps + (max(least, 0) + kBk - 1) / kBk;
+      f1 = span.sink_steps + most / kBk + 1;
     }
+  }
+  auto scores = [&](const unsigned char* st, f16v (&s)[2]) {
+    feed<2 * KD, 8>([&](int i) { return key(st, i & 1, i >> 1); },
+                    [&](int i, h8 f) { s[i & 1] = mfma32_of<BF>(f, qreg[i >> 1], s[i & 1]); });
+  };
+  // the running maximum (it may lag kLag behind), and the probabilities
+  auto probabilities = [&](f16v (&s)[2], h8 (&p)[2][2]) {
     float mx = s[0][0];
 #pragma unroll
     for (int e = 1; e < 32; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
     mx = both_max(mx) * a.scale_log2;
-    if (__any(mx > m + kLag)) {  // the maximum may lag kLag behind
+    if (__any(mx > m + kLag)) {
       const float mn = fmaxf(m, mx);
       const float f = __builtin_amdgcn_exp2f(m - mn);
-      l *= f;
+      l[0] *= f;
+      l[1] *= f;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] *= f;
       m = mn;
     }
     const float shift = p_shift<BF>() - m;
-    h8 p[2][2];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -217,69 +208,97 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, int padded, float* __res
         for (int e = 0; e < 4; ++e) {
           const float y = __builtin_amdgcn_exp2f(fmaf(s[b][8 * g + 2 * e], a.scale_log2, shift));
           const float z = __builtin_amdgcn_exp2f(fmaf(s[b][8 * g + 2 * e + 1], a.scale_log2, shift));
-          l += y;
-          l += z;
           x[e] = pack2<BF>(y, z);
+          l[e & 1] = add_pair<BF>(x[e], l[e & 1]);
         }
         p[b][g] = __builtin_bit_cast(h8, x);
       }
-    if (full) {
+  };
+  auto whole = [&](int stage) {  // a step that every row sees
+    const unsigned char* st = lds + stage * STAGE;
+    f16v s[2] = {f16v{}, f16v{}};
+    h8 p[2][2];
+    scores(st, s);
+    probabilities(s, p);
+    feed<4 * ND, 8>(
+        [&](int i) { return value(st, i / (2 * ND), i % ND, i / ND % 2); },
+        [&](int i, h8 f) { o[i % ND] = mfma32_of<BF>(f, p[i / (2 * ND)][i / ND % 2], o[i % ND]); });
+  };
+  auto masked = [&](int step, int stage) {
+    const int t = span.token<kBk>(step);
+    if (nrows <= 0 || t > wlast || (a.window != 0 && t + kBk - 1 <= wfirst - a.window && t >= a.sinks)) return;
+    const unsigned char* st = lds + stage * STAGE;
+    uint32_t seen = 0;  // bit 16 b + e: score e of the 32 tokens b
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+    for (int x = 0; x < 32; ++x) {
+      const bool there = BS == 0 || ((held[stage] >> (BS == 32 ? x >> 4 : x >> 3)) & 1);
+      seen |= (uint32_t)(there && sees(t + 16 * (x >> 3) + 8 * half + (x & 7), last, before, a.sinks)) << x;
+    }
+    f16v s[2] = {f16v{}, f16v{}};
+    h8 p[2][2];
+    scores(st, s);
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+    for (int x = 0; x < 32; ++x) s[x >> 4][x & 15] = seen >> x & 1 ? s[x >> 4][x & 15] : -INFINITY;
+    probabilities(s, p);
+    // a value that some rows do not see (or that no row does) must not reach
+    // them as 0 * inf: where there is one, its part is added apart
+    bool odd = false;
 #pragma unroll
-          for (int d = 0; d < ND; ++d) o[d] = mfma32_of<BF>(value(st, b, d, g), p[b][g], o[d]);
-    } else {
-      // a value that some rows do not see (or that no row does) must not reach
-      // them as 0 * inf: where there is one, its part is added apart
+    for (int x = 0; x < 4; ++x)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        h8 v[2][2];
-        bool odd = false;
+      for (int d = 0; d < ND; ++d) odd |= any_nonfinite<BF>(value(st, x >> 1, d, x & 1));
+    odd = __any(odd);
+    if (odd) {
+      for (uint32_t sign = 0; sign <= 0x8000u; sign += 0x8000u) {
+        const float inf = sign ? -INFINITY : INFINITY;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int d = 0; d < ND; ++d) {
+          f16v count = {};
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            v[b][g] = value(st, b, d, g);
-            odd |= any_nonfinite<BF>(v[b][g]);
-          }
-        if (__any(odd)) {
-          f16v up = {}, down = {};
+          for (int x = 0; x < 4; ++x)
+            count = mfma32_of<BF>(infinite_part<BF>(value(st, x >> 1, d, x & 1), sign), ones_of<BF>(seen >> (8 * x)), count);
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              u4 w;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t one = BF ? 0x3F80u : 0x3C00u;
-                w[e] = (visible(b, 8 * g + 2 * e) ? one : 0u) | (visible(b, 8 * g + 2 * e + 1) ? one << 16 : 0u);
-              }
-              h8 pn, nn;
-              split_nonfinite<BF>(v[b][g], pn, nn);
-              up = mfma32_of<BF>(pn, __builtin_bit_cast(h8, w), up);
-              down = mfma32_of<BF>(nn, __builtin_bit_cast(h8, w), down);
-            }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if (up[e] > 0.f) o[d][e] += INFINITY;
-            if (down[e] > 0.f) o[d][e] -= INFINITY;
-          }
+          for (int e = 0; e < 16; ++e)
+            if (count[e] > 0.f) o[d][e] += inf;
         }
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int g = 0; g < 2; ++g) o[d] = mfma32_of<BF>(v[b][g], p[b][g], o[d]);
       }
     }
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        h8 v = value(st, x >> 1, d, x & 1);
+        if (odd) v = finite_part<BF>(v);
+        o[d] = mfma32_of<BF>(v, p[x >> 1][x & 1], o[d]);
+      }
+  };
+  int stage = 0, step = s0;
+  auto begin = [&]() {
+    wait_copies();
+    if (step + 1 < s1) issue(step + 1, stage ^ 1);
+  };
+  auto is_whole = [&]() { return step >= f0 && step < f1 && held[stage] == (1u << NB) - 1; };
+  while (step < s1) {
+    begin();
+    if (is_whole()) {
+      do {
+        whole(stage);
+        stage ^= 1;
+        if (++step == s1) break;
+        begin();
+      } while (is_whole());
+      if (step == s1) break;
+    }
+    masked(step, stage);
+    stage ^= 1;
+    ++step;
   }
 
-  l = both_sum(l);
+  const float sum = both_sum(l[0] + l[1]);
   if (c >= nrows) return;
   const int token = q0 + row / G, head = kvh * G + row % G;
   if (splits == 1) {
-    const float f = l == 0.f ? 1.f : 1.f / l;  // no visible token: zeros
+    const float f = sum == 0.f ? 1.f : 1.f / sum;  // no visible token: zeros
     uint16_t* op = a.out + (size_t)token * a.o_stride + (size_t)head * HS;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -291,7 +310,7 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, int padded, float* __res
                                            pack2<BF>(o[d][e + 2] * f, o[d][e + 3] * f));
       }
     if (a.lse != nullptr && half == 0)
-      a.lse[(size_t)token * a.num_heads + head] = m + __builtin_amdgcn_logf(l) - p_shift<BF>();
+      a.lse[(size_t)token * a.num_heads + head] = m + __builtin_amdgcn_logf(sum) - p_shift<BF>();
   } else {
     const size_t slot = ((size_t)token * a.num_heads + head) * splits + split;
 #pragma unroll
@@ -304,7 +323,7 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, int padded, float* __res
       }
     if (half == 0) {
       ws_ml[2 * slot] = m;
-      ws_ml[2 * slot + 1] = l;
+      ws_ml[2 * slot + 1] = sum;
     }
   }
 }
@@ -315,9 +334,8 @@ hipError_t launch_tile_bs(const WindowArgs& a, const WindowPlan& p, float* ws, h
   auto kern = &window_tile_kernel<HS, BS, BF>;
   const hipError_t e = allow_lds(reinterpret_cast<const void*>(kern), win_tile_smem(HS), done);
   if (e != hipSuccess) return e;
-  const int total = a.num_seqs * a.num_kv_heads * p.tiles * p.splits, padded = (total + 7) / 8 * 8;
-  kern<<<(unsigned)padded, 256, win_tile_smem(HS), stream>>>(
-      a, p.tiles, p.splits, padded, ws, ws + 2 * (size_t)a.total_rows * a.num_heads * p.splits);
+  kern<<<win_grid(a.num_seqs * a.num_kv_heads, p.tiles * p.splits), 256, win_tile_smem(HS), stream>>>(
+      a, p.tiles, p.splits, ws, ws + 2 * (size_t)a.total_rows * a.num_heads * p.splits);
   return hipGetLastError();
 }
 

@@ -8,6 +8,7 @@
 #include <cstdint>
 
 #include "drofell_w4a16.h"
+#include "w4a16_blocks.h"
 #include "w4a16_internal.h"
 #include "w4a16_window.h"
 
@@ -198,6 +199,128 @@ int dw4_window_attention_dense_backward(int dtype, int num_seqs, int num_heads, 
   g.scale = scale;
   auto launch = g.f.bf16 ? &dw4::launch_window_grad<true> : &dw4::launch_window_grad<false>;
   return status_of(launch(g, static_cast<float*>(workspace), static_cast<hipStream_t>(stream)));
+}
+
+// ---- the block pool
+
+int dw4_blocks_workspace_size(int num_rows, int num_blocks, size_t* workspace_bytes) {
+  if (num_rows < 0 || num_blocks < 0 || workspace_bytes == nullptr) return DW4_ERR_INVALID_ARG;
+  *workspace_bytes = sizeof(int32_t) * dw4::pool_ws_ints(num_rows, num_blocks);
+  return DW4_OK;
+}
+
+static int pool_layers(dw4::PoolArgs& a, int num_layers, const int64_t* kp, const int64_t* vp, int num_blocks,
+                       int64_t part_bytes) {
+  if (num_layers < 0 || num_blocks < 0 || part_bytes < 0) return DW4_ERR_INVALID_ARG;
+  if (num_layers > 0 && (!kp || !vp || part_bytes == 0)) return DW4_ERR_INVALID_ARG;
+  if (part_bytes % 16 != 0) return DW4_ERR_MISALIGNED;
+  a.layers = num_layers;
+  a.key_tables = kp;
+  a.value_tables = vp;
+  a.num_blocks = num_blocks;
+  a.part_bytes = part_bytes;
+  return DW4_OK;
+}
+
+static int pool_state(dw4::PoolArgs& a, int num_rows, int max_blocks, int num_blocks, const int32_t* tables,
+                      const int32_t* lens, const int32_t* refs, int32_t* tables_out, int32_t* lens_out, int32_t* refs_out,
+                      int32_t* shortage) {
+  if (num_rows < 0 || max_blocks < 0 || num_blocks < 0 || !shortage) return DW4_ERR_INVALID_ARG;
+  if (num_rows > 0 && (!lens || !lens_out || lens == lens_out)) return DW4_ERR_INVALID_ARG;
+  if (num_rows > 0 && max_blocks > 0 && (!tables || !tables_out || tables == tables_out)) return DW4_ERR_INVALID_ARG;
+  if (num_blocks > 0 && (!refs || !refs_out || refs == refs_out)) return DW4_ERR_INVALID_ARG;
+  if (num_blocks > 1 << 28 || num_rows > 1 << 24) return DW4_ERR_UNSUPPORTED;
+  a.rows = num_rows;
+  a.max_blocks = max_blocks;
+  a.num_blocks = num_blocks;
+  a.tables = tables;
+  a.lens = lens;
+  a.refs = refs;
+  a.tables_out = tables_out;
+  a.lens_out = lens_out;
+  a.refs_out = refs_out;
+  a.shortage = shortage;
+  return DW4_OK;
+}
+
+static int pool_workspace(dw4::PoolArgs& a, void* workspace, size_t workspace_bytes) {
+  if (workspace == nullptr || workspace_bytes < sizeof(int32_t) * dw4::pool_ws_ints(a.rows, a.num_blocks))
+    return DW4_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return DW4_ERR_MISALIGNED;
+  a.ws = static_cast<int32_t*>(workspace);
+  return DW4_OK;
+}
+
+static bool good_block(int block_size) { return block_size == 16 || block_size == 32; }
+
+int dw4_copy_blocks(int num_layers, const int64_t* layer_key_ptrs, const int64_t* layer_value_ptrs, int num_blocks,
+                    int64_t part_bytes, int count, const int32_t* pairs, void* stream) {
+  dw4::PoolArgs a = {};
+  const int st = pool_layers(a, num_layers, layer_key_ptrs, layer_value_ptrs, num_blocks, part_bytes);
+  if (st != DW4_OK) return st;
+  if (count < 0 || (count > 0 && !pairs)) return DW4_ERR_INVALID_ARG;
+  if (count == 0 || num_layers == 0) return DW4_OK;
+  return status_of(dw4::launch_copy_blocks(a, count, pairs, dw4::cu_count(), static_cast<hipStream_t>(stream)));
+}
+
+int dw4_extend_blocks(int num_rows, int max_blocks, int num_blocks, int block_size, const int32_t* tables,
+                      const int32_t* lens, const int32_t* refs, const int32_t* add, int32_t* tables_out, int32_t* lens_out,
+                      int32_t* refs_out, int32_t* shortage, void* workspace, size_t workspace_bytes, void* stream) {
+  dw4::PoolArgs a = {};
+  int st = pool_state(a, num_rows, max_blocks, num_blocks, tables, lens, refs, tables_out, lens_out, refs_out, shortage);
+  if (st != DW4_OK) return st;
+  if (!good_block(block_size)) return DW4_ERR_UNSUPPORTED;
+  if (num_rows > 0 && !add) return DW4_ERR_INVALID_ARG;
+  if ((st = pool_workspace(a, workspace, workspace_bytes)) != DW4_OK) return st;
+  a.block_size = block_size;
+  a.by_row = add;
+  return status_of(dw4::launch_extend_blocks(a, static_cast<hipStream_t>(stream)));
+}
+
+int dw4_fork_blocks(int num_layers, const int64_t* layer_key_ptrs, const int64_t* layer_value_ptrs, int64_t part_bytes,
+                    int num_rows, int max_blocks, int num_blocks, int block_size, const int32_t* tables,
+                    const int32_t* lens, const int32_t* refs, const int32_t* parents, int32_t* tables_out,
+                    int32_t* lens_out, int32_t* refs_out, int32_t* shortage, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  dw4::PoolArgs a = {};
+  int st = pool_state(a, num_rows, max_blocks, num_blocks, tables, lens, refs, tables_out, lens_out, refs_out, shortage);
+  if (st == DW4_OK) st = pool_layers(a, num_layers, layer_key_ptrs, layer_value_ptrs, num_blocks, part_bytes);
+  if (st != DW4_OK) return st;
+  if (!good_block(block_size) || num_rows > dw4::kPoolMaxRows) return DW4_ERR_UNSUPPORTED;
+  if (num_rows > 0 && !parents) return DW4_ERR_INVALID_ARG;
+  if ((st = pool_workspace(a, workspace, workspace_bytes)) != DW4_OK) return st;
+  a.block_size = block_size;
+  a.by_row = parents;
+  return status_of(dw4::launch_fork_blocks(a, dw4::cu_count(), static_cast<hipStream_t>(stream)));
+}
+
+int dw4_free_blocks(int num_rows, int max_blocks, int num_blocks, int block_size, const int32_t* tables,
+                    const int32_t* lens, const int32_t* refs, const uint8_t* finished, int window, int sinks,
+                    int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, int32_t* shortage, void* stream) {
+  dw4::PoolArgs a = {};
+  const int st = pool_state(a, num_rows, max_blocks, num_blocks, tables, lens, refs, tables_out, lens_out, refs_out, shortage);
+  if (st != DW4_OK) return st;
+  if (!good_block(block_size)) return DW4_ERR_UNSUPPORTED;
+  if (window < 0 || sinks < 0) return DW4_ERR_INVALID_ARG;
+  a.block_size = block_size;
+  a.finished = finished;
+  a.window = window;
+  a.sinks = sinks;
+  return status_of(dw4::launch_free_blocks(a, static_cast<hipStream_t>(stream)));
+}
+
+int dw4_compact_blocks(int num_layers, const int64_t* layer_key_ptrs, const int64_t* layer_value_ptrs, int64_t part_bytes,
+                       int num_rows, int max_blocks, int num_blocks, const int32_t* tables, const int32_t* lens,
+                       const int32_t* refs, int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, int32_t* shortage,
+                       int32_t* live, void* workspace, size_t workspace_bytes, void* stream) {
+  dw4::PoolArgs a = {};
+  int st = pool_state(a, num_rows, max_blocks, num_blocks, tables, lens, refs, tables_out, lens_out, refs_out, shortage);
+  if (st == DW4_OK) st = pool_layers(a, num_layers, layer_key_ptrs, layer_value_ptrs, num_blocks, part_bytes);
+  if (st != DW4_OK) return st;
+  if (!live) return DW4_ERR_INVALID_ARG;
+  if ((st = pool_workspace(a, workspace, workspace_bytes)) != DW4_OK) return st;
+  a.live = live;
+  return status_of(dw4::launch_compact_blocks(a, dw4::cu_count(), static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -139,6 +139,14 @@ SIGNATURES = {
                                             + [_P, _c.c_int, _c.c_int, _c.c_float, _c.c_int,
                                                _c.c_int, _P, _c.c_size_t, _P]),
     "dw4_window_attention_dense_backward_workspace_size": (_c.c_int, [_c.c_int] * 5 + [_SZ]),
+    "dw4_blocks_workspace_size": (_c.c_int, [_c.c_int, _c.c_int, _SZ]),
+    "dw4_copy_blocks": (_c.c_int, [_c.c_int, _P, _P, _c.c_int, _c.c_int64, _c.c_int, _P, _P]),
+    "dw4_extend_blocks": (_c.c_int, [_c.c_int] * 4 + [_P] * 9 + [_c.c_size_t, _P]),
+    "dw4_fork_blocks": (_c.c_int, [_c.c_int, _P, _P, _c.c_int64] + [_c.c_int] * 4 + [_P] * 9
+                        + [_c.c_size_t, _P]),
+    "dw4_free_blocks": (_c.c_int, [_c.c_int] * 4 + [_P] * 4 + [_c.c_int, _c.c_int] + [_P] * 5),
+    "dw4_compact_blocks": (_c.c_int, [_c.c_int, _P, _P, _c.c_int64] + [_c.c_int] * 3 + [_P] * 9
+                           + [_c.c_size_t, _P]),
     "dw4_gemm_group": (_c.c_int, [_c.c_int, _IP, _c.c_int, _P, _c.c_int64, _P, _c.c_size_t, _P]),
     "dw4_gemm_silu_mul": (_c.c_int, [_c.c_int, _P, _c.c_int64, _IP, _IP, _P, _c.c_int64,
                                      _P, _c.c_size_t, _P]),
@@ -313,4 +321,12 @@ def window_attention_backward_workspace_size(num_seqs: int, num_heads: int, num_
     fn = "dw4_window_attention_dense_backward_workspace_size"
     check(fn, getattr(load(), fn)(num_seqs, num_heads, num_kv_heads, total_rows, max_seq_len,
                                   ctypes.byref(out)))
+    return out.value
+
+
+@functools.lru_cache(maxsize=4096)
+def blocks_workspace_size(num_rows: int, num_blocks: int) -> int:
+    out = ctypes.c_size_t(0)
+    check("dw4_blocks_workspace_size",
+          load().dw4_blocks_workspace_size(num_rows, num_blocks, ctypes.byref(out)))
     return out.value

@@ -549,6 +549,70 @@ int dw4_window_attention_dense_backward_workspace_size(int num_seqs, int num_hea
                                                        int total_rows, int max_seq_len,
                                                        size_t* workspace_bytes);
 
+/* ---------------------------------------------------------------------------
+ * Cache-block pool: the blocks of a paged cache given to rows, shared, copied,
+ * given back and moved together on the device.  No counterpart in the reference
+ * (its block tables live on the host).  State, all int32 device memory: tables
+ * [num_rows][max_blocks] of block numbers (-1, or any number outside 0 ..
+ * num_blocks - 1: none), lens [num_rows] (tokens per row) and refs
+ * [num_blocks] (table entries that hold a block; 0: free).  A call reads one
+ * state and writes another (*_out; no array may be both).  Blocks are handed
+ * out from the lowest free number up, in the order of rows.  shortage (int32
+ * [1]): how many blocks were missing; unless it is 0 the state written is the
+ * state read and nothing is copied.  Contents move in every layer of the
+ * pool: layer_key_ptrs / layer_value_ptrs (int64 device [num_layers]) hold the
+ * addresses of the layers' pointer tables (key_block_ptrs / value_block_ptrs
+ * above), part_bytes is the size of a block's key part (and of its value part),
+ * a multiple of 16, blocks 16-byte aligned.  num_layers 0: tables and counts
+ * alone.  workspace: dw4_blocks_workspace_size bytes.  Never synchronises.
+ * ------------------------------------------------------------------------- */
+int dw4_blocks_workspace_size(int num_rows, int num_blocks, size_t* workspace_bytes);
+
+/* Block pairs[i][0] copied to pairs[i][1] for each of `count` pairs (int32 device).
+ * Pairs with a number outside the pool are skipped; no block may be written
+ * twice, or written and read. */
+int dw4_copy_blocks(int num_layers, const int64_t* layer_key_ptrs, const int64_t* layer_value_ptrs,
+                    int num_blocks, int64_t part_bytes, int count, const int32_t* pairs,
+                    void* stream);
+
+/* lens_out = lens + max(add, 0), and the blocks that takes (the entries from
+ * ceil(lens / block_size) on).  A row longer than max_blocks blocks counts as short
+ * of those beyond. */
+int dw4_extend_blocks(int num_rows, int max_blocks, int num_blocks, int block_size,
+                      const int32_t* tables, const int32_t* lens, const int32_t* refs,
+                      const int32_t* add, int32_t* tables_out, int32_t* lens_out, int32_t* refs_out,
+                      int32_t* shortage, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Row r continues row parents[r] (int32 device; outside 0 .. num_rows - 1: it
+ * ends, with no blocks and length 0).  Full blocks are shared.  A half-filled last
+ * block stays with the first row that continues its row, if no other entry
+ * holds it; every other row gets a copy of its own.  Blocks that this leaves free
+ * are not handed out by the same call.  num_rows at most 8192. */
+int dw4_fork_blocks(int num_layers, const int64_t* layer_key_ptrs, const int64_t* layer_value_ptrs,
+                    int64_t part_bytes, int num_rows, int max_blocks, int num_blocks,
+                    int block_size, const int32_t* tables, const int32_t* lens, const int32_t* refs,
+                    const int32_t* parents, int32_t* tables_out, int32_t* lens_out,
+                    int32_t* refs_out, int32_t* shortage, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/* Entries given back: all of the rows with finished[r] != 0 (bytes, device, or
+ * NULL), whose length becomes 0, and with a window > 0 those whose tokens neither the
+ * next token of the row nor any later one sees (dw4_window_attention's rule). */
+int dw4_free_blocks(int num_rows, int max_blocks, int num_blocks, int block_size,
+                    const int32_t* tables, const int32_t* lens, const int32_t* refs,
+                    const uint8_t* finished, int window, int sinks, int32_t* tables_out,
+                    int32_t* lens_out, int32_t* refs_out, int32_t* shortage, void* stream);
+
+/* The live blocks (refs > 0; *live of them, int32 device [1]) moved into the numbers
+ * below *live: the lowest free number takes the lowest block from *live on, and so
+ * forth; tables and refs follow. */
+int dw4_compact_blocks(int num_layers, const int64_t* layer_key_ptrs,
+                       const int64_t* layer_value_ptrs, int64_t part_bytes, int num_rows,
+                       int max_blocks, int num_blocks, const int32_t* tables, const int32_t* lens,
+                       const int32_t* refs, int32_t* tables_out, int32_t* lens_out,
+                       int32_t* refs_out, int32_t* shortage, int32_t* live, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Decode chain: one launch over a list of projections at m <= 4 (no single
  * reference call: it runs the per-projection q4_matmul_cuda_v2 calls,

@@ -588,10 +588,11 @@ def _plain_fork(s):
     fresh = listed_free[(need.cumsum(0) - 1).clamp(min=0)].clamp(max=len(refs) - 1)
     new.scatter_(1, last[:, None], torch.where(need, fresh, page)[:, None].to(torch.int32))
     new_refs = _add_refs(_add_refs(refs, tables, -1), new, 1)
-    dst = torch.where(need & ok, fresh, page.clamp(min=0))
+    copied = (need & ok).nonzero()[:, 0]
+    src, dst = page[copied], fresh[copied]
     for pair in s["pages"]:
         for t in pair:
-            t[dst] = t[page.clamp(min=0)]
+            t[dst] = t[src]
     return (torch.where(ok, new, tables), torch.where(ok, new_lens, lens),
             torch.where(ok, new_refs, refs), short.to(torch.int32).view(1), s["pages"])
 

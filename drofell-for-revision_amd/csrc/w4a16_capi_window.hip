@@ -144,14 +144,17 @@ static int dense_args(int dtype, int num_seqs, int num_heads, int num_kv_heads, 
 
 int dw4_window_attention_dense(int dtype, int num_seqs, int num_heads, int num_kv_heads, int head_size,
                                const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
-                               const uint16_t* v, int64_t v_stride, uint16_t* out, int64_t o_stride, float* lse,
+                               const uint16_t* v, int64_t v_stride, uint16_t* out, int64_t o_stride, float* lse, uint16_t* out_rest,
                                const int32_t* seq_starts, int total_rows, int max_seq_len, float scale, int window,
                                int sinks, void* stream) {
   dw4::WindowArgs a = {};
   const int st = dense_args(dtype, num_seqs, num_heads, num_kv_heads, head_size, q, q_stride, k, k_stride, v, v_stride, out,
                             o_stride, seq_starts, total_rows, max_seq_len, scale, window, sinks, a);
   if (st != DW4_OK || a.q == nullptr) return st;
+  if ((lse == nullptr) != (out_rest == nullptr)) return DW4_ERR_INVALID_ARG;
+  if (!aligned16(out_rest)) return DW4_ERR_MISALIGNED;
   a.lse = lse;
+  a.rest = out_rest;
   return status_of(dw4::launch_window(a, dw4::plan_window(a, a.max_query, dw4::cu_count()), nullptr,
                                       static_cast<hipStream_t>(stream)));
 }
@@ -169,7 +172,7 @@ int dw4_window_attention_dense_backward_workspace_size(int num_seqs, int num_hea
 int dw4_window_attention_dense_backward(int dtype, int num_seqs, int num_heads, int num_kv_heads, int head_size,
                                         const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
                                         const uint16_t* v, int64_t v_stride, const uint16_t* out, int64_t o_stride,
-                                        const float* lse, const uint16_t* dout, int64_t do_stride, uint16_t* dq,
+                                        const float* lse, const uint16_t* out_rest, const uint16_t* dout, int64_t do_stride, uint16_t* dq,
                                         int64_t dq_stride, uint16_t* dk, int64_t dk_stride, uint16_t* dv,
                                         int64_t dv_stride, const int32_t* seq_starts, int total_rows, int max_seq_len,
                                         float scale, int window, int sinks, void* workspace, size_t workspace_bytes,
@@ -178,16 +181,17 @@ int dw4_window_attention_dense_backward(int dtype, int num_seqs, int num_heads, 
   const int st = dense_args(dtype, num_seqs, num_heads, num_kv_heads, head_size, q, q_stride, k, k_stride, v, v_stride, out,
                             o_stride, seq_starts, total_rows, max_seq_len, scale, window, sinks, g.f);
   if (st != DW4_OK || g.f.q == nullptr) return st;
-  if (!lse || !dout || !dq || !dk || !dv) return DW4_ERR_INVALID_ARG;
+  if (!lse || !out_rest || !dout || !dq || !dk || !dv) return DW4_ERR_INVALID_ARG;
   const int64_t row = (int64_t)num_heads * head_size, kv = (int64_t)num_kv_heads * head_size;
   if (do_stride < row || dq_stride < row || dk_stride < kv || dv_stride < kv) return DW4_ERR_INVALID_ARG;
-  if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || do_stride % 8 != 0 || dq_stride % 8 != 0 ||
+  if (!aligned16(out_rest) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || do_stride % 8 != 0 || dq_stride % 8 != 0 ||
       dk_stride % 8 != 0 || dv_stride % 8 != 0)
     return DW4_ERR_MISALIGNED;
   const size_t need = dw4::window_grad_ws_bytes(num_seqs, total_rows, num_heads, num_kv_heads, g.f.max_query);
   if (workspace == nullptr || workspace_bytes < need) return DW4_ERR_WORKSPACE;
   if (!aligned16(workspace)) return DW4_ERR_MISALIGNED;
   g.f.lse = const_cast<float*>(lse);
+  g.f.rest = const_cast<uint16_t*>(out_rest);
   g.dout = dout;
   g.do_stride = do_stride;
   g.dq = dq;

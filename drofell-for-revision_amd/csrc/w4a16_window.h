@@ -32,7 +32,8 @@ struct WindowArgs {
   const uint16_t* k;
   const uint16_t* v;
   int64_t k_stride, v_stride;
-  float* lse;  // [rows][num_heads] log2 of the softmax's sum, or null
+  float* lse;      // [rows][num_heads] log2 of the softmax's sum, or null
+  uint16_t* rest;  // [rows][num_heads][head_size] what rounding the output left off, or null
 };
 
 // rows: the kernel whose waves share 32 rows and split the tokens; else the

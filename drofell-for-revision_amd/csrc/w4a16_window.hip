@@ -149,15 +149,14 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restr
     const int first_pos = p0 + base / G, last_pos = p0 + (base + nrows - 1) / G;
     const bool full = held == (1u << NB) - 1 && t + 31 <= min(first_pos, cap - 1) &&
                       (a.window == 0 || t > last_pos - a.window || t + 31 < a.sinks);
+    uint32_t seen = 0;  // bit e: score e
     if (!full) {
+      seen = own_scores(seen_of(t, last, before, a.sinks), half);
+      if constexpr (NB == 1) seen = held ? seen : 0u;
+      else seen &= (held & 1 ? 0xFFu : 0u) | (held & 2 ? 0xFF00u : 0u);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int in = 16 * (e >> 3) + 8 * half + (e & 7);
-        const bool there = (held >> (NB == 2 ? e >> 3 : 0)) & 1;
-        s[e] = there && sees(t + in, last, before, a.sinks) ? s[e] : -INFINITY;
-      }
+      for (int e = 0; e < 16; ++e) s[e] = where_seen(seen, e, s[e], -INFINITY);
     }
-    const uint32_t held_now = held;
     if (i + 1 < nsw) load_k(i + 1);
     held = held_next;
     float mx = s[0];
@@ -193,17 +192,15 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restr
     if (!full) {
       // a value that some rows do not see (or that is behind the context) must
       // not reach them as 0 * inf
+      uint32_t bits = 0;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) odd |= any_nonfinite<BF>(vreg[d][0]) | any_nonfinite<BF>(vreg[d][1]);
-      odd = __any(odd);
+      for (int d = 0; d < ND; ++d) {
+        add_nonfinite<BF>(vreg[d][0], bits);
+        add_nonfinite<BF>(vreg[d][1], bits);
+      }
+      odd = __any((bits & kNonfinite) != 0);
     }
     if (odd) {
-      uint32_t seen = 0;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const bool there = (held_now >> (NB == 2 ? e >> 3 : 0)) & 1;
-        seen |= (uint32_t)(there && sees(t + 16 * (e >> 3) + 8 * half + (e & 7), last, before, a.sinks)) << e;
-      }
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         for (uint32_t sign = 0; sign <= 0x8000u; sign += 0x8000u) {

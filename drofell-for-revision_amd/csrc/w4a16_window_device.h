@@ -115,19 +115,16 @@ __device__ __forceinline__ bool work_of(int b, int pairs, int items, int& pair, 
   return item < items;
 }
 
-// Non-finite elements of a 16-byte operand (eight 16-bit values).
+// Sets bit 15 or 31 of a word of `bits` if an element of x is not finite (the
+// exponent's carry; other bits of `bits` mean nothing).
 template <bool BF>
-__device__ __forceinline__ bool any_nonfinite(h8 x) {
-  constexpr uint32_t kExp = BF ? 0x7F80u : 0x7C00u;
+__device__ __forceinline__ void add_nonfinite(h8 x, uint32_t& bits) {
+  constexpr uint32_t kExp = BF ? 0x7F807F80u : 0x7C007C00u, kLow = BF ? 0x00800080u : 0x04000400u;
   const u4 v = __builtin_bit_cast(u4, x);
-  bool bad = false;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    bad |= (v[e] & kExp) == kExp;
-    bad |= (v[e] & (kExp << 16)) == kExp << 16;
-  }
-  return bad;
+  for (int e = 0; e < 4; ++e) bits |= (v[e] & kExp) + kLow;
 }
+constexpr uint32_t kNonfinite = 0x80008000u;
 
 // x without its non-finite elements.
 template <bool BF>
@@ -168,6 +165,25 @@ __device__ __forceinline__ h8 ones_of(uint32_t bits) {
 // the cache), and after `before` or a sink.
 __device__ __forceinline__ bool sees(int j, int last, int before, int sinks) {
   return j <= last && (j > before || j < sinks);
+}
+// The n lowest of 32 bits (none for n <= 0).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+// Bit e: whether a row sees token t + e, of 32.
+__device__ __forceinline__ uint32_t seen_of(int t, int last, int before, int sinks) {
+  // before - t may pass the 32-bit range below (no window: every token is after it)
+  const int b = before < t ? -1 : before - t;
+  return low_bits(last - t + 1) & (~low_bits(b + 1) | low_bits(sinks - t));
+}
+// Of 32 tokens' bits (per row) the lane's own scores' (register i: token
+// 16 (i / 8) + 8 (lane / 32) + i % 8), in bits 0 .. 15.
+__device__ __forceinline__ uint32_t own_scores(uint32_t seen, int half) {
+  const uint32_t x = seen >> (8 * half);
+  return (x & 0xFFu) | ((x >> 8) & 0xFF00u);
+}
+// v where bit i of `seen` is set, else `other`.
+__device__ __forceinline__ float where_seen(uint32_t seen, int i, float v, float other) {
+  const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)seen, i, 1);
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) & m) | (__builtin_bit_cast(uint32_t, other) & ~m));
 }
 
 // global -> LDS copy of 16 / 4 bytes per active lane, to lds + lane * 16 / 4 (a

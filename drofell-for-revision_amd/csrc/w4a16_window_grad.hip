@@ -15,12 +15,14 @@
 // Both read a tile from LDS in both directions, rows in plain and columns in
 // transposing reads.  Matrix-core and LDS-read bound.
 //
-// Roundings: P and dS enter the products in 16 bits, as the matrix cores take
-// them, with independent errors.  fp16 holds neither small probabilities nor
-// small gradients, so P goes in as 2^10 P and dS times a power of two that
-// brings the largest |dO| of the rows it is summed with to 1/16 .. 1/8; bf16
-// needs neither.  delta comes from the rounded output: its error is half a
-// step of O, one part in some thousands of |dO| |O|, beside dS's own rounding.
+// Roundings: P enters its product in 16 bits, as the matrix cores take it, with
+// independent errors.  dS, whose errors would add up with those of delta, enters
+// as two 16-bit parts, over operands that are in registers already, and delta
+// sums the forward's output and what its rounding left off.  (With one part
+// and the rounded output alone dq and dk were 1.7 times as far from float64 as their
+// own rounding is.)  fp16 holds neither small probabilities nor small gradients,
+// so P goes in as 2^10 P and dS times a power of two that brings the largest
+// |dO| of the rows it is summed with to 1/16 .. 1/8; bf16 needs neither.
 // A sequence's non-finite values may reach any gradient of that sequence.
 
 #include <hip/hip_runtime.h>
@@ -47,16 +49,30 @@ __device__ __forceinline__ float grad_scale(float most) {
   return __builtin_amdgcn_ldexpf(1.f, -3 - __builtin_amdgcn_frexp_expf(most));
 }
 
+// sum of x (y + z), and the largest |x|
 template <bool BF>
-__device__ __forceinline__ void dot8(u4 x, u4 y, float& sum, float& most) {
+__device__ __forceinline__ void dot8(u4 x, u4 y, u4 z, float& sum, float& most) {
 #pragma unroll
   for (int e = 0; e < 4; ++e)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float a = unpack<BF>(x[e], h);
-      sum = fmaf(a, unpack<BF>(y[e], h), sum);
+      sum = fmaf(a, unpack<BF>(y[e], h) + unpack<BF>(z[e], h), sum);
       most = fmaxf(most, fabsf(a));
     }
+}
+
+// Eight values as an operand, and what its rounding leaves off as another.
+template <bool BF>
+__device__ __forceinline__ void two_parts(const float* v, h8& hi, h8& lo) {
+  u4 h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = pack2<BF>(v[2 * e], v[2 * e + 1]);
+    l[e] = pack2<BF>(v[2 * e] - unpack<BF>(h[e], 0), v[2 * e + 1] - unpack<BF>(h[e], 1));
+  }
+  hi = __builtin_bit_cast(h8, h);
+  lo = __builtin_bit_cast(h8, l);
 }
 
 template <int HS, bool BF>
@@ -111,11 +127,12 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
     const uint16_t* qp = a.q + (size_t)token * a.q_stride + col;
     const uint16_t* dp = g.dout + (size_t)token * g.do_stride + col;
     const uint16_t* op = a.out + (size_t)token * a.o_stride + col;
+    const uint16_t* rp = a.rest + (size_t)token * a.num_heads * HS + col;
 #pragma unroll
     for (int j = 0; j < KD; ++j) {
       qreg[j] = *(const h8*)(qp + 16 * j);
       oreg[j] = *(const h8*)(dp + 16 * j);
-      dot8<BF>(__builtin_bit_cast(u4, oreg[j]), *(const u4*)(op + 16 * j), dl, mo);
+      dot8<BF>(__builtin_bit_cast(u4, oreg[j]), *(const u4*)(op + 16 * j), *(const u4*)(rp + 16 * j), dl, mo);
     }
   }
   dl = both_sum(dl);
@@ -158,17 +175,18 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
 #pragma unroll
       for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * ((p[e] - dl) * gs);
       if (!full) {
+        const uint32_t seen = own_scores(seen_of(tb, pos, before, a.sinks), half);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          ds[e] = sees(tb + 16 * (e >> 3) + 8 * half + (e & 7), pos, before, a.sinks) ? ds[e] : 0.f;
+        for (int e = 0; e < 16; ++e) ds[e] = where_seen(seen, e, ds[e], 0.f);
       }
-      h8 w[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        w[x] = __builtin_bit_cast(h8, u4{pack2<BF>(ds[8 * x], ds[8 * x + 1]), pack2<BF>(ds[8 * x + 2], ds[8 * x + 3]),
-                                         pack2<BF>(ds[8 * x + 4], ds[8 * x + 5]), pack2<BF>(ds[8 * x + 6], ds[8 * x + 7])});
+      h8 hi[2], lo[2];
+      two_parts<BF>(ds, hi[0], lo[0]);
+      two_parts<BF>(ds + 8, hi[1], lo[1]);
       feed<2 * ND, 6>([&](int i) { return column_unit<HS>(st, 32 * b + 16 * (i / ND), i % ND); },
-                      [&](int i, h8 f) { dq[i % ND] = mfma32_of<BF>(f, w[i / ND], dq[i % ND]); });
+                      [&](int i, h8 f) {
+                        dq[i % ND] = mfma32_of<BF>(f, hi[i / ND], dq[i % ND]);
+                        dq[i % ND] = mfma32_of<BF>(f, lo[i / ND], dq[i % ND]);
+                      });
     }
   }
   if (c >= nrows) return;
@@ -282,7 +300,7 @@ window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, uint32_t magic,
             if (i & 1) p = mfma32_of<BF>(f, vreg[i >> 1], p);
             else s = mfma32_of<BF>(f, kreg[i >> 1], s);
           });
-      h8 pw[2], dw[2];
+      h8 pw[2], hi[2], lo[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int r = 32 * b + 16 * x + 8 * half;  // the lane's eight rows
@@ -302,14 +320,18 @@ window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, uint32_t magic,
           }
         }
         pw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(pr[0], pr[1]), pack2<BF>(pr[2], pr[3]), pack2<BF>(pr[4], pr[5]), pack2<BF>(pr[6], pr[7])});
-        dw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(ds[0], ds[1]), pack2<BF>(ds[2], ds[3]), pack2<BF>(ds[4], ds[5]), pack2<BF>(ds[6], ds[7])});
+        two_parts<BF>(ds, hi[x], lo[x]);
       }
       feed<4 * ND, 6>(  // of each 16 rows and 32 dims: dO, then Q
           [&](int i) { return column_unit<HS>(st + (1 - (i & 1)) * TILE, 32 * b + 16 * (i / (2 * ND)), i / 2 % ND); },
           [&](int i, h8 f) {
             const int x = i / (2 * ND), d = i / 2 % ND;
-            if (i & 1) dk[d] = mfma32_of<BF>(f, dw[x], dk[d]);
-            else dv[d] = mfma32_of<BF>(f, pw[x], dv[d]);
+            if (i & 1) {
+              dk[d] = mfma32_of<BF>(f, hi[x], dk[d]);
+              dk[d] = mfma32_of<BF>(f, lo[x], dk[d]);
+            } else {
+              dv[d] = mfma32_of<BF>(f, pw[x], dv[d]);
+            }
           });
     }
   }

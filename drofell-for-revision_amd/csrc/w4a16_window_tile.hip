@@ -230,24 +230,24 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
     const unsigned char* st = lds + stage * STAGE;
     uint32_t seen = 0;  // bit 16 b + e: score e of the 32 tokens b
 #pragma unroll
-    for (int x = 0; x < 32; ++x) {
-      const bool there = BS == 0 || ((held[stage] >> (BS == 32 ? x >> 4 : x >> 3)) & 1);
-      seen |= (uint32_t)(there && sees(t + 16 * (x >> 3) + 8 * half + (x & 7), last, before, a.sinks)) << x;
+    for (int b = 0; b < 2; ++b) {
+      uint32_t x = own_scores(seen_of(t + 32 * b, last, before, a.sinks), half);
+      if constexpr (BS == 32) x = held[stage] >> b & 1 ? x : 0u;
+      if constexpr (BS == 16) x &= (held[stage] >> (2 * b) & 1 ? 0xFFu : 0u) | (held[stage] >> (2 * b + 1) & 1 ? 0xFF00u : 0u);
+      seen |= x << (16 * b);
     }
     f16v s[2] = {f16v{}, f16v{}};
     h8 p[2][2];
     scores(st, s);
 #pragma unroll
-    for (int x = 0; x < 32; ++x) s[x >> 4][x & 15] = seen >> x & 1 ? s[x >> 4][x & 15] : -INFINITY;
+    for (int x = 0; x < 32; ++x) s[x >> 4][x & 15] = where_seen(seen, x, s[x >> 4][x & 15], -INFINITY);
     probabilities(s, p);
     // a value that some rows do not see (or that no row does) must not reach
     // them as 0 * inf: where there is one, its part is added apart
-    bool odd = false;
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) odd |= any_nonfinite<BF>(value(st, x >> 1, d, x & 1));
-    odd = __any(odd);
+    uint32_t bits = 0;
+    feed<4 * ND, 8>([&](int i) { return value(st, i / (2 * ND), i % ND, i / ND % 2); },
+                    [&](int, h8 f) { add_nonfinite<BF>(f, bits); });
+    const bool odd = __any((bits & kNonfinite) != 0);
     if (odd) {
       for (uint32_t sign = 0; sign <= 0x8000u; sign += 0x8000u) {
         const float inf = sign ? -INFINITY : INFINITY;
@@ -263,14 +263,11 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
         }
       }
     }
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        h8 v = value(st, x >> 1, d, x & 1);
-        if (odd) v = finite_part<BF>(v);
-        o[d] = mfma32_of<BF>(v, p[x >> 1][x & 1], o[d]);
-      }
+    feed<4 * ND, 8>([&](int i) { return value(st, i / (2 * ND), i % ND, i / ND % 2); },
+                    [&](int i, h8 f) {
+                      if (odd) f = finite_part<BF>(f);
+                      o[i % ND] = mfma32_of<BF>(f, p[i / (2 * ND)][i / ND % 2], o[i % ND]);
+                    });
   };
   int stage = 0, step = s0;
   auto begin = [&]() {
@@ -300,14 +297,24 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   if (splits == 1) {
     const float f = sum == 0.f ? 1.f : 1.f / sum;  // no visible token: zeros
     uint16_t* op = a.out + (size_t)token * a.o_stride + (size_t)head * HS;
+    uint16_t* rp = a.rest + ((size_t)token * a.num_heads + head) * HS;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const int dim = d * 32 + 2 * e + 4 * half;
-        if (!VTAIL || dim < HS)
-          *(uint2*)(op + dim) = make_uint2(pack2<BF>(o[d][e] * f, o[d][e + 1] * f),
-                                           pack2<BF>(o[d][e + 2] * f, o[d][e + 3] * f));
+        if (VTAIL && dim >= HS) continue;
+        float y[4];
+        uint32_t x[2], r[2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = o[d][e + k] * f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          x[k] = pack2<BF>(y[2 * k], y[2 * k + 1]);
+          r[k] = pack2<BF>(y[2 * k] - unpack<BF>(x[k], 0), y[2 * k + 1] - unpack<BF>(x[k], 1));
+        }
+        *(uint2*)(op + dim) = make_uint2(x[0], x[1]);
+        if (BS == 0 && a.rest != nullptr) *(uint2*)(rp + dim) = make_uint2(r[0], r[1]);
       }
     if (a.lse != nullptr && half == 0)
       a.lse[(size_t)token * a.num_heads + head] = m + __builtin_amdgcn_logf(sum) - p_shift<BF>();

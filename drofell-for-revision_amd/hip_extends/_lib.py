@@ -132,9 +132,9 @@ SIGNATURES = {
                                         _c.c_size_t, _P]),
     "dw4_window_attention_workspace_size": (_c.c_int, [_c.c_int] * 10 + [_SZ]),
     "dw4_window_attention_dense": (_c.c_int, [_c.c_int] * 5 + [_P, _c.c_int64] * 4
-                                   + [_P, _P, _c.c_int, _c.c_int, _c.c_float, _c.c_int,
+                                   + [_P, _P, _P, _c.c_int, _c.c_int, _c.c_float, _c.c_int,
                                       _c.c_int, _P]),
-    "dw4_window_attention_dense_backward": (_c.c_int, [_c.c_int] * 5 + [_P, _c.c_int64] * 4 + [_P]
+    "dw4_window_attention_dense_backward": (_c.c_int, [_c.c_int] * 5 + [_P, _c.c_int64] * 4 + [_P, _P]
                                             + [_P, _c.c_int64] * 4
                                             + [_P, _c.c_int, _c.c_int, _c.c_float, _c.c_int,
                                                _c.c_int, _P, _c.c_size_t, _P]),

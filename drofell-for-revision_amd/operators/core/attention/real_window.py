@@ -191,15 +191,16 @@ class _WindowDense(torch.autograd.Function):
             out = torch.empty(q.shape, dtype=q.dtype, device=device)
             need = any(ctx.needs_input_grad[:3])
             lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if need else None
+            rest = torch.empty(q.shape, dtype=q.dtype, device=device) if need else None
             _lib.call("dw4_window_attention_dense", *_WindowDense._shape(att, q, starts),
                       q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v),
                       out.data_ptr(), _stride(out), None if lse is None else lse.data_ptr(),
-                      starts.data_ptr(), q.shape[0], seq_len_max, float(att.scale), att._window,
+                      None if rest is None else rest.data_ptr(), starts.data_ptr(), q.shape[0], seq_len_max, float(att.scale), att._window,
                       att._sinks, torch.cuda.current_stream(device).cuda_stream)
         ctx.empty = False
         ctx.att, ctx.seq_len_max = att, seq_len_max
         if need:
-            ctx.save_for_backward(q, k, v, out, lse, starts)
+            ctx.save_for_backward(q, k, v, out, lse, rest, starts)
         return out
 
     @staticmethod
@@ -208,7 +209,7 @@ class _WindowDense(torch.autograd.Function):
         if ctx.empty:
             return (*(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in ctx.saved_tensors),
                     None, None, None)
-        q, k, v, out, lse, starts = ctx.saved_tensors
+        q, k, v, out, lse, rest, starts = ctx.saved_tensors
         att, device = ctx.att, q.device
         with _on(device):
             do = _rows(dout)
@@ -218,7 +219,7 @@ class _WindowDense(torch.autograd.Function):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
             _lib.call("dw4_window_attention_dense_backward", *shape, q.data_ptr(), _stride(q),
                       k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), out.data_ptr(), _stride(out),
-                      lse.data_ptr(), do.data_ptr(), _stride(do), dq.data_ptr(), _stride(dq),
+                      lse.data_ptr(), rest.data_ptr(), do.data_ptr(), _stride(do), dq.data_ptr(), _stride(dq),
                       dk.data_ptr(), _stride(dk), dv.data_ptr(), _stride(dv), starts.data_ptr(),
                       q.shape[0], ctx.seq_len_max, float(att.scale), att._window, att._sinks,
                       ws.data_ptr(), nbytes, torch.cuda.current_stream(device).cuda_stream)

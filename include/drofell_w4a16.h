@@ -523,23 +523,25 @@ int dw4_window_attention_workspace_size(int num_seqs, int num_heads, int num_kv_
  * [total_rows][num_kv_heads][head_size] with row strides, sequence s in the rows
  * seq_starts[s] .. seq_starts[s + 1] - 1 (int32 device, ascending), each at most
  * max_seq_len long.  Output rows of no sequence become zeros.  lse: float
- * [total_rows][num_heads], the base-2 logarithm of each row's softmax sum, for
- * the backward pass, or NULL. */
+ * [total_rows][num_heads], the base-2 logarithm of each row's softmax sum, and
+ * out_rest, of dtype and contiguous [total_rows][num_heads][head_size], what
+ * rounding the output left off: both for the backward pass, or both NULL. */
 int dw4_window_attention_dense(int dtype, int num_seqs, int num_heads, int num_kv_heads,
                                int head_size, const uint16_t* q, int64_t q_stride, const uint16_t* k,
                                int64_t k_stride, const uint16_t* v, int64_t v_stride, uint16_t* out,
-                               int64_t o_stride, float* lse, const int32_t* seq_starts, int total_rows,
-                               int max_seq_len, float scale, int window, int sinks, void* stream);
+                               int64_t o_stride, float* lse, uint16_t* out_rest,
+                               const int32_t* seq_starts, int total_rows, int max_seq_len, float scale, int window, int sinks, void* stream);
 
 /* Its gradients dq, dk, dv (shapes of q, k, v; rows of no sequence become
- * zeros) for the output gradient dout, from the forward's inputs, out and lse.
+ * zeros) for the output gradient dout, from the forward's inputs, out, lse and out_rest.
  * Deterministic, also where query heads share a kv head.  workspace:
  * dw4_window_attention_dense_backward_workspace_size bytes. */
 int dw4_window_attention_dense_backward(int dtype, int num_seqs, int num_heads, int num_kv_heads,
                                         int head_size, const uint16_t* q, int64_t q_stride,
                                         const uint16_t* k, int64_t k_stride, const uint16_t* v,
                                         int64_t v_stride, const uint16_t* out, int64_t o_stride,
-                                        const float* lse, const uint16_t* dout, int64_t do_stride,
+                                        const float* lse, const uint16_t* out_rest,
+                                        const uint16_t* dout, int64_t do_stride,
                                         uint16_t* dq, int64_t dq_stride, uint16_t* dk,
                                         int64_t dk_stride, uint16_t* dv, int64_t dv_stride,
                                         const int32_t* seq_starts, int total_rows, int max_seq_len,

@@ -5,8 +5,8 @@ Roundings counted, u = half a step of the 16-bit type relative to the value:
 * the output, dq, dk, dv rounded once: u |result|;
 * probabilities rounded before p . v and P^T . dO: u sum p |v| (independent errors
   may all point one way in a bound);
-* dS rounded before its products: u sum |dS| |k|;
-* delta = dO . O from the rounded O: P (u |O| + error of O) . |dO|;
+* dS as two 16-bit parts in its products: u^2 sum |dS| |k|;
+* delta = dO . O from the unrounded O (as two parts): P (u^2 |O| + error of p . v) . |dO|;
 * everything else in float32: sums of n terms n 2^-24 of the sum of absolute
   values; an exponent (a logit of up to 2^5 times log2 e, formed from float32 sums
   of the head size's terms) 2^-16 of p.
@@ -55,13 +55,14 @@ def gradients(q, k, v, dout, seen, scale, dtype):
     u, n = half_step(dtype), len(q)
     out, spread, p = attend(q, k, v, seen, scale)
     e_out = out_bound(out, spread, n, dtype)
+    e_sum = e_out - (u - u * u) * out.abs()
     dp = dout @ v.T
     delta = (dout * out).sum(1, keepdim=True)
     ds = p * (dp - delta)
     dq, dk, dv = scale * ds @ k, scale * ds.T @ q, p.T @ dout
     f = SLACK + n * 2.0 ** -23
     size = dout.abs() @ v.abs().T + (dout.abs() * out.abs()).sum(1, keepdim=True)
-    e_ds = (u + f) * ds.abs() + p * ((dout.abs() * e_out).sum(1, keepdim=True) + f * size)
+    e_ds = (u * u + f) * ds.abs() + p * ((dout.abs() * e_sum).sum(1, keepdim=True) + f * size)
     tiny = torch.finfo(dtype).smallest_normal * u * 2
     e_dq = u * dq.abs() + scale * (e_ds + f * ds.abs()) @ k.abs() * (1 + u) + tiny
     e_dk = u * dk.abs() + scale * (e_ds + f * ds.abs()).T @ q.abs() * (1 + u) + tiny

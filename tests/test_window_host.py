@@ -55,12 +55,12 @@ def test_window_attention_refusals():
 
 
 def dense(back=False, dtype=1, seqs=2, heads=8, kvh=4, hd=64, q=FAKE, qs=512, k=FAKE, ks=256, o=FAKE, starts=FAKE, rows=100,
-          most=60, scale=0.1, window=0, sinks=0, lse=FAKE, do=FAKE, dk=FAKE, dks=256, ws=FAKE, wsb=1 << 20):
+          most=60, scale=0.1, window=0, sinks=0, lse=FAKE, rest=FAKE, do=FAKE, dk=FAKE, dks=256, ws=FAKE, wsb=1 << 20):
     lib = _lib.load()
     if not back:
-        return lib.dw4_window_attention_dense(dtype, seqs, heads, kvh, hd, q, qs, k, ks, k, ks, o, 512, lse, starts, rows,
+        return lib.dw4_window_attention_dense(dtype, seqs, heads, kvh, hd, q, qs, k, ks, k, ks, o, 512, lse, rest, starts, rows,
                                               most, scale, window, sinks, None)
-    return lib.dw4_window_attention_dense_backward(dtype, seqs, heads, kvh, hd, q, qs, k, ks, k, ks, o, 512, lse, do, 512,
+    return lib.dw4_window_attention_dense_backward(dtype, seqs, heads, kvh, hd, q, qs, k, ks, k, ks, o, 512, lse, rest, do, 512,
                                                    FAKE, 512, dk, dks, FAKE, 256, starts, rows, most, scale, window, sinks,
                                                    ws, wsb, None)
 
@@ -76,6 +76,7 @@ def test_dense_refusals(back):
     assert call(q=ODD) == MISAL and call(k=ODD) == MISAL and call(qs=516) == MISAL and call(ks=260) == MISAL
     for empty in (dict(seqs=0), dict(rows=0), dict(most=0)):
         assert call(**empty) == OK
+    assert call(rest=None) == BAD and call(rest=ODD) == MISAL
     if back:
         assert call(lse=None) == BAD and call(do=None) == BAD and call(dk=None) == BAD and call(dks=128) == BAD
         assert call(dk=ODD) == MISAL and call(dks=260) == MISAL

@@ -159,13 +159,16 @@ int dw4_window_attention_dense(int dtype, int num_seqs, int num_heads, int num_k
                                       static_cast<hipStream_t>(stream)));
 }
 
-int dw4_window_attention_dense_backward_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int total_rows,
-                                                       int max_seq_len, size_t* workspace_bytes) {
-  const int st = check_window(DW4_F16, num_seqs, num_heads, num_kv_heads, 64, total_rows, max_seq_len, 0, 0);
+int dw4_window_attention_dense_backward_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_size,
+                                                       int total_rows, int max_seq_len, int window, int sinks,
+                                                       size_t* workspace_bytes) {
+  const int st = check_window(DW4_F16, num_seqs, num_heads, num_kv_heads, head_size, total_rows, max_seq_len, window, sinks);
   if (st != DW4_OK) return st;
   if (workspace_bytes == nullptr) return DW4_ERR_INVALID_ARG;
-  *workspace_bytes = dw4::window_grad_ws_bytes(num_seqs, total_rows, num_heads, num_kv_heads,
-                                               max_seq_len < total_rows ? max_seq_len : total_rows);
+  *workspace_bytes = 0;
+  if (num_seqs > 0 && total_rows > 0 && max_seq_len > 0)
+    *workspace_bytes = dw4::window_grad_ws_bytes(
+        window_args(DW4_F16, num_seqs, num_heads, num_kv_heads, head_size, total_rows, max_seq_len, 1.f, window, sinks));
   return DW4_OK;
 }
 
@@ -187,7 +190,7 @@ int dw4_window_attention_dense_backward(int dtype, int num_seqs, int num_heads, 
   if (!aligned16(out_rest) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || do_stride % 8 != 0 || dq_stride % 8 != 0 ||
       dk_stride % 8 != 0 || dv_stride % 8 != 0)
     return DW4_ERR_MISALIGNED;
-  const size_t need = dw4::window_grad_ws_bytes(num_seqs, total_rows, num_heads, num_kv_heads, g.f.max_query);
+  const size_t need = dw4::window_grad_ws_bytes(g.f);
   if (workspace == nullptr || workspace_bytes < need) return DW4_ERR_WORKSPACE;
   if (!aligned16(workspace)) return DW4_ERR_MISALIGNED;
   g.f.lse = const_cast<float*>(lse);

@@ -59,7 +59,6 @@ inline unsigned win_grid(int pairs, int items) {
 inline size_t win_rows_smem(int hs, int cols, int waves) {
   return sizeof(float) * (size_t)waves * cols * (hs + 2);
 }
-inline size_t win_tile_smem(int hs) { return (size_t)2 * 2 * kWinTileTokens * hs * 2; }
 
 WindowPlan plan_window(const WindowArgs& a, int max_context, int cus);
 size_t window_ws_bytes(const WindowPlan& p, int total_rows, int num_heads, int head_size);
@@ -81,7 +80,7 @@ struct WindowGradArgs {
   int64_t dq_stride, dk_stride, dv_stride;
   float scale;
 };
-size_t window_grad_ws_bytes(int num_seqs, int total_rows, int num_heads, int num_kv_heads, int max_query);
+size_t window_grad_ws_bytes(const WindowArgs& a);
 template <bool BF>
 hipError_t launch_window_grad(const WindowGradArgs& a, float* ws, hipStream_t stream);
 

@@ -213,7 +213,7 @@ __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt((7 << 
 template <int N, int AHEAD, typename Load, typename Use>
 __device__ __forceinline__ void feed(Load&& load, Use&& use) {
   constexpr int kMoves = 0x2 | 0x4 | 0x400;  // vector ALU, scalar ALU, transcendental
-  h8 f[N];
+  decltype(load(0)) f[N];
 #pragma unroll
   for (int i = 0; i < (AHEAD < N ? AHEAD : N); ++i) f[i] = load(i);
   __builtin_amdgcn_sched_barrier(kMoves);
@@ -226,19 +226,31 @@ __device__ __forceinline__ void feed(Load&& load, Use&& use) {
   }
 }
 
-// Row-major tiles in LDS ([row][HS], as the tensors have them): 16-byte unit u
-// of row r stands at unit u ^ swizzle<HS>(r), so that both reads, a unit of 32
-// rows (row_unit) and four rows by 32 dims (column_unit), spread over the banks.
+// Row-major tiles in LDS ([row][HS], as the tensors have them), laid out so that
+// both reads, a unit of 32 rows (row_unit) and four rows by 32 dims (column_unit),
+// spread over the banks, and so that few addresses differ by more than a constant:
+//   * HS 128 and 256: 16-byte unit u of row r stands at unit u ^ 4 (r % 4), and
+//     every four rows 16 bytes further;
+//   * HS 64: at unit u ^ (2 (r & 2) + r / 4 % 4);
+//   * HS 80, 96 and 112: as it is, the rows' own stride does it.
 template <int HS>
 __device__ __forceinline__ int swizzle(int r) {
-  if constexpr (HS == 64) return ((r & 2) << 1) | ((r >> 2) & 3);
-  else if constexpr (HS % 128 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
-  else return 0;  // 80, 96 and 112: the rows' own stride does it
+  if constexpr (HS % 128 == 0) return (r & 3) << 2;
+  else if constexpr (HS == 64) return ((r & 2) << 1) | ((r >> 2) & 3);
+  else return 0;
 }
-// A operand: row r, units 2 kk + lane / 32.
+template <int HS>
+__host__ __device__ constexpr int row_at(int r) {
+  return HS % 128 == 0 ? (r >> 2) * (8 * HS + 16) + (r & 3) * (2 * HS) : r * (2 * HS);
+}
+template <int HS>  // of 64 units (1 KiB), as a copy instruction writes them
+__device__ __forceinline__ int chunk_at(int ch) {
+  return ch * 1024 + (HS % 128 == 0 ? ch / (HS / 128) * 16 : 0);
+}
+// A operand: unit `unit` of row r.
 template <int HS>
 __device__ __forceinline__ h8 row_unit(const unsigned char* tile, int r, int unit) {
-  return *(const h8*)(tile + r * (HS * 2) + ((unit ^ swizzle<HS>(r)) << 4));
+  return *(const h8*)(tile + row_at<HS>(r) + ((unit ^ swizzle<HS>(r)) << 4));
 }
 // A operand of the transposed tile: dims 32 dt + lane % 32 (below HS), rows
 // r0 + 8 (lane / 32) .. + 7, by two transposing reads.  Lane l of 16 gives the
@@ -251,12 +263,12 @@ __device__ __forceinline__ h8 column_unit(const unsigned char* tile, int r0, int
   int d = dt * 32 + (lane & 16);
   if (HS % 32 != 0) d = min(d, HS - 16);
   d += 4 * (lane & 3);
-  const int r = r0 + ((lane >> 5) << 3) + ((lane >> 2) & 3);
+  const int r = ((lane >> 5) << 3) + ((lane >> 2) & 3);
+  tile += row_at<HS>(r0);  // r0 is a multiple of 16
   s4 x[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const unsigned char* at = tile + (r + 4 * h) * (HS * 2) +
-                              ((((d >> 3) ^ swizzle<HS>(r + 4 * h)) << 4) | ((d & 7) << 1));
+    const unsigned char* at = tile + row_at<HS>(r + 4 * h) + ((((d >> 3) ^ swizzle<HS>(r + 4 * h)) << 4) | ((d & 7) << 1));
     x[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
   }
   typedef short s8 __attribute__((ext_vector_type(8)));

@@ -10,8 +10,11 @@
 //   * window_dq_kernel: as the forward, 128 rows (tokens x query heads of a kv
 //     head) of a workgroup, steps of 64 tokens through LDS; it writes delta too;
 //   * window_dkv_kernel: 128 tokens of a workgroup, a wave's 32 as the columns
-//     of its products, steps of 64 rows through LDS; the heads of a group are
+//     of its products, steps of 32 rows through LDS; the heads of a group are
 //     rows like any others, so that shared heads' gradients add up in registers.
+//     The tokens' values stay in LDS beside the steps, which leaves registers
+//     for two waves per SIMD (one wave, with steps of 64 rows and the values in
+//     registers: 1372 us for 2 x 6000 tokens, 32 heads of 128, window 2048).
 // Both read a tile from LDS in both directions, rows in plain and columns in
 // transposing reads.  Matrix-core and LDS-read bound.
 //
@@ -80,7 +83,7 @@ __global__ void __launch_bounds__(256, HS <= 128 ? 2 : 1)
 window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* __restrict__ most) {
   constexpr int KD = HS / 16, ND = (HS + 31) / 32;
   constexpr bool VTAIL = HS % 32 != 0;
-  constexpr int TILE = kBk * HS * 2, STAGE = 2 * TILE;  // keys, values
+  constexpr int TILE = row_at<HS>(kBk), STAGE = 2 * TILE;  // keys, values
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const WindowArgs& a = g.f;
   zero_outside(g.dq, g.dq_stride, a.num_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, gridDim.x);
@@ -115,8 +118,8 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
       const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
       const int64_t tok = q0 + min(t + r, n - 1);
       const size_t col = (size_t)kvh * HS + at * 8;
-      copy16(a.k + tok * a.k_stride + col, dst + ch * 1024);
-      copy16(a.v + tok * a.v_stride + col, dst + TILE + ch * 1024);
+      copy16(a.k + tok * a.k_stride + col, dst + chunk_at<HS>(ch));
+      copy16(a.v + tok * a.v_stride + col, dst + TILE + chunk_at<HS>(ch));
     }
   };
   if (span.steps > 0) issue(0, 0);
@@ -166,14 +169,14 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
       const bool full = tb + 31 <= wfirst && (a.window == 0 || tb > wlast - a.window || tb + 31 < a.sinks);
       f16v s = {}, p = {};
       feed<2 * KD, 8>(
-          [&](int i) { return row_unit<HS>(st + (i & 1) * TILE, 32 * b + row_token(c), (i & ~1) + half); },
+          [&](int i) { return row_unit<HS>(st + (i & 1) * TILE + row_at<HS>(32 * b), row_token(c), (i & ~1) + half); },
           [&](int i, h8 f) {
             if (i & 1) p = mfma32_of<BF>(f, oreg[i >> 1], p);
             else s = mfma32_of<BF>(f, qreg[i >> 1], s);
           });
       float ds[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * ((p[e] - dl) * gs);
+      for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * (BF ? p[e] - dl : (p[e] - dl) * gs);
       if (!full) {
         const uint32_t seen = own_scores(seen_of(tb, pos, before, a.sinks), half);
 #pragma unroll
@@ -203,20 +206,40 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
     }
 }
 
+// Floats of a workspace part, whole 16-byte units.
+constexpr size_t grad_rows(size_t a, size_t b) { return (a * b + 3) / 4 * 4; }
+
+// The row steps (of kDkvRows rows) of a tile of tokens are split into parts where
+// that many workgroups are wanted: sink tiles, which a window does not bound, by
+// `sink_parts`, the others by `parts`.  Items of a pair: the sink tiles' parts, then
+// the other tiles'.
+struct DkvPlan {
+  int tiles, sink_tiles, parts, sink_parts;
+  __host__ __device__ int items() const { return sink_tiles * sink_parts + (tiles - sink_tiles) * parts; }
+  __host__ __device__ bool joined() const { return (sink_tiles > 0 && sink_parts > 1) || (tiles > sink_tiles && parts > 1); }
+};
+constexpr int kDkvRows = 32;
+
 template <int HS, bool BF>
-__global__ void __launch_bounds__(256, 1)
-window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, uint32_t magic,
-                  const float* __restrict__ delta, const float* __restrict__ most) {
+__global__ void __launch_bounds__(256, HS <= 128 ? 2 : 1)
+window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic, const float* __restrict__ delta,
+                  const float* __restrict__ most, float* __restrict__ partial) {
   constexpr int KD = HS / 16, ND = (HS + 31) / 32;
   constexpr bool VTAIL = HS % 32 != 0;
-  constexpr int TILE = kBk * HS * 2;
-  constexpr int STAGE = 2 * TILE + 3 * kBk * 4;  // rows of Q and of dO, log-sums, deltas, positions
+  constexpr int AHEAD = HS <= 96 ? 3 : 2;  // operands in flight (registers)
+  constexpr int TILE = row_at<HS>(kDkvRows);
+  constexpr int STAGE = 2 * TILE + 3 * kDkvRows * 4;  // rows of Q and of dO, log-sums, deltas, positions
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  unsigned char* const vtile = lds + 2 * STAGE;  // the tokens' values [128][HS]
   const WindowArgs& a = g.f;
   zero_outside(g.dk, g.dk_stride, a.num_kv_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, gridDim.x);
   zero_outside(g.dv, g.dv_stride, a.num_kv_heads * HS, a.starts, a.num_seqs, a.total_rows, blockIdx.x, gridDim.x);
-  int pair, tile;
-  if (!work_of(blockIdx.x, a.num_seqs * a.num_kv_heads, tiles, pair, tile)) return;
+  int pair, item;
+  if (!work_of(blockIdx.x, a.num_seqs * a.num_kv_heads, plan.items(), pair, item)) return;
+  const int far = plan.sink_tiles * plan.sink_parts;
+  const int parts = item < far ? plan.sink_parts : plan.parts;
+  const int tile = item < far ? item / parts : plan.sink_tiles + (item - far) / parts;
+  const int part = item < far ? item % parts : (item - far) % parts;
   const int seq = pair / a.num_kv_heads, kvh = pair % a.num_kv_heads;
   const int G = a.num_heads / a.num_kv_heads;
   int q0, q1;
@@ -227,44 +250,47 @@ window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, uint32_t magic,
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t0 >= n) return;
   const int c = lane & 31, half = lane >> 5;
-  // rows that see a token of the tile
+  // rows that see a token of the tile, and this part of them
   const int64_t reach = a.window == 0 || t0 < a.sinks ? n : (int64_t)t0 + kGradTile - 1 + a.window;
   const int r0 = t0 * G, r1 = (int)min<int64_t>(n, reach) * G;
-  const int steps = (r1 - r0 + kBk - 1) / kBk;
+  const int all = (r1 - r0 + kDkvRows - 1) / kDkvRows, per = (all + parts - 1) / parts;
+  const int s0 = part * per, s1 = min(all, s0 + per);
   const int wa = t0 + 32 * wave, wb = min(wa + 31, n - 1);  // this wave's tokens
   const int tk = min(wa + c, n - 1);
 
   const uint32_t lds0 = lds_offset(lds);
+  constexpr int UNITS = HS / 8;
   auto issue = [&](int s, int stage) {
     const uint32_t dst = lds0 + stage * STAGE;
-    constexpr int UNITS = HS / 8, CHUNKS = kBk * UNITS / 64;
+    constexpr int CHUNKS = kDkvRows * UNITS / 64;
     for (int ch = wave; ch < CHUNKS; ch += 4) {
       const int u = ch * 64 + lane;
       const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
-      const int row = min(r0 + s * kBk + r, r1 - 1), i = div_by_magic(row, magic);
+      const int row = min(r0 + s * kDkvRows + r, r1 - 1), i = div_by_magic(row, magic);
       const size_t col = (size_t)(kvh * G + row - i * G) * HS + at * 8;
-      copy16(a.q + (size_t)(q0 + i) * a.q_stride + col, dst + ch * 1024);
-      copy16(g.dout + (size_t)(q0 + i) * g.do_stride + col, dst + TILE + ch * 1024);
+      copy16(a.q + (size_t)(q0 + i) * a.q_stride + col, dst + chunk_at<HS>(ch));
+      copy16(g.dout + (size_t)(q0 + i) * g.do_stride + col, dst + TILE + chunk_at<HS>(ch));
     }
-    if (wave < 3) {
-      const int row = r0 + s * kBk + lane, in = min(row, r1 - 1), i = div_by_magic(in, magic);
+    if (wave < 3 && lane < kDkvRows) {
+      const int row = r0 + s * kDkvRows + lane, in = min(row, r1 - 1), i = div_by_magic(in, magic);
       const size_t at = (size_t)(q0 + i) * a.num_heads + kvh * G + in - i * G;
       if (wave == 0) copy4(a.lse + at, dst + 2 * TILE);
-      else if (wave == 1) copy4(delta + at, dst + 2 * TILE + kBk * 4);
-      else *(int*)(lds + stage * STAGE + 2 * TILE + 2 * kBk * 4 + lane * 4) = row < r1 ? i : -1;
+      else if (wave == 1) copy4(delta + at, dst + 2 * TILE + kDkvRows * 4);
+      else *(int*)(lds + stage * STAGE + 2 * TILE + 2 * kDkvRows * 4 + lane * 4) = row < r1 ? i : -1;
     }
   };
-  issue(0, 0);
-  h8 kreg[KD], vreg[KD];  // B operands: this token's key and value
+  if (s0 < s1) issue(s0, 0);
+  for (int ch = wave; ch < kGradTile * UNITS / 64; ch += 4) {
+    const int u = ch * 64 + lane;
+    const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
+    copy16(a.v + (size_t)(q0 + min(t0 + r, n - 1)) * a.v_stride + (size_t)kvh * HS + at * 8,
+           lds0 + 2 * STAGE + chunk_at<HS>(ch));
+  }
+  h8 kreg[KD];  // B operand: this token's key
   {
-    const size_t col = (size_t)kvh * HS + 8 * half;
-    const uint16_t* kp = a.k + (size_t)(q0 + tk) * a.k_stride + col;
-    const uint16_t* vp = a.v + (size_t)(q0 + tk) * a.v_stride + col;
+    const uint16_t* kp = a.k + (size_t)(q0 + tk) * a.k_stride + (size_t)kvh * HS + 8 * half;
 #pragma unroll
-    for (int j = 0; j < KD; ++j) {
-      kreg[j] = *(const h8*)(kp + 16 * j);
-      vreg[j] = *(const h8*)(vp + 16 * j);
-    }
+    for (int j = 0; j < KD; ++j) kreg[j] = *(const h8*)(kp + 16 * j);
   }
   float gs = 1.f;
   if constexpr (!BF) {
@@ -280,75 +306,126 @@ window_dkv_kernel(WindowGradArgs g, int tiles, int row_tiles, uint32_t magic,
   f16v dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f16v{};
-  for (int step = 0; step < steps; ++step) {
+  for (int step = s0; step < s1; ++step) {
+    const int stage = (step - s0) & 1;
     wait_copies();
-    if (step + 1 < steps) issue(step + 1, (step + 1) & 1);
-    if (wa >= n) continue;
-    const unsigned char* st = lds + (step & 1) * STAGE;
-    const float* ls = (const float*)(st + 2 * TILE);
-    const int* at = (const int*)(st + 2 * TILE + 2 * kBk * 4);
-    for (int b = 0; b < 2; ++b) {
-      const int ra = r0 + step * kBk + 32 * b;
-      if (ra >= r1) continue;
-      const int ia = div_by_magic(ra, magic), ib = div_by_magic(min(ra + 31, r1 - 1), magic);
-      if (ib < wa || (a.window != 0 && ia - a.window >= wb && wa >= a.sinks)) continue;
-      const bool full = ra + 31 < r1 && ia >= wb && (a.window == 0 || ib < wa + a.window || wb < a.sinks);
-      f16v s = {}, p = {};
-      feed<2 * KD, 8>(
-          [&](int i) { return row_unit<HS>(st + (i & 1) * TILE, 32 * b + row_token(c), (i & ~1) + half); },
-          [&](int i, h8 f) {
-            if (i & 1) p = mfma32_of<BF>(f, vreg[i >> 1], p);
-            else s = mfma32_of<BF>(f, kreg[i >> 1], s);
-          });
-      h8 pw[2], hi[2], lo[2];
+    if (step + 1 < s1) issue(step + 1, stage ^ 1);
+    const unsigned char* st = lds + stage * STAGE;
+    const int ra = r0 + step * kDkvRows;
+    const int ia = div_by_magic(ra, magic), ib = div_by_magic(min(ra + kDkvRows, r1) - 1, magic);
+    if (wa >= n || ib < wa || (a.window != 0 && ia - a.window >= wb && wa >= a.sinks)) continue;
+    const bool full = ra + kDkvRows <= r1 && ia >= wb && (a.window == 0 || ib < wa + a.window || wb < a.sinks);
+    f16v s = {}, p = {};
+    struct Operands {
+      h8 q, o, v;
+    };
+    feed<KD, AHEAD>(
+        [&](int j) {
+          return Operands{row_unit<HS>(st, row_token(c), 2 * j + half), row_unit<HS>(st + TILE, row_token(c), 2 * j + half),
+                          row_unit<HS>(vtile + row_at<HS>(32 * wave), c, 2 * j + half)};
+        },
+        [&](int j, const Operands& f) {
+          s = mfma32_of<BF>(f.q, kreg[j], s);
+          p = mfma32_of<BF>(f.o, f.v, p);
+        });
+    h8 pw[2], hi[2], lo[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int r = 32 * b + 16 * x + 8 * half;  // the lane's eight rows
-        float pr[8], ds[8];
+    for (int x = 0; x < 2; ++x) {
+      const float* ls = (const float*)(st + 2 * TILE) + 16 * x + 8 * half;  // of the lane's eight rows
+      float pr[8], ds[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pr[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * x + e], a.scale_log2, ps - ls[e]));
+        ds[e] = pr[e] * (p[8 * x + e] - ls[kDkvRows + e]);
+        if constexpr (!BF) ds[e] *= gp;
+      }
+      if (!full) {
+        const int* at = (const int*)(ls + 2 * kDkvRows);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          pr[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * x + e], a.scale_log2, ps - ls[r + e]));
-          ds[e] = pr[e] * ((p[8 * x + e] - ls[kBk + r + e]) * gp);
+          const int i = at[e];
+          const bool seen = sees(wa + c, i, a.window == 0 ? INT32_MIN : i - a.window, i < 0 ? 0 : a.sinks);
+          pr[e] = seen ? pr[e] : 0.f;
+          ds[e] = seen ? ds[e] : 0.f;
         }
-        if (!full) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int i = at[r + e];
-            const bool seen = sees(wa + c, i, a.window == 0 ? INT32_MIN : i - a.window, i < 0 ? 0 : a.sinks);
-            pr[e] = seen ? pr[e] : 0.f;
-            ds[e] = seen ? ds[e] : 0.f;
-          }
-        }
-        pw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(pr[0], pr[1]), pack2<BF>(pr[2], pr[3]), pack2<BF>(pr[4], pr[5]), pack2<BF>(pr[6], pr[7])});
-        two_parts<BF>(ds, hi[x], lo[x]);
       }
-      feed<4 * ND, 6>(  // of each 16 rows and 32 dims: dO, then Q
-          [&](int i) { return column_unit<HS>(st + (1 - (i & 1)) * TILE, 32 * b + 16 * (i / (2 * ND)), i / 2 % ND); },
-          [&](int i, h8 f) {
-            const int x = i / (2 * ND), d = i / 2 % ND;
-            if (i & 1) {
-              dk[d] = mfma32_of<BF>(f, hi[x], dk[d]);
-              dk[d] = mfma32_of<BF>(f, lo[x], dk[d]);
-            } else {
-              dv[d] = mfma32_of<BF>(f, pw[x], dv[d]);
-            }
-          });
+      pw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(pr[0], pr[1]), pack2<BF>(pr[2], pr[3]), pack2<BF>(pr[4], pr[5]), pack2<BF>(pr[6], pr[7])});
+      two_parts<BF>(ds, hi[x], lo[x]);
     }
+    feed<4 * ND, 6>(  // of each 16 rows and 32 dims: dO, then Q
+        [&](int i) { return column_unit<HS>(st + (1 - (i & 1)) * TILE, 16 * (i / (2 * ND)), i / 2 % ND); },
+        [&](int i, h8 f) {
+          const int x = i / (2 * ND), d = i / 2 % ND;
+          if (i & 1) {
+            dk[d] = mfma32_of<BF>(f, hi[x], dk[d]);
+            dk[d] = mfma32_of<BF>(f, lo[x], dk[d]);
+          } else {
+            dv[d] = mfma32_of<BF>(f, pw[x], dv[d]);
+          }
+        });
   }
   if (wa + c >= n) return;
   const float fk = g.scale / gs, fv = __builtin_amdgcn_exp2f(-ps);
   uint16_t* ok = g.dk + (size_t)(q0 + tk) * g.dk_stride + (size_t)kvh * HS;
   uint16_t* ov = g.dv + (size_t)(q0 + tk) * g.dv_stride + (size_t)kvh * HS;
+  float* pk = partial + (((size_t)pair * plan.items() + item) * kGradTile + 32 * wave + c) * (2 * HS);
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
       const int dim = d * 32 + 2 * e + 4 * half;
-      if (!VTAIL || dim < HS) {
-        *(uint2*)(ok + dim) = make_uint2(pack2<BF>(dk[d][e] * fk, dk[d][e + 1] * fk), pack2<BF>(dk[d][e + 2] * fk, dk[d][e + 3] * fk));
-        *(uint2*)(ov + dim) = make_uint2(pack2<BF>(dv[d][e] * fv, dv[d][e + 1] * fv), pack2<BF>(dv[d][e + 2] * fv, dv[d][e + 3] * fv));
+      if (VTAIL && dim >= HS) continue;
+      const f4 x = f4{dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]} * fk;
+      const f4 y = f4{dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]} * fv;
+      if (parts == 1) {
+        *(uint2*)(ok + dim) = make_uint2(pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]));
+        *(uint2*)(ov + dim) = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
+      } else {
+        *(f4*)(pk + dim) = x;
+        *(f4*)(pk + HS + dim) = y;
       }
     }
+}
+
+// The parts of a tile summed in their order, four dims per thread.
+template <int HS, bool BF>
+__global__ void __launch_bounds__(256)
+window_dkv_join_kernel(WindowGradArgs g, DkvPlan plan, int tiles, const float* __restrict__ partial) {
+  const WindowArgs& a = g.f;
+  constexpr int PER = kGradTile * (2 * HS / 4) / 256;  // workgroups of 256 units per tile
+  const int chunk = blockIdx.x % PER, tile = blockIdx.x / PER % tiles, pair = blockIdx.x / PER / tiles;
+  const int parts = tile < plan.sink_tiles ? plan.sink_parts : plan.parts;
+  if (parts == 1) return;
+  const int item = tile < plan.sink_tiles ? tile * parts : plan.sink_tiles * plan.sink_parts + (tile - plan.sink_tiles) * parts;
+  const int seq = pair / a.num_kv_heads, kvh = pair % a.num_kv_heads;
+  int q0, q1;
+  seq_rows(a.starts, seq, a.total_rows, q0, q1);
+  const int u = chunk * 256 + threadIdx.x, t = u / (2 * HS / 4), dim = u % (2 * HS / 4) * 4;
+  const int token = tile * kGradTile + t;
+  if (token >= min(q1 - q0, a.max_query)) return;
+  const float* src = partial + (((size_t)pair * plan.items() + item) * kGradTile + t) * (2 * HS) + dim;
+  f4 sum = {};
+  for (int p = 0; p < parts; ++p) sum += *(const f4*)(src + (size_t)p * kGradTile * (2 * HS));
+  uint16_t* out = dim < HS ? g.dk + (size_t)(q0 + token) * g.dk_stride + (size_t)kvh * HS + dim
+                           : g.dv + (size_t)(q0 + token) * g.dv_stride + (size_t)kvh * HS + dim - HS;
+  *(uint2*)out = make_uint2(pack2<BF>(sum[0], sum[1]), pack2<BF>(sum[2], sum[3]));
+}
+
+// Tiles of tokens split into parts: all of them where they leave more than half
+// of the CUs (two workgroups each) without one, down to eight steps a part; sink
+// tiles, whose rows a window does not bound, to about twice a bounded tile's rows.
+DkvPlan plan_dkv(const WindowArgs& a, int cus) {
+  DkvPlan p = {};
+  const int64_t G = a.num_heads / a.num_kv_heads, pairs = (int64_t)a.num_seqs * a.num_kv_heads;
+  p.tiles = (a.max_query + kGradTile - 1) / kGradTile;
+  const int64_t bound = a.window == 0 ? a.max_query : std::min<int64_t>(a.max_query, (int64_t)a.window + kGradTile);
+  const int64_t steps = (bound * G + kDkvRows - 1) / kDkvRows;
+  p.parts = 1;
+  if (pairs * p.tiles <= cus) p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / (pairs * p.tiles), steps / 8));
+  p.sink_tiles = a.window == 0 ? 0 : (int)std::min<int64_t>(p.tiles, ((int64_t)a.sinks + kGradTile - 1) / kGradTile);
+  p.sink_parts = p.parts;
+  if (p.sink_tiles > 0 && a.max_query >= 3 * bound) p.sink_parts = (int)std::max<int64_t>(p.parts, std::min<int64_t>(64, a.max_query / (2 * bound) * p.parts));
+  return p;
 }
 
 template <int HS, bool BF>
@@ -356,7 +433,8 @@ hipError_t launch_grad_hs(const WindowGradArgs& g, float* ws, hipStream_t stream
   static std::atomic<uint64_t> done_q{0}, done_kv{0};
   const WindowArgs& a = g.f;
   const int G = a.num_heads / a.num_kv_heads;
-  const size_t smem = win_tile_smem(HS), smem_kv = smem + 2 * 3 * kBk * 4;
+  const size_t smem = 4 * row_at<HS>(kBk);
+  const size_t smem_kv = 2 * (2 * row_at<HS>(kDkvRows) + 3 * kDkvRows * 4) + row_at<HS>(kGradTile);
   auto dq = &window_dq_kernel<HS, BF>;
   auto dkv = &window_dkv_kernel<HS, BF>;
   hipError_t e = allow_lds(reinterpret_cast<const void*>(dq), smem, done_q);
@@ -364,14 +442,20 @@ hipError_t launch_grad_hs(const WindowGradArgs& g, float* ws, hipStream_t stream
   if (e != hipSuccess) return e;
   const int pairs = a.num_seqs * a.num_kv_heads;
   const int row_tiles = (int)(((int64_t)a.max_query * G + kGradTile - 1) / kGradTile);
-  const int tiles = (a.max_query + kGradTile - 1) / kGradTile;
+  const DkvPlan plan = plan_dkv(a, cu_count());
   float* delta = ws;
-  float* most = ws + (size_t)a.total_rows * a.num_heads;
+  float* most = delta + grad_rows(a.total_rows, a.num_heads);
+  float* partial = most + grad_rows(pairs, row_tiles);
   dq<<<win_grid(pairs, row_tiles), 256, smem, stream>>>(g, row_tiles, delta, most);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   const uint32_t magic = G == 1 ? 0u : (uint32_t)((0x100000000ull + G - 1) / G);
-  dkv<<<win_grid(pairs, tiles), 256, smem_kv, stream>>>(g, tiles, row_tiles, magic, delta, most);
+  dkv<<<win_grid(pairs, plan.items()), 256, smem_kv, stream>>>(g, plan, row_tiles, magic, delta, most, partial);
+  e = hipGetLastError();
+  if (e != hipSuccess || !plan.joined()) return e;
+  const int tiles = plan.parts > 1 ? plan.tiles : plan.sink_tiles;
+  window_dkv_join_kernel<HS, BF><<<(unsigned)(pairs * tiles * (kGradTile * (2 * HS / 4) / 256)), 256, 0, stream>>>(
+      g, plan, tiles, partial);
   return hipGetLastError();
 }
 
@@ -392,9 +476,12 @@ hipError_t launch_window_grad(const WindowGradArgs& g, float* ws, hipStream_t st
 template hipError_t launch_window_grad<WINDOW_BF16>(const WindowGradArgs&, float*, hipStream_t);
 
 #if !WINDOW_BF16
-size_t window_grad_ws_bytes(int num_seqs, int total_rows, int num_heads, int num_kv_heads, int max_query) {
-  const int64_t row_tiles = ((int64_t)max_query * (num_heads / num_kv_heads) + kGradTile - 1) / kGradTile;
-  return sizeof(float) * ((size_t)total_rows * num_heads + (size_t)num_seqs * num_kv_heads * row_tiles);
+size_t window_grad_ws_bytes(const WindowArgs& a) {
+  const int64_t row_tiles = ((int64_t)a.max_query * (a.num_heads / a.num_kv_heads) + kGradTile - 1) / kGradTile;
+  const DkvPlan p = plan_dkv(a, cu_count());
+  const size_t pairs = (size_t)a.num_seqs * a.num_kv_heads;
+  return sizeof(float) * (grad_rows(a.total_rows, a.num_heads) + grad_rows(pairs, row_tiles) +
+                          (p.joined() ? pairs * p.items() * kGradTile * 2 * a.head_size : 0));
 }
 #endif
 

@@ -46,7 +46,8 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   constexpr int NB = BS == 0 ? 1 : kBk / BS;  // blocks of a step
   constexpr int STEPS = 64 / NB;              // steps whose block addresses the lanes hold
   constexpr int SUB = HS * 64;                // bytes of 32 tokens' keys (or values)
-  constexpr int STAGE = 4 * SUB;              // keys of 64 tokens, then their values
+  constexpr int HALF = BS == 0 ? row_at<HS>(kBk) : 2 * SUB;
+  constexpr int STAGE = 2 * HALF;             // keys of 64 tokens, then their values
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
 
   if constexpr (BS == 0)
@@ -112,8 +113,8 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
         const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
         const int64_t token = q0 + min(t + r, cap - 1);
         const size_t col = (size_t)kvh * HS + at * 8;
-        copy16(a.k + token * a.k_stride + col, dst + ch * 1024);
-        copy16(a.v + token * a.v_stride + col, dst + 2 * SUB + ch * 1024);
+        copy16(a.k + token * a.k_stride + col, dst + chunk_at<HS>(ch));
+        copy16(a.v + token * a.v_stride + col, dst + HALF + chunk_at<HS>(ch));
       }
     } else {
       if ((s - s0) % STEPS == 0) fetch(s);
@@ -130,28 +131,28 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
           const uint64_t kb = block_of(kp, l0 + sub), vb = block_of(vp, l0 + sub);
           if (kb != 0) {
             copy16((const void*)(kb + u * 16), dst + ch * 1024);
-            copy16((const void*)(vb + d * 64 + at * 16), dst + 2 * SUB + ch * 1024);
+            copy16((const void*)(vb + d * 64 + at * 16), dst + HALF + ch * 1024);
           }
         } else {
           const uint64_t ka = block_of(kp, l0 + 2 * sub), kb = block_of(kp, l0 + 2 * sub + 1);
           const uint64_t va = block_of(vp, l0 + 2 * sub), vb = block_of(vp, l0 + 2 * sub + 1);
           const uint64_t k = u & 16 ? kb : ka, v = at & 2 ? vb : va;
           if (k != 0) copy16((const void*)(k + (u >> 5) * 256 + (u & 15) * 16), dst + ch * 1024);
-          if (v != 0) copy16((const void*)(v + d * 32 + (at & 1) * 16), dst + 2 * SUB + ch * 1024);
+          if (v != 0) copy16((const void*)(v + d * 32 + (at & 1) * 16), dst + HALF + ch * 1024);
         }
       }
     }
   };
   auto key = [&](const unsigned char* st, int sub, int kk) {
-    if constexpr (BS == 0) return row_unit<HS>(st, 32 * sub + row_token(c), 2 * kk + half);
+    if constexpr (BS == 0) return row_unit<HS>(st + row_at<HS>(32 * sub), row_token(c), 2 * kk + half);
     else return *(const h8*)(st + sub * SUB + ((2 * kk + half) * 32 + row_token(c)) * 16);
   };
   auto value = [&](const unsigned char* st, int sub, int d, int s) {
     if constexpr (BS == 0) {
-      return column_unit<HS>(st + 2 * SUB, 32 * sub + 16 * s, d);
+      return column_unit<HS>(st + HALF, 32 * sub + 16 * s, d);
     } else {
       const int dim = VTAIL ? min(32 * d + c, HS - 1) : 32 * d + c;
-      return *(const h8*)(st + 2 * SUB + sub * SUB + dim * 64 + (((2 * s + half) ^ ((dim >> 2) & 3)) << 4));
+      return *(const h8*)(st + HALF + sub * SUB + dim * 64 + (((2 * s + half) ^ ((dim >> 2) & 3)) << 4));
     }
   };
 
@@ -339,9 +340,10 @@ template <int HS, int BS, bool BF>
 hipError_t launch_tile_bs(const WindowArgs& a, const WindowPlan& p, float* ws, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   auto kern = &window_tile_kernel<HS, BS, BF>;
-  const hipError_t e = allow_lds(reinterpret_cast<const void*>(kern), win_tile_smem(HS), done);
+  constexpr size_t smem = BS == 0 ? 4 * row_at<HS>(kBk) : 4 * kBk * HS * 2;
+  const hipError_t e = allow_lds(reinterpret_cast<const void*>(kern), smem, done);
   if (e != hipSuccess) return e;
-  kern<<<win_grid(a.num_seqs * a.num_kv_heads, p.tiles * p.splits), 256, win_tile_smem(HS), stream>>>(
+  kern<<<win_grid(a.num_seqs * a.num_kv_heads, p.tiles * p.splits), 256, smem, stream>>>(
       a, p.tiles, p.splits, ws, ws + 2 * (size_t)a.total_rows * a.num_heads * p.splits);
   return hipGetLastError();
 }

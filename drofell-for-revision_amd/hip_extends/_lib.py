@@ -138,7 +138,7 @@ SIGNATURES = {
                                             + [_P, _c.c_int64] * 4
                                             + [_P, _c.c_int, _c.c_int, _c.c_float, _c.c_int,
                                                _c.c_int, _P, _c.c_size_t, _P]),
-    "dw4_window_attention_dense_backward_workspace_size": (_c.c_int, [_c.c_int] * 5 + [_SZ]),
+    "dw4_window_attention_dense_backward_workspace_size": (_c.c_int, [_c.c_int] * 8 + [_SZ]),
     "dw4_blocks_workspace_size": (_c.c_int, [_c.c_int, _c.c_int, _SZ]),
     "dw4_copy_blocks": (_c.c_int, [_c.c_int, _P, _P, _c.c_int, _c.c_int64, _c.c_int, _P, _P]),
     "dw4_extend_blocks": (_c.c_int, [_c.c_int] * 4 + [_P] * 9 + [_c.c_size_t, _P]),
@@ -315,12 +315,17 @@ def window_attention_workspace_size(num_seqs: int, num_heads: int, num_kv_heads:
     return out.value
 
 
+@functools.lru_cache(maxsize=4096)
 def window_attention_backward_workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int,
-                                             total_rows: int, max_seq_len: int) -> int:
+                                             head_size: int, total_rows: int, max_seq_len: int,
+                                             window: int, sinks: int,
+                                             device: Optional[int] = None) -> int:
+    """Bytes of one such dw4_window_attention_dense_backward call on the current
+    device (``device``, its index, only tells several devices' sizes apart)."""
     out = ctypes.c_size_t(0)
     fn = "dw4_window_attention_dense_backward_workspace_size"
-    check(fn, getattr(load(), fn)(num_seqs, num_heads, num_kv_heads, total_rows, max_seq_len,
-                                  ctypes.byref(out)))
+    check(fn, getattr(load(), fn)(num_seqs, num_heads, num_kv_heads, head_size, total_rows,
+                                  max_seq_len, window, sinks, ctypes.byref(out)))
     return out.value
 
 

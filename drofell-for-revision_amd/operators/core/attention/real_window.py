@@ -215,7 +215,8 @@ class _WindowDense(torch.autograd.Function):
             do = _rows(dout)
             dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
             shape = _WindowDense._shape(att, q, starts)
-            nbytes = _lib.window_attention_backward_workspace_size(*shape[1:4], q.shape[0], ctx.seq_len_max)
+            nbytes = _lib.window_attention_backward_workspace_size(
+                *shape[1:], q.shape[0], ctx.seq_len_max, att._window, att._sinks, device.index)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
             _lib.call("dw4_window_attention_dense_backward", *shape, q.data_ptr(), _stride(q),
                       k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), out.data_ptr(), _stride(out),

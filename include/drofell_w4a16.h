@@ -548,8 +548,8 @@ int dw4_window_attention_dense_backward(int dtype, int num_seqs, int num_heads, 
                                         float scale, int window, int sinks, void* workspace,
                                         size_t workspace_bytes, void* stream);
 int dw4_window_attention_dense_backward_workspace_size(int num_seqs, int num_heads, int num_kv_heads,
-                                                       int total_rows, int max_seq_len,
-                                                       size_t* workspace_bytes);
+                                                       int head_size, int total_rows, int max_seq_len,
+                                                       int window, int sinks, size_t* workspace_bytes);
 
 /* ---------------------------------------------------------------------------
  * Cache-block pool: the blocks of a paged cache given to rows, shared, copied,

@@ -320,6 +320,7 @@ TRAIN = [
     ([260], 12, 1, 64, 33, 140),      # sinks over more than a tile of tokens
     ([150, 33], 2, 1, 256, 70, 2),
     ([400], 24, 2, 64, 100000, 1),
+    ([2000, 30], 2, 1, 64, 40, 5),    # the sinks' rows, far beyond a window's, in parts
 ]
 
 

@@ -199,6 +199,18 @@ __device__ __forceinline__ void copy16(const void* g, uint32_t lds) {
 __device__ __forceinline__ void copy4(const void* g, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory");
 }
+// The same from a wave-uniform address and an offset per lane, whose 64-bit
+// sum then takes no vector ALU.
+__device__ __forceinline__ void copy16(uint64_t g, uint32_t lane_offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               ::"v"(lane_offset), "s"(g), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void copy4(uint64_t g, uint32_t lane_offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+               ::"v"(lane_offset), "s"(g), "s"(lds) : "memory");
+}
+// Rows at most so far apart (elements) that 128 of them lie within 32-bit offsets.
+constexpr int64_t kNearRows = 1 << 23;
 // Every copy of this workgroup has landed and every wave has left the stage before.
 __device__ __forceinline__ void wait_copies() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -214,6 +226,7 @@ template <int N, int AHEAD, typename Load, typename Use>
 __device__ __forceinline__ void feed(Load&& load, Use&& use) {
   constexpr int kMoves = 0x2 | 0x4 | 0x400;  // vector ALU, scalar ALU, transcendental
   decltype(load(0)) f[N];
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int i = 0; i < (AHEAD < N ? AHEAD : N); ++i) f[i] = load(i);
   __builtin_amdgcn_sched_barrier(kMoves);
@@ -224,6 +237,7 @@ __device__ __forceinline__ void feed(Load&& load, Use&& use) {
     use(i, f[i]);
     __builtin_amdgcn_sched_barrier(kMoves);
   }
+  __builtin_amdgcn_s_setprio(0);
 }
 
 // Row-major tiles in LDS ([row][HS], as the tensors have them), laid out so that

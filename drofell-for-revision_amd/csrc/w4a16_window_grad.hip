@@ -109,10 +109,23 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
   const int token = q0 + pos, head = kvh * G + row % G;
 
   const uint32_t lds0 = lds_offset(lds);
+  const bool near = a.k_stride <= kNearRows && a.v_stride <= kNearRows;
   auto issue = [&](int s, int stage) {
     const uint32_t dst = lds0 + stage * STAGE;
     const int t = span.token<kBk>(s);
     constexpr int UNITS = HS / 8, CHUNKS = kBk * UNITS / 64;
+    if (near && t + kBk <= n) {
+      const size_t col = (size_t)kvh * HS;
+      const uint64_t kb = (uint64_t)(a.k + (size_t)(q0 + t) * a.k_stride + col);
+      const uint64_t vb = (uint64_t)(a.v + (size_t)(q0 + t) * a.v_stride + col);
+      for (int ch = wave; ch < CHUNKS; ch += 4) {
+        const int u = ch * 64 + lane;
+        const uint32_t r = u / UNITS, at = ((u % UNITS) ^ swizzle<HS>(r)) * 16;
+        copy16(kb, r * (uint32_t)(a.k_stride * 2) + at, dst + chunk_at<HS>(ch));
+        copy16(vb, r * (uint32_t)(a.v_stride * 2) + at, dst + TILE + chunk_at<HS>(ch));
+      }
+      return;
+    }
     for (int ch = wave; ch < CHUNKS; ch += 4) {
       const int u = ch * 64 + lane;
       const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
@@ -260,9 +273,31 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
 
   const uint32_t lds0 = lds_offset(lds);
   constexpr int UNITS = HS / 8;
+  const int log_g = 31 - __builtin_clz(G);
+  const bool near = kDkvRows % G == 0 && a.q_stride <= kNearRows && g.do_stride <= kNearRows;
   auto issue = [&](int s, int stage) {
     const uint32_t dst = lds0 + stage * STAGE;
     constexpr int CHUNKS = kDkvRows * UNITS / 64;
+    if (near && r0 + (s + 1) * kDkvRows <= r1) {  // whole tokens' rows: G divides the step's
+      const int first = t0 + ((s * kDkvRows) >> log_g);
+      const size_t col = (size_t)kvh * G * HS;
+      const uint64_t qb = (uint64_t)(a.q + (size_t)(q0 + first) * a.q_stride + col);
+      const uint64_t ob = (uint64_t)(g.dout + (size_t)(q0 + first) * g.do_stride + col);
+      for (int ch = wave; ch < CHUNKS; ch += 4) {
+        const int u = ch * 64 + lane;
+        const uint32_t r = u / UNITS, at = ((u % UNITS) ^ swizzle<HS>(r)) * 16 + (r & (G - 1)) * (HS * 2);
+        copy16(qb, (r >> log_g) * (uint32_t)(a.q_stride * 2) + at, dst + chunk_at<HS>(ch));
+        copy16(ob, (r >> log_g) * (uint32_t)(g.do_stride * 2) + at, dst + TILE + chunk_at<HS>(ch));
+      }
+      if (wave < 3 && lane < kDkvRows) {
+        const size_t at = (size_t)(q0 + first) * a.num_heads + kvh * G;
+        const uint32_t off = ((lane >> log_g) * a.num_heads + (lane & (G - 1))) * 4;
+        if (wave == 0) copy4((uint64_t)(a.lse + at), off, dst + 2 * TILE);
+        else if (wave == 1) copy4((uint64_t)(delta + at), off, dst + 2 * TILE + kDkvRows * 4);
+        else *(int*)(lds + stage * STAGE + 2 * TILE + 2 * kDkvRows * 4 + lane * 4) = first + (lane >> log_g);
+      }
+      return;
+    }
     for (int ch = wave; ch < CHUNKS; ch += 4) {
       const int u = ch * 64 + lane;
       const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);

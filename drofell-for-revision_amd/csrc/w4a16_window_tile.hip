@@ -9,9 +9,8 @@
 // Scores are formed transposed, S^T = K Q^T, so that a row's scores lie in one
 // lane pair, and the probabilities are the B operand of O^T = V^T P^T as they
 // stand (w4a16_window_device.h).
-//   * cache blocks lie in LDS as in memory, keys [dims / 8][32 tokens][8], values
-//     [dims][32 tokens] with the four 16-byte units of a row rotated against
-//     bank conflicts;
+//   * cache blocks lie in LDS as in memory, those of 32 tokens with the four
+//     16-byte units of a dim's values rotated against bank conflicts;
 //   * token rows lie as [token][dims], and values reach the second product
 //     through LDS's transposing reads.
 // Matrix-core and vector-ALU bound.  Probabilities enter p . v rounded to the
@@ -45,8 +44,8 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   constexpr bool VTAIL = HS % 32 != 0;
   constexpr int NB = BS == 0 ? 1 : kBk / BS;  // blocks of a step
   constexpr int STEPS = 64 / NB;              // steps whose block addresses the lanes hold
-  constexpr int SUB = HS * 64;                // bytes of 32 tokens' keys (or values)
-  constexpr int HALF = BS == 0 ? row_at<HS>(kBk) : 2 * SUB;
+  constexpr int BB = HS * BS * 2;             // bytes of a block's keys (or values)
+  constexpr int HALF = BS == 0 ? row_at<HS>(kBk) : kBk * HS * 2;
   constexpr int STAGE = 2 * HALF;             // keys of 64 tokens, then their values
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
 
@@ -83,6 +82,7 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   const int wfirst = p0 + min(wbase, rows - 1) / G, wlast = p0 + min(wbase + 31, rows - 1) / G;
 
   // ---- the copies of one step into a stage
+  const bool near = a.k_stride <= kNearRows && a.v_stride <= kNearRows;
   uint64_t kp = 0, vp = 0;  // lane l: block l % NB of step l / NB (of STEPS), 0: not in the table
   auto fetch = [&](int s) {
     kp = vp = 0;
@@ -108,13 +108,25 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
     if constexpr (BS == 0) {
       const int t = span.token<kBk>(s);
       constexpr int UNITS = HS / 8, CHUNKS = kBk * UNITS / 64;
-      for (int ch = wave; ch < CHUNKS; ch += 4) {
-        const int u = ch * 64 + lane;
-        const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
-        const int64_t token = q0 + min(t + r, cap - 1);
-        const size_t col = (size_t)kvh * HS + at * 8;
-        copy16(a.k + token * a.k_stride + col, dst + chunk_at<HS>(ch));
-        copy16(a.v + token * a.v_stride + col, dst + HALF + chunk_at<HS>(ch));
+      if (near && t + kBk <= cap) {
+        const size_t col = (size_t)kvh * HS;
+        const uint64_t kb = (uint64_t)(a.k + (size_t)(q0 + t) * a.k_stride + col);
+        const uint64_t vb = (uint64_t)(a.v + (size_t)(q0 + t) * a.v_stride + col);
+        for (int ch = wave; ch < CHUNKS; ch += 4) {
+          const int u = ch * 64 + lane;
+          const uint32_t r = u / UNITS, at = ((u % UNITS) ^ swizzle<HS>(r)) * 16;
+          copy16(kb, r * (uint32_t)(a.k_stride * 2) + at, dst + chunk_at<HS>(ch));
+          copy16(vb, r * (uint32_t)(a.v_stride * 2) + at, dst + HALF + chunk_at<HS>(ch));
+        }
+      } else {
+        for (int ch = wave; ch < CHUNKS; ch += 4) {
+          const int u = ch * 64 + lane;
+          const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
+          const int64_t token = q0 + min(t + r, cap - 1);
+          const size_t col = (size_t)kvh * HS + at * 8;
+          copy16(a.k + token * a.k_stride + col, dst + chunk_at<HS>(ch));
+          copy16(a.v + token * a.v_stride + col, dst + HALF + chunk_at<HS>(ch));
+        }
       }
     } else {
       if ((s - s0) % STEPS == 0) fetch(s);
@@ -123,37 +135,30 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
 #pragma unroll
       for (int b = 0; b < NB; ++b) there |= (uint32_t)(block_of(kp, l0 + b) != 0) << b;
       held[stage] = there;
-      constexpr int CHUNKS = SUB / 1024;  // of 64 units, per 32 tokens
-      for (int ch = wave; ch < 2 * CHUNKS; ch += 4) {
-        const int sub = ch / CHUNKS, u = ch % CHUNKS * 64 + lane;
-        const int d = u >> 2, at = (u & 3) ^ ((d >> 2) & 3);  // value row and unit
-        if constexpr (BS == 32) {
-          const uint64_t kb = block_of(kp, l0 + sub), vb = block_of(vp, l0 + sub);
-          if (kb != 0) {
-            copy16((const void*)(kb + u * 16), dst + ch * 1024);
-            copy16((const void*)(vb + d * 64 + at * 16), dst + HALF + ch * 1024);
-          }
-        } else {
-          const uint64_t ka = block_of(kp, l0 + 2 * sub), kb = block_of(kp, l0 + 2 * sub + 1);
-          const uint64_t va = block_of(vp, l0 + 2 * sub), vb = block_of(vp, l0 + 2 * sub + 1);
-          const uint64_t k = u & 16 ? kb : ka, v = at & 2 ? vb : va;
-          if (k != 0) copy16((const void*)(k + (u >> 5) * 256 + (u & 15) * 16), dst + ch * 1024);
-          if (v != 0) copy16((const void*)(v + d * 32 + (at & 1) * 16), dst + HALF + ch * 1024);
-        }
+      // a block's keys as they lie; its values too, for 32-token blocks with the
+      // four 16-byte units of a row rotated by dim / 4 (mod 4)
+      constexpr int CHUNKS = (BB + 1023) / 1024;
+      const uint32_t koff = lane * 16;
+      const uint32_t voff = BS == 32 ? (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) * 16) : lane * 16;
+      for (int it = wave; it < NB * CHUNKS; it += 4) {
+        const int b = it / CHUNKS, at = it % CHUNKS * 1024;
+        const uint64_t kb = block_of(kp, l0 + b), vb = block_of(vp, l0 + b);
+        if (kb == 0 || (BB % 1024 != 0 && at + (int)koff >= BB)) continue;
+        copy16(kb + at, koff, dst + b * BB + at);
+        copy16(vb + at, voff, dst + HALF + b * BB + at);
       }
     }
   };
   auto key = [&](const unsigned char* st, int sub, int kk) {
-    if constexpr (BS == 0) return row_unit<HS>(st + row_at<HS>(32 * sub), row_token(c), 2 * kk + half);
-    else return *(const h8*)(st + sub * SUB + ((2 * kk + half) * 32 + row_token(c)) * 16);
+    const int t = row_token(c);  // of the 32 tokens `sub`
+    if constexpr (BS == 0) return row_unit<HS>(st + row_at<HS>(32 * sub), t, 2 * kk + half);
+    else return *(const h8*)(st + 32 / (BS + !BS) * sub * BB + t / (BS + !BS) * BB + ((2 * kk + half) * BS + t % (BS + !BS)) * 16);
   };
   auto value = [&](const unsigned char* st, int sub, int d, int s) {
-    if constexpr (BS == 0) {
-      return column_unit<HS>(st + HALF, 32 * sub + 16 * s, d);
-    } else {
-      const int dim = VTAIL ? min(32 * d + c, HS - 1) : 32 * d + c;
-      return *(const h8*)(st + HALF + sub * SUB + dim * 64 + (((2 * s + half) ^ ((dim >> 2) & 3)) << 4));
-    }
+    const int dim = VTAIL ? min(32 * d + c, HS - 1) : 32 * d + c;
+    if constexpr (BS == 0) return column_unit<HS>(st + HALF, 32 * sub + 16 * s, d);
+    else if constexpr (BS == 16) return *(const h8*)(st + HALF + (2 * sub + s) * BB + dim * 32 + half * 16);
+    else return *(const h8*)(st + HALF + sub * BB + dim * 64 + (((2 * s + half) ^ ((dim >> 2) & 3)) << 4));
   };
 
   if (s0 < s1) issue(s0, 0);
@@ -263,12 +268,13 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
             if (count[e] > 0.f) o[d][e] += inf;
         }
       }
+#pragma unroll
+      for (int i = 0; i < 4 * ND; ++i)
+        o[i % ND] = mfma32_of<BF>(finite_part<BF>(value(st, i / (2 * ND), i % ND, i / ND % 2)), p[i / (2 * ND)][i / ND % 2], o[i % ND]);
+      return;
     }
     feed<4 * ND, 8>([&](int i) { return value(st, i / (2 * ND), i % ND, i / ND % 2); },
-                    [&](int i, h8 f) {
-                      if (odd) f = finite_part<BF>(f);
-                      o[i % ND] = mfma32_of<BF>(f, p[i / (2 * ND)][i / ND % 2], o[i % ND]);
-                    });
+                    [&](int i, h8 f) { o[i % ND] = mfma32_of<BF>(f, p[i / (2 * ND)][i / ND % 2], o[i % ND]); });
   };
   int stage = 0, step = s0;
   auto begin = [&]() {

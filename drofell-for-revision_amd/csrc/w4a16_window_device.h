@@ -226,7 +226,6 @@ template <int N, int AHEAD, typename Load, typename Use>
 __device__ __forceinline__ void feed(Load&& load, Use&& use) {
   constexpr int kMoves = 0x2 | 0x4 | 0x400;  // vector ALU, scalar ALU, transcendental
   decltype(load(0)) f[N];
-  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int i = 0; i < (AHEAD < N ? AHEAD : N); ++i) f[i] = load(i);
   __builtin_amdgcn_sched_barrier(kMoves);
@@ -237,7 +236,6 @@ __device__ __forceinline__ void feed(Load&& load, Use&& use) {
     use(i, f[i]);
     __builtin_amdgcn_sched_barrier(kMoves);
   }
-  __builtin_amdgcn_s_setprio(0);
 }
 
 // Row-major tiles in LDS ([row][HS], as the tensors have them), laid out so that

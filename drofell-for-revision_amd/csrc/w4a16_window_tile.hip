@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #include "w4a16_device.h"
 #include "w4a16_window.h"
@@ -103,50 +104,78 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   };
   uint32_t held[2] = {(1u << NB) - 1, (1u << NB) - 1};  // by stage: the blocks that are there
   const uint32_t lds0 = lds_offset(lds);
-  auto issue = [&](int s, int stage) {
-    const uint32_t dst = lds0 + stage * STAGE;
+  // A step's copies are PARTS per wave, keys and values in turn (part()), from
+  // addresses that next_step() sets; steps with missing blocks and the last tokens of
+  // a sequence, which need a bound each, go as a whole (slowly()).
+  constexpr int UNITS = HS / 8, CHUNKS = BS == 0 ? kBk * UNITS / 64 : (BB + 1023) / 1024;
+  constexpr int ITEMS = BS == 0 ? CHUNKS : NB * CHUNKS, PARTS = (ITEMS + 3) / 4 * 2;
+  uint64_t next_k = 0, next_v = 0;  // token rows: their addresses
+  int next_l = 0;                   // blocks: the lane that holds the first one's
+  uint32_t next_dst = 0;
+  auto next_step = [&](int s, int stage) {  // false: slowly()
+    next_dst = lds0 + stage * STAGE;
     if constexpr (BS == 0) {
       const int t = span.token<kBk>(s);
-      constexpr int UNITS = HS / 8, CHUNKS = kBk * UNITS / 64;
-      if (near && t + kBk <= cap) {
-        const size_t col = (size_t)kvh * HS;
-        const uint64_t kb = (uint64_t)(a.k + (size_t)(q0 + t) * a.k_stride + col);
-        const uint64_t vb = (uint64_t)(a.v + (size_t)(q0 + t) * a.v_stride + col);
-        for (int ch = wave; ch < CHUNKS; ch += 4) {
-          const int u = ch * 64 + lane;
-          const uint32_t r = u / UNITS, at = ((u % UNITS) ^ swizzle<HS>(r)) * 16;
-          copy16(kb, r * (uint32_t)(a.k_stride * 2) + at, dst + chunk_at<HS>(ch));
-          copy16(vb, r * (uint32_t)(a.v_stride * 2) + at, dst + HALF + chunk_at<HS>(ch));
-        }
-      } else {
-        for (int ch = wave; ch < CHUNKS; ch += 4) {
-          const int u = ch * 64 + lane;
-          const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
-          const int64_t token = q0 + min(t + r, cap - 1);
-          const size_t col = (size_t)kvh * HS + at * 8;
-          copy16(a.k + token * a.k_stride + col, dst + chunk_at<HS>(ch));
-          copy16(a.v + token * a.v_stride + col, dst + HALF + chunk_at<HS>(ch));
-        }
-      }
+      if (!near || t + kBk > cap) return false;
+      const size_t col = (size_t)kvh * HS;
+      next_k = (uint64_t)(a.k + (size_t)(q0 + t) * a.k_stride + col);
+      next_v = (uint64_t)(a.v + (size_t)(q0 + t) * a.v_stride + col);
     } else {
-      if ((s - s0) % STEPS == 0) fetch(s);
-      const int l0 = (s - s0) % STEPS * NB;
+      if ((s - s0) % STEPS == 0) {
+        fetch(s);
+        wait_loads();
+      }
+      next_l = (s - s0) % STEPS * NB;
       uint32_t there = 0;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) there |= (uint32_t)(block_of(kp, l0 + b) != 0) << b;
+      for (int b = 0; b < NB; ++b) there |= (uint32_t)(block_of(kp, next_l + b) != 0) << b;
       held[stage] = there;
+      return there == (1u << NB) - 1;
+    }
+    return true;
+  };
+  auto part = [&](int i, auto all) {  // all: no block of the step is missing
+    const int it = wave + 4 * (i >> 1);
+    const bool values = i & 1;
+    if (ITEMS % 4 != 0 && it >= ITEMS) return;
+    if constexpr (BS == 0) {
+      const int u = it * 64 + lane;
+      const uint32_t r = u / UNITS, at = ((u % UNITS) ^ swizzle<HS>(r)) * 16;
+      if (values) copy16(next_v, r * (uint32_t)(a.v_stride * 2) + at, next_dst + HALF + chunk_at<HS>(it));
+      else copy16(next_k, r * (uint32_t)(a.k_stride * 2) + at, next_dst + chunk_at<HS>(it));
+    } else {
       // a block's keys as they lie; its values too, for 32-token blocks with the
       // four 16-byte units of a row rotated by dim / 4 (mod 4)
-      constexpr int CHUNKS = (BB + 1023) / 1024;
-      const uint32_t koff = lane * 16;
-      const uint32_t voff = BS == 32 ? (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) * 16) : lane * 16;
-      for (int it = wave; it < NB * CHUNKS; it += 4) {
-        const int b = it / CHUNKS, at = it % CHUNKS * 1024;
-        const uint64_t kb = block_of(kp, l0 + b), vb = block_of(vp, l0 + b);
-        if (kb == 0 || (BB % 1024 != 0 && at + (int)koff >= BB)) continue;
-        copy16(kb + at, koff, dst + b * BB + at);
-        copy16(vb + at, voff, dst + HALF + b * BB + at);
-      }
+      const int b = it / CHUNKS, at = it % CHUNKS * 1024;
+      const uint64_t p = block_of(values ? vp : kp, next_l + b);
+      if (!decltype(all)::value && p == 0) return;
+      if (BB % 1024 != 0 && at + lane * 16 >= BB) return;
+      const uint32_t off = BS == 32 && values ? (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) * 16) : lane * 16;
+      copy16(p + at, off, next_dst + (values ? HALF : 0) + b * BB + at);
+    }
+  };
+  auto slowly = [&](int s) {
+    if constexpr (BS != 0) {
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) part(i, std::false_type{});
+      return;
+    }
+    const int t = span.token<kBk>(s);
+    for (int ch = wave; ch < CHUNKS; ch += 4) {
+      const int u = ch * 64 + lane;
+      const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
+      const int64_t token = q0 + min(t + r, cap - 1);
+      const size_t col = (size_t)kvh * HS + at * 8;
+      copy16(a.k + token * a.k_stride + col, next_dst + chunk_at<HS>(ch));
+      copy16(a.v + token * a.v_stride + col, next_dst + HALF + chunk_at<HS>(ch));
+    }
+  };
+  auto issue = [&](int s, int stage) {
+    if (next_step(s, stage)) {
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) part(i, std::true_type{});
+    } else {
+      slowly(s);
     }
   };
   auto key = [&](const unsigned char* st, int sub, int kk) {
@@ -185,9 +214,18 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
       f1 = span.sink_steps + most / kBk + 1;
     }
   }
-  auto scores = [&](const unsigned char* st, f16v (&s)[2]) {
+  // with `copies`, the next step's go out among the products: at once they would
+  // hold up the wave until the memory pipeline has taken them all
+  auto scores = [&](const unsigned char* st, f16v (&s)[2], auto copies) {
+    constexpr bool kCopies = decltype(copies)::value;
     feed<2 * KD, 8>([&](int i) { return key(st, i & 1, i >> 1); },
-                    [&](int i, h8 f) { s[i & 1] = mfma32_of<BF>(f, qreg[i >> 1], s[i & 1]); });
+                    [&](int i, h8 f) {
+                      s[i & 1] = mfma32_of<BF>(f, qreg[i >> 1], s[i & 1]);
+                      if constexpr (kCopies) {
+#pragma unroll
+                        for (int c = i * PARTS / (2 * KD); c < (i + 1) * PARTS / (2 * KD); ++c) part(c, std::true_type{});
+                      }
+                    });
   };
   // the running maximum (it may lag kLag behind), and the probabilities
   auto probabilities = [&](f16v (&s)[2], h8 (&p)[2][2]) {
@@ -220,11 +258,12 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
         p[b][g] = __builtin_bit_cast(h8, x);
       }
   };
-  auto whole = [&](int stage) {  // a step that every row sees
+  auto whole = [&](int stage, bool more) {  // a step that every row sees
     const unsigned char* st = lds + stage * STAGE;
     f16v s[2] = {f16v{}, f16v{}};
     h8 p[2][2];
-    scores(st, s);
+    if (more) scores(st, s, std::true_type{});
+    else scores(st, s, std::false_type{});
     probabilities(s, p);
     feed<4 * ND, 8>(
         [&](int i) { return value(st, i / (2 * ND), i % ND, i / ND % 2); },
@@ -244,7 +283,7 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
     }
     f16v s[2] = {f16v{}, f16v{}};
     h8 p[2][2];
-    scores(st, s);
+    scores(st, s, std::false_type{});
 #pragma unroll
     for (int x = 0; x < 32; ++x) s[x >> 4][x & 15] = where_seen(seen, x, s[x >> 4][x & 15], -INFINITY);
     probabilities(s, p);
@@ -277,22 +316,19 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
                     [&](int i, h8 f) { o[i % ND] = mfma32_of<BF>(f, p[i / (2 * ND)][i / ND % 2], o[i % ND]); });
   };
   int stage = 0, step = s0;
-  auto begin = [&]() {
-    wait_copies();
-    if (step + 1 < s1) issue(step + 1, stage ^ 1);
-  };
   auto is_whole = [&]() { return step >= f0 && step < f1 && held[stage] == (1u << NB) - 1; };
   while (step < s1) {
-    begin();
-    if (is_whole()) {
-      do {
-        whole(stage);
-        stage ^= 1;
-        if (++step == s1) break;
-        begin();
-      } while (is_whole());
-      if (step == s1) break;
+    wait_copies();
+    while (is_whole()) {
+      const bool more = step + 1 < s1, parts = more && next_step(step + 1, stage ^ 1);
+      if (more && !parts) slowly(step + 1);
+      whole(stage, parts);
+      stage ^= 1;
+      if (++step == s1) break;
+      wait_copies();
     }
+    if (step == s1) break;
+    if (step + 1 < s1) issue(step + 1, stage ^ 1);
     masked(step, stage);
     stage ^= 1;
     ++step;

@@ -9,8 +9,8 @@
 // order of rows; counts are integer sums.
 //
 // Each of extend, fork and compact is two launches.  In the first, one workgroup of
-// 1024 threads reads the counts (each thread a run of them, one scan over the
-// threads' sums) and lists the blocks to hand out or to move, while others copy
+// 1024 threads reads the counts (each wave a run of them, ranks by ballot after one
+// scan over the waves' sums) and lists the blocks to hand out or to move, while others copy
 // the state's unchanged parts.  The second applies the lists to the tables and counts
 // and, where blocks' contents move, copies them in every layer: 16-byte units,
 // 16 KiB of one block at a time per workgroup, as many workgroups as stay
@@ -60,11 +60,50 @@ __device__ __forceinline__ int up(int64_t tokens, int bs) { return (int)min<int6
 
 __device__ __forceinline__ bool is_block(const PoolArgs& a, int e) { return e >= 0 && e < a.num_blocks; }
 
-// The blocks of the thread's run of counts.
-__device__ __forceinline__ void run_of(int n, int& from, int& to) {
-  const int per = (n + kPlanThreads - 1) / kPlanThreads;
-  from = min((int)threadIdx.x * per, n);
-  to = min(from + per, n);
+// The counts in ascending order of blocks: each wave takes one run of them, 256 at
+// a time; f(first, counts, which): lane l has the counts of blocks first + l + 64 e, e
+// = 0 .. 3, and bit e of `which` says that there is such a block.
+template <typename F>
+__device__ __forceinline__ void sweep(const int32_t* __restrict__ refs, int n, F&& f) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int run = (n + 256 * (kPlanThreads / 64) - 1) / (256 * (kPlanThreads / 64)) * 256;
+  const int to = min(n, (wave + 1) * run);
+#pragma unroll 4
+  for (int p = wave * run; p < to; p += 256) {
+    int v[4], which = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = p + 64 * e + lane;
+      which |= (at < to) << e;
+      v[e] = at < to ? refs[at] : 0;
+    }
+    f(p, v, which);
+  }
+}
+// How many blocks of the pool are free (LIVE: held), and of those before the wave's run.
+template <bool LIVE>
+__device__ __forceinline__ int64_t count_blocks(const int32_t* __restrict__ refs, int n, int64_t* tmp, int64_t& total) {
+  int64_t own = 0;
+  sweep(refs, n, [&](int, const int (&v)[4], int which) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own += (which >> e & 1) && (LIVE ? v[e] > 0 : v[e] == 0);
+  });
+  const int64_t before = scan(own, tmp, total);
+  return __shfl(before, 0);  // of the wave's first lane
+}
+// f(rank, block) of every free (LIVE: held) block, by its rank among them.
+template <bool LIVE, typename F>
+__device__ __forceinline__ void rank_blocks(const int32_t* __restrict__ refs, int n, int64_t before, F&& f) {
+  const int lane = threadIdx.x & 63;
+  sweep(refs, n, [&](int p, const int (&v)[4], int which) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool in = (which >> e & 1) && (LIVE ? v[e] > 0 : v[e] == 0);
+      const uint64_t all = __ballot(in);
+      if (in) f(before + __popcll(all & ((1ull << lane) - 1)), p + 64 * e + lane);
+      before += __popcll(all);
+    }
+  });
 }
 
 // The workgroups beside the planning one copy n ints.
@@ -138,13 +177,11 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(PoolArgs a) {
   }
   scan(wide, tmp, total);
   const int64_t beyond = total;
-  int from, to;
-  run_of(a.num_blocks, from, to);
-  int free = 0;
-  for (int p = from; p < to; ++p) free += a.refs[p] == 0;
-  int64_t k = scan(free, tmp, total);
-  for (int p = from; p < to && k < need; ++p)
-    if (a.refs[p] == 0) list[k++] = p;
+  const int64_t before = count_blocks<false>(a.refs, a.num_blocks, tmp, total);
+  if (before < need)
+    rank_blocks<false>(a.refs, a.num_blocks, before, [&](int64_t k, int p) {
+      if (k < need) list[k] = p;
+    });
   if (threadIdx.x == 0) a.shortage[0] = clamp_int(max<int64_t>(need - total, 0) + beyond);
 }
 
@@ -212,20 +249,17 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(PoolArgs a) {
     if (copy) needy[need + before] = r;
     need += total;
   }
-  int from, to;
-  run_of(a.num_blocks, from, to);
-  int free = 0;
-  for (int p = from; p < to; ++p) free += a.refs[p] == 0;
-  int64_t k = scan(free, tmp, total);  // its barriers also publish needy and fresh
-  for (int p = from; p < to && k < need; ++p) {
-    if (a.refs[p] != 0) continue;
-    const int r = needy[k];
-    int at;
-    pairs[2 * k] = last_block(a, parent_of(a, r), at);
-    pairs[2 * k + 1] = p;
-    fresh[r] = p;
-    ++k;
-  }
+  // (its barriers also publish needy and fresh)
+  const int64_t before = count_blocks<false>(a.refs, a.num_blocks, tmp, total);
+  if (before < need)
+    rank_blocks<false>(a.refs, a.num_blocks, before, [&](int64_t k, int p) {
+      if (k >= need) return;
+      const int r = needy[k];
+      int at;
+      pairs[2 * k] = last_block(a, parent_of(a, r), at);
+      pairs[2 * k + 1] = p;
+      fresh[r] = p;
+    });
   if (threadIdx.x == 0) {
     a.shortage[0] = clamp_int(max<int64_t>(need - total, 0));
     a.ws[0] = need > total ? 0 : (int)need;
@@ -288,25 +322,32 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PoolArgs a) 
   __shared__ int64_t tmp[kPlanThreads / 64];
   int32_t* moved = a.ws + kPoolHead;
   int32_t* pairs = moved + a.num_blocks;
-  int from, to;
-  run_of(a.num_blocks, from, to);
-  int alive = 0;
-  for (int p = from; p < to; ++p) alive += a.refs[p] > 0;
-  int64_t live, count;
-  scan(alive, tmp, live);
+  int64_t live, below, count;
+  const int64_t held = count_blocks<true>(a.refs, a.num_blocks, tmp, live);
   // holes below `live` and live blocks from there on: as many of one as of the other
-  int holes = 0, movers = 0;
-  for (int p = from; p < to; ++p) {
-    const bool is_live = a.refs[p] > 0;
-    holes += p < live && !is_live;
-    movers += p >= live && is_live;
-  }
-  int64_t h = scan(holes, tmp, count), m = scan(movers, tmp, count);
-  for (int p = from; p < to; ++p) {
-    const bool is_live = a.refs[p] > 0;
-    if (p < live && !is_live) pairs[2 * h++ + 1] = p;
-    if (p >= live && is_live) pairs[2 * m++] = p;
-  }
+  int64_t own = 0;
+  sweep(a.refs, a.num_blocks, [&](int p, const int (&v)[4], int which) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own += (which >> e & 1) && v[e] > 0 && p + 64 * e + (int)(threadIdx.x & 63) < live;
+  });
+  scan(own, tmp, below);
+  count = live - below;
+  rank_blocks<true>(a.refs, a.num_blocks, held, [&](int64_t k, int p) {
+    if (p >= live) pairs[2 * (k - below)] = p;
+  });
+  // a hole's rank: the blocks before it less the live ones among them
+  const int lane = threadIdx.x & 63;
+  int64_t before = held;
+  sweep(a.refs, a.num_blocks, [&](int p, const int (&v)[4], int which) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool is_live = (which >> e & 1) && v[e] > 0;
+      const uint64_t all = __ballot(is_live);
+      const int64_t at = p + 64 * e + lane;
+      if ((which >> e & 1) && !is_live && at < live) pairs[2 * (at - before - __popcll(all & ((1ull << lane) - 1))) + 1] = (int)at;
+      before += __popcll(all);
+    }
+  });
   __syncthreads();
   for (int64_t k = threadIdx.x; k < count; k += kPlanThreads) {
     moved[pairs[2 * k]] = pairs[2 * k + 1];

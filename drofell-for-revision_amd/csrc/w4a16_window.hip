@@ -392,6 +392,24 @@ static int64_t window_steps(const WindowArgs& a, int max_context, int tile_rows,
   return (span + bk - 1) / bk + (far + bk - 1) / bk;
 }
 
+// Splits over the tokens, for calls that leave CUs without a workgroup; g
+// workgroups without splits, n steps of tokens each.
+//
+// Rows kernel (32-token steps): one 8-wave workgroup per CU, at least 12 steps in a
+// part; not for contexts under 24 steps, nor for two parts unless they are long
+// (160 steps), which the join's launch costs more than it gains.  Measured (us,
+// one part / these / more; heads 32 on 8 unless said): 1 x 300 tokens 6.7 / - / 7.5 (4
+// parts), 1 x 3000 24.8 / 10.2 / 10.5 (16), 1 x 8000 58 / 17.8 / 19 (32), 4 x 3000 28.5
+// / 17.0 / 17.4 (8), 16 x 3000 33.4 / - / 35.0 (2), 16 x 8000 118 / 95 / 98.5 (4), 8 x
+// 600, 32 on 32, 15.8 / - / 22.4 (2).  More workgroups than CUs: four waves each (32 x
+// 128 tokens, 32 on 32, 23.5 with eight, 16.5).
+//
+// Tile kernel (64-token steps): one workgroup per CU, or two where that leaves
+// fewer than four parts of a long context (64 steps), at least three steps in a
+// part and at most 16 parts below 128 steps.  Measured (us, one part / these /
+// twice as many): 16 new tokens over 2000 42 / 14.2 / 18, over 8000 153 / 26.5 /
+// 26.9; 200 over 8000 157 / 53 / 63; 600 over 2000 45 / - / 48.5, over 8000 158 / 107
+// / 118; 4 x 200 over 700 23.5 / - / 38.6, over 8000 160 / 139 / 136.
 WindowPlan plan_window(const WindowArgs& a, int max_context, int cus) {
   WindowPlan p;
   const int G = a.num_heads / a.num_kv_heads;
@@ -400,12 +418,19 @@ WindowPlan plan_window(const WindowArgs& a, int max_context, int cus) {
   p.rows = a.block_size != 0 && most <= kWinRowsTile;
   const int tile_rows = p.rows ? kWinRowsTile : 4 * 32;
   p.tiles = (int)((most + tile_rows - 1) / tile_rows);
-  const int64_t groups = pairs * p.tiles;
-  const int64_t steps = window_steps(a, max_context, tile_rows, p.rows ? kWinRowsTokens : kWinTileTokens);
-  if (a.block_size == 0 || groups >= cus) return p;
-  const int64_t least = p.rows ? 4 : 4;  // steps of a split, at least
-  const int64_t parts = std::min((2 * (int64_t)cus + groups - 1) / groups, (steps + least - 1) / least);
-  p.splits = (int)std::max<int64_t>(1, parts);
+  const int64_t g = pairs * p.tiles;
+  const int64_t n = window_steps(a, max_context, tile_rows, p.rows ? kWinRowsTokens : kWinTileTokens);
+  if (p.rows && a.head_size <= 128 && g <= cus) p.waves = 8;
+  if (a.block_size == 0 || g == 0) return p;
+  int64_t s = cus / g;
+  if (p.rows) {
+    s = std::min(s, (n + 11) / 12);
+    if (n < 24 || (s < 3 && n < 160)) s = 1;
+  } else {
+    if (n >= 64 && s < 4) s = 2 * cus / g;
+    s = std::min({s, (n + 2) / 3, std::max<int64_t>(16, n / 8)});
+  }
+  p.splits = (int)std::max<int64_t>(1, s);
   return p;
 }
 

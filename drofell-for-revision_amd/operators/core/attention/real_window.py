@@ -31,12 +31,15 @@ from .common import AttentionConfig
 _DTYPES = {torch.float16: _lib.DW4_F16, torch.bfloat16: _lib.DW4_BF16}
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """The library launches on the current device."""
     if device.type != "cuda":
         raise ValueError("windowed attention runs on a HIP device")
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index is None or device.index == _lib.current_device():
+        return _HERE
     return torch.cuda.device(device)
 
 
@@ -148,7 +151,7 @@ class WindowAttention:
                       float(self.scale), self._window, self._sinks, tables.data_ptr(),
                       tables.shape[1], lens.data_ptr(), int(context_len_max),
                       None if ws is None else ws.data_ptr(), nbytes,
-                      torch.cuda.current_stream(device).cuda_stream)
+                      _lib.current_stream(device.index))
         return output
 
     def dense(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: torch.Tensor,
@@ -196,7 +199,7 @@ class _WindowDense(torch.autograd.Function):
                       q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v),
                       out.data_ptr(), _stride(out), None if lse is None else lse.data_ptr(),
                       None if rest is None else rest.data_ptr(), starts.data_ptr(), q.shape[0], seq_len_max, float(att.scale), att._window,
-                      att._sinks, torch.cuda.current_stream(device).cuda_stream)
+                      att._sinks, _lib.current_stream(device.index))
         ctx.empty = False
         ctx.att, ctx.seq_len_max = att, seq_len_max
         if need:
@@ -223,5 +226,5 @@ class _WindowDense(torch.autograd.Function):
                       lse.data_ptr(), rest.data_ptr(), do.data_ptr(), _stride(do), dq.data_ptr(), _stride(dq),
                       dk.data_ptr(), _stride(dk), dv.data_ptr(), _stride(dv), starts.data_ptr(),
                       q.shape[0], ctx.seq_len_max, float(att.scale), att._window, att._sinks,
-                      ws.data_ptr(), nbytes, torch.cuda.current_stream(device).cuda_stream)
+                      ws.data_ptr(), nbytes, _lib.current_stream(device.index))
         return dq, dk, dv, None, None, None

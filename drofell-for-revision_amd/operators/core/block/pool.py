@@ -17,8 +17,7 @@ given, and nothing is copied.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -28,8 +27,7 @@ from ... import flags
 from .real import LayerBlocksHolder
 
 
-@dataclass(frozen=True)
-class BlockState:
+class BlockState(NamedTuple):
     block_tables: torch.Tensor  # int32 [rows, blocks per row], -1: none
     context_lens: torch.Tensor  # int32 [rows]
     refs: torch.Tensor          # int32 [blocks of the pool]: table entries that hold each
@@ -82,12 +80,15 @@ class BlockPool:
             torch.zeros(self.num_blocks, dtype=torch.int32, device=self.device))
 
     def _check(self, state: BlockState) -> Tuple[int, int]:
-        rows, width = state.block_tables.shape
-        for name, t, shape in (("block_tables", state.block_tables, (rows, width)),
-                               ("context_lens", state.context_lens, (rows,)),
-                               ("refs", state.refs, (self.num_blocks,))):
-            if t.dtype != torch.int32 or t.shape != shape or t.device != self.device or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous int32 {list(shape)} on {self.device}")
+        tables, lens, refs = state[:3]
+        if tables.dim() != 2:
+            raise ValueError("block_tables must be [rows, blocks per row]")
+        rows, width = tables.shape
+        if lens.shape != (rows,) or refs.shape != (self.num_blocks,):
+            raise ValueError(f"context_lens must be [{rows}] and refs [{self.num_blocks}]")
+        for t in (tables, lens, refs):
+            if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
+                raise ValueError(f"a block state is contiguous int32 on {self.device}")
         return rows, width
 
     def _by_row(self, x: torch.Tensor, rows: int, name: str) -> torch.Tensor:
@@ -116,11 +117,12 @@ class BlockPool:
 
     def _call(self, fn: str, *args) -> None:
         """On the pool's device, on its current stream."""
-        if torch.cuda.current_device() == self.device.index:
-            _lib.call(fn, *args, torch.cuda.current_stream(self.device).cuda_stream)
+        index = self.device.index
+        if _lib.current_device() == index:
+            _lib.call(fn, *args, _lib.current_stream(index))
         else:
-            with torch.cuda.device(self.device):
-                _lib.call(fn, *args, torch.cuda.current_stream(self.device).cuda_stream)
+            with torch.cuda.device(index):
+                _lib.call(fn, *args, _lib.current_stream(index))
 
     # ---- operators
     def copy(self, pairs: torch.Tensor) -> None:

@@ -397,11 +397,14 @@ static int64_t window_steps(const WindowArgs& a, int max_context, int tile_rows,
 //
 // Rows kernel (32-token steps): one 8-wave workgroup per CU, at least 12 steps in a
 // part; not for contexts under 24 steps, nor for two parts unless they are long
-// (160 steps), which the join's launch costs more than it gains.  Measured (us,
+// (100 steps), which the join's launch costs more than it gains.  Between one and
+// two workgroups per CU, of which some CUs then have two and others one, long
+// contexts go in two parts, or three where those fill two per CU better.  Measured (us,
 // one part / these / more; heads 32 on 8 unless said): 1 x 300 tokens 6.7 / - / 7.5 (4
 // parts), 1 x 3000 24.8 / 10.2 / 10.5 (16), 1 x 8000 58 / 17.8 / 19 (32), 4 x 3000 28.5
 // / 17.0 / 17.4 (8), 16 x 3000 33.4 / - / 35.0 (2), 16 x 8000 118 / 95 / 98.5 (4), 8 x
-// 600, 32 on 32, 15.8 / - / 22.4 (2).  More workgroups than CUs: four waves each (32 x
+// 600, 32 on 32, 15.8 / - / 22.4 (2), 40 x 4100 150 / 124 / 126 (4), 48 x 4100 155 / 145 /
+// 150 (3), 12 x 3500 with 7 new tokens 36.3 / 31.9 / 39.1 (3).  More workgroups than CUs: four waves each (32 x
 // 128 tokens, 32 on 32, 23.5 with eight, 16.5).
 //
 // Tile kernel (64-token steps): one workgroup per CU, or two where that leaves
@@ -425,7 +428,8 @@ WindowPlan plan_window(const WindowArgs& a, int max_context, int cus) {
   int64_t s = cus / g;
   if (p.rows) {
     s = std::min(s, (n + 11) / 12);
-    if (n < 24 || (s < 3 && n < 160)) s = 1;
+    if (n < 24 || (s < 3 && n < 100)) s = 1;
+    if (g > cus && g < 2 * cus && n >= 100) s = 3 * g <= 4 * cus ? 3 : 2;
   } else {
     if (n >= 64 && s < 4) s = 2 * cus / g;
     s = std::min({s, (n + 2) / 3, std::max<int64_t>(16, n / 8)});

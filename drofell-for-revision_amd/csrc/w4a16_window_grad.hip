@@ -33,6 +33,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #include "w4a16_device.h"
 #include "w4a16_window.h"
@@ -110,32 +111,42 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
 
   const uint32_t lds0 = lds_offset(lds);
   const bool near = a.k_stride <= kNearRows && a.v_stride <= kNearRows;
-  auto issue = [&](int s, int stage) {
-    const uint32_t dst = lds0 + stage * STAGE;
+  // a step's copies, PARTS per wave, go out among the products of the one before
+  // (at once they would hold up the wave); the last tokens' in one go, bounded
+  constexpr int UNITS = HS / 8, CHUNKS = kBk * UNITS / 64, PARTS = (CHUNKS + 3) / 4 * 2;
+  uint64_t next_k = 0, next_v = 0;
+  uint32_t next_dst = 0;
+  auto part = [&](int i) {
+    const int ch = wave + 4 * (i >> 1);
+    if (CHUNKS % 4 != 0 && ch >= CHUNKS) return;
+    const int u = ch * 64 + lane;
+    const uint32_t r = u / UNITS, at = ((u % UNITS) ^ swizzle<HS>(r)) * 16;
+    if (i & 1) copy16(next_v, r * (uint32_t)(a.v_stride * 2) + at, next_dst + TILE + chunk_at<HS>(ch));
+    else copy16(next_k, r * (uint32_t)(a.k_stride * 2) + at, next_dst + chunk_at<HS>(ch));
+  };
+  auto next_step = [&](int s, int stage) {  // whether part() is to copy it
+    next_dst = lds0 + stage * STAGE;
     const int t = span.token<kBk>(s);
-    constexpr int UNITS = HS / 8, CHUNKS = kBk * UNITS / 64;
     if (near && t + kBk <= n) {
       const size_t col = (size_t)kvh * HS;
-      const uint64_t kb = (uint64_t)(a.k + (size_t)(q0 + t) * a.k_stride + col);
-      const uint64_t vb = (uint64_t)(a.v + (size_t)(q0 + t) * a.v_stride + col);
-      for (int ch = wave; ch < CHUNKS; ch += 4) {
-        const int u = ch * 64 + lane;
-        const uint32_t r = u / UNITS, at = ((u % UNITS) ^ swizzle<HS>(r)) * 16;
-        copy16(kb, r * (uint32_t)(a.k_stride * 2) + at, dst + chunk_at<HS>(ch));
-        copy16(vb, r * (uint32_t)(a.v_stride * 2) + at, dst + TILE + chunk_at<HS>(ch));
-      }
-      return;
+      next_k = (uint64_t)(a.k + (size_t)(q0 + t) * a.k_stride + col);
+      next_v = (uint64_t)(a.v + (size_t)(q0 + t) * a.v_stride + col);
+      return true;
     }
     for (int ch = wave; ch < CHUNKS; ch += 4) {
       const int u = ch * 64 + lane;
       const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
       const int64_t tok = q0 + min(t + r, n - 1);
       const size_t col = (size_t)kvh * HS + at * 8;
-      copy16(a.k + tok * a.k_stride + col, dst + chunk_at<HS>(ch));
-      copy16(a.v + tok * a.v_stride + col, dst + TILE + chunk_at<HS>(ch));
+      copy16(a.k + tok * a.k_stride + col, next_dst + chunk_at<HS>(ch));
+      copy16(a.v + tok * a.v_stride + col, next_dst + TILE + chunk_at<HS>(ch));
     }
+    return false;
   };
-  if (span.steps > 0) issue(0, 0);
+  if (span.steps > 0 && next_step(0, 0)) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) part(i);
+  }
   h8 qreg[KD], oreg[KD];  // B operands: this row of Q and of dO
   float dl = 0.f, mo = 0.f;
   {
@@ -172,21 +183,29 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
   for (int d = 0; d < ND; ++d) dq[d] = f16v{};
   for (int step = 0; step < span.steps; ++step) {
     wait_copies();
-    if (step + 1 < span.steps) issue(step + 1, (step + 1) & 1);
+    bool copies = step + 1 < span.steps && next_step(step + 1, (step + 1) & 1);
     const int t = span.token<kBk>(step);
-    if (nrows <= 0) continue;
     const unsigned char* st = lds + (step & 1) * STAGE;
     for (int b = 0; b < 2; ++b) {
       const int tb = t + 32 * b;
-      if (tb > wlast || (a.window != 0 && tb + 31 <= wfirst - a.window && tb >= a.sinks)) continue;
+      if (nrows <= 0 || tb > wlast || (a.window != 0 && tb + 31 <= wfirst - a.window && tb >= a.sinks)) continue;
       const bool full = tb + 31 <= wfirst && (a.window == 0 || tb > wlast - a.window || tb + 31 < a.sinks);
       f16v s = {}, p = {};
-      feed<2 * KD, 8>(
-          [&](int i) { return row_unit<HS>(st + (i & 1) * TILE + row_at<HS>(32 * b), row_token(c), (i & ~1) + half); },
-          [&](int i, h8 f) {
-            if (i & 1) p = mfma32_of<BF>(f, oreg[i >> 1], p);
-            else s = mfma32_of<BF>(f, qreg[i >> 1], s);
-          });
+      auto products = [&](auto with) {
+        feed<2 * KD, 6>(
+            [&](int i) { return row_unit<HS>(st + (i & 1) * TILE + row_at<HS>(32 * b), row_token(c), (i & ~1) + half); },
+            [&](int i, h8 f) {
+              if (i & 1) p = mfma32_of<BF>(f, oreg[i >> 1], p);
+              else s = mfma32_of<BF>(f, qreg[i >> 1], s);
+              if constexpr (decltype(with)::value) {
+#pragma unroll
+                for (int k = i * PARTS / (2 * KD); k < (i + 1) * PARTS / (2 * KD); ++k) part(k);
+              }
+            });
+      };
+      if (copies) products(std::true_type{});
+      else products(std::false_type{});
+      copies = false;
       float ds[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * (BF ? p[e] - dl : (p[e] - dl) * gs);
@@ -203,6 +222,10 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
                         dq[i % ND] = mfma32_of<BF>(f, hi[i / ND], dq[i % ND]);
                         dq[i % ND] = mfma32_of<BF>(f, lo[i / ND], dq[i % ND]);
                       });
+    }
+    if (copies) {  // the wave sees nothing of this step
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) part(i);
     }
   }
   if (c >= nrows) return;

@@ -68,7 +68,7 @@ struct Span {
     Span s;
     const int hi = min(last + 1, cap);
     s.lo = (window == 0 ? 0 : max(0, first - window + 1)) & ~(BK - 1);
-    s.sink_steps = hi > 0 ? (min(sinks, s.lo) + BK - 1) / BK : 0;
+    s.sink_steps = (max(min(min(sinks, s.lo), hi), 0) + BK - 1) / BK;
     s.steps = s.sink_steps + (hi > s.lo ? (hi - s.lo + BK - 1) / BK : 0);
     return s;
   }

@@ -338,7 +338,7 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
     }
   };
   if (s0 < s1) issue(s0, 0);
-  for (int ch = wave; ch < kGradTile * UNITS / 64; ch += 4) {
+  for (int ch = wave; s0 < s1 && ch < kGradTile * UNITS / 64; ch += 4) {
     const int u = ch * 64 + lane;
     const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
     copy16(a.v + (size_t)(q0 + min(t0 + r, n - 1)) * a.v_stride + (size_t)kvh * HS + at * 8,

@@ -49,6 +49,8 @@ class PagedAttention:
             raise AssertionError("query shape does not match the attention config")
         if query.dtype != torch.float16:
             raise TypeError("paged attention runs on fp16 queries")
+        if kv_cacher.dtype != torch.float16:
+            raise TypeError("paged attention reads fp16 caches (WindowAttention reads bf16 ones too)")
         q = query if query.is_contiguous() else query.contiguous()
         output = torch.empty_like(q)
         tables = block_tables.to(torch.int32).contiguous()

@@ -120,6 +120,8 @@ class LayerBlocksHolder:
         for t in (q, k, v):
             if t.dtype != torch.float16 or not t.is_contiguous():
                 raise TypeError("q, k, v must be contiguous fp16")
+        if self.dtype != torch.float16:
+            raise TypeError("the rotary embedding runs in fp16: its rows do not go into a bf16 cache")
         s16, c16, max_pos = rope_tables(sin, cos, hd)
         if context_lens_out is not None and (context_lens_out.dtype != torch.int32 or
                                              context_lens_out.numel() < seqs):

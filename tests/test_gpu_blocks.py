@@ -357,6 +357,21 @@ def test_serving_run(hip_device):
     assert not state.refs.any() and (state.block_tables == -1).all()
 
 
+def test_empty_states(hip_device):
+    """No rows, tables without columns, a pool without blocks."""
+    say("empty states")
+    for rows, width, blocks in ((0, 4, 10), (3, 0, 10), (3, 4, 0), (0, 0, 0)):
+        pool, _ = make_pool(hip_device, blocks, layers=0)
+        state = pool.new_state(rows, width)
+        ints = torch.zeros(rows, dtype=torch.int32, device=hip_device)
+        for got in (pool.extend(state, ints), pool.fork(state, ints), pool.free(state, 4, 1), pool.compact(state)[0]):
+            check_state(got, [[-1] * width] * rows, [0] * rows, [0] * blocks, 0)
+        if rows:
+            got = pool.extend(state, ints + 5)
+            want = 0 if width and blocks >= rows else max(rows - blocks, 0) + (0 if width else rows)
+            assert got.shortage.item() == want
+
+
 def test_two_streams(hip_device):
     """Two states of one pool worked on at once."""
     rng = random.Random(8)

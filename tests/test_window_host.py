@@ -10,6 +10,7 @@ import torch
 
 from hip_extends import _lib
 from operators.core.attention.common import AttentionConfig
+from operators.core.attention.real_page import PagedAttention
 from operators.core.attention.real_window import WindowAttention
 from operators.core.block.common import BlockInfo
 from operators.core.block.pool import BlockPool
@@ -168,6 +169,22 @@ def test_python_refusals():
         BlockPool([holder], num_blocks=5)
     with pytest.raises(TypeError):                                       # rows of another type than the cache's
         holder.kv_tensor_to_slots_with_convert(kv.bfloat16(), kv.bfloat16(), torch.arange(3))
+
+
+def test_bf16_caches_are_refused_where_fp16_is_read():
+    info = BlockInfo(head_dim=64, num_key_value_heads=2, dtype=torch.bfloat16)
+    holder = LayerBlocksHolder.create_contigious_cacher(info, 4, torch.device("cpu"), torch.bfloat16)
+    q = torch.zeros(3, 8, 64, dtype=torch.float16)
+    kv = torch.zeros(3, 2, 64, dtype=torch.float16)
+    one = torch.ones(3, dtype=torch.int32)
+    with pytest.raises(TypeError):
+        PagedAttention(AttentionConfig(512, 64, 8, 2, 4)).forward(q, 1, one, torch.zeros(3, 1, dtype=torch.int32), holder)
+    with pytest.raises(TypeError):
+        holder.rope_and_cache(q, kv, kv, torch.zeros(4, 64), torch.zeros(4, 64), one, torch.zeros(3, 1, dtype=torch.int32))
+    with pytest.raises(TypeError):
+        holder.kv_tensor_to_slots_with_convert(kv, kv, torch.arange(3))
+    with pytest.raises(TypeError):
+        WindowAttention(AttentionConfig(512, 64, 8, 2, 4)).forward(q, 1, one, torch.zeros(3, 1, dtype=torch.int32), holder)
 
 
 def test_oracle_against_a_masked_softmax():

@@ -18,6 +18,11 @@
 // too few (sequence, kv head) pairs for the CUs, the steps are split among
 // workgroups, which leave max, sum and unnormalised fp32 outputs for
 // window_join_kernel, in a fixed order (deterministic).
+//
+// Measured: 48 streams, window 4096 and 4 sinks, heads 32 on 8 of 128, bf16: 800 MB
+// of cache in 143 us, 5.6 TB/s (a copy of 1 GiB reaches 5.1, reading alone 6.5).  One
+// stream with window 512, where no load hides another (table, pointer, block, then
+// the join in LDS): 7 to 10 us.
 
 #include <hip/hip_runtime.h>
 
@@ -273,7 +278,8 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restr
   }
 }
 
-// The splits of each row joined in their order, a wave per (row, head).
+// The splits of each row joined in their order, a wave per (row, head).  Launch-bound: 4 to
+// 5 us for the splits of 48 tokens with 32 heads as for those of 84.
 template <int HS, bool BF>
 __global__ void __launch_bounds__(256)
 window_join_kernel(WindowArgs a, int splits, const float* __restrict__ ws_ml,

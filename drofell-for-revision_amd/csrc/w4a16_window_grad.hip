@@ -4,8 +4,8 @@
 //   delta_i = dO_i . O_i          dV_j = sum_i P_ij dO_i
 //   dS_ij   = P_ij (dO_i . V_j - delta_i)
 //   dQ_i = c sum_j dS_ij K_j      dK_j = c sum_i dS_ij Q_i
-// P is formed again from the forward's log-sums.  Two kernels, seven products
-// where one pass with atomic sums would need five, so that every sum has one
+// P is formed again from the forward's log-sums.  Two kernels, seven products (nine,
+// dS being in two parts) where one pass with atomic sums would need five, so that every sum has one
 // order and results repeat bit for bit:
 //   * window_dq_kernel: as the forward, 128 rows (tokens x query heads of a kv
 //     head) of a workgroup, steps of 64 tokens through LDS; it writes delta too;
@@ -13,10 +13,15 @@
 //     of its products, steps of 32 rows through LDS; the heads of a group are
 //     rows like any others, so that shared heads' gradients add up in registers.
 //     The tokens' values stay in LDS beside the steps, which leaves registers
-//     for two waves per SIMD (one wave, with steps of 64 rows and the values in
-//     registers: 1372 us for 2 x 6000 tokens, 32 heads of 128, window 2048).
+//     for two waves per SIMD (1003 us when that was measured against one wave, with
+//     steps of 64 rows and the values in registers, 1372 us; sizes as below).
 // Both read a tile from LDS in both directions, rows in plain and columns in
-// transposing reads.  Matrix-core and LDS-read bound.
+// transposing reads.  Bound by matrix cores and vector ALU together, as the forward
+// (busy 50 and 38 % of the cycles in dq, 41 and 36 % in dkv, whose copies cost 13 %:
+// registers do not reach for issuing them among its products).  Measured, for
+// sequences of 6000 and 4100 tokens, 32 heads of 128, window 2048, bf16 (0.155 TFLOP a
+// product): dq 670 us for its four products (dS in two parts), dkv 970 to 1030 us for
+// its five, 0.93 and 0.78 PFLOP/s.
 //
 // Roundings: P enters its product in 16 bits, as the matrix cores take it, with
 // independent errors.  dS, whose errors would add up with those of delta, enters
@@ -445,7 +450,8 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
     }
 }
 
-// The parts of a tile summed in their order, four dims per thread.
+// The parts of a tile summed in their order, four dims per thread.  Launch-bound where
+// parts are made (few tiles): 4 us for five sequences of 333 tokens, 4 kv heads of 80.
 template <int HS, bool BF>
 __global__ void __launch_bounds__(256)
 window_dkv_join_kernel(WindowGradArgs g, DkvPlan plan, int tiles, const float* __restrict__ partial) {

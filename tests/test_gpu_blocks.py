@@ -372,6 +372,25 @@ def test_empty_states(hip_device):
             assert got.shortage.item() == want
 
 
+@pytest.mark.parametrize("blocks", [2047, 32768, 32769, 70001])
+def test_many_blocks(hip_device, blocks):
+    """Runs of counts that just fit what is read at once, and that take several reads."""
+    rng = random.Random(blocks)
+    rows, width, bs = 60, blocks // 80, 16
+    pool, _ = make_pool(hip_device, blocks, layers=0, bs=bs)
+    tables, lens, refs = random_state(rng, rows, width, blocks, bs)
+    state = to_state(hip_device, tables, lens, refs, width)
+    say(f"{blocks} blocks")
+    add = [rng.randint(0, min(width * bs - n, 5 * bs)) for n in lens]
+    check_state(pool.extend(state, torch.tensor(add, dtype=torch.int32, device=hip_device)), *B.extend(tables, lens, refs, add, bs))
+    parents = [rng.randint(-1, rows - 1) for _ in range(rows)]
+    check_state(pool.fork(state, torch.tensor(parents, device=hip_device)), *B.fork(tables, lens, refs, parents, bs)[:4])
+    got, live = pool.compact(state)
+    want_tables, want_refs, want_live, _ = B.compact(tables, refs)
+    check_state(got, want_tables, lens, want_refs, 0)
+    assert live.tolist() == [want_live]
+
+
 def test_two_streams(hip_device):
     """Two states of one pool worked on at once."""
     rng = random.Random(8)

@@ -220,6 +220,13 @@ __device__ __forceinline__ void wait_copies() {
 // into registers used in a loop would make it wait in every round of it).
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }
 
+// threadIdx.x once more: what is computed from it holds no register before.
+__device__ __forceinline__ int thread_again() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // N operands, each loaded (from LDS) AHEAD uses before its use.  The loads and
 // the matrix instructions keep this order; vector-ALU work may move among them.
 template <int N, int AHEAD, typename Load, typename Use>

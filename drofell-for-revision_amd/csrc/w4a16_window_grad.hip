@@ -361,7 +361,7 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
     for (int i = lane; i < (n * G + kGradTile - 1) / kGradTile; i += 64) w = fmaxf(w, most[(size_t)pair * row_tiles + i]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) w = fmaxf(w, __shfl_xor(w, off));
-    gs = grad_scale<BF>(w);
+    gs = grad_scale<BF>(__builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, w))));
   }
   const float ps = p_shift<BF>(), gp = gs * __builtin_amdgcn_exp2f(-ps);
 
@@ -404,10 +404,11 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
       }
       if (!full) {
         const int* at = (const int*)(ls + 2 * kDkvRows);
+        const int own = HS <= 128 ? wa + (thread_again() & 31) : wa + c;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int i = at[e];
-          const bool seen = sees(wa + c, i, a.window == 0 ? INT32_MIN : i - a.window, i < 0 ? 0 : a.sinks);
+          const bool seen = sees(own, i, a.window == 0 ? INT32_MIN : i - a.window, i < 0 ? 0 : a.sinks);
           pr[e] = seen ? pr[e] : 0.f;
           ds[e] = seen ? ds[e] : 0.f;
         }
@@ -427,16 +428,17 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
           }
         });
   }
-  if (wa + c >= n) return;
+  const int thread = HS <= 128 ? thread_again() : (int)threadIdx.x, col = thread & 31, hi = thread >> 5 & 1, token = wa + col;
+  if (token >= n) return;
   const float fk = g.scale / gs, fv = __builtin_amdgcn_exp2f(-ps);
-  uint16_t* ok = g.dk + (size_t)(q0 + tk) * g.dk_stride + (size_t)kvh * HS;
-  uint16_t* ov = g.dv + (size_t)(q0 + tk) * g.dv_stride + (size_t)kvh * HS;
-  float* pk = partial + (((size_t)pair * plan.items() + item) * kGradTile + 32 * wave + c) * (2 * HS);
+  uint16_t* ok = g.dk + (size_t)(q0 + token) * g.dk_stride + (size_t)kvh * HS;
+  uint16_t* ov = g.dv + (size_t)(q0 + token) * g.dv_stride + (size_t)kvh * HS;
+  float* pk = partial + (((size_t)pair * plan.items() + item) * kGradTile + 32 * wave + col) * (2 * HS);
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
-      const int dim = d * 32 + 2 * e + 4 * half;
+      const int dim = d * 32 + 2 * e + 4 * hi;
       if (VTAIL && dim >= HS) continue;
       const f4 x = f4{dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]} * fk;
       const f4 y = f4{dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]} * fv;

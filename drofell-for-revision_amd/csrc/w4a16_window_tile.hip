@@ -88,7 +88,6 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   const int nrows = min(32, rows - wbase);
   const int row = min(wbase + c, rows - 1);
   const int pos = p0 + row / G;
-  const int last = min(pos, cap - 1), before = a.window == 0 ? INT32_MIN : pos - a.window;
   const int wfirst = p0 + min(wbase, rows - 1) / G, wlast = p0 + min(wbase + 31, rows - 1) / G;
 
   // ---- the copies of one step into a stage
@@ -282,6 +281,9 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
     const int t = span.token<kBk>(step);
     if (nrows <= 0 || t > wlast || (a.window != 0 && t + kBk - 1 <= wfirst - a.window && t >= a.sinks)) return;
     const unsigned char* st = lds + stage * STAGE;
+    int at = pos;  // (what follows from it holds no register across the steps)
+    asm volatile("" : "+v"(at));
+    const int last = min(at, cap - 1), before = a.window == 0 ? INT32_MIN : at - a.window;
     uint32_t seen = 0;  // bit 16 b + e: score e of the 32 tokens b
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -302,7 +304,7 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
     feed<4 * ND, 8>([&](int i) { return value(st, i / (2 * ND), i % ND, i / ND % 2); },
                     [&](int, h8 f) { add_nonfinite<BF>(f, bits); });
     const bool odd = __any((bits & kNonfinite) != 0);
-    if (odd) {
+    if (odd) {  // (a fragment at a time: scheduled together they take registers from the usual steps)
       for (uint32_t sign = 0; sign <= 0x8000u; sign += 0x8000u) {
         const float inf = sign ? -INFINITY : INFINITY;
 #pragma unroll
@@ -314,11 +316,14 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (count[e] > 0.f) o[d][e] += inf;
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4 * ND; ++i)
+      for (int i = 0; i < 4 * ND; ++i) {
         o[i % ND] = mfma32_of<BF>(finite_part<BF>(value(st, i / (2 * ND), i % ND, i / ND % 2)), p[i / (2 * ND)][i / ND % 2], o[i % ND]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       return;
     }
     feed<4 * ND, 8>([&](int i) { return value(st, i / (2 * ND), i % ND, i / ND % 2); },
@@ -328,6 +333,7 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   auto is_whole = [&]() { return step >= f0 && step < f1 && held[stage] == (1u << NB) - 1; };
   while (step < s1) {
     wait_copies();
+    wait_loads();  // (registers that the masked steps put aside: none may be waited for in the loop)
     while (is_whole()) {
       const bool more = step + 1 < s1, parts = more && next_step(step + 1, stage ^ 1);
       if (more && !parts) slowly(step + 1);
@@ -344,8 +350,9 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   }
 
   const float sum = both_sum(l[0] + l[1]);
-  if (c >= nrows) return;
-  const int token = q0 + row / G, head = kvh * G + row % G;
+  const int thread = thread_again(), col = thread & 31, hi = thread >> 5 & 1;
+  if (col >= nrows) return;
+  const int own = wbase + col, token = q0 + own / G, head = kvh * G + own % G;
   if (splits == 1) {
     const float f = sum == 0.f ? 1.f : 1.f / sum;  // no visible token: zeros
     uint16_t* op = a.out + (size_t)token * a.o_stride + (size_t)head * HS;
@@ -354,7 +361,7 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        const int dim = d * 32 + 2 * e + 4 * half;
+        const int dim = d * 32 + 2 * e + 4 * hi;
         if (VTAIL && dim >= HS) continue;
         float y[4];
         uint32_t x[2], r[2];
@@ -368,7 +375,7 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
         *(uint2*)(op + dim) = make_uint2(x[0], x[1]);
         if (BS == 0 && a.rest != nullptr) *(uint2*)(rp + dim) = make_uint2(r[0], r[1]);
       }
-    if (a.lse != nullptr && half == 0)
+    if (a.lse != nullptr && hi == 0)
       a.lse[(size_t)token * a.num_heads + head] = m + __builtin_amdgcn_logf(sum) - p_shift<BF>();
   } else {
     const size_t slot = ((size_t)token * a.num_heads + head) * splits + split;
@@ -376,11 +383,11 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        const int dim = d * 32 + 2 * e + 4 * half;
+        const int dim = d * 32 + 2 * e + 4 * hi;
         if (!VTAIL || dim < HS)
           *(f4*)(ws_out + slot * HS + dim) = f4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
       }
-    if (half == 0) {
+    if (hi == 0) {
       ws_ml[2 * slot] = m;
       ws_ml[2 * slot + 1] = sum;
     }

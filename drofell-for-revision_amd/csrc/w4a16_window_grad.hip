@@ -303,26 +303,34 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
   constexpr int UNITS = HS / 8;
   const int log_g = 31 - __builtin_clz(G);
   const bool near = kDkvRows % G == 0 && a.q_stride <= kNearRows && g.do_stride <= kNearRows;
+  constexpr int CHUNKS = kDkvRows * UNITS / 64, TURNS = (CHUNKS + 3) / 4;
+  // Whole tokens' rows (G divides a step's): uniform addresses that advance by the step,
+  // and one offset per lane; a wave's turns are 256 units apart, whole rows where a row
+  // is a power of two.
+  const uint64_t q_first = (uint64_t)(a.q + (size_t)(q0 + t0) * a.q_stride + (size_t)kvh * G * HS);
+  const uint64_t o_first = (uint64_t)(g.dout + (size_t)(q0 + t0) * g.do_stride + (size_t)kvh * G * HS);
+  const uint64_t l_first = (uint64_t)((wave == 0 ? a.lse : delta) + (size_t)(q0 + t0) * a.num_heads + kvh * G);
   auto issue = [&](int s, int stage) {
     const uint32_t dst = lds0 + stage * STAGE;
-    constexpr int CHUNKS = kDkvRows * UNITS / 64;
-    if (near && r0 + (s + 1) * kDkvRows <= r1) {  // whole tokens' rows: G divides the step's
-      const int first = t0 + ((s * kDkvRows) >> log_g);
-      const size_t col = (size_t)kvh * G * HS;
-      const uint64_t qb = (uint64_t)(a.q + (size_t)(q0 + first) * a.q_stride + col);
-      const uint64_t ob = (uint64_t)(g.dout + (size_t)(q0 + first) * g.do_stride + col);
-      for (int ch = wave; ch < CHUNKS; ch += 4) {
-        const int u = ch * 64 + lane;
+    if (near && r0 + (s + 1) * kDkvRows <= r1) {
+      const uint32_t tokens = (uint32_t)(s * kDkvRows) >> log_g, q2 = (uint32_t)(a.q_stride * 2), o2 = (uint32_t)(g.do_stride * 2);
+      const uint64_t qb = q_first + (uint64_t)tokens * q2, ob = o_first + (uint64_t)tokens * o2;
+      constexpr bool EVEN = 256 % UNITS == 0;
+      const int l = BF || HS != 128 ? lane : thread_again() & 63;  // (fp16's powers of two leave no register for offsets)
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        const int ch = wave + 4 * i;
+        if (CHUNKS % 4 != 0 && ch >= CHUNKS) break;
+        const int u = (EVEN ? wave : ch) * 64 + l, rows = EVEN ? i * (256 / UNITS) : 0;
         const uint32_t r = u / UNITS, at = ((u % UNITS) ^ swizzle<HS>(r)) * 16 + (r & (G - 1)) * (HS * 2);
-        copy16(qb, (r >> log_g) * (uint32_t)(a.q_stride * 2) + at, dst + chunk_at<HS>(ch));
-        copy16(ob, (r >> log_g) * (uint32_t)(g.do_stride * 2) + at, dst + TILE + chunk_at<HS>(ch));
+        const uint32_t on = (rows & (G - 1)) * (HS * 2), by = (uint32_t)rows >> log_g;
+        copy16(qb + on + by * q2, (r >> log_g) * q2 + at, dst + chunk_at<HS>(ch));
+        copy16(ob + on + by * o2, (r >> log_g) * o2 + at, dst + TILE + chunk_at<HS>(ch));
       }
-      if (wave < 3 && lane < kDkvRows) {
-        const size_t at = (size_t)(q0 + first) * a.num_heads + kvh * G;
-        const uint32_t off = ((lane >> log_g) * a.num_heads + (lane & (G - 1))) * 4;
-        if (wave == 0) copy4((uint64_t)(a.lse + at), off, dst + 2 * TILE);
-        else if (wave == 1) copy4((uint64_t)(delta + at), off, dst + 2 * TILE + kDkvRows * 4);
-        else *(int*)(lds + stage * STAGE + 2 * TILE + 2 * kDkvRows * 4 + lane * 4) = first + (lane >> log_g);
+      if (wave < 3 && l < kDkvRows) {
+        const uint32_t off = ((l >> log_g) * a.num_heads + (l & (G - 1))) * 4;
+        if (wave == 2) *(int*)(lds + stage * STAGE + 2 * TILE + 2 * kDkvRows * 4 + l * 4) = t0 + tokens + (l >> log_g);
+        else copy4(l_first + 4 * (uint64_t)tokens * a.num_heads, off, dst + 2 * TILE + wave * kDkvRows * 4);
       }
       return;
     }

@@ -357,6 +357,13 @@ def test_dense_and_gradients(hip_device, lens, heads, kvh, hd, window, sinks, dt
         assert torch.equal(att.dense(*dev, starts, max(lens)), got[0])
 
 
+@pytest.mark.parametrize("hd", [64, 80, 128, 256])
+@pytest.mark.parametrize("group", [8, 16, 32, 64])
+def test_gradients_of_wide_groups(hip_device, group, hd):
+    """Groups of as many heads as a step, a copy's turn or half a turn has rows, and more."""
+    test_dense_and_gradients(hip_device, [140, 37], 2 * group, 2, hd, 90, 3, torch.bfloat16 if group < 32 else torch.float16)
+
+
 def test_small_fp16_gradients(hip_device):
     """Output gradients of a mean loss, far below fp16's normal range after the product
     with the probabilities: as exact, relative to their size, as gradients of size one.  The

@@ -117,6 +117,8 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   // a sequence, which need a bound each, go as a whole (slowly()).
   constexpr int UNITS = HS / 8, CHUNKS = BS == 0 ? kBk * UNITS / 64 : (BB + 1023) / 1024;
   constexpr int ITEMS = BS == 0 ? CHUNKS : NB * CHUNKS, PARTS = (ITEMS + 3) / 4 * 2;
+  const uint64_t k_first = (uint64_t)(a.k + (size_t)q0 * a.k_stride + (size_t)kvh * HS);
+  const uint64_t v_first = (uint64_t)(a.v + (size_t)q0 * a.v_stride + (size_t)kvh * HS);
   uint64_t next_k = 0, next_v = 0;  // token rows: their addresses
   int next_l = 0;                   // blocks: the lane that holds the first one's
   uint32_t next_dst = 0;
@@ -125,9 +127,8 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
     if constexpr (BS == 0) {
       const int t = span.token<kBk>(s);
       if (!near || t + kBk > cap) return false;
-      const size_t col = (size_t)kvh * HS;
-      next_k = (uint64_t)(a.k + (size_t)(q0 + t) * a.k_stride + col);
-      next_v = (uint64_t)(a.v + (size_t)(q0 + t) * a.v_stride + col);
+      next_k = k_first + (uint64_t)(uint32_t)t * (uint32_t)(a.k_stride * 2);
+      next_v = v_first + (uint64_t)(uint32_t)t * (uint32_t)(a.v_stride * 2);
     } else {
       if ((s - s0) % STEPS == 0) {
         fetch(s);
@@ -147,10 +148,13 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
     const bool values = i & 1;
     if (ITEMS % 4 != 0 && it >= ITEMS) return;
     if constexpr (BS == 0) {
-      const int u = it * 64 + lane;
+      // (256 units further are whole rows where a row is a power of two: one offset per lane)
+      constexpr bool EVEN = 256 % UNITS == 0;
+      const int u = (EVEN ? wave : it) * 64 + lane;
       const uint32_t r = u / UNITS, at = ((u % UNITS) ^ swizzle<HS>(r)) * 16;
-      if (values) copy16(next_v, r * (uint32_t)(a.v_stride * 2) + at, next_dst + HALF + chunk_at<HS>(it));
-      else copy16(next_k, r * (uint32_t)(a.k_stride * 2) + at, next_dst + chunk_at<HS>(it));
+      const uint32_t k2 = (uint32_t)(a.k_stride * 2), v2 = (uint32_t)(a.v_stride * 2), on = EVEN ? (i >> 1) * (256 / UNITS) : 0;
+      if (values) copy16(next_v + on * v2, r * v2 + at, next_dst + HALF + chunk_at<HS>(it));
+      else copy16(next_k + on * k2, r * k2 + at, next_dst + chunk_at<HS>(it));
     } else {
       // a block's keys as they lie; its values too, for 32-token blocks with the
       // four 16-byte units of a row rotated by dim / 4 (mod 4)

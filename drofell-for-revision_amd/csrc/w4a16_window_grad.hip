@@ -17,11 +17,11 @@
 //     steps of 64 rows and the values in registers, 1372 us; sizes as below).
 // Both read a tile from LDS in both directions, rows in plain and columns in
 // transposing reads.  Bound by matrix cores and vector ALU together, as the forward
-// (busy 50 and 38 % of the cycles in dq, 41 and 36 % in dkv, whose copies cost 13 %:
+// (busy 49 and 38 % of the cycles in dq, 43 and 33 % in dkv, whose copies cost 10 %:
 // registers do not reach for issuing them among its products).  Measured, for
 // sequences of 6000 and 4100 tokens, 32 heads of 128, window 2048, bf16 (0.155 TFLOP a
-// product): dq 670 us for its four products (dS in two parts), dkv 970 to 1030 us for
-// its five, 0.93 and 0.78 PFLOP/s.
+// product): dq 668 us for its four products (dS in two parts), dkv 940 us for its
+// five, 0.93 and 0.82 PFLOP/s.
 //
 // Roundings: P enters its product in 16 bits, as the matrix cores take it, with
 // independent errors.  dS, whose errors would add up with those of delta, enters

@@ -14,10 +14,10 @@
 //   * token rows lie as [token][dims], and values reach the second product
 //     through LDS's transposing reads.
 // Matrix cores and vector ALU bound it together, each busy for half of the cycles at
-// the 1.75 to 1.9 GHz that the card holds under this load.  Measured: four prompts of
-// 900 to 12000 tokens, window 4096, heads 32 on 8 of 128, bf16 (1.7 TFLOP) 1770 us, 0.97
+// the 1.8 to 1.9 GHz that the card holds under this load.  Measured: four prompts of
+// 900 to 12000 tokens, window 4096, heads 32 on 8 of 128, bf16 (1.7 TFLOP) 1726 us, 0.99
 // PFLOP/s (a 16384^3 library product 1.32); dense rows of 6000 and 4100 tokens, window
-// 2048, 32 heads of 128 (0.31 TFLOP) 440 us.  Two workgroups of four waves per CU, so that one's
+// 2048, 32 heads of 128 (0.31 TFLOP) 415 us.  Two workgroups of four waves per CU, so that one's
 // softmax runs beside another's products: eight waves on one step's copies won 2.6 %
 // on the prompts and lost 17 % on the dense rows, 64 rows a wave with one wave per SIMD took 11 % and
 // 45 % longer, copies issued together instead of among the products 6 % longer.

@@ -64,10 +64,20 @@ def _stride(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _int32(x: torch.Tensor) -> torch.Tensor:
+    if x.dtype is torch.int32 and x.is_contiguous():
+        return x
+    return x.to(torch.int32).contiguous()
+
+
 def _ints(x: torch.Tensor, count: int, device: torch.device, name: str) -> torch.Tensor:
     if x.dim() != 1 or x.numel() != count or x.device != device or x.is_floating_point():
         raise ValueError(f"{name} must be {count} integers on the queries' device")
-    return x.to(torch.int32).contiguous()
+    return _int32(x)
 
 
 class WindowAttention:
@@ -128,13 +138,12 @@ class WindowAttention:
         lens = _ints(context_lens, num_seqs, device, "context_lens")
         starts = None if query_starts is None else _ints(query_starts, num_seqs + 1, device, "query_starts")
         if output is None:
-            output = torch.empty(query.shape, dtype=query.dtype, device=device)
+            output = _like(query)
         elif output.shape != query.shape or output.dtype != query.dtype or output.device != device:
             raise ValueError("output must have the queries' shape, type and device")
-        out = output
-        if _rows(output) is not output:
+        elif _rows(output) is not output:
             raise ValueError("output rows must be contiguous and 16-byte aligned")
-        tables = block_tables.to(torch.int32).contiguous()
+        tables = _int32(block_tables)
         with _on(device):
             q = _rows(query)
             nbytes = _lib.window_attention_workspace_size(
@@ -145,7 +154,7 @@ class WindowAttention:
             _lib.call("dw4_window_attention", dtype, num_seqs, cfg.num_query_heads,
                       cfg.num_key_value_heads, cfg.head_dim, flags.BLOCK_SIZE,
                       kv_cacher.layer_key_ptr_table_device.numel(), q.data_ptr(), _stride(q),
-                      out.data_ptr(), _stride(out), None if starts is None else starts.data_ptr(),
+                      output.data_ptr(), _stride(output), None if starts is None else starts.data_ptr(),
                       rows, int(query_len_max), kv_cacher.layer_key_ptr_table_device.data_ptr(),
                       kv_cacher.layer_val_ptr_table_device.data_ptr(), info.head_stride,
                       float(self.scale), self._window, self._sinks, tables.data_ptr(),
@@ -191,10 +200,10 @@ class _WindowDense(torch.autograd.Function):
                 ctx.empty = True
                 ctx.save_for_backward(q, k, v)
                 return torch.zeros(q.shape, dtype=q.dtype, device=device)
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            out = _like(q)
             need = any(ctx.needs_input_grad[:3])
             lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if need else None
-            rest = torch.empty(q.shape, dtype=q.dtype, device=device) if need else None
+            rest = _like(q) if need else None
             _lib.call("dw4_window_attention_dense", *_WindowDense._shape(att, q, starts),
                       q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v),
                       out.data_ptr(), _stride(out), None if lse is None else lse.data_ptr(),
@@ -216,7 +225,7 @@ class _WindowDense(torch.autograd.Function):
         att, device = ctx.att, q.device
         with _on(device):
             do = _rows(dout)
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
+            dq, dk, dv = _like(q), _like(k), _like(v)
             shape = _WindowDense._shape(att, q, starts)
             nbytes = _lib.window_attention_backward_workspace_size(
                 *shape[1:], q.shape[0], ctx.seq_len_max, att._window, att._sinks, device.index)

@@ -94,7 +94,7 @@ class BlockPool:
     def _by_row(self, x: torch.Tensor, rows: int, name: str) -> torch.Tensor:
         if x.shape != (rows,) or x.device != self.device or x.is_floating_point():
             raise ValueError(f"{name} must be one integer per row on {self.device}")
-        return x.to(torch.int32).contiguous()
+        return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
 
     def _next(self, state: BlockState) -> BlockState:
         return BlockState(torch.empty_like(state.block_tables), torch.empty_like(state.context_lens),

@@ -247,6 +247,15 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
     }
 }
 
+// Token of a row (row / G), by the magic ceil(2^32 / G).  The product's quotient is one
+// too large for the last rows of far tokens (rows times the magic's excess, up to G - 1,
+// pass 2^32: with 1023 heads from token 4120 on, with 77 from 764093), never more, which
+// the product back tells.
+__device__ __forceinline__ int token_of(int row, int G, uint32_t magic) {
+  const int i = div_by_magic(row, magic);
+  return i * G > row ? i - 1 : i;
+}
+
 // Floats of a workspace part, whole 16-byte units.
 constexpr size_t grad_rows(size_t a, size_t b) { return (a * b + 3) / 4 * 4; }
 
@@ -337,13 +346,13 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
     for (int ch = wave; ch < CHUNKS; ch += 4) {
       const int u = ch * 64 + lane;
       const int r = u / UNITS, at = (u % UNITS) ^ swizzle<HS>(r);
-      const int row = min(r0 + s * kDkvRows + r, r1 - 1), i = div_by_magic(row, magic);
+      const int row = min(r0 + s * kDkvRows + r, r1 - 1), i = token_of(row, G, magic);
       const size_t col = (size_t)(kvh * G + row - i * G) * HS + at * 8;
       copy16(a.q + (size_t)(q0 + i) * a.q_stride + col, dst + chunk_at<HS>(ch));
       copy16(g.dout + (size_t)(q0 + i) * g.do_stride + col, dst + TILE + chunk_at<HS>(ch));
     }
     if (wave < 3 && lane < kDkvRows) {
-      const int row = r0 + s * kDkvRows + lane, in = min(row, r1 - 1), i = div_by_magic(in, magic);
+      const int row = r0 + s * kDkvRows + lane, in = min(row, r1 - 1), i = token_of(in, G, magic);
       const size_t at = (size_t)(q0 + i) * a.num_heads + kvh * G + in - i * G;
       if (wave == 0) copy4(a.lse + at, dst + 2 * TILE);
       else if (wave == 1) copy4(delta + at, dst + 2 * TILE + kDkvRows * 4);
@@ -383,7 +392,7 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
     if (step + 1 < s1) issue(step + 1, stage ^ 1);
     const unsigned char* st = lds + stage * STAGE;
     const int ra = r0 + step * kDkvRows;
-    const int ia = div_by_magic(ra, magic), ib = div_by_magic(min(ra + kDkvRows, r1) - 1, magic);
+    const int ia = token_of(ra, G, magic), ib = token_of(min(ra + kDkvRows, r1) - 1, G, magic);
     if (wa >= n || ib < wa || (a.window != 0 && ia - a.window >= wb && wa >= a.sinks)) continue;
     const bool full = ra + kDkvRows <= r1 && ia >= wb && (a.window == 0 || ib < wa + a.window || wb < a.sinks);
     f16v s = {}, p = {};

@@ -364,6 +364,32 @@ def test_gradients_of_wide_groups(hip_device, group, hd):
     test_dense_and_gradients(hip_device, [140, 37], 2 * group, 2, hd, 90, 3, torch.bfloat16 if group < 32 else torch.float16)
 
 
+@pytest.mark.parametrize("heads,n", [(1023, 4200), (1000, 6200)])
+def test_gradients_of_far_tokens_of_wide_groups(hip_device, heads, n):
+    """Groups whose rows at far tokens an inexact division by the group's size (one product
+    with ceil(2^32 / heads)) counts to the next token: the last head's rows from token 4120
+    on with 1023 heads, 6100 with 1000.  Only that head has an output gradient, so that its
+    part of dk and dv is not lost among the others'."""
+    hd, window, tail = 64, 6, 150
+    say(f"{n} tokens of {heads} heads on one")
+    g = torch.Generator(device=hip_device).manual_seed(heads)
+    q, k, v, dout = (torch.randn(n, h, hd, generator=g, device=hip_device, dtype=torch.float16).to(torch.bfloat16)
+                     for h in (heads, 1, 1, 1))
+    full = torch.zeros_like(q)
+    full[:, -1:] = dout
+    att = WindowAttention(config(heads, 1, hd), window)
+    dev = [t.requires_grad_(True) for t in (q, k, v)]
+    out = att.dense(*dev, torch.tensor([0, n], dtype=torch.int32, device=hip_device), n)
+    dq, dk, dv = torch.autograd.grad(out, dev, full)
+    torch.cuda.synchronize()
+    # the last tokens as a sequence of their own, less those whose window starts before it
+    x = [t[n - tail:].detach().double().cpu() for t in (q[:, -1:], k, v, dout)]
+    ref, bounds = O.dense(*x, [tail], window, 0, att.scale, torch.bfloat16)
+    for name, y, r, b in zip(("out", "dq", "dk", "dv"), (out[:, -1:].detach(), dq[:, -1:], dk, dv), ref, bounds):
+        ok, worst = O.within(y[n - tail + window:], r[window:], b[window:])
+        assert ok, f"{name}: worst error / bound {worst:.3f}"
+
+
 def test_small_fp16_gradients(hip_device):
     """Output gradients of a mean loss, far below fp16's normal range after the product
     with the probabilities: as exact, relative to their size, as gradients of size one.  The

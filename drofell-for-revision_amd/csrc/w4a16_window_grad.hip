@@ -28,9 +28,9 @@
 // as two 16-bit parts, over operands that are in registers already, and delta
 // sums the forward's output and what its rounding left off.  (With one part
 // and the rounded output alone dq and dk were 1.7 times as far from float64 as their
-// own rounding is.)  fp16 holds neither small probabilities nor small gradients,
-// so P goes in as 2^10 P and dS times a power of two that brings the largest
-// |dO| of the rows it is summed with to 1/16 .. 1/8; bf16 needs neither.
+// own rounding is.)  fp16 holds neither small probabilities nor small or large gradients,
+// so P goes in as 2^10 P and dS times a power of two per row (dq) or token (dkv) that
+// follows the largest of what it is summed from (keep_in_range()); bf16 needs neither.
 // A sequence's non-finite values may reach any gradient of that sequence.
 
 #include <hip/hip_runtime.h>
@@ -51,24 +51,39 @@ namespace {
 constexpr int kBk = kWinTileTokens;
 constexpr int kGradTile = 128;  // rows of a dq workgroup, tokens of a dkv workgroup
 
-// The power of two that brings a largest |dO| to 1/16 .. 1/8 (1 for 0, inf and NaN, and for bf16).
-template <bool BF>
-__device__ __forceinline__ float grad_scale(float most) {
-  if (BF || !(most > 0.f) || !(most < INFINITY)) return 1.f;
-  return __builtin_amdgcn_ldexpf(1.f, -3 - __builtin_amdgcn_frexp_expf(most));
+// fp16: the factors dO . V - delta of a step (of this lane's column: a row in dq, a token in
+// dkv) times a power of two that keeps the largest so far at MOST / 16 or above and at MOST
+// or below, and with them the sums, as a softmax keeps its running maximum: nothing
+// overflows, and nothing that counts beside the largest is lost, whatever the sizes of dO
+// and V.  (The largest of the factors, not of dS = P times them, which a P <= 1 only makes
+// smaller: it is known before the exponentials are.  A power of two from |dO| alone, which takes
+// no step's time, overflowed at coherent values and lost small gradients beside large ones;
+// this costs 2 % of fp16 training with heads of 128, 2 x 6000 tokens, 4 % with heads of 64 and 256.)
+constexpr float kFirstScale = 0x1p100f;
+template <int MOST, int ND>
+__device__ __forceinline__ void keep_in_range(float (&v)[16], float& scale, f16v (&sums)[ND]) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(v[e]));
+  if (__any(top * scale > (float)(1 << MOST))) {
+    top = both_max(top);
+    const float to = top * scale > (float)(1 << MOST) ? __builtin_amdgcn_ldexpf(1.f, MOST - 3 - __builtin_amdgcn_frexp_expf(top)) : scale;
+    const float f = to * __builtin_amdgcn_rcpf(scale);  // (exact: powers of two)
+#pragma unroll
+    for (int d = 0; d < ND; ++d) sums[d] *= f;
+    scale = to;
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] *= scale;
 }
 
-// sum of x (y + z), and the largest |x|
+// sum of x (y + z)
 template <bool BF>
-__device__ __forceinline__ void dot8(u4 x, u4 y, u4 z, float& sum, float& most) {
+__device__ __forceinline__ void dot8(u4 x, u4 y, u4 z, float& sum) {
 #pragma unroll
   for (int e = 0; e < 4; ++e)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float a = unpack<BF>(x[e], h);
-      sum = fmaf(a, unpack<BF>(y[e], h) + unpack<BF>(z[e], h), sum);
-      most = fmaxf(most, fabsf(a));
-    }
+    for (int h = 0; h < 2; ++h) sum = fmaf(unpack<BF>(x[e], h), unpack<BF>(y[e], h) + unpack<BF>(z[e], h), sum);
 }
 
 // Eight values as an operand, and what its rounding leaves off as another.
@@ -86,7 +101,7 @@ __device__ __forceinline__ void two_parts(const float* v, h8& hi, h8& lo) {
 
 template <int HS, bool BF>
 __global__ void __launch_bounds__(256, HS <= 128 ? 2 : 1)
-window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* __restrict__ most) {
+window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta) {
   constexpr int KD = HS / 16, ND = (HS + 31) / 32;
   constexpr bool VTAIL = HS % 32 != 0;
   constexpr int TILE = row_at<HS>(kBk), STAGE = 2 * TILE;  // keys, values
@@ -153,7 +168,7 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
     for (int i = 0; i < PARTS; ++i) part(i);
   }
   h8 qreg[KD], oreg[KD];  // B operands: this row of Q and of dO
-  float dl = 0.f, mo = 0.f;
+  float dl = 0.f;
   {
     const size_t col = (size_t)head * HS + 8 * half;
     const uint16_t* qp = a.q + (size_t)token * a.q_stride + col;
@@ -164,23 +179,13 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
     for (int j = 0; j < KD; ++j) {
       qreg[j] = *(const h8*)(qp + 16 * j);
       oreg[j] = *(const h8*)(dp + 16 * j);
-      dot8<BF>(__builtin_bit_cast(u4, oreg[j]), *(const u4*)(op + 16 * j), *(const u4*)(rp + 16 * j), dl, mo);
+      dot8<BF>(__builtin_bit_cast(u4, oreg[j]), *(const u4*)(op + 16 * j), *(const u4*)(rp + 16 * j), dl);
     }
   }
   dl = both_sum(dl);
-  mo = both_max(mo);
   const float lse = a.lse[(size_t)token * a.num_heads + head];
   if (c < nrows && half == 0) delta[(size_t)token * a.num_heads + head] = dl;
-  const float gs = grad_scale<BF>(mo);
-  if constexpr (!BF) {  // the largest |dO| of the tile, for the dkv kernel
-    __shared__ float top[4];
-    float w = mo;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) w = fmaxf(w, __shfl_xor(w, off));
-    if (lane == 0) top[wave] = w;
-    __syncthreads();
-    if (threadIdx.x == 0) most[(size_t)pair * tiles + tile] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  }
+  float gs = BF ? 1.f : kFirstScale;
 
   wait_loads();
   f16v dq[ND];
@@ -211,9 +216,15 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta, float* 
       if (copies) products(std::true_type{});
       else products(std::false_type{});
       copies = false;
-      float ds[16];
+      float pr[16], ds[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * (BF ? p[e] - dl : (p[e] - dl) * gs);
+      for (int e = 0; e < 16; ++e) {
+        pr[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse));
+        ds[e] = p[e] - dl;
+      }
+      if constexpr (!BF) keep_in_range<15>(ds, gs, dq);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ds[e] *= pr[e];
       if (!full) {
         const uint32_t seen = own_scores(seen_of(tb, pos, before, a.sinks), half);
 #pragma unroll
@@ -272,8 +283,8 @@ constexpr int kDkvRows = 32;
 
 template <int HS, bool BF>
 __global__ void __launch_bounds__(256, HS <= 128 ? 2 : 1)
-window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic, const float* __restrict__ delta,
-                  const float* __restrict__ most, float* __restrict__ partial) {
+window_dkv_kernel(WindowGradArgs g, DkvPlan plan, uint32_t magic, const float* __restrict__ delta,
+                  float* __restrict__ partial) {
   constexpr int KD = HS / 16, ND = (HS + 31) / 32;
   constexpr bool VTAIL = HS % 32 != 0;
   constexpr int AHEAD = HS <= 96 ? 3 : 2;  // operands in flight (registers)
@@ -372,15 +383,8 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
 #pragma unroll
     for (int j = 0; j < KD; ++j) kreg[j] = *(const h8*)(kp + 16 * j);
   }
-  float gs = 1.f;
-  if constexpr (!BF) {
-    float w = 0.f;
-    for (int i = lane; i < (n * G + kGradTile - 1) / kGradTile; i += 64) w = fmaxf(w, most[(size_t)pair * row_tiles + i]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) w = fmaxf(w, __shfl_xor(w, off));
-    gs = grad_scale<BF>(__builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, w))));
-  }
-  const float ps = p_shift<BF>(), gp = gs * __builtin_amdgcn_exp2f(-ps);
+  const float ps = p_shift<BF>();
+  float gs = BF ? 1.f : kFirstScale;  // of 2^ps dS
 
   wait_loads();
   f16v dk[ND], dv[ND];
@@ -409,29 +413,31 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
           p = mfma32_of<BF>(f.o, f.v, p);
         });
     h8 pw[2], hi[2], lo[2];
+    float pr[16], ds[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float* ls = (const float*)(st + 2 * TILE) + 16 * (e / 8) + 8 * half + e % 8;  // of the lane's rows
+      pr[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, ps - ls[0]));
+      ds[e] = p[e] - ls[kDkvRows];
+    }
+    if constexpr (!BF) keep_in_range<5>(ds, gs, dk);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ds[e] *= pr[e];
+    if (!full) {
+      const int own = HS <= 128 ? wa + (thread_again() & 31) : wa + c;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int i = ((const int*)(st + 2 * TILE))[2 * kDkvRows + 16 * (e / 8) + 8 * half + e % 8];
+        const bool seen = sees(own, i, a.window == 0 ? INT32_MIN : i - a.window, i < 0 ? 0 : a.sinks);
+        pr[e] = seen ? pr[e] : 0.f;
+        ds[e] = seen ? ds[e] : 0.f;
+      }
+    }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const float* ls = (const float*)(st + 2 * TILE) + 16 * x + 8 * half;  // of the lane's eight rows
-      float pr[8], ds[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        pr[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * x + e], a.scale_log2, ps - ls[e]));
-        ds[e] = pr[e] * (p[8 * x + e] - ls[kDkvRows + e]);
-        if constexpr (!BF) ds[e] *= gp;
-      }
-      if (!full) {
-        const int* at = (const int*)(ls + 2 * kDkvRows);
-        const int own = HS <= 128 ? wa + (thread_again() & 31) : wa + c;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int i = at[e];
-          const bool seen = sees(own, i, a.window == 0 ? INT32_MIN : i - a.window, i < 0 ? 0 : a.sinks);
-          pr[e] = seen ? pr[e] : 0.f;
-          ds[e] = seen ? ds[e] : 0.f;
-        }
-      }
-      pw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(pr[0], pr[1]), pack2<BF>(pr[2], pr[3]), pack2<BF>(pr[4], pr[5]), pack2<BF>(pr[6], pr[7])});
-      two_parts<BF>(ds, hi[x], lo[x]);
+      const float* v = pr + 8 * x;
+      pw[x] = __builtin_bit_cast(h8, u4{pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7])});
+      two_parts<BF>(ds + 8 * x, hi[x], lo[x]);
     }
     feed<4 * ND, 6>(  // of each 16 rows and 32 dims: dO, then Q
         [&](int i) { return column_unit<HS>(st + (1 - (i & 1)) * TILE, 16 * (i / (2 * ND)), i / 2 % ND); },
@@ -447,7 +453,7 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, int row_tiles, uint32_t magic,
   }
   const int thread = HS <= 128 ? thread_again() : (int)threadIdx.x, col = thread & 31, hi = thread >> 5 & 1, token = wa + col;
   if (token >= n) return;
-  const float fk = g.scale / gs, fv = __builtin_amdgcn_exp2f(-ps);
+  const float fv = __builtin_amdgcn_exp2f(-ps), fk = g.scale * fv / gs;
   uint16_t* ok = g.dk + (size_t)(q0 + token) * g.dk_stride + (size_t)kvh * HS;
   uint16_t* ov = g.dv + (size_t)(q0 + token) * g.dv_stride + (size_t)kvh * HS;
   float* pk = partial + (((size_t)pair * plan.items() + item) * kGradTile + 32 * wave + col) * (2 * HS);
@@ -527,13 +533,12 @@ hipError_t launch_grad_hs(const WindowGradArgs& g, float* ws, hipStream_t stream
   const int row_tiles = (int)(((int64_t)a.max_query * G + kGradTile - 1) / kGradTile);
   const DkvPlan plan = plan_dkv(a, cu_count());
   float* delta = ws;
-  float* most = delta + grad_rows(a.total_rows, a.num_heads);
-  float* partial = most + grad_rows(pairs, row_tiles);
-  dq<<<win_grid(pairs, row_tiles), 256, smem, stream>>>(g, row_tiles, delta, most);
+  float* partial = delta + grad_rows(a.total_rows, a.num_heads);
+  dq<<<win_grid(pairs, row_tiles), 256, smem, stream>>>(g, row_tiles, delta);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   const uint32_t magic = G == 1 ? 0u : (uint32_t)((0x100000000ull + G - 1) / G);
-  dkv<<<win_grid(pairs, plan.items()), 256, smem_kv, stream>>>(g, plan, row_tiles, magic, delta, most, partial);
+  dkv<<<win_grid(pairs, plan.items()), 256, smem_kv, stream>>>(g, plan, magic, delta, partial);
   e = hipGetLastError();
   if (e != hipSuccess || !plan.joined()) return e;
   const int tiles = plan.parts > 1 ? plan.tiles : plan.sink_tiles;
@@ -560,11 +565,9 @@ template hipError_t launch_window_grad<WINDOW_BF16>(const WindowGradArgs&, float
 
 #if !WINDOW_BF16
 size_t window_grad_ws_bytes(const WindowArgs& a) {
-  const int64_t row_tiles = ((int64_t)a.max_query * (a.num_heads / a.num_kv_heads) + kGradTile - 1) / kGradTile;
   const DkvPlan p = plan_dkv(a, cu_count());
   const size_t pairs = (size_t)a.num_seqs * a.num_kv_heads;
-  return sizeof(float) * (grad_rows(a.total_rows, a.num_heads) + grad_rows(pairs, row_tiles) +
-                          (p.joined() ? pairs * p.items() * kGradTile * 2 * a.head_size : 0));
+  return sizeof(float) * (grad_rows(a.total_rows, a.num_heads) + (p.joined() ? pairs * p.items() * kGradTile * 2 * a.head_size : 0));
 }
 #endif
 

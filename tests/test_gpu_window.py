@@ -411,6 +411,48 @@ def test_small_fp16_gradients(hip_device):
         assert ok, f"{name}: {worst:.3f}"
 
 
+def check_gradients(dev, q, k, v, dout, lens, window, sinks):
+    """dq, dk, dv of packed fp16 sequences against the oracle, element by element."""
+    heads, kvh, hd = q.shape[1], k.shape[1], q.shape[2]
+    att = WindowAttention(config(heads, kvh, hd), window or None, sinks)
+    starts = torch.tensor(starts_of(lens), dtype=torch.int32, device=dev)
+    x = [t.to(dev).requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(att.dense(*x, starts, max(lens)), x, dout.to(dev))
+    torch.cuda.synchronize()
+    ref, bounds = O.dense(*[t.double() for t in (q, k, v, dout)], lens, window, sinks, att.scale, q.dtype)
+    for name, y, r, b in zip(("dq", "dk", "dv"), grads, ref[1:], bounds[1:]):
+        ok, worst = O.within(y, r, b)
+        assert ok, f"{name}: worst error / bound {worst:.3f}"
+
+
+@pytest.mark.parametrize("hd,kvh,lens,window", [(256, 1, [2, 40, 3], 0), (128, 2, [300, 2, 5], 70), (64, 1, [4, 700], 0)])
+def test_fp16_gradients_of_large_values(hip_device, hd, kvh, lens, window):
+    """Values of one size and alternating sign by token, every dim of a token alike, under output
+    gradients of one: dO . V is 2^22, far beyond fp16, where dq and dk, with small keys
+    and queries, are not."""
+    say(f"fp16 gradients of large values, {lens} tokens, head size {hd}")
+    g = torch.Generator().manual_seed(hd)
+    q, k, v, dout = leaves(g, lens, 2, kvh, hd, torch.float16)
+    q, k = (q.float() * 0.02).half(), (k.float() * 0.02).half()
+    v[:] = min(2.0 ** 22 / hd, 65504)
+    v[::2] *= -1
+    check_gradients(hip_device, q, k, v, torch.ones_like(dout), lens, window, 2)
+
+
+@pytest.mark.parametrize("where", ["first", "last", "middle"])
+@pytest.mark.parametrize("n,window,hd,low", [(2048, 512, 128, -10), (1024, 200, 64, -12), (512, 64, 128, -10), (300, 0, 80, -12)])
+def test_uneven_fp16_gradients(hip_device, n, window, hd, low, where):
+    """Eight rows with output gradients of size one among rows of 2^-10 or 2^-12, as at the end of a
+    masked loss: the others' gradients are as exact as without them."""
+    say(f"uneven fp16 gradients {n} tokens, window {window}, 2^{low}, large ones {where}")
+    g = torch.Generator().manual_seed(n + low)
+    q, k, v, dout = leaves(g, [n], 2, 1, hd, torch.float16)
+    at = {"first": 0, "last": n - 8, "middle": n // 2}[where]
+    size = torch.full((n, 1, 1), 2.0 ** low)
+    size[at:at + 8] = 1
+    check_gradients(hip_device, q, k, v, (dout.float() * size).half(), [n], window, 0)
+
+
 def test_gradients_against_differences(hip_device):
     """(f(x + h d) - f(x - h d)) / 2 h in float64 of the oracle's forward against the
     kernels' gradient along d: the formula itself, not the oracle's."""

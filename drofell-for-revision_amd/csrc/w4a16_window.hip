@@ -154,7 +154,7 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restr
     const int first_pos = p0 + base / G, last_pos = p0 + (base + nrows - 1) / G;
     const bool full = held == (1u << NB) - 1 && t + 31 <= min(first_pos, cap - 1) &&
                       (a.window == 0 || t > last_pos - a.window || t + 31 < a.sinks);
-    uint32_t seen = 0;  // bit e: score e
+    uint32_t seen = 0xFFFF;  // bit e: score e
     if (!full) {
       seen = own_scores(seen_of(t, last, before, a.sinks), half);
       if constexpr (NB == 1) seen = held ? seen : 0u;
@@ -193,18 +193,16 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restr
       hi[g] = __builtin_bit_cast(h8, h);
       lo[g] = __builtin_bit_cast(h8, r);
     }
-    bool odd = false;
-    if (!full) {
-      // a value that some rows do not see (or that is behind the context) must
-      // not reach them as 0 * inf
-      uint32_t bits = 0;
+    // a value that some rows do not see (or that is behind the context) must not reach
+    // them as 0 * inf, nor an infinity a row that sees it as inf - inf, by a negative
+    // second part
+    uint32_t bits = 0;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        add_nonfinite<BF>(vreg[d][0], bits);
-        add_nonfinite<BF>(vreg[d][1], bits);
-      }
-      odd = __any((bits & kNonfinite) != 0);
+    for (int d = 0; d < ND; ++d) {
+      add_nonfinite<BF>(vreg[d][0], bits);
+      add_nonfinite<BF>(vreg[d][1], bits);
     }
+    const bool odd = __any((bits & kNonfinite) != 0);
     if (odd) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) {

@@ -233,6 +233,43 @@ def test_nonfinite_of_later_tokens(hip_device, hd, bs):
     assert torch.equal(o[..., rest], clean[hit][:, :2][..., rest])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("hd,bs,token", [(128, 32, 140), (64, 16, 140), (256, 32, 140), (128, 32, 195), (80, 16, 101)])
+def test_nonfinite_values_that_rows_see(hip_device, hd, bs, token, dtype):
+    """Decode and a few new tokens: an infinity gives infinity, a NaN NaN, in the dims that hold
+    them and nowhere else, whether every row sees the whole step of tokens (140), or some of it
+    is behind the context (195) or before the window (101)."""
+    holder, g = cache(hip_device, 20, 2, hd, bs, dtype, 5)
+    tables = tables_of(g, [200], bs, 20)
+    kt, vt = holder.contigious_kv_tenosr
+    att = WindowAttention(config(4, 2, hd), 100, 2)
+    lens = torch.tensor([200], dtype=torch.int32, device=hip_device)
+    for n in (1, 3):
+        say(f"visible non-finite values, token {token}, {n} rows, hd={hd} bs={bs} {dtype}")
+        q = torch.randn(n, 4, hd, generator=g).to(dtype).to(hip_device)
+        starts = torch.tensor([0, n], dtype=torch.int32, device=hip_device)
+
+        def call():
+            return att.prefill(q, starts, n, 200, lens, tables.to(hip_device), holder)
+
+        clean = call()
+        kept = vt.clone()
+        blk = int(tables[0, token // bs])
+        for dim, value in ((3, torch.inf), (5, -torch.inf), (7, torch.nan), (hd - 1, torch.inf)):
+            vt[blk, 0, dim, token % bs] = value
+        out = call()
+        vt.copy_(kept)
+        torch.cuda.synchronize()
+        hit = torch.arange(200 - n, 200) < token + 100
+        assert hit.any()
+        o = out[hit][:, :2]
+        assert (o[..., 3] == torch.inf).all() and (o[..., 5] == -torch.inf).all()
+        assert o[..., 7].isnan().all() and (o[..., hd - 1] == torch.inf).all()
+        rest = [d for d in range(hd) if d not in (3, 5, 7, hd - 1)]
+        assert torch.equal(o[..., rest], clean[hit][:, :2][..., rest])
+        assert torch.equal(out[:, 2:], clean[:, 2:]) and torch.equal(out[~hit], clean[~hit])
+
+
 def test_rows_behind_the_last_sequence_and_strides(hip_device):
     """Queries inside a wider tensor, an output with a stride of its own, rows that
     belong to no sequence."""

@@ -277,7 +277,8 @@ constexpr size_t grad_rows(size_t a, size_t b) { return (a * b + 3) / 4 * 4; }
 struct DkvPlan {
   int tiles, sink_tiles, parts, sink_parts;
   __host__ __device__ int items() const { return sink_tiles * sink_parts + (tiles - sink_tiles) * parts; }
-  __host__ __device__ bool joined() const { return (sink_tiles > 0 && sink_parts > 1) || (tiles > sink_tiles && parts > 1); }
+  // Items of a pair that are parts, the first ones (sink_parts >= parts): they leave sums in the workspace.
+  __host__ __device__ int partial_items() const { return parts > 1 ? items() : sink_parts > 1 ? sink_tiles * sink_parts : 0; }
 };
 constexpr int kDkvRows = 32;
 
@@ -456,7 +457,7 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, uint32_t magic, const float* _
   const float fv = __builtin_amdgcn_exp2f(-ps), fk = g.scale * fv / gs;
   uint16_t* ok = g.dk + (size_t)(q0 + token) * g.dk_stride + (size_t)kvh * HS;
   uint16_t* ov = g.dv + (size_t)(q0 + token) * g.dv_stride + (size_t)kvh * HS;
-  float* pk = partial + (((size_t)pair * plan.items() + item) * kGradTile + 32 * wave + col) * (2 * HS);
+  float* pk = partial + (((size_t)pair * plan.partial_items() + item) * kGradTile + 32 * wave + col) * (2 * HS);
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -492,7 +493,7 @@ window_dkv_join_kernel(WindowGradArgs g, DkvPlan plan, int tiles, const float* _
   const int u = chunk * 256 + threadIdx.x, t = u / (2 * HS / 4), dim = u % (2 * HS / 4) * 4;
   const int token = tile * kGradTile + t;
   if (token >= min(q1 - q0, a.max_query)) return;
-  const float* src = partial + (((size_t)pair * plan.items() + item) * kGradTile + t) * (2 * HS) + dim;
+  const float* src = partial + (((size_t)pair * plan.partial_items() + item) * kGradTile + t) * (2 * HS) + dim;
   f4 sum = {};
   for (int p = 0; p < parts; ++p) sum += *(const f4*)(src + (size_t)p * kGradTile * (2 * HS));
   uint16_t* out = dim < HS ? g.dk + (size_t)(q0 + token) * g.dk_stride + (size_t)kvh * HS + dim
@@ -502,7 +503,8 @@ window_dkv_join_kernel(WindowGradArgs g, DkvPlan plan, int tiles, const float* _
 
 // Tiles of tokens split into parts: all of them where they leave more than half
 // of the CUs (two workgroups each) without one, down to eight steps a part; sink
-// tiles, whose rows a window does not bound, to about twice a bounded tile's rows.
+// tiles, whose rows a window does not bound, to about twice a bounded tile's rows, or
+// until their parts, which go first, fill every CU once: more would only cost workspace.
 DkvPlan plan_dkv(const WindowArgs& a, int cus) {
   DkvPlan p = {};
   const int64_t G = a.num_heads / a.num_kv_heads, pairs = (int64_t)a.num_seqs * a.num_kv_heads;
@@ -513,7 +515,8 @@ DkvPlan plan_dkv(const WindowArgs& a, int cus) {
   if (pairs * p.tiles <= cus) p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / (pairs * p.tiles), steps / 8));
   p.sink_tiles = a.window == 0 ? 0 : (int)std::min<int64_t>(p.tiles, ((int64_t)a.sinks + kGradTile - 1) / kGradTile);
   p.sink_parts = p.parts;
-  if (p.sink_tiles > 0 && a.max_query >= 3 * bound) p.sink_parts = (int)std::max<int64_t>(p.parts, std::min<int64_t>(64, a.max_query / (2 * bound) * p.parts));
+  if (p.sink_tiles > 0 && a.max_query >= 3 * bound)
+    p.sink_parts = (int)std::max<int64_t>(p.parts, std::min({(int64_t)64, a.max_query / (2 * bound) * p.parts, 2 * cus / (pairs * p.sink_tiles)}));
   return p;
 }
 
@@ -540,7 +543,7 @@ hipError_t launch_grad_hs(const WindowGradArgs& g, float* ws, hipStream_t stream
   const uint32_t magic = G == 1 ? 0u : (uint32_t)((0x100000000ull + G - 1) / G);
   dkv<<<win_grid(pairs, plan.items()), 256, smem_kv, stream>>>(g, plan, magic, delta, partial);
   e = hipGetLastError();
-  if (e != hipSuccess || !plan.joined()) return e;
+  if (e != hipSuccess || plan.partial_items() == 0) return e;
   const int tiles = plan.parts > 1 ? plan.tiles : plan.sink_tiles;
   window_dkv_join_kernel<HS, BF><<<(unsigned)(pairs * tiles * (kGradTile * (2 * HS / 4) / 256)), 256, 0, stream>>>(
       g, plan, tiles, partial);
@@ -567,7 +570,7 @@ template hipError_t launch_window_grad<WINDOW_BF16>(const WindowGradArgs&, float
 size_t window_grad_ws_bytes(const WindowArgs& a) {
   const DkvPlan p = plan_dkv(a, cu_count());
   const size_t pairs = (size_t)a.num_seqs * a.num_kv_heads;
-  return sizeof(float) * (grad_rows(a.total_rows, a.num_heads) + (p.joined() ? pairs * p.items() * kGradTile * 2 * a.head_size : 0));
+  return sizeof(float) * (grad_rows(a.total_rows, a.num_heads) + pairs * p.partial_items() * kGradTile * 2 * a.head_size);
 }
 #endif
 

@@ -448,6 +448,14 @@ def test_small_fp16_gradients(hip_device):
         assert ok, f"{name}: {worst:.3f}"
 
 
+@pytest.mark.parametrize("lens,heads,kvh,hd,window,sinks", [
+    ([2000, 40], 20, 20, 64, 40, 140),   # sink tiles in parts, the others whole
+    ([1500], 6, 3, 128, 30, 200),        # both in parts, of different numbers
+])
+def test_gradients_of_cut_sink_tiles(hip_device, lens, heads, kvh, hd, window, sinks):
+    test_dense_and_gradients(hip_device, lens, heads, kvh, hd, window, sinks, torch.bfloat16)
+
+
 def check_gradients(dev, q, k, v, dout, lens, window, sinks):
     """dq, dk, dv of packed fp16 sequences against the oracle, element by element."""
     heads, kvh, hd = q.shape[1], k.shape[1], q.shape[2]

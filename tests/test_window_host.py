@@ -84,6 +84,16 @@ def test_dense_refusals(back):
         assert call(ws=None) == WORK and call(wsb=100) == WORK and call(ws=ODD) == MISAL
 
 
+@pytest.mark.parametrize("seqs,heads,kvh,hd,rows,most,window,sinks", [
+    (2, 32, 32, 128, 12000, 6000, 1024, 4), (1, 32, 32, 128, 32768, 32768, 4096, 4), (4, 32, 32, 128, 65536, 16384, 1024, 4),
+    (1, 32, 32, 128, 16384, 16384, 128, 4096), (1, 32, 32, 128, 32768, 32768, 256, 1024),
+    (64, 64, 8, 128, 65536, 8192, 1024, 4), (1000, 8, 8, 128, 100000, 50000, 1024, 4)])
+def test_gradient_workspace_holds_parts_alone(seqs, heads, kvh, hd, rows, most, window, sinks):
+    """Where only the sinks' tiles are cut, only their parts take room: a fraction of dk and dv."""
+    size = _lib.window_attention_backward_workspace_size(seqs, heads, kvh, hd, rows, most, window, sinks)
+    assert size - 4 * rows * heads <= 2 * 2 * rows * kvh * hd / 2
+
+
 def test_pool_refusals():
     lib = _lib.load()
     out = [ctypes.c_void_p((1 << 20) + 4096 * i) for i in range(1, 9)]

@@ -100,6 +100,13 @@ __device__ __forceinline__ void zero_outside(uint16_t* x, int64_t stride, int wi
   }
 }
 
+// The rows of a sequence longer than the call said, beyond what it works on (first .. end - 1,
+// usually none), become zeros: those of a pair's columns by its workgroups in turn.
+__device__ __forceinline__ void zero_beyond(uint16_t* x, int64_t stride, int width, int first, int end, int item, int items) {
+  for (int64_t row = (int64_t)first + item; row < end; row += items)
+    for (int d = threadIdx.x * 8; d < width; d += blockDim.x * 8) *(u4*)(x + row * stride + d) = u4{};
+}
+
 // Workgroup b's (sequence, kv head) pair and its item of `items` (row tiles,
 // longest spans first, x splits), false where there is none.  Workgroups go
 // round-robin to the eight XCDs, each with an L2 of its own: kWinUnit

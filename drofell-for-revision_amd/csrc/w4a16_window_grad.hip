@@ -119,6 +119,7 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta) {
   const int rows = n * G, base = tile * kGradTile;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  zero_beyond(g.dq + (size_t)kvh * G * HS, g.dq_stride, G * HS, q0 + n, q1, tile, tiles);
   if (base >= rows) return;
   const int c = lane & 31, half = lane >> 5;
   const Span span = Span::of<kBk>(base / G, (min(base + kGradTile, rows) - 1) / G, n, a.window, a.sinks);
@@ -310,6 +311,8 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, uint32_t magic, const float* _
   const int t0 = tile * kGradTile;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  zero_beyond(g.dk + (size_t)kvh * HS, g.dk_stride, HS, q0 + n, q1, item, plan.items());
+  zero_beyond(g.dv + (size_t)kvh * HS, g.dv_stride, HS, q0 + n, q1, item, plan.items());
   if (t0 >= n) return;
   const int c = lane & 31, half = lane >> 5;
   // rows that see a token of the tile, and this part of them

@@ -71,6 +71,7 @@ window_tile_kernel(WindowArgs a, int tiles, int splits, float* __restrict__ ws_m
   seq_rows(a.starts, seq, a.total_rows, q0, q1);
   const int n = min(q1 - q0, a.max_query);
   const int rows = n * G, base = tile * 128;
+  if (BS == 0) zero_beyond(a.out + (size_t)kvh * G * HS, a.o_stride, G * HS, q0 + n, q1, tile, tiles);
   if (base >= rows) return;
 
   const int lane = threadIdx.x & 63;

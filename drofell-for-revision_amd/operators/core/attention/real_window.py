@@ -167,8 +167,9 @@ class WindowAttention:
               seq_len_max: int) -> torch.Tensor:
         """Packed sequences: q [rows, query heads, head_dim], k and v [rows, kv heads,
         head_dim], sequence s in the rows ``seq_starts[s]`` to ``seq_starts[s + 1]``
-        (int32 [seqs + 1], ascending), each at most ``seq_len_max`` long -> out like q, rows
-        of no sequence zero.  Differentiable in q, k and v (once)."""
+        (int32 [seqs + 1], ascending), each at most ``seq_len_max`` long -> out like q; rows of
+        no sequence, and those of a longer one beyond ``seq_len_max``, are zero and get zero
+        gradients.  Differentiable in q, k and v (once)."""
         cfg = self.cfg
         self._check(q, cfg.num_query_heads, "q")
         self._check(k, cfg.num_key_value_heads, "k")

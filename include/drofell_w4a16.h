@@ -522,7 +522,8 @@ int dw4_window_attention_workspace_size(int num_seqs, int num_heads, int num_kv_
 /* Packed sequences: q, out [total_rows][num_heads][head_size], k, v
  * [total_rows][num_kv_heads][head_size] with row strides, sequence s in the rows
  * seq_starts[s] .. seq_starts[s + 1] - 1 (int32 device, ascending), each at most
- * max_seq_len long.  Output rows of no sequence become zeros.  lse: float
+ * max_seq_len long.  Output rows of no sequence, and those of a longer one beyond
+ * max_seq_len, become zeros (with no sequence, row or length at all nothing is written).  lse: float
  * [total_rows][num_heads], the base-2 logarithm of each row's softmax sum, and
  * out_rest, of dtype and contiguous [total_rows][num_heads][head_size], what
  * rounding the output left off: both for the backward pass, or both NULL. */
@@ -532,8 +533,7 @@ int dw4_window_attention_dense(int dtype, int num_seqs, int num_heads, int num_k
                                int64_t o_stride, float* lse, uint16_t* out_rest,
                                const int32_t* seq_starts, int total_rows, int max_seq_len, float scale, int window, int sinks, void* stream);
 
-/* Its gradients dq, dk, dv (shapes of q, k, v; rows of no sequence become
- * zeros) for the output gradient dout, from the forward's inputs, out, lse and out_rest.
+/* Its gradients dq, dk, dv (shapes of q, k, v; zeros in the same rows) for the output gradient dout, from the forward's inputs, out, lse and out_rest.
  * Deterministic, also where query heads share a kv head.  workspace:
  * dw4_window_attention_dense_backward_workspace_size bytes. */
 int dw4_window_attention_dense_backward(int dtype, int num_seqs, int num_heads, int num_kv_heads,

@@ -427,6 +427,32 @@ def test_gradients_of_far_tokens_of_wide_groups(hip_device, heads, n):
         assert ok, f"{name}: worst error / bound {worst:.3f}"
 
 
+@pytest.mark.parametrize("lens,most,heads,kvh,hd,sinks", [([100, 30], 64, 4, 2, 128, 0), ([5, 700, 1], 1, 2, 1, 80, 2),
+                                                          ([1500, 900], 1000, 20, 20, 64, 3)])
+def test_rows_beyond_the_stated_length(hip_device, lens, most, heads, kvh, hd, sinks):
+    """Sequences longer than the call says: their further rows are zeros, in the output and
+    in every gradient, whatever the memory held; the others are those of shorter sequences."""
+    say(f"{lens} tokens said to be {most}")
+    g = torch.Generator().manual_seed(6)
+    q, k, v, dout = leaves(g, lens, heads, kvh, hd, torch.bfloat16)
+    att = WindowAttention(config(heads, kvh, hd), 40, sinks)
+    starts = starts_of(lens)
+    dev = [t.to(hip_device).requires_grad_(True) for t in (q, k, v)]
+    spoilt = [torch.full_like(t, torch.nan, device=hip_device) for t in (q, q, k, v) for _ in range(3)]
+    del spoilt  # torch gives this memory out again
+    out = att.dense(*dev, torch.tensor(starts, dtype=torch.int32, device=hip_device), most)
+    grads = torch.autograd.grad(out, dev, dout.to(hip_device))
+    torch.cuda.synchronize()
+    keep = torch.cat([torch.arange(a, min(b, a + most)) for a, b in zip(starts, starts[1:])])
+    rest = torch.ones(sum(lens), dtype=torch.bool)
+    rest[keep] = False
+    ref, bounds = O.dense(*[t[keep].double() for t in (q, k, v, dout)], [min(n, most) for n in lens], 40, sinks, att.scale, torch.bfloat16)
+    for name, y, r, b in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), ref, bounds):
+        assert not y.cpu()[rest].any(), name
+        ok, worst = O.within(y.cpu()[keep], r, b)
+        assert ok, f"{name}: worst error / bound {worst:.3f}"
+
+
 def test_small_fp16_gradients(hip_device):
     """Output gradients of a mean loss, far below fp16's normal range after the product
     with the probabilities: as exact, relative to their size, as gradients of size one.  The

@@ -61,6 +61,10 @@ inline size_t win_rows_smem(int hs, int cols, int waves) {
 }
 
 WindowPlan plan_window(const WindowArgs& a, int max_context, int cus);
+// Floats of a split call's maxima and sums, whole 16-byte units; the outputs follow.
+inline size_t win_ml_floats(int total_rows, int num_heads, int splits) {
+  return (2 * (size_t)total_rows * num_heads * splits + 3) / 4 * 4;
+}
 size_t window_ws_bytes(const WindowPlan& p, int total_rows, int num_heads, int head_size);
 hipError_t launch_window(const WindowArgs& a, const WindowPlan& p, float* ws, hipStream_t stream);
 // The kernels by storage: rows kernel (blocks), tile kernel (blocks or rows).

@@ -345,7 +345,7 @@ hipError_t launch_rows_w(const WindowArgs& a, const WindowPlan& p, float* ws_ml,
 template <int HS, bool BF>
 hipError_t launch_rows_hs(const WindowArgs& a, const WindowPlan& p, float* ws, hipStream_t stream) {
   float* ws_ml = ws;
-  float* ws_out = ws + 2 * (size_t)a.total_rows * a.num_heads * p.splits;
+  float* ws_out = ws + win_ml_floats(a.total_rows, a.num_heads, p.splits);
   hipError_t e = hipErrorInvalidValue;
   if (p.rows) {
     if (p.waves == 4)
@@ -443,7 +443,8 @@ WindowPlan plan_window(const WindowArgs& a, int max_context, int cus) {
 }
 
 size_t window_ws_bytes(const WindowPlan& p, int total_rows, int num_heads, int head_size) {
-  return p.splits == 1 ? 0 : sizeof(float) * (size_t)total_rows * num_heads * p.splits * (2 + (size_t)head_size);
+  if (p.splits == 1) return 0;
+  return sizeof(float) * (win_ml_floats(total_rows, num_heads, p.splits) + (size_t)total_rows * num_heads * p.splits * head_size);
 }
 #endif
 

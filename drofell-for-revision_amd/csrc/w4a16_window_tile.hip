@@ -407,7 +407,7 @@ hipError_t launch_tile_bs(const WindowArgs& a, const WindowPlan& p, float* ws, h
   const hipError_t e = allow_lds(reinterpret_cast<const void*>(kern), smem, done);
   if (e != hipSuccess) return e;
   kern<<<win_grid(a.num_seqs * a.num_kv_heads, p.tiles * p.splits), 256, smem, stream>>>(
-      a, p.tiles, p.splits, ws, ws + 2 * (size_t)a.total_rows * a.num_heads * p.splits);
+      a, p.tiles, p.splits, ws, ws + win_ml_floats(a.total_rows, a.num_heads, p.splits));
   return hipGetLastError();
 }
 

@@ -152,6 +152,14 @@ def test_prefill(hip_device, new, ctxs, heads, kvh, bs, window, sinks, dtype):
     check_paged(hip_device, new, ctxs, heads, kvh, 128, bs, dtype, window, sinks)
 
 
+def test_prefill_in_an_odd_number_of_slots(hip_device):
+    """Odd heads, rows and parts: the parts' outputs start behind maxima and sums that do not
+    fill whole 16-byte units."""
+    for n, dtype in ((41, torch.float16), (1, torch.bfloat16)):
+        say(f"odd heads, rows and parts, {n} new tokens")
+        check_paged(hip_device, [n], [540], 5, 5, 128, 32, dtype, 0, 0)
+
+
 @pytest.mark.parametrize("hd", HEAD_SIZES)
 @pytest.mark.parametrize("bs", [16, 32])
 def test_prefill_head_sizes(hip_device, hd, bs):

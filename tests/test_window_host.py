@@ -84,6 +84,17 @@ def test_dense_refusals(back):
         assert call(ws=None) == WORK and call(wsb=100) == WORK and call(ws=ODD) == MISAL
 
 
+def test_split_outputs_are_aligned():
+    """An odd number of (row, head, part) slots: their maxima and sums, 8 bytes each, are
+    followed by 8 bytes more, so that the outputs behind them start at 16-byte units."""
+    def size(rows, heads):
+        return _lib.window_attention_workspace_size(1, heads, heads, 128, 32, rows, rows, 0, 0, 540)
+
+    slots = 41 * 5 * 3          # 540 tokens in nine steps of 64: three parts
+    assert size(41, 5) == slots * 4 * 128 + slots * 8 + 8
+    assert size(42, 5) == 42 * 5 * 3 * (4 * 128 + 8)
+
+
 @pytest.mark.parametrize("seqs,heads,kvh,hd,rows,most,window,sinks", [
     (2, 32, 32, 128, 12000, 6000, 1024, 4), (1, 32, 32, 128, 32768, 32768, 4096, 4), (4, 32, 32, 128, 65536, 16384, 1024, 4),
     (1, 32, 32, 128, 16384, 16384, 128, 4096), (1, 32, 32, 128, 32768, 32768, 256, 1024),

@@ -35,7 +35,11 @@ class LayerBlocksHolder:
                  layer_val_ptr_table_device: torch.Tensor,
                  layer_key_ptr_table_cpu: torch.Tensor, layer_val_ptr_table_cpu: torch.Tensor,
                  layer_key_ptr_table_list: List[int], layer_val_ptr_table_list: List[int],
-                 contigious_kv_tensor: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> None:
+                 contigious_kv_tensor: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                 dtype: Optional[torch.dtype] = None) -> None:
+        """``dtype``: fp16 or bf16, the type of the keys and values that the blocks hold; by
+        default that of the contiguous backing, and fp16 without one, whatever type the
+        geometry was given with (of which only the size counts)."""
         for t in (layer_key_ptr_table_device, layer_val_ptr_table_device):
             if t.dtype != torch.int64 or t.requires_grad:
                 raise AssertionError("pointer tables must be int64 without grad")
@@ -48,11 +52,14 @@ class LayerBlocksHolder:
         self.layer_val_ptr_table_list = layer_val_ptr_table_list
         self._contigious_kv_tensor = contigious_kv_tensor
         self.device = layer_key_ptr_table_device.device
-
-    @property
-    def dtype(self) -> torch.dtype:
-        """Type of the cached keys and values: bf16 for a bf16 geometry, else fp16."""
-        return torch.bfloat16 if self.block_info.dtype == torch.bfloat16 else torch.float16
+        held = None if contigious_kv_tensor is None else contigious_kv_tensor[0].dtype
+        if dtype is None:
+            dtype = torch.bfloat16 if held == torch.bfloat16 else torch.float16
+        elif dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError("KV blocks hold fp16 or bf16")
+        elif held is not None and held != dtype:
+            raise TypeError(f"the contiguous backing holds {held}, not {dtype}")
+        self.dtype = dtype
 
     @property
     def is_contigious(self) -> bool:

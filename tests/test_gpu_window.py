@@ -313,6 +313,55 @@ def test_no_window_is_paged_attention(hip_device):
     assert torch.allclose(out.float(), ref.float(), rtol=2 ** -10, atol=2 ** -13)
 
 
+def test_fp16_rows_of_a_geometry_given_with_bf16(hip_device):
+    """A holder whose geometry says bf16 but whose blocks were not made so takes, gives back and
+    attends over fp16 rows."""
+    flags.BLOCK_SIZE = 16
+    info = BlockInfo(head_dim=64, num_key_value_heads=2, dtype=torch.bfloat16)
+    made = LayerBlocksHolder.create_contigious_cacher(info, 5, hip_device)
+    k, v = made.contigious_kv_tenosr
+    bare = LayerBlocksHolder(info, made.layer_key_ptr_table_device, made.layer_val_ptr_table_device,
+                             made.layer_key_ptr_table_cpu, made.layer_val_ptr_table_cpu,
+                             made.layer_key_ptr_table_list, made.layer_val_ptr_table_list)
+    g = torch.Generator().manual_seed(3)
+    rows = [torch.randn(70, 2, 64, generator=g).half().to(hip_device) for _ in range(2)]
+    q = torch.randn(1, 4, 64, generator=g).half().to(hip_device)
+    slots = torch.arange(70, device=hip_device)
+    tables = torch.arange(5, dtype=torch.int32, device=hip_device)[None]
+    lens = torch.tensor([70], dtype=torch.int32, device=hip_device)
+    for holder in (made, bare):
+        say(f"fp16 rows, geometry given with bf16, backing: {holder.is_contigious}")
+        k.zero_(), v.zero_()
+        holder.kv_tensor_to_slots_with_convert(*rows, slots)
+        back = holder.kv_tensor_from_slots_with_convert_with_create(slots)
+        a = PagedAttention(config(4, 2, 64)).forward(q, 70, lens, tables, holder)
+        b = WindowAttention(config(4, 2, 64)).forward(q, 70, lens, tables, holder)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(back, rows))
+        ref, bound = O.paged(q.cpu().double(), [0, 1], [70], tables.cpu(), k.cpu(), v.cpu(), 16, 0, 0, 64 ** -0.5)
+        ok, worst = O.within(b, ref, bound)
+        assert ok, worst
+        assert torch.allclose(a.float(), b.float(), rtol=2 ** -10, atol=2 ** -13)
+
+
+def test_bf16_rows_come_back(hip_device):
+    """Rows written to a bf16 cache and read back, bit for bit, infinities and NaN among them."""
+    for hd, kvh, bs in ((128, 8, 32), (80, 3, 16), (256, 1, 32)):
+        say(f"bf16 rows hd={hd} bs={bs}")
+        flags.BLOCK_SIZE = bs
+        info = BlockInfo(head_dim=hd, num_key_value_heads=kvh, dtype=torch.bfloat16)
+        holder = LayerBlocksHolder.create_contigious_cacher(info, 9, hip_device, torch.bfloat16)
+        g = torch.Generator().manual_seed(hd)
+        rows = [torch.randint(-2 ** 15, 2 ** 15, (77, kvh, hd), generator=g).to(torch.int16).view(torch.bfloat16).to(hip_device)
+                for _ in range(2)]
+        slots = torch.randperm(9 * bs, generator=g)[:77].to(hip_device)
+        holder.kv_tensor_to_slots_with_convert(*rows, slots)
+        back = holder.kv_tensor_from_slots_with_convert_with_create(slots)
+        torch.cuda.synchronize()
+        for x, y in zip(back, rows):
+            assert x.dtype == torch.bfloat16 and torch.equal(x.view(torch.int16), y.view(torch.int16))
+
+
 def test_long_position_and_large_cache_offsets(hip_device):
     """A stream far beyond its window, its early blocks given back, and blocks whose byte
     offset in the cache passes 2^32."""

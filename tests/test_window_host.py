@@ -208,6 +208,29 @@ def test_bf16_caches_are_refused_where_fp16_is_read():
         WindowAttention(AttentionConfig(512, 64, 8, 2, 4)).forward(q, 1, one, torch.zeros(3, 1, dtype=torch.int32), holder)
 
 
+def test_cache_type_is_the_backings_or_the_stated_one():
+    """A geometry given with bf16 alone says no more than its size: such holders take fp16 rows,
+    as before there were bf16 caches; bf16 is what the backing holds or the caller states."""
+    info, cpu = BlockInfo(head_dim=64, num_key_value_heads=2, dtype=torch.bfloat16), torch.device("cpu")
+    made = LayerBlocksHolder.create_contigious_cacher(info, 4, cpu)
+    assert made.dtype == torch.float16 == made.contigious_kv_tenosr[0].dtype
+    assert LayerBlocksHolder.create_contigious_cacher(info, 4, cpu, torch.bfloat16).dtype == torch.bfloat16
+    none, tables = torch.zeros(4, dtype=torch.int64), [0] * 4
+    args = (info, none, none, none, none, tables, tables)
+    assert LayerBlocksHolder(*args).dtype == torch.float16
+    assert LayerBlocksHolder(*args, dtype=torch.bfloat16).dtype == torch.bfloat16
+    with pytest.raises(TypeError):
+        LayerBlocksHolder(*args, dtype=torch.float32)
+    with pytest.raises(TypeError):
+        LayerBlocksHolder(*args, made.contigious_kv_tenosr, dtype=torch.bfloat16)
+    q, kv = torch.zeros(0, 8, 64, dtype=torch.float16), torch.zeros(0, 2, 64, dtype=torch.float16)
+    for holder in (made, LayerBlocksHolder(*args)):
+        with pytest.raises(TypeError):
+            holder.kv_tensor_to_slots_with_convert(kv.bfloat16(), kv.bfloat16(), torch.arange(0))
+        with pytest.raises(TypeError):
+            WindowAttention(AttentionConfig(512, 64, 8, 2, 4)).forward(q.bfloat16(), 1, none[:0], none[:0, None], holder)
+
+
 def test_oracle_against_a_masked_softmax():
     """oracle/window.py against torch's own softmax and autograd in float64."""
     g = torch.Generator().manual_seed(1)

@@ -175,14 +175,32 @@ class BlockPool:
                    refs, rest[0], min(window or 0, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1), *rest[1:])
         return new
 
-    def compact(self, state: BlockState) -> Tuple[BlockState, torch.Tensor]:
+    def compact(self, state: BlockState, held: Optional[torch.Tensor] = None):
         """The live blocks moved, in every layer, into the numbers below their count, which
         is returned too (int32 [1], on the device): the blocks from there on are free, and
-        their memory may go elsewhere."""
+        their memory may go elsewhere.  Blocks that ``refs`` counts for a holder outside the
+        tables (a cache of prefixes) move like any other: ``held`` gives their numbers (integers
+        of any shape), and the numbers they have now (int32) are the third result."""
         rows, width = self._check(state)
-        new, ws = self._next(state), self._workspace(rows)
+        extra = 0
+        if held is not None:
+            if held.device != self.device or held.is_floating_point():
+                raise ValueError(f"held must be integers on {self.device}")
+            # as rows of the tables, without tokens
+            wide = max(width, 1)
+            extra = -(-held.numel() // wide)
+            tables = torch.full((rows + extra, wide), -1, dtype=torch.int32, device=self.device)
+            tables[:rows, :width] = state.block_tables
+            tables[rows:].view(-1)[:held.numel()] = held.reshape(-1)
+            lens = torch.cat([state.context_lens, state.context_lens.new_zeros(extra)])
+            state = BlockState(tables, lens, state.refs)
+        new, ws = self._next(state), self._workspace(rows + extra)
         live = torch.empty(1, dtype=torch.int32, device=self.device)
-        self._call("dw4_compact_blocks", *self._layer_args(), self.part_bytes, rows, width,
+        self._call("dw4_compact_blocks", *self._layer_args(), self.part_bytes, *state.block_tables.shape,
                    self.num_blocks, *self._pointers(state, new), live.data_ptr(), ws.data_ptr(),
                    ws.numel())
-        return new, live
+        if held is None:
+            return new, live
+        now = new.block_tables[rows:].reshape(-1)[:held.numel()].view(held.shape)
+        return new._replace(block_tables=new.block_tables[:rows, :width].contiguous(),
+                            context_lens=new.context_lens[:rows]), live, now

@@ -607,7 +607,8 @@ int dw4_free_blocks(int num_rows, int max_blocks, int num_blocks, int block_size
 
 /* The live blocks (refs > 0; *live of them, int32 device [1]) moved into the numbers
  * below *live: the lowest free number takes the lowest block from *live on, and so
- * forth; tables and refs follow. */
+ * forth; tables and refs follow.  Blocks that refs counts for a holder outside the
+ * tables move too: to learn where, give their numbers as rows of the tables, of length 0. */
 int dw4_compact_blocks(int num_layers, const int64_t* layer_key_ptrs,
                        const int64_t* layer_value_ptrs, int64_t part_bytes, int num_rows,
                        int max_blocks, int num_blocks, const int32_t* tables, const int32_t* lens,

@@ -187,6 +187,36 @@ def test_compact(hip_device, rows, width, blocks, bs):
     assert all(torch.equal(a, b) for a, b in zip(contents(held), before))
 
 
+@pytest.mark.parametrize("rows,width,blocks,count", [(5, 9, 200, 30), (1, 7, 40, 1), (3, 4, 50, 0), (0, 4, 60, 9), (4, 0, 60, 9)])
+def test_compact_tells_where_held_blocks_went(hip_device, rows, width, blocks, count):
+    """Blocks counted for a holder outside the tables: their contents are found at the numbers
+    returned; numbers that are no block stay what they are."""
+    rng = random.Random(blocks)
+    pool, layers = make_pool(hip_device, blocks, layers=2, kvh=1)
+    tables, lens, refs = random_state(rng, rows, width, blocks, 16)
+    free = [p for p in range(blocks) if refs[p] == 0]
+    held = rng.sample(free, count)
+    for p in held:
+        refs[p] += 1
+    if count > 2:
+        held[0], held[2] = -1, blocks       # (their old blocks stay counted)
+    say(f"compact with {count} blocks held outside, {rows} rows of {width}")
+    before = contents(layers)
+    got, live, now = pool.compact(to_state(hip_device, tables, lens, refs, width),
+                                  torch.tensor(held, dtype=torch.int64, device=hip_device))
+    want_tables, want_refs, want_live, pairs = B.compact(tables, refs)
+    check_state(got, want_tables, lens, want_refs, 0)
+    assert got.block_tables.shape == (rows, width) and live.tolist() == [want_live]
+    to = dict(pairs)
+    assert now.dtype == torch.int32 and now.tolist() == [to.get(p, p) for p in held]
+    for old, p in zip(held, now.tolist()):
+        if 0 <= old < blocks:
+            assert p < want_live
+            assert all(torch.equal(a[p], b[old]) for a, b in zip(contents(layers), before))
+    # the state goes on into other calls
+    pool.extend(got, torch.zeros(rows, dtype=torch.int32, device=hip_device))
+
+
 @pytest.mark.parametrize("kvh,hd,bs,dtype", [(1, 64, 16, torch.float16), (3, 80, 16, torch.bfloat16),
                                              (32, 128, 32, torch.float16), (2, 256, 32, torch.bfloat16)])
 def test_copy(hip_device, kvh, hd, bs, dtype):

@@ -9,7 +9,7 @@ whatever their distance.  No counterpart in the reference; it stands beside
   of ``PagedAttention.forward``;
 * ``prefill``  several new tokens per sequence over the same cache;
 * ``dense``    packed sequences whose keys and values stand beside the queries,
-  with gradients.
+  with gradients (the cached calls have none: a backward pass through them raises).
 
 All take fp16 or bf16 and any number of query heads per kv head.  Every call
 runs on the current stream of its tensors' device, never synchronises, and may
@@ -78,6 +78,19 @@ def _ints(x: torch.Tensor, count: int, device: torch.device, name: str) -> torch
     if x.dim() != 1 or x.numel() != count or x.device != device or x.is_floating_point():
         raise ValueError(f"{name} must be {count} integers on the queries' device")
     return _int32(x)
+
+
+class _NoGradient(torch.autograd.Function):
+    """The cached calls have no backward pass: one that reaches them fails instead of
+    finding no gradient."""
+
+    @staticmethod
+    def forward(ctx, query, output):
+        return output.detach()  # (of the same memory: a given output stays outside the graph)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("windowed attention over a cache has no gradients (WindowAttention.dense has)")
 
 
 class WindowAttention:
@@ -161,6 +174,8 @@ class WindowAttention:
                       tables.shape[1], lens.data_ptr(), int(context_len_max),
                       None if ws is None else ws.data_ptr(), nbytes,
                       _lib.current_stream(device.index))
+        if query.requires_grad and torch.is_grad_enabled():
+            return _NoGradient.apply(query, output)
         return output
 
     def dense(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: torch.Tensor,

@@ -692,6 +692,32 @@ def test_captured_and_replayed(hip_device):
             assert torch.equal(a.view(torch.int16), b.view(torch.int16)), r
 
 
+def test_no_gradient_through_a_cache(hip_device):
+    """Queries that require a gradient: the call runs, also into a given output, and a backward
+    pass through it raises."""
+    holder, g = cache(hip_device, 4, 2, 64, 32, torch.float16, 1)
+    att = WindowAttention(config(4, 2, 64), 8, 1)
+    lens = torch.tensor([40, 7], dtype=torch.int32, device=hip_device)
+    tables = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=hip_device)
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=hip_device)
+    q = torch.randn(2, 4, 64, generator=g).half().to(hip_device)
+    say("no gradient through a cache")
+    want = att.forward(q, 40, lens, tables, holder)
+    x = q.clone().requires_grad_(True)
+    given = torch.empty_like(q)
+    for y in (att.forward(x, 40, lens, tables, holder), att.prefill(x * 1, starts, 1, 40, lens, tables, holder),
+              att.forward(x, 40, lens, tables, holder, output=given)):
+        assert torch.equal(y.detach(), want)
+        with pytest.raises(RuntimeError, match="no gradients"):
+            y.sum().backward()
+    assert given.data_ptr() == y.data_ptr() and not given.requires_grad and x.grad is None
+    both = (att.forward(x, 40, lens, tables, holder) + x).sum()  # beside a path that has gradients
+    with pytest.raises(RuntimeError, match="no gradients"):
+        both.backward()
+    with torch.no_grad():
+        assert not att.forward(x, 40, lens, tables, holder).requires_grad
+
+
 def test_two_streams(hip_device):
     """Two calls of one object at once, each on a stream of its own."""
     dev = hip_device

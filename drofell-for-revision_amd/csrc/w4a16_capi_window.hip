@@ -86,7 +86,9 @@ int dw4_window_attention(int dtype, int num_seqs, int num_heads, int num_kv_head
   if (!good_scale(scale) || max_context_len < 0 || max_blocks_per_seq < 0 || num_blocks < 0) return DW4_ERR_INVALID_ARG;
   if (query_starts == nullptr && (total_rows != num_seqs || max_query_len != 1)) return DW4_ERR_INVALID_ARG;
   if (num_seqs == 0 || total_rows == 0 || max_query_len == 0) return DW4_OK;
-  if (!query || !out || !key_block_ptrs || !value_block_ptrs || !block_tables || !context_lens) return DW4_ERR_INVALID_ARG;
+  if (!query || !out || !context_lens) return DW4_ERR_INVALID_ARG;
+  if ((num_blocks > 0 && (!key_block_ptrs || !value_block_ptrs)) || (max_blocks_per_seq > 0 && !block_tables))
+    return DW4_ERR_INVALID_ARG;
   const int64_t row = (int64_t)num_heads * head_size;
   if (q_stride < row || o_stride < row || kv_head_stride < block_size * head_size ||
       (int64_t)max_blocks_per_seq * block_size < max_context_len || (int64_t)max_blocks_per_seq * block_size > dw4::kWinMaxWindow)

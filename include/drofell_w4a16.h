@@ -505,7 +505,8 @@ int dw4_rope_and_cache(int num_seqs, int num_heads, int num_kv_heads, int head_d
  * addresses 16-byte aligned; a table entry outside 0 .. num_blocks - 1 means
  * that the block is not there (freed behind the window): its tokens are not
  * seen, and nothing is read.  Keys and values of tokens that a row does not see
- * do not reach it, whatever they hold.  context_lens at most max_context_len.
+ * do not reach it, whatever they hold.  context_lens at most max_context_len.  A cache
+ * without blocks has no pointer tables, and tables without columns no address.
  * workspace: dw4_window_attention_workspace_size bytes (0 for most calls). */
 int dw4_window_attention(int dtype, int num_seqs, int num_heads, int num_kv_heads, int head_size,
                          int block_size, int num_blocks, const uint16_t* query, int64_t q_stride,

@@ -743,6 +743,23 @@ def test_two_streams(hip_device):
             assert torch.equal(y, want[i])
 
 
+def test_tables_without_columns_and_caches_without_blocks(hip_device):
+    """Empty contexts give zeros also where there is no table entry, or no block, at all."""
+    dev = hip_device
+    att = WindowAttention(config(4, 2, 64), 8, 1)
+    lens = torch.zeros(2, dtype=torch.int32, device=dev)
+    starts = torch.tensor([0, 1, 41], dtype=torch.int32, device=dev)
+    for blocks, width in ((2, 0), (0, 0), (0, 3)):
+        holder, _ = cache(dev, blocks, 2, 64, 32, torch.float16, 1)
+        tab = torch.full((2, width), -1, dtype=torch.int32, device=dev)
+        q = torch.ones(41, 4, 64, dtype=torch.float16, device=dev)
+        say(f"{blocks} blocks, tables of {width} columns")
+        out = torch.ones_like(q)
+        assert not att.forward(q[:2], 0, lens, tab, holder, output=out[:2]).any()
+        out.fill_(1)
+        assert not att.prefill(q, starts, 40, 0, lens, tab, holder, output=out).any()
+
+
 def test_empty_calls(hip_device):
     say("empty calls")
     dev = hip_device

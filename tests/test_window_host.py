@@ -55,6 +55,13 @@ def test_window_attention_refusals():
     assert size(0, 8, 2, 128, 16, 0, 5, 7, 2, 1000, ctypes.byref(out)) == OK and out.value == 0
 
 
+def test_window_attention_without_blocks_or_columns():
+    """No address is asked for what has no entries (the calls go on to the next refusal)."""
+    assert paged(tab=None, width=0, ctx=0, window=0, o=ODD) == MISAL
+    assert paged(kp=None, nb=0, o=ODD) == MISAL
+    assert paged(tab=None, width=0, ctx=1) == BAD
+
+
 def dense(back=False, dtype=1, seqs=2, heads=8, kvh=4, hd=64, q=FAKE, qs=512, k=FAKE, ks=256, o=FAKE, starts=FAKE, rows=100,
           most=60, scale=0.1, window=0, sinks=0, lse=FAKE, rest=FAKE, do=FAKE, dk=FAKE, dks=256, ws=FAKE, wsb=1 << 20):
     lib = _lib.load()

@@ -29,6 +29,7 @@ int check_window(int dtype, int num_seqs, int num_heads, int num_kv_heads, int h
   // rows of (token, head) and workgroups are counted in 32 bits
   const int64_t G = num_heads / num_kv_heads;
   if (G > 1024 || (int64_t)total_rows * num_heads > (int64_t)1 << 26) return DW4_ERR_UNSUPPORTED;
+  max_query = max_query < total_rows ? max_query : total_rows;  // (a bound that the caller may have taken wide)
   const int64_t tiles = (max_query * G + 31) / 32 + 1;
   if ((int64_t)num_seqs * num_kv_heads > INT32_MAX / 4 || (int64_t)num_seqs * num_kv_heads * tiles > INT32_MAX / 4 ||
       (int64_t)num_seqs * max_query * num_heads > INT32_MAX)

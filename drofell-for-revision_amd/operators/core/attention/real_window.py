@@ -74,6 +74,11 @@ def _int32(x: torch.Tensor) -> torch.Tensor:
     return x.to(torch.int32).contiguous()
 
 
+def _bound(n: int) -> int:
+    """An upper bound as the library takes it (longer than any sequence is as good)."""
+    return min(int(n), 2 ** 31 - 1)
+
+
 def _ints(x: torch.Tensor, count: int, device: torch.device, name: str) -> torch.Tensor:
     if x.dim() != 1 or x.numel() != count or x.device != device or x.is_floating_point():
         raise ValueError(f"{name} must be {count} integers on the queries' device")
@@ -147,7 +152,7 @@ class WindowAttention:
             raise ValueError("cache and block tables must be on the queries' device")
         if block_tables.dim() != 2 or block_tables.shape[0] != num_seqs or block_tables.is_floating_point():
             raise ValueError("block_tables must hold one row of block numbers per sequence")
-        rows = query.shape[0]
+        rows, query_len_max, context_len_max = query.shape[0], _bound(query_len_max), _bound(context_len_max)
         lens = _ints(context_lens, num_seqs, device, "context_lens")
         starts = None if query_starts is None else _ints(query_starts, num_seqs + 1, device, "query_starts")
         if output is None:
@@ -161,17 +166,17 @@ class WindowAttention:
             q = _rows(query)
             nbytes = _lib.window_attention_workspace_size(
                 num_seqs, cfg.num_query_heads, cfg.num_key_value_heads, cfg.head_dim,
-                flags.BLOCK_SIZE, rows, int(query_len_max), self._window, self._sinks,
-                int(context_len_max), device.index)
+                flags.BLOCK_SIZE, rows, query_len_max, self._window, self._sinks,
+                context_len_max, device.index)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
             _lib.call("dw4_window_attention", dtype, num_seqs, cfg.num_query_heads,
                       cfg.num_key_value_heads, cfg.head_dim, flags.BLOCK_SIZE,
                       kv_cacher.layer_key_ptr_table_device.numel(), q.data_ptr(), _stride(q),
                       output.data_ptr(), _stride(output), None if starts is None else starts.data_ptr(),
-                      rows, int(query_len_max), kv_cacher.layer_key_ptr_table_device.data_ptr(),
+                      rows, query_len_max, kv_cacher.layer_key_ptr_table_device.data_ptr(),
                       kv_cacher.layer_val_ptr_table_device.data_ptr(), info.head_stride,
                       float(self.scale), self._window, self._sinks, tables.data_ptr(),
-                      tables.shape[1], lens.data_ptr(), int(context_len_max),
+                      tables.shape[1], lens.data_ptr(), context_len_max,
                       None if ws is None else ws.data_ptr(), nbytes,
                       _lib.current_stream(device.index))
         if query.requires_grad and torch.is_grad_enabled():
@@ -197,7 +202,7 @@ class WindowAttention:
         if seq_starts.numel() < 1:
             raise ValueError("seq_starts must hold one entry more than there are sequences")
         starts = _ints(seq_starts, seq_starts.numel(), q.device, "seq_starts")
-        return _WindowDense.apply(q, k, v, starts, int(seq_len_max), self)
+        return _WindowDense.apply(q, k, v, starts, _bound(seq_len_max), self)
 
 
 class _WindowDense(torch.autograd.Function):

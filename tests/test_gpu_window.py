@@ -760,6 +760,27 @@ def test_tables_without_columns_and_caches_without_blocks(hip_device):
         assert not att.prefill(q, starts, 40, 0, lens, tab, holder, output=out).any()
 
 
+def test_wide_bounds(hip_device):
+    """Bounds far above the lengths, past 32 bits too: the same results."""
+    dev = hip_device
+    holder, g = cache(dev, 10, 2, 64, 32, torch.bfloat16, 1)
+    att = WindowAttention(config(4, 2, 64), 20, 1)
+    starts = torch.tensor([0, 50, 51], dtype=torch.int32, device=dev)
+    lens = torch.tensor([60, 90], dtype=torch.int32, device=dev)
+    tables = torch.arange(6, dtype=torch.int32, device=dev).view(2, 3)
+    q, k, v, dout = [t.to(dev) for t in leaves(g, [50, 1], 4, 2, 64, torch.bfloat16)]
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    results = []
+    for most in (50, 51, 2 ** 20, 2 ** 31 - 1, 2 ** 32, 2 ** 40):
+        say(f"bound {most}")
+        out = att.dense(*x, starts, most)
+        results.append([att.prefill(q.detach(), starts, most, 90, lens, tables, holder), out.detach(),
+                        *torch.autograd.grad(out, x, dout)])
+    torch.cuda.synchronize()
+    for r in results[1:]:
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(r, results[0]))
+
+
 def test_empty_calls(hip_device):
     say("empty calls")
     dev = hip_device

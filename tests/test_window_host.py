@@ -62,6 +62,16 @@ def test_window_attention_without_blocks_or_columns():
     assert paged(tab=None, width=0, ctx=1) == BAD
 
 
+def test_wide_bounds_are_taken():
+    """Lengths bounded by more than there are rows: the limits count the rows (the calls go on to the
+    next refusal)."""
+    assert paged(most=1 << 30, o=ODD) == MISAL
+    assert paged(seqs=1000, rows=5000, most=1 << 20, o=ODD) == MISAL
+    assert dense(most=2 ** 31 - 1, q=ODD) == MISAL
+    assert dense(back=True, most=2 ** 31 - 1, q=ODD) == MISAL
+    assert paged(seqs=1 << 26, rows=1 << 20, most=9) == UNSUP  # (sequence, kv head) pairs in 32 bits
+
+
 def dense(back=False, dtype=1, seqs=2, heads=8, kvh=4, hd=64, q=FAKE, qs=512, k=FAKE, ks=256, o=FAKE, starts=FAKE, rows=100,
           most=60, scale=0.1, window=0, sinks=0, lse=FAKE, rest=FAKE, do=FAKE, dk=FAKE, dks=256, ws=FAKE, wsb=1 << 20):
     lib = _lib.load()

@@ -25,6 +25,7 @@ import torch
 from hip_extends import _lib
 
 from ... import flags
+from ..block.common import int32
 from ..block.real import LayerBlocksHolder
 from .common import AttentionConfig
 
@@ -68,21 +69,15 @@ def _like(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
-def _int32(x: torch.Tensor) -> torch.Tensor:
-    if x.dtype is torch.int32 and x.is_contiguous():
-        return x
-    return x.to(torch.int32).contiguous()
-
-
 def _bound(n: int) -> int:
     """An upper bound as the library takes it (longer than any sequence is as good)."""
     return min(int(n), 2 ** 31 - 1)
 
 
 def _ints(x: torch.Tensor, count: int, device: torch.device, name: str) -> torch.Tensor:
-    if x.dim() != 1 or x.numel() != count or x.device != device or x.is_floating_point():
+    if x.dim() != 1 or x.numel() != count or x.device != device:
         raise ValueError(f"{name} must be {count} integers on the queries' device")
-    return _int32(x)
+    return int32(x, name)
 
 
 class _NoGradient(torch.autograd.Function):
@@ -150,7 +145,7 @@ class WindowAttention:
             raise TypeError(f"queries of {query.dtype} over a cache of {kv_cacher.dtype}")
         if kv_cacher.device != device or block_tables.device != device:
             raise ValueError("cache and block tables must be on the queries' device")
-        if block_tables.dim() != 2 or block_tables.shape[0] != num_seqs or block_tables.is_floating_point():
+        if block_tables.dim() != 2 or block_tables.shape[0] != num_seqs:
             raise ValueError("block_tables must hold one row of block numbers per sequence")
         rows, query_len_max, context_len_max = query.shape[0], _bound(query_len_max), _bound(context_len_max)
         lens = _ints(context_lens, num_seqs, device, "context_lens")
@@ -161,7 +156,7 @@ class WindowAttention:
             raise ValueError("output must have the queries' shape, type and device")
         elif _rows(output) is not output:
             raise ValueError("output rows must be contiguous and 16-byte aligned")
-        tables = _int32(block_tables)
+        tables = int32(block_tables, "block_tables")
         with _on(device):
             q = _rows(query)
             nbytes = _lib.window_attention_workspace_size(

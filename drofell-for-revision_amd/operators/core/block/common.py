@@ -16,6 +16,18 @@ import torch
 from ... import flags
 
 
+def int32(x: torch.Tensor, name: str) -> torch.Tensor:
+    """Integers as the library reads them; those outside 32 bits become the nearest ones inside,
+    so that no number that is no block, row or position turns into one that is."""
+    if x.dtype is torch.int32:
+        return x if x.is_contiguous() else x.contiguous()
+    if x.dtype is torch.int64:
+        x = x.clamp(-2 ** 31, 2 ** 31 - 1)
+    elif x.dtype not in (torch.int16, torch.int8, torch.uint8, torch.bool):
+        raise ValueError(f"{name} must be integers")
+    return x.to(torch.int32).contiguous()
+
+
 @dataclass
 class BlockInfo:
     head_dim: int

@@ -24,6 +24,7 @@ import torch
 from hip_extends import _lib
 
 from ... import flags
+from .common import int32
 from .real import LayerBlocksHolder
 
 
@@ -92,9 +93,9 @@ class BlockPool:
         return rows, width
 
     def _by_row(self, x: torch.Tensor, rows: int, name: str) -> torch.Tensor:
-        if x.shape != (rows,) or x.device != self.device or x.is_floating_point():
+        if x.shape != (rows,) or x.device != self.device:
             raise ValueError(f"{name} must be one integer per row on {self.device}")
-        return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+        return int32(x, name)
 
     def _next(self, state: BlockState) -> BlockState:
         return BlockState(torch.empty_like(state.block_tables), torch.empty_like(state.context_lens),
@@ -129,9 +130,9 @@ class BlockPool:
         """Block pairs[i, 0] copied to pairs[i, 1] in every layer (int32 [n, 2]; a pair with
         a number outside the pool is skipped).  No block may be written twice, or written
         and read."""
-        if pairs.dim() != 2 or pairs.shape[1] != 2 or pairs.device != self.device or pairs.is_floating_point():
+        if pairs.dim() != 2 or pairs.shape[1] != 2 or pairs.device != self.device:
             raise ValueError(f"pairs must be integers [n, 2] on {self.device}")
-        p = pairs.to(torch.int32).contiguous()
+        p = int32(pairs, "pairs")
         n, kt, vt = self._layer_args()
         self._call("dw4_copy_blocks", n, kt, vt, self.num_blocks, self.part_bytes, p.shape[0],
                    p.data_ptr())
@@ -184,14 +185,14 @@ class BlockPool:
         rows, width = self._check(state)
         extra = 0
         if held is not None:
-            if held.device != self.device or held.is_floating_point():
+            if held.device != self.device:
                 raise ValueError(f"held must be integers on {self.device}")
             # as rows of the tables, without tokens
             wide = max(width, 1)
             extra = -(-held.numel() // wide)
             tables = torch.full((rows + extra, wide), -1, dtype=torch.int32, device=self.device)
             tables[:rows, :width] = state.block_tables
-            tables[rows:].view(-1)[:held.numel()] = held.reshape(-1)
+            tables[rows:].view(-1)[:held.numel()] = int32(held, "held").reshape(-1)
             lens = torch.cat([state.context_lens, state.context_lens.new_zeros(extra)])
             state = BlockState(tables, lens, state.refs)
         new, ws = self._next(state), self._workspace(rows + extra)

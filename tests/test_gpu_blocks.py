@@ -234,6 +234,25 @@ def test_copy(hip_device, kvh, hd, bs, dtype):
     assert all(torch.equal(a, b) for a, b in zip(contents(held), before))
 
 
+def test_numbers_past_32_bits(hip_device):
+    """64-bit numbers of no block and no row, whose low 32 bits name one, and tokens by the
+    billion: skipped, ended, missing."""
+    pool, held = make_pool(hip_device, 6, bs=16)
+    before = contents(held)
+    say("numbers past 32 bits")
+    pool.copy(torch.tensor([[2 ** 32, 3], [1, 2 ** 33 + 4], [-2 ** 32 + 2, 5]], device=hip_device))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(contents(held), before))
+    tables, lens, refs = [[0, 1], [2, -1]], [20, 5], [1, 1, 1, 0, 0, 0]
+    state = to_state(hip_device, tables, lens, refs, 2)
+    *want, _ = B.fork(tables, lens, refs, [-1, 1], 16)
+    check_state(pool.fork(state, torch.tensor([2 ** 32, 1], device=hip_device)), *want)
+    got = pool.extend(state, torch.tensor([2 ** 32, 2 ** 40 + 1], device=hip_device))
+    assert got.shortage.item() > 2 ** 27 and got.context_lens.tolist() == lens and got.block_tables.tolist() == tables
+    got = pool.extend(state, torch.tensor([-2 ** 32 + 9, 0], device=hip_device))
+    check_state(got, tables, lens, refs, 0)
+
+
 def test_separately_allocated_blocks(hip_device):
     """Layers whose blocks were allocated one by one (pointer tables without contiguous backing)."""
     flags.BLOCK_SIZE = 16

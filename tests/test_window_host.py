@@ -12,7 +12,7 @@ from hip_extends import _lib
 from operators.core.attention.common import AttentionConfig
 from operators.core.attention.real_page import PagedAttention
 from operators.core.attention.real_window import WindowAttention
-from operators.core.block.common import BlockInfo
+from operators.core.block.common import BlockInfo, int32
 from operators.core.block.pool import BlockPool
 from operators.core.block.real import LayerBlocksHolder
 from oracle import blocks as B
@@ -246,6 +246,19 @@ def test_cache_type_is_the_backings_or_the_stated_one():
             holder.kv_tensor_to_slots_with_convert(kv.bfloat16(), kv.bfloat16(), torch.arange(0))
         with pytest.raises(TypeError):
             WindowAttention(AttentionConfig(512, 64, 8, 2, 4)).forward(q.bfloat16(), 1, none[:0], none[:0, None], holder)
+
+
+def test_integers_outside_32_bits_stay_outside_every_range():
+    """Not cut to their low bits, which may name a block, a row or a length."""
+    x = torch.tensor([5, -1, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 40 + 3, -2 ** 32 + 3, -2 ** 63])
+    top, low = 2 ** 31 - 1, -2 ** 31
+    assert int32(x, "x").tolist() == [5, -1, top, top, top, top, low, low] and int32(x, "x").dtype == torch.int32
+    assert int32(x[:3].int(), "x").tolist() == [5, -1, top]
+    assert int32(torch.tensor([True, False]), "x").tolist() == [1, 0]
+    assert int32(torch.arange(6).view(3, 2).T.int(), "x").is_contiguous()
+    for bad in (torch.float32, torch.complex64, torch.uint64):
+        with pytest.raises(ValueError):
+            int32(torch.zeros(3).to(bad), "x")
 
 
 def test_oracle_against_a_masked_softmax():

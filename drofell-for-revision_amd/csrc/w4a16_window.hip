@@ -1,6 +1,6 @@
 // Windowed attention of few rows over a paged KV cache: decode steps, and up
-// to 32 rows (new tokens x query heads of a kv head) at a time of short
-// prompts and drafts.
+// to 32 rows (new tokens x query heads) per kv head of short prompts and
+// drafts.
 //
 //   out[i][h] = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max),
 // over the tokens j <= i with j > i - window or j < sinks, positions i counted
@@ -40,26 +40,22 @@ namespace {
 
 template <int HS, int BS, bool BF, int W>
 __global__ void __launch_bounds__(W * 64, W == 8 || HS <= 128 ? 2 : 1)
-window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restrict__ ws_ml,
-                   float* __restrict__ ws_out) {
+window_rows_kernel(WindowArgs a, int splits, int cols, float* __restrict__ ws_ml, float* __restrict__ ws_out) {
   constexpr int KD = HS / 16;         // 16-dim reduction steps of q . k
   constexpr int ND = (HS + 31) / 32;  // 32-dim tiles of p . v (the last may be half empty)
   constexpr int NB = 32 / BS;         // blocks of a step
   constexpr bool VTAIL = HS % 32 != 0;
   extern __shared__ __attribute__((aligned(16))) float sm[];
 
-  int pair, item;
-  if (!work_of(blockIdx.x, a.num_seqs * a.num_kv_heads, tiles * splits, pair, item)) return;
-  const int split = item % splits;
-  const int tile = item / splits;
+  int pair, split;
+  if (!work_of(blockIdx.x, a.num_seqs * a.num_kv_heads, splits, pair, split)) return;
   const int seq = pair / a.num_kv_heads, kvh = pair % a.num_kv_heads;
   const int G = a.num_heads / a.num_kv_heads;
   int q0, q1;
   seq_rows(a.starts, seq, a.total_rows, q0, q1);
   const int n = min(q1 - q0, a.max_query);
-  const int rows = n * G, base = tile * kWinRowsTile;
-  if (base >= rows) return;
-  const int nrows = min(kWinRowsTile, rows - base);
+  const int nrows = n * G;  // at most kWinRowsTile
+  if (nrows <= 0) return;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -67,13 +63,13 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restr
   const int len = a.lens[seq];
   const int cap = min(len, a.max_blocks * BS);  // a table shorter than the context ends it
   const int p0 = len - (q1 - q0);                // position of the first new token
-  const Span span = Span::of<32>(p0 + base / G, p0 + (base + nrows - 1) / G, cap, a.window, a.sinks);
+  const Span span = Span::of<32>(p0, p0 + n - 1, cap, a.window, a.sinks);
   const int per = (span.steps + splits - 1) / splits;
   const int s0 = split * per, s1 = min(span.steps, s0 + per);
   const int nsw = s0 + wave < s1 ? (s1 - s0 - wave + W - 1) / W : 0;  // this wave's steps
 
-  // row c of the tile (rows past the last repeat it; they are not stored)
-  const int row = base + min(c, nrows - 1);
+  // row c (rows past the last repeat it; they are not stored)
+  const int row = min(c, nrows - 1);
   const int pos = p0 + row / G;
   const int last = min(pos, cap - 1), before = a.window == 0 ? INT32_MIN : pos - a.window;
 
@@ -151,9 +147,8 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restr
 #pragma unroll
     for (int j = 0; j < KD; ++j) s = mfma32_of<BF>(kreg[j], qreg[j], s);
     // every row sees every token of the step?
-    const int first_pos = p0 + base / G, last_pos = p0 + (base + nrows - 1) / G;
-    const bool full = held == (1u << NB) - 1 && t + 31 <= min(first_pos, cap - 1) &&
-                      (a.window == 0 || t > last_pos - a.window || t + 31 < a.sinks);
+    const bool full = held == (1u << NB) - 1 && t + 31 <= min(p0, cap - 1) &&
+                      (a.window == 0 || t > p0 + n - 1 - a.window || t + 31 < a.sinks);
     uint32_t seen = 0xFFFF;  // bit e: score e
     if (!full) {
       seen = own_scores(seen_of(t, last, before, a.sinks), half);
@@ -261,7 +256,7 @@ window_rows_kernel(WindowArgs a, int tiles, int splits, int cols, float* __restr
       sum += f * ml[(w * cols + r) * 2 + 1];
       acc += f * red[(w * cols + r) * HS + d];
     }
-    const int at = base + r, token = q0 + at / G, head = kvh * G + at % G;
+    const int token = q0 + r / G, head = kvh * G + r % G;
     if (splits == 1) {
       const float y = sum == 0.f ? acc : acc / sum;  // no visible token: zeros
       a.out[(size_t)token * a.o_stride + (size_t)head * HS + d] = (uint16_t)pack2<BF>(y, 0.f);
@@ -319,8 +314,6 @@ window_join_kernel(WindowArgs a, int splits, const float* __restrict__ ws_ml,
       }
     }
   }
-  if (a.lse != nullptr && lane == 0)
-    a.lse[(size_t)(q0 + i) * a.num_heads + head] = gm + __builtin_amdgcn_logf(sum) - p_shift<BF>();
 #pragma unroll
   for (int d = 0; d < D; ++d)
     if (HS % 64 == 0 || lane + 64 * d < HS)
@@ -337,8 +330,7 @@ hipError_t launch_rows_w(const WindowArgs& a, const WindowPlan& p, float* ws_ml,
   auto kern = &window_rows_kernel<HS, BS, BF, W>;
   const hipError_t e = allow_lds(reinterpret_cast<const void*>(kern), win_rows_smem(HS, kWinRowsTile, W), done);
   if (e != hipSuccess) return e;
-  kern<<<win_grid(a.num_seqs * a.num_kv_heads, p.tiles * p.splits), W * 64, smem, stream>>>(a, p.tiles, p.splits, cols, ws_ml,
-                                                                                         ws_out);
+  kern<<<win_grid(a.num_seqs * a.num_kv_heads, p.splits), W * 64, smem, stream>>>(a, p.splits, cols, ws_ml, ws_out);
   return hipGetLastError();
 }
 

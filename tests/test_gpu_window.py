@@ -130,6 +130,39 @@ def test_decode_head_sizes(hip_device, hd, bs):
         check_paged(hip_device, [1, 1, 1], [1, 97, 700], 6, 2, hd, bs, dtype, 200, 5, decode=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("ctxs,heads,kvh,hd,bs", [([37, 5, 12, 40], 16, 2, 128, 32), ([3, 64, 20, 33], 18, 3, 80, 16),
+                                                  ([9, 30, 2, 50], 16, 4, 256, 32)])
+def test_decode_probabilities_in_two_parts(hip_device, ctxs, heads, kvh, hd, bs, dtype):
+    """Values that cancel, so that the output's own rounding hides little: within the bound of
+    probabilities kept to 2^-16, which one 16-bit part does not hold."""
+    say(f"two parts {ctxs} hd={hd} bs={bs} {dtype}")
+    blocks = sum((c + bs - 1) // bs for c in ctxs) + 1
+    holder, g = cache(hip_device, blocks, kvh, hd, bs, dtype, hd)
+    tables = tables_of(g, ctxs, bs, blocks)
+    kt, vt = holder.contigious_kv_tenosr
+    vt[..., 0::2], vt[..., 1::2] = 1, -1   # by token
+    q = torch.randn(len(ctxs), heads, hd, generator=g).to(dtype)
+    att = WindowAttention(config(heads, kvh, hd))
+    out = att.forward(q.to(hip_device), max(ctxs), torch.tensor(ctxs, dtype=torch.int32, device=hip_device),
+                      tables.to(hip_device), holder)
+    torch.cuda.synchronize()
+    ref, bound = O.paged(q.double(), range(len(ctxs) + 1), ctxs, tables, kt.cpu(), vt.cpu(), bs, 0, 0, att.scale, rounded_p=False)
+    ok, worst = O.within(out, ref, bound)
+    assert ok, f"worst error / bound {worst:.3f}"
+    # (one part: the same from probabilities rounded to the type)
+    ratios = []
+    for s, ctx in enumerate(ctxs):
+        k, v, _ = O.slots_to_rows(kt.cpu(), vt.cpu(), tables[s], ctx, bs)
+        for h in range(heads):
+            x = h // (heads // kvh)
+            seen = torch.ones(1, ctx, dtype=torch.bool)
+            _, _, p = O.attend(q[s:s + 1, h].double(), k[:, x].double(), v[:, x].double(), seen, att.scale)
+            rough = p.to(dtype).double() @ v[:, x].double()
+            ratios.append(float(((rough - ref[s, h]).abs() / bound[s, h]).max()))
+    assert max(ratios) > 1
+
+
 PREFILL = [
     # new tokens, contexts, heads, kv heads, block size, window, sinks
     ([7, 1, 0, 3], [100, 1, 50, 3], 8, 2, 16, 0, 0),           # few rows: the rows kernel
@@ -503,7 +536,8 @@ def test_rows_beyond_the_stated_length(hip_device, lens, most, heads, kvh, hd, s
     keep = torch.cat([torch.arange(a, min(b, a + most)) for a, b in zip(starts, starts[1:])])
     rest = torch.ones(sum(lens), dtype=torch.bool)
     rest[keep] = False
-    ref, bounds = O.dense(*[t[keep].double() for t in (q, k, v, dout)], [min(n, most) for n in lens], 40, sinks, att.scale, torch.bfloat16)
+    ref, bounds = O.dense(*[t[keep].double() for t in (q, k, v, dout)], [min(n, most) for n in lens], 40, sinks,
+                          att.scale, torch.bfloat16)
     for name, y, r, b in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), ref, bounds):
         assert not y.cpu()[rest].any(), name
         ok, worst = O.within(y.cpu()[keep], r, b)
@@ -641,6 +675,84 @@ def test_strided_and_broadcast_inputs(hip_device):
     # torch sums the two heads' gradients in fp16: one more rounding
     ok, worst = O.within(grad, total, bounds[2].sum(1, keepdim=True) + 2.0 ** -11 * total.abs() * 2)
     assert ok, worst
+
+
+@pytest.mark.parametrize("far", ["q", "k and v"])
+def test_rows_far_apart(hip_device, far):
+    """Rows 16 MiB and more apart, whose offsets within a step pass 31 bits."""
+    n, heads, kvh, hd, stride = 140, 2, 1, 64, (1 << 23) + 64
+    g = torch.Generator().manual_seed(5)
+    q, k, v, dout = leaves(g, [n], heads, kvh, hd, torch.bfloat16)
+    say(f"rows of {far} {2 * stride} bytes apart")
+    flat = torch.empty(n * stride, dtype=torch.bfloat16, device=hip_device)
+
+    def spread(x, at):
+        y = flat.as_strided(x.shape, (stride, hd, 1), at)
+        y.copy_(x)
+        return y
+
+    x = [t.to(hip_device) for t in (q, k, v)]
+    d = dout.to(hip_device)
+    if far == "q":
+        x[0], d = spread(q, 0), spread(dout, 1024)
+    else:
+        x[1], x[2] = spread(k, 0), spread(v, 1024)
+    x = [t.requires_grad_(True) for t in x]
+    att = WindowAttention(config(heads, kvh, hd), 50, 2)
+    out = att.dense(*x, torch.tensor([0, n], dtype=torch.int32, device=hip_device), n)
+    grads = torch.autograd.grad(out, x, d)
+    torch.cuda.synchronize()
+    ref, bounds = O.dense(*[t.double() for t in (q, k, v, dout)], [n], 50, 2, att.scale, torch.bfloat16)
+    for name, y, r, b in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), ref, bounds):
+        ok, worst = O.within(y, r, b)
+        assert ok, f"{name}: worst error / bound {worst:.3f}"
+
+
+def test_misaligned_inputs(hip_device):
+    """Tensors that start at 2 bytes past a 16-byte unit, and rows of odd strides: the
+    results of aligned ones."""
+    n, heads, kvh, hd = 50, 4, 2, 128
+    g = torch.Generator().manual_seed(5)
+    plain = [t.to(hip_device) for t in leaves(g, [n], heads, kvh, hd, torch.float16)]
+    att = WindowAttention(config(heads, kvh, hd), 20, 1)
+    starts = torch.tensor([0, n], dtype=torch.int32, device=hip_device)
+    holder, _ = cache(hip_device, 4, kvh, hd, 32, torch.float16, 2)
+    tables = torch.arange(4, dtype=torch.int32, device=hip_device)[None]
+    lens = torch.tensor([90], dtype=torch.int32, device=hip_device)
+
+    def moved(t, pad):
+        row = t.shape[1] * t.shape[2] + pad
+        buf = torch.empty(n * row + 1, dtype=t.dtype, device=hip_device)
+        y = buf[1:].as_strided(t.shape, (row, t.shape[2], 1))
+        y.copy_(t)
+        return y
+
+    results = []
+    for place in (lambda t: t, lambda t: moved(t, 0), lambda t: moved(t, 3)):
+        say("misaligned inputs")
+        x = [place(t).requires_grad_(True) for t in plain[:3]]
+        out = att.dense(*x, starts, n)
+        results.append([out.detach(), *torch.autograd.grad(out, x, place(plain[3])),
+                        att.prefill(x[0].detach(), starts, n, 90, lens, tables, holder)])
+    torch.cuda.synchronize()
+    for r in results[1:]:
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(r, results[0]))
+    with pytest.raises(ValueError):
+        att.prefill(plain[0], starts, n, 90, lens, tables, holder, output=moved(plain[0], 0))
+
+
+@pytest.mark.parametrize("heads,kvh", [(100, 1), (130, 2), (333, 1)])
+def test_wide_groups_over_a_cache(hip_device, heads, kvh):
+    """More query heads per kv head than a tile has rows, in tiles that end inside a token's heads."""
+    for dtype in (torch.float16, torch.bfloat16):
+        say(f"{heads} heads on {kvh} over a cache {dtype}")
+        check_paged(hip_device, [1, 1], [70, 300], heads, kvh, 64, 32, dtype, 100, 3, decode=True)
+        check_paged(hip_device, [5, 17], [70, 300], heads, kvh, 64, 16, dtype, 100, 3)
+
+
+@pytest.mark.parametrize("group", [65, 77, 100, 255])
+def test_gradients_of_groups_that_no_step_holds(hip_device, group):
+    test_dense_and_gradients(hip_device, [90, 37], 2 * group, 2, 64, 50, 3, torch.bfloat16)
 
 
 def test_captured_and_replayed(hip_device):

@@ -58,7 +58,8 @@ constexpr int kGradTile = 128;  // rows of a dq workgroup, tokens of a dkv workg
 // and V.  (The largest of the factors, not of dS = P times them, which a P <= 1 only makes
 // smaller: it is known before the exponentials are.  A power of two from |dO| alone, which takes
 // no step's time, overflowed at coherent values and lost small gradients beside large ones;
-// this costs 2 % of fp16 training with heads of 128, 2 x 6000 tokens, 4 % with heads of 64 and 256.)
+// this costs 2 % of fp16 training with heads of 128, 2 x 6000 tokens, 4 % with heads of 64, 3 %
+// with heads of 256.)
 constexpr float kFirstScale = 0x1p100f;
 template <int MOST, int ND>
 __device__ __forceinline__ void keep_in_range(float (&v)[16], float& scale, f16v (&sums)[ND]) {
@@ -68,7 +69,7 @@ __device__ __forceinline__ void keep_in_range(float (&v)[16], float& scale, f16v
   if (__any(top * scale > (float)(1 << MOST))) {
     top = both_max(top);
     const float to = top * scale > (float)(1 << MOST) ? __builtin_amdgcn_ldexpf(1.f, MOST - 3 - __builtin_amdgcn_frexp_expf(top)) : scale;
-    const float f = to * __builtin_amdgcn_rcpf(scale);  // (exact: powers of two)
+    const float f = __builtin_amdgcn_ldexpf(to, 1 - __builtin_amdgcn_frexp_expf(scale));  // to / scale, powers of two
 #pragma unroll
     for (int d = 0; d < ND; ++d) sums[d] *= f;
     scale = to;
@@ -428,7 +429,7 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, uint32_t magic, const float* _
 #pragma unroll
     for (int e = 0; e < 16; ++e) ds[e] *= pr[e];
     if (!full) {
-      const int own = HS <= 128 ? wa + (thread_again() & 31) : wa + c;
+      const int own = wa + (thread_again() & 31);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int i = ((const int*)(st + 2 * TILE))[2 * kDkvRows + 16 * (e / 8) + 8 * half + e % 8];

@@ -28,7 +28,11 @@
 // as two 16-bit parts, over operands that are in registers already, and delta
 // sums the forward's output and what its rounding left off.  (With one part
 // and the rounded output alone dq and dk were 1.7 times as far from float64 as their
-// own rounding is.)  fp16 holds neither small probabilities nor small or large gradients,
+// own rounding is.)  What is left of delta's error, from the forward's 16-bit
+// probabilities, is seen in a row's dS, whose sum over the tokens is zero: dq takes
+// the sum off again, by the probabilities of the row's last tokens, and dkv gets delta
+// with it.  (Else keys that share a vector, 8 times what tells them apart, put dq 7
+// times its rounding off; so it is 1.0 to 1.4 times, 1 to 2 % of the pass dearer.)  fp16 holds neither small probabilities nor small or large gradients,
 // so P goes in as 2^10 P and dS times a power of two per row (dq) or token (dkv) that
 // follows the largest of what it is summed from (keep_in_range()); bf16 needs neither.
 // A sequence's non-finite values may reach any gradient of that sequence.
@@ -62,7 +66,7 @@ constexpr int kGradTile = 128;  // rows of a dq workgroup, tokens of a dkv workg
 // with heads of 256.)
 constexpr float kFirstScale = 0x1p100f;
 template <int MOST, int ND>
-__device__ __forceinline__ void keep_in_range(float (&v)[16], float& scale, f16v (&sums)[ND]) {
+__device__ __forceinline__ void keep_in_range(float (&v)[16], float& scale, f16v (&sums)[ND], float& total) {
   float top = 0.f;
 #pragma unroll
   for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(v[e]));
@@ -72,6 +76,7 @@ __device__ __forceinline__ void keep_in_range(float (&v)[16], float& scale, f16v
     const float f = __builtin_amdgcn_ldexpf(to, 1 - __builtin_amdgcn_frexp_expf(scale));  // to / scale, powers of two
 #pragma unroll
     for (int d = 0; d < ND; ++d) sums[d] *= f;
+    total *= f;
     scale = to;
   }
 #pragma unroll
@@ -186,8 +191,7 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta) {
   }
   dl = both_sum(dl);
   const float lse = a.lse[(size_t)token * a.num_heads + head];
-  if (c < nrows && half == 0) delta[(size_t)token * a.num_heads + head] = dl;
-  float gs = BF ? 1.f : kFirstScale;
+  float gs = BF ? 1.f : kFirstScale, total = 0.f;  // total: of this lane's dS
 
   wait_loads();
   f16v dq[ND];
@@ -201,7 +205,7 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta) {
     for (int b = 0; b < 2; ++b) {
       const int tb = t + 32 * b;
       if (nrows <= 0 || tb > wlast || (a.window != 0 && tb + 31 <= wfirst - a.window && tb >= a.sinks)) continue;
-      const bool full = tb + 31 <= wfirst && (a.window == 0 || tb > wlast - a.window || tb + 31 < a.sinks);
+      const bool full = tb + 31 < wfirst && (a.window == 0 || tb > wlast - a.window || tb + 31 < a.sinks);
       f16v s = {}, p = {};
       auto products = [&](auto with) {
         feed<2 * KD, 6>(
@@ -224,13 +228,27 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta) {
         pr[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse));
         ds[e] = p[e] - dl;
       }
-      if constexpr (!BF) keep_in_range<15>(ds, gs, dq);
+      if constexpr (!BF) keep_in_range<15>(ds, gs, dq, total);
 #pragma unroll
       for (int e = 0; e < 16; ++e) ds[e] *= pr[e];
       if (!full) {
         const uint32_t seen = own_scores(seen_of(tb, pos, before, a.sinks), half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[e] = where_seen(seen, e, ds[e], 0.f);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) total += (ds[e] + ds[e + 1]) + (ds[e + 2] + ds[e + 3]);
+      // Some rows' own tokens, their last, are among these (`full` leaves them out): what all
+      // their dS sum to is known.  (Not by parts of a softmax below 2^-40.)
+      if (tb + 31 >= wfirst) {
+        const uint32_t seen = own_scores(seen_of(tb, pos, before, a.sinks), half);
+        float own = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) own += where_seen(seen, e, pr[e], 0.f);
+        own = both_sum(own);
+        const float left = both_sum(total), r = pos >= tb && pos < tb + 32 && own > 0x1p-40f ? left / own : 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[e] = fmaf(-r, where_seen(seen, e, pr[e], 0.f), ds[e]);
       }
       h8 hi[2], lo[2];
       two_parts<BF>(ds, hi[0], lo[0]);
@@ -246,14 +264,18 @@ window_dq_kernel(WindowGradArgs g, int tiles, float* __restrict__ delta) {
       for (int i = 0; i < PARTS; ++i) part(i);
     }
   }
-  if (c >= nrows) return;
+  total = both_sum(total);
+  const int thread = thread_again(), col = thread & 31, hi = thread >> 5 & 1;
+  if (col >= nrows) return;
+  const int own = wbase + col, at = q0 + own / G, to = kvh * G + own % G;
+  if (hi == 0) delta[(size_t)at * a.num_heads + to] = dl + total / gs;
   const float f = g.scale / gs;
-  uint16_t* out = g.dq + (size_t)token * g.dq_stride + (size_t)head * HS;
+  uint16_t* out = g.dq + (size_t)at * g.dq_stride + (size_t)to * HS;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
-      const int dim = d * 32 + 2 * e + 4 * half;
+      const int dim = d * 32 + 2 * e + 4 * hi;
       if (!VTAIL || dim < HS)
         *(uint2*)(out + dim) = make_uint2(pack2<BF>(dq[d][e] * f, dq[d][e + 1] * f),
                                           pack2<BF>(dq[d][e + 2] * f, dq[d][e + 3] * f));
@@ -425,7 +447,8 @@ window_dkv_kernel(WindowGradArgs g, DkvPlan plan, uint32_t magic, const float* _
       pr[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, ps - ls[0]));
       ds[e] = p[e] - ls[kDkvRows];
     }
-    if constexpr (!BF) keep_in_range<5>(ds, gs, dk);
+    float none = 0.f;
+    if constexpr (!BF) keep_in_range<5>(ds, gs, dk, none);
 #pragma unroll
     for (int e = 0; e < 16; ++e) ds[e] *= pr[e];
     if (!full) {

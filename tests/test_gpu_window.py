@@ -601,6 +601,36 @@ def test_fp16_gradients_of_large_values(hip_device, hd, kvh, lens, window):
     check_gradients(hip_device, q, k, v, torch.ones_like(dout), lens, window, 2)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("lens,heads,kvh,hd,window,sinks", [([16, 40], 4, 4, 128, 0, 0), ([300], 6, 2, 64, 0, 0),
+                                                            ([700, 33], 4, 4, 80, 200, 4), ([150], 10, 2, 256, 60, 0)])
+def test_gradients_with_keys_of_a_common_part(hip_device, lens, heads, kvh, hd, window, sinks, dtype):
+    """Keys that share a vector eight times as large as what tells them apart, as a bias makes
+    them: dS sums to zero over a row's tokens, so that the shared part must not reach dq,
+    and an error of delta, which every token of a row gets, must not bring it back.
+
+    In the 2-norm over many elements: the result's own rounding is one (relative u / sqrt(3)
+    of a mantissa of 1, 0.42 u on average).  Of the rest the largest is delta's error from the
+    forward's 16-bit probabilities, at most u / sqrt(3) = 0.58 u of what tells the keys apart, as
+    dq is: together sqrt(0.42^2 + 0.58^2) / 0.42 = 1.7.  Uncorrected it is 0.58 u times 8 beside
+    0.42 u, 5 and more."""
+    say(f"keys of a common part {lens} {heads}/{kvh} hd={hd} window={window} {dtype}")
+    g = torch.Generator().manual_seed(hd)
+    q, k, v, dout = leaves(g, lens, heads, kvh, hd, dtype)
+    k = (k.float() + 8 * torch.randn(1, kvh, hd, generator=g)).to(dtype)
+    att = WindowAttention(config(heads, kvh, hd), window or None, sinks)
+    x = [t.to(hip_device).requires_grad_(True) for t in (q, k, v)]
+    out = att.dense(*x, torch.tensor(starts_of(lens), dtype=torch.int32, device=hip_device), max(lens))
+    grads = torch.autograd.grad(out, x, dout.to(hip_device))
+    torch.cuda.synchronize()
+    ref, bounds = O.dense(*[t.double() for t in (q, k, v, dout)], lens, window, sinks, att.scale, dtype)
+    for name, y, r, b in zip(("dq", "dk", "dv"), grads, ref[1:], bounds[1:]):
+        ok, worst = O.within(y, r, b)
+        assert ok, f"{name}: worst error / bound {worst:.3f}"
+        ratio = float((y.double().cpu() - r).norm() / (r.to(dtype).double() - r).norm())
+        assert ratio < 1.7, f"{name}: {ratio:.2f} times its own rounding"
+
+
 @pytest.mark.parametrize("where", ["first", "last", "middle"])
 @pytest.mark.parametrize("n,window,hd,low", [(2048, 512, 128, -10), (1024, 200, 64, -12), (512, 64, 128, -10), (300, 0, 80, -12)])
 def test_uneven_fp16_gradients(hip_device, n, window, hd, low, where):

@@ -14,13 +14,15 @@
 // of it as the columns of 32 x 32 x 16 products; its waves take steps of 32
 // tokens round-robin, keep a running max and sum per row, and meet once in LDS.
 // Probabilities enter p . v as two 16-bit parts (22 bits of fp16's 2^10 p, 16 of
-// bf16's p): the products' time is hidden behind the stream.  Where there are
+// bf16's p): the products' time is hidden behind the stream, and so is a look at every
+// value for NaN and infinities, which take a path of their own (48 streams 146.5 us without
+// it, 146.8 with it).  Where there are
 // too few (sequence, kv head) pairs for the CUs, the steps are split among
 // workgroups, which leave max, sum and unnormalised fp32 outputs for
 // window_join_kernel, in a fixed order (deterministic).
 //
 // Measured: 48 streams, window 4096 and 4 sinks, heads 32 on 8 of 128, bf16: 800 MB
-// of cache in 143 us, 5.6 TB/s (a copy of 1 GiB reaches 5.1, reading alone 6.5).  One
+// of cache in 144 us, 5.5 TB/s (a copy of 1 GiB reaches 5.2, reading alone 6.5).  One
 // stream with window 512, where no load hides another (table, pointer, block, then
 // the join in LDS): 7 to 10 us.
 

@@ -17,11 +17,11 @@
 //     steps of 64 rows and the values in registers, 1372 us; sizes as below).
 // Both read a tile from LDS in both directions, rows in plain and columns in
 // transposing reads.  Bound by matrix cores and vector ALU together, as the forward
-// (busy 49 and 38 % of the cycles in dq, 43 and 33 % in dkv, whose copies cost 10 %:
+// (busy 48 and 42 % of the cycles in dq, 44 and 34 % in dkv, whose copies cost 10 %:
 // registers do not reach for issuing them among its products).  Measured, for
 // sequences of 6000 and 4100 tokens, 32 heads of 128, window 2048, bf16 (0.155 TFLOP a
-// product): dq 668 us for its four products (dS in two parts), dkv 940 us for its
-// five, 0.93 and 0.82 PFLOP/s.
+// product): dq 700 us for its four products (dS in two parts), dkv 955 us for its
+// five, 0.89 and 0.81 PFLOP/s; fp16 756 and 1076 us.
 //
 // Roundings: P enters its product in 16 bits, as the matrix cores take it, with
 // independent errors.  dS, whose errors would add up with those of delta, enters
@@ -32,9 +32,10 @@
 // probabilities, is seen in a row's dS, whose sum over the tokens is zero: dq takes
 // the sum off again, by the probabilities of the row's last tokens, and dkv gets delta
 // with it.  (Else keys that share a vector, 8 times what tells them apart, put dq 7
-// times its rounding off; so it is 1.0 to 1.4 times, 1 to 2 % of the pass dearer.)  fp16 holds neither small probabilities nor small or large gradients,
-// so P goes in as 2^10 P and dS times a power of two per row (dq) or token (dkv) that
-// follows the largest of what it is summed from (keep_in_range()); bf16 needs neither.
+// times its rounding off; so it is 1.0 to 1.4 times, 1 to 2 % of the pass dearer.)
+// fp16 holds neither small probabilities nor small or large gradients, so P goes in
+// as 2^10 P and dS times a power of two per row (dq) or token (dkv) that follows the
+// largest of what it is summed from (keep_in_range()); bf16 needs neither.
 // A sequence's non-finite values may reach any gradient of that sequence.
 
 #include <hip/hip_runtime.h>

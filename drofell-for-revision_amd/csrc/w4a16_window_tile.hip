@@ -15,9 +15,11 @@
 //     through LDS's transposing reads.
 // Matrix cores and vector ALU bound it together, each busy for half of the cycles at
 // the 1.8 to 1.9 GHz that the card holds under this load.  Measured: four prompts of
-// 900 to 12000 tokens, window 4096, heads 32 on 8 of 128, bf16 (1.7 TFLOP) 1726 us, 0.99
-// PFLOP/s (a 16384^3 library product 1.32); dense rows of 6000 and 4100 tokens, window
-// 2048, 32 heads of 128 (0.31 TFLOP) 415 us.  Two workgroups of four waves per CU, so that one's
+// 900 to 12000 tokens, window 4096, heads 32 on 8 of 128, bf16 (1.7 TFLOP) 1717 to 1800 us
+// from box to box, 0.95 to 1.0 PFLOP/s (a 16384^3 library product 1.32 to 1.37); dense rows of
+// 6000 and 4100 tokens, window 2048, 32 heads of 128 (0.31 TFLOP) 428 us, 0.72 PFLOP/s: its
+// spans are half as long, and their masked steps, which issue their copies at once and
+// read every value twice, weigh double.  Two workgroups of four waves per CU, so that one's
 // softmax runs beside another's products: eight waves on one step's copies won 2.6 %
 // on the prompts and lost 17 % on the dense rows, 64 rows a wave with one wave per SIMD took 11 % and
 // 45 % longer, copies issued together instead of among the products 6 % longer.
@@ -26,6 +28,8 @@
 // value type (fp16: of 2^10 p), as the matrix cores take it: their errors are
 // independent of each other, and add to the output's own rounding about as much
 // again; the denominator sums the rounded ones, so that the weights add up to 1.
+// Values of NaN and infinity reach the rows that see them and no others; where a step is
+// seen whole an infinity whose probability rounds to zero (fp16: below 2^-35) gives NaN.
 
 #include <hip/hip_runtime.h>
 

@@ -11,7 +11,7 @@ whatever their distance.  No counterpart in the reference; it stands beside
 * ``dense``    packed sequences whose keys and values stand beside the queries,
   with gradients (the cached calls have none: a backward pass through them raises).
 
-All take fp16 or bf16 and any number of query heads per kv head.  Every call
+All take fp16 or bf16 and up to 1024 query heads per kv head.  Every call
 runs on the current stream of its tensors' device, never synchronises, and may
 be captured into a graph; scratch memory is torch's, allocated per call.
 """
@@ -117,6 +117,7 @@ class WindowAttention:
                 output: Optional[torch.Tensor] = None) -> torch.Tensor:
         """query [seqs, query heads, head_dim], one new token per sequence (its key
         and value cached, ``context_lens`` counting it) -> out of the same shape.
+        ``context_len_max``, an upper bound of them, lies within the tables' columns.
         A block table entry that is no block (-1) means that the block was given
         back; an empty context gives zeros."""
         return self._paged(query, None, query.shape[0], 1, context_len_max, context_lens,

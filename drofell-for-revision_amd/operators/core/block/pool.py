@@ -150,7 +150,7 @@ class BlockPool:
         """Row r continues row parents[r] (integers [rows]; outside the rows: it ends).  Full
         blocks are shared; a half-filled last block stays with the first row that
         continues its row, if nothing else holds it, and is copied for the others, in every
-        layer, so that each row may write the slots that follow its tokens."""
+        layer, so that each row may write the slots that follow its tokens.  Up to 8192 rows."""
         rows, width = self._check(state)
         p, new, ws = self._by_row(parents, rows, "parents"), self._next(state), self._workspace(rows)
         self._call("dw4_fork_blocks", *self._layer_args(), self.part_bytes, rows, width,

@@ -488,8 +488,9 @@ int dw4_rope_and_cache(int num_seqs, int num_heads, int num_kv_heads, int head_d
  * tokens whatever their distance.  No counterpart in the reference.  Softmax
  * and both products are summed in fp32; results are deterministic.  A row that
  * sees nothing is zero.  dtype: DW4_F16 or DW4_BF16, of queries, keys, values and
- * outputs; head_size as in dw4_paged_attention, any number of query heads per
- * kv head; scale > 0.
+ * outputs; head_size as in dw4_paged_attention, up to 1024 query heads per kv head;
+ * scale > 0.  Refused as unsupported: total_rows * num_heads above 2^26, and num_seqs *
+ * min(stated length, total_rows) * num_heads of 2^31 or more.
  * ------------------------------------------------------------------------- */
 #define DW4_F16 0
 #define DW4_BF16 1

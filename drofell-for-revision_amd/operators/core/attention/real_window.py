@@ -167,7 +167,8 @@ class WindowAttention:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
             _lib.call("dw4_window_attention", dtype, num_seqs, cfg.num_query_heads,
                       cfg.num_key_value_heads, cfg.head_dim, flags.BLOCK_SIZE,
-                      kv_cacher.layer_key_ptr_table_device.numel(), q.data_ptr(), _stride(q),
+                      min(kv_cacher.layer_key_ptr_table_device.numel(),
+                          kv_cacher.layer_val_ptr_table_device.numel()), q.data_ptr(), _stride(q),
                       output.data_ptr(), _stride(output), None if starts is None else starts.data_ptr(),
                       rows, query_len_max, kv_cacher.layer_key_ptr_table_device.data_ptr(),
                       kv_cacher.layer_val_ptr_table_device.data_ptr(), info.head_stride,

@@ -39,7 +39,8 @@ class LayerBlocksHolder:
                  dtype: Optional[torch.dtype] = None) -> None:
         """``dtype``: fp16 or bf16, the type of the keys and values that the blocks hold; by
         default that of the contiguous backing, and fp16 without one, whatever type the
-        geometry was given with (of which only the size counts)."""
+        geometry was given with (of which only the size counts: blocks of one byte an element
+        hold what it says, and the calls that move 16-bit rows refuse them)."""
         for t in (layer_key_ptr_table_device, layer_val_ptr_table_device):
             if t.dtype != torch.int64 or t.requires_grad:
                 raise AssertionError("pointer tables must be int64 without grad")
@@ -55,6 +56,10 @@ class LayerBlocksHolder:
         held = None if contigious_kv_tensor is None else contigious_kv_tensor[0].dtype
         if dtype is None:
             dtype = torch.bfloat16 if held == torch.bfloat16 else torch.float16
+            if block_info.element_size < 2:
+                dtype = block_info.dtype
+        elif block_info.element_size < 2:
+            raise TypeError(f"blocks of {block_info.dtype} have no room for {dtype}")
         elif dtype not in (torch.float16, torch.bfloat16):
             raise TypeError("KV blocks hold fp16 or bf16")
         elif held is not None and held != dtype:
@@ -75,7 +80,7 @@ class LayerBlocksHolder:
               slot_mapping: torch.Tensor) -> None:
         if key_states.shape[0] != slot_mapping.shape[0] or key_states.shape != val_states.shape:
             raise AssertionError("key/value rows must match slot_mapping")
-        if key_states.dtype != self.dtype or val_states.dtype != self.dtype:
+        if key_states.dtype != self.dtype or val_states.dtype != self.dtype or self.dtype.itemsize != 2:
             raise TypeError(f"the KV cache holds {self.dtype}")
         n, heads, hs = key_states.shape
         if heads != self.block_info.num_key_value_heads or hs != self.block_info.head_dim:

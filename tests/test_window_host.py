@@ -248,6 +248,32 @@ def test_cache_type_is_the_backings_or_the_stated_one():
             WindowAttention(AttentionConfig(512, 64, 8, 2, 4)).forward(q.bfloat16(), 1, none[:0], none[:0, None], holder)
 
 
+def test_caches_of_one_byte_are_refused():
+    """Their blocks are half as long as what 16-bit rows take: reading or writing them would
+    leave the memory."""
+    info = BlockInfo(head_dim=64, num_key_value_heads=2, dtype=torch.float8_e4m3fn)
+    holder = LayerBlocksHolder.create_contigious_cacher(info, 4, torch.device("cpu"), torch.float8_e4m3fn)
+    bare = LayerBlocksHolder(info, *[getattr(holder, f"layer_{x}_ptr_table_{y}") for y in ("device", "cpu", "list")
+                                     for x in ("key", "val")])
+    cfg, tab, one = AttentionConfig(512, 64, 8, 2, 4), torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    for h in (holder, bare):
+        assert h.dtype == torch.float8_e4m3fn
+        with pytest.raises(TypeError):
+            h.kv_tensor_from_slots_with_convert_with_create(torch.arange(3))
+        for dtype in (torch.float16, torch.bfloat16, torch.float8_e4m3fn):
+            q, kv = torch.zeros(3, 8, 64, dtype=dtype), torch.zeros(3, 2, 64, dtype=dtype)
+            for call in (lambda: h.kv_tensor_to_slots_with_convert(kv, kv, torch.arange(3)),
+                         lambda: h.kv_tensor_from_slots_with_convert(kv, kv, torch.arange(3)),
+                         lambda: h.rope_and_cache(q, kv, kv, torch.zeros(4, 64), torch.zeros(4, 64), one, tab),
+                         lambda: PagedAttention(cfg).forward(q, 1, one, tab, h),
+                         lambda: WindowAttention(cfg).forward(q, 1, one, tab, h)):
+                with pytest.raises(TypeError):
+                    call()
+    with pytest.raises(TypeError):
+        LayerBlocksHolder(info, *[getattr(holder, f"layer_{x}_ptr_table_{y}") for y in ("device", "cpu", "list")
+                                  for x in ("key", "val")], dtype=torch.float16)
+
+
 def test_integers_outside_32_bits_stay_outside_every_range():
     """Not cut to their low bits, which may name a block, a row or a length."""
     x = torch.tensor([5, -1, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 40 + 3, -2 ** 32 + 3, -2 ** 63])

@@ -34,6 +34,21 @@ inline size_t pool_ws_ints(int rows, int num_blocks) {
 }
 constexpr int kPoolMaxRows = 8192;   // a fork keeps one LDS word per row
 
+// Positions and cache slots of rows' last tokens.
+struct SlotArgs {
+  int rows, max_blocks, num_blocks, block_size, num_tokens;
+  const int32_t* tables;  // [rows][max_blocks]
+  const int32_t* lens;
+  const int32_t* new_tokens;  // [rows]
+  int32_t* starts;            // [rows + 1]
+  int32_t* positions;         // [num_tokens]
+  int64_t* slots;
+  int32_t* row_of;
+  int32_t* excess;            // [1]
+};
+constexpr int kSlotMaxRows = 8192;  // each workgroup keeps the rows' starts in LDS
+
+hipError_t launch_token_slots(const SlotArgs& a, hipStream_t stream);
 hipError_t launch_copy_blocks(const PoolArgs& a, int count, const int32_t* pairs, int cus, hipStream_t stream);
 hipError_t launch_extend_blocks(const PoolArgs& a, hipStream_t stream);
 hipError_t launch_fork_blocks(const PoolArgs& a, int cus, hipStream_t stream);

@@ -204,6 +204,53 @@ __global__ void __launch_bounds__(kThreads) extend_apply_kernel(PoolArgs a) {
   }
 }
 
+// ---- the slots of rows' last tokens: every workgroup sums up the rows' new tokens
+// (a few thousand integers from L2, so that one launch does) and maps 1024 tokens, each to its row by
+// bisection.
+
+__global__ void __launch_bounds__(kPlanThreads) token_slots_kernel(SlotArgs a) {
+  extern __shared__ int start[];  // [rows + 1]
+  __shared__ int64_t tmp[kPlanThreads / 64];
+  int64_t sum = 0, total;
+  for (int r0 = 0; r0 < a.rows; r0 += kPlanThreads) {
+    const int r = r0 + threadIdx.x;
+    const int64_t n = r < a.rows ? max(min(a.new_tokens[r], a.lens[r]), 0) : 0;
+    const int64_t before = scan(n, tmp, total);
+    if (r < a.rows) start[r] = clamp_int(sum + before);
+    sum += total;
+  }
+  const int64_t excess = max<int64_t>(sum - a.num_tokens, 0);
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int r = threadIdx.x; r <= a.rows; r += kPlanThreads)
+      a.starts[r] = excess > 0 ? 0 : r < a.rows ? start[r] : (int)sum;
+    if (threadIdx.x == 0) a.excess[0] = clamp_int(excess);
+  }
+  const int t = blockIdx.x * kPlanThreads + threadIdx.x;
+  if (t >= a.num_tokens) return;
+  int row = -1, pos = 0;
+  int64_t slot = -1;
+  if (excess == 0 && t < sum) {
+    int lo = 0, hi = a.rows - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (start[mid] <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    row = lo;
+    const int len = a.lens[row];
+    pos = len - max(min(a.new_tokens[row], len), 0) + t - start[row];
+    const int at = pos / a.block_size;
+    if (at < a.max_blocks) {
+      const int block = a.tables[(int64_t)row * a.max_blocks + at];
+      if (block >= 0 && block < a.num_blocks) slot = (int64_t)block * a.block_size + pos % a.block_size;
+    }
+  }
+  a.positions[t] = pos;
+  a.slots[t] = slot;
+  a.row_of[t] = row;
+}
+
 // ---- fork: workspace [head][fresh block per row][rows that need one][pairs]
 
 __device__ __forceinline__ int parent_of(const PoolArgs& a, int r) {
@@ -395,6 +442,12 @@ int copy_groups(const PoolArgs& a, int64_t most_pairs, int cus) {
 unsigned plan_groups(int64_t ints) { return (unsigned)(1 + std::min<int64_t>(64, (ints + kPlanThreads - 1) / kPlanThreads)); }
 
 }  // namespace
+
+hipError_t launch_token_slots(const SlotArgs& a, hipStream_t stream) {
+  const unsigned grid = std::max(1u, ((unsigned)a.num_tokens + kPlanThreads - 1) / kPlanThreads);
+  token_slots_kernel<<<grid, kPlanThreads, sizeof(int) * ((size_t)a.rows + 1), stream>>>(a);
+  return hipGetLastError();
+}
 
 hipError_t launch_copy_blocks(const PoolArgs& a, int count, const int32_t* pairs, int cus, hipStream_t stream) {
   copy_blocks_kernel<<<(unsigned)copy_groups(a, count, cus), kThreads, 0, stream>>>(a, count, pairs);

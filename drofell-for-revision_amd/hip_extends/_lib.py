@@ -6,11 +6,12 @@ object is missing or fails to load, every entry point raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
 import threading
-from typing import Optional
+from typing import Optional, Tuple
 
 LIB_NAME = "libdrofell_w4a16.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
@@ -147,6 +148,18 @@ SIGNATURES = {
     "dw4_free_blocks": (_c.c_int, [_c.c_int] * 4 + [_P] * 4 + [_c.c_int, _c.c_int] + [_P] * 5),
     "dw4_compact_blocks": (_c.c_int, [_c.c_int, _P, _P, _c.c_int64] + [_c.c_int] * 3 + [_P] * 9
                            + [_c.c_size_t, _P]),
+    "dw4_token_slots": (_c.c_int, [_c.c_int] * 4 + [_P] * 3 + [_c.c_int] + [_P] * 6),
+    "dw4_adapter_plan_size": (_c.c_int, [_c.c_int, _c.c_int, _SZ]),
+    "dw4_adapter_plan": (_c.c_int, [_c.c_int, _c.c_int, _P, _P, _c.c_size_t, _P]),
+    "dw4_adapters_workspace_size": (_c.c_int, [_c.c_int] * 6 + [_SZ, _SZ]),
+    "dw4_adapters": (_c.c_int, [_c.c_int] * 6 + [_P, _c.c_int64] * 3 + [_P] * 4 + [_c.c_int, _P, _P, _P,
+                                                                             _c.c_size_t, _P]),
+    "dw4_adapters_backward": (_c.c_int, [_c.c_int] * 6 + [_P, _c.c_int64] * 2 + [_P] * 4
+                              + [_c.c_int, _P, _P, _P, _c.c_int64, _P, _P, _P, _c.c_size_t, _P]),
+    "dw4_dropout": (_c.c_int, [_c.c_int] * 3 + [_P, _c.c_int64] * 2 + [_c.c_int, _P, _P]),
+    "dw4_rotary": (_c.c_int, [_c.c_int] * 8 + [_P, _c.c_int64] * 4 + [_P, _P, _c.c_float, _P]),
+    "dw4_rotary_and_cache": (_c.c_int, [_c.c_int] * 7 + [_P, _c.c_int64] * 4 + [_P, _P, _c.c_float, _P, _c.c_int,
+                                                                              _c.c_int, _P, _P, _c.c_int, _P]),
     "dw4_gemm_group": (_c.c_int, [_c.c_int, _IP, _c.c_int, _P, _c.c_int64, _P, _c.c_size_t, _P]),
     "dw4_gemm_silu_mul": (_c.c_int, [_c.c_int, _P, _c.c_int64, _IP, _IP, _P, _c.c_int64,
                                      _P, _c.c_size_t, _P]),
@@ -240,6 +253,20 @@ def current_stream(index: int) -> int:
     """The handle of torch's current stream of a device, without a Stream object (1.7 us)."""
     import torch
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """The context in which a call on tensors of ``device`` runs: the library launches on the
+    current device."""
+    import torch
+    if device.type != "cuda":
+        raise ValueError(f"the library runs on HIP devices, not on {device}")
+    if device.index is None or device.index == current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def query_sizes(k: int, n: int, group_size: int, act_order: bool, max_m: int) -> dict:
@@ -348,3 +375,21 @@ def blocks_workspace_size(num_rows: int, num_blocks: int) -> int:
     check("dw4_blocks_workspace_size",
           load().dw4_blocks_workspace_size(num_rows, num_blocks, ctypes.byref(out)))
     return out.value
+
+
+@functools.lru_cache(maxsize=4096)
+def adapter_plan_size(num_rows: int, num_adapters: int) -> int:
+    out = ctypes.c_size_t(0)
+    check("dw4_adapter_plan_size", load().dw4_adapter_plan_size(num_rows, num_adapters, ctypes.byref(out)))
+    return out.value
+
+
+@functools.lru_cache(maxsize=4096)
+def adapters_workspace_size(num_rows: int, num_adapters: int, k: int, n: int, rank: int, backward: bool,
+                            device: Optional[int] = None) -> Tuple[int, int]:
+    """Bytes of the workspace of one such dw4_adapters (or dw4_adapters_backward) call on the
+    current device, and of its h (``device``, its index, only tells several devices' sizes apart)."""
+    out, h = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    check("dw4_adapters_workspace_size", load().dw4_adapters_workspace_size(
+        num_rows, num_adapters, k, n, rank, int(backward), ctypes.byref(out), ctypes.byref(h)))
+    return out.value, h.value

@@ -5,7 +5,8 @@ a pool spans the layers of a stage, which share block numbers, and gives blocks
 to the rows of a running batch (``extend``), lets rows continue other rows
 (``fork``: beam steps, parallel samples, shared prompts), takes blocks back
 (``free``: finished rows, blocks behind an attention window), copies them
-(``copy``) and moves the live ones together (``compact``).  No counterpart in the
+(``copy``), moves the live ones together (``compact``) and says which slots new tokens go
+to (``slots``).  No counterpart in the
 reference, whose block tables live on the host.
 
 A ``BlockState`` is never changed in place: each call returns the next one, on
@@ -33,6 +34,15 @@ class BlockState(NamedTuple):
     context_lens: torch.Tensor  # int32 [rows]
     refs: torch.Tensor          # int32 [blocks of the pool]: table entries that hold each
     shortage: Optional[torch.Tensor] = None  # int32 [1]: blocks missing in the call that gave this state
+
+
+class SlotMap(NamedTuple):
+    """Where the rows' new tokens go (all on the device, token by token, row after row)."""
+    query_starts: torch.Tensor  # int32 [rows + 1]: each row's first token
+    positions: torch.Tensor     # int32 [tokens]: its position in the row
+    slots: torch.Tensor         # int64 [tokens]: its cache slot, -1: none
+    rows: torch.Tensor          # int32 [tokens]: its row, -1 behind the last token
+    excess: torch.Tensor        # int32 [1]: tokens that the arrays had no room for
 
 
 class BlockPool:
@@ -145,6 +155,27 @@ class BlockPool:
         self._call("dw4_extend_blocks", rows, width, self.num_blocks, flags.BLOCK_SIZE,
                    *self._pointers(state, new, n), ws.data_ptr(), ws.numel())
         return new
+
+    def slots(self, state: BlockState, new_tokens: torch.Tensor, tokens: int) -> SlotMap:
+        """Query starts, positions and cache slots of each row's last ``new_tokens`` tokens
+        (integers [rows], counted in ``context_lens`` already: those that ``extend`` has added),
+        in arrays of ``tokens`` entries, which the host knows to be enough.  What
+        ``WindowAttention.prefill``, ``RotaryEmbedding.forward_cached`` and
+        ``kv_tensor_to_slots_with_convert`` take.  Entries behind the last token have position 0,
+        slot -1 and row -1.  Where the rows have more tokens, ``excess`` says how many and none is
+        mapped.  Up to 8192 rows."""
+        rows, width = self._check(state)
+        n, tokens = self._by_row(new_tokens, rows, "new_tokens"), int(tokens)
+        if tokens < 0:
+            raise ValueError("tokens must not be negative")
+        ints = torch.empty(rows + 2 + 2 * tokens, dtype=torch.int32, device=self.device)
+        excess, starts, positions, row_of = ints.split([1, rows + 1, tokens, tokens])
+        slots = torch.empty(tokens, dtype=torch.int64, device=self.device)
+        self._call("dw4_token_slots", rows, width, self.num_blocks, flags.BLOCK_SIZE,
+                   state.block_tables.data_ptr(), state.context_lens.data_ptr(), n.data_ptr(), tokens,
+                   starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), row_of.data_ptr(),
+                   excess.data_ptr())
+        return SlotMap(starts, positions, slots, row_of, excess)
 
     def fork(self, state: BlockState, parents: torch.Tensor) -> BlockState:
         """Row r continues row parents[r] (integers [rows]; outside the rows: it ends).  Full

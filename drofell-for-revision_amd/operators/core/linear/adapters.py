@@ -1,0 +1,292 @@
+"""Low-rank adapters of many requests beside a shared projection, on the HIP library.
+
+A batch's rows go through one projection (a ``QuantLinear``, a ``MarlinQuantLinear``, or any
+other), and each row adds the low-rank product of its own adapter, or of none:
+
+    y_t = W x_t + scaling_a B_a (A_a d(x_t)),   a the row's adapter, d dropout (training).
+
+* ``AdapterRows``     which adapter each row of a batch has, sorted once on the device for all
+                      projections of all layers;
+* ``LowRankAdapters`` the adapters of one projection, with gradients;
+* ``AdaptedLinear``   a projection with its adapters;
+* ``CounterDropout``  the adapters' dropout by itself: its mask comes from a counter and is
+                      never stored.
+
+The reference's adapters (``operators/core/lora``, paths relative to
+``/root/reference/After-Revision-DROFELL``) are dense products of one adapter.
+
+All take fp16 or bf16.  Every call runs on the current stream of its tensors' device, never
+synchronises, keeps nothing between calls and may be captured into a graph; scratch memory is
+torch's, allocated per call.  Give a training step to a graph when no eager autograd graph over the
+same leaves is alive.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import nn
+from torch.autograd.graph import increment_version
+
+from hip_extends import _lib
+
+from ..block.common import int32
+from .real import Linear
+
+_DTYPES = {torch.float16: _lib.DW4_F16, torch.bfloat16: _lib.DW4_BF16}
+
+
+def _matrix(x: torch.Tensor) -> torch.Tensor:
+    """x [rows, width] as the kernels read it, in 16-byte units of its rows; a copy where it is not so."""
+    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < x.shape[1])):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _drop(p: float) -> int:
+    """A probability as the generator takes it, of 65536."""
+    if not 0 <= p <= 1:
+        raise ValueError("the probability of dropout lies between 0 and 1")
+    return round(p * 65536)
+
+
+def _seed(seed: Optional[torch.Tensor], device: torch.device) -> torch.Tensor:
+    if seed is None:
+        raise ValueError("dropout needs a seed (int64 [2], on the device: seed and offset)")
+    if seed.dtype != torch.int64 or seed.shape != (2,) or seed.device != device:
+        raise ValueError(f"the seed must be int64 [2] on {device}")
+    return seed.contiguous()
+
+
+class AdapterRows:
+    """Which adapter each row of a batch has (``adapters``, integers [rows] on the device; a number
+    outside 0 .. num_adapters - 1: none), sorted by adapter.  Made once per batch: every
+    projection of every layer takes it.  Up to 2^24 rows and 1024 adapters."""
+
+    def __init__(self, adapters: torch.Tensor, num_adapters: int) -> None:
+        if adapters.dim() != 1:
+            raise ValueError("adapters must hold one integer per row")
+        self.num_rows, self.num_adapters, self.device = adapters.shape[0], int(num_adapters), adapters.device
+        with _lib.on_device(self.device):
+            self.plan = torch.empty(_lib.adapter_plan_size(self.num_rows, self.num_adapters) // 4, dtype=torch.int32,
+                                    device=self.device)
+        self.update(adapters)
+
+    def update(self, adapters: torch.Tensor) -> None:
+        """The same rows with other adapters, in the memory that captured calls read."""
+        if adapters.shape != (self.num_rows,) or adapters.device != self.device:
+            raise ValueError(f"adapters must be {self.num_rows} integers on {self.device}")
+        index = int32(adapters, "adapters")
+        with _lib.on_device(self.device):
+            _lib.call("dw4_adapter_plan", self.num_rows, self.num_adapters, index.data_ptr(), self.plan.data_ptr(),
+                      self.plan.numel() * 4, _lib.current_stream(self.device.index))
+        increment_version(self.plan)  # a backward pass that was to read the old one fails
+
+
+class LowRankAdapters(nn.Module):
+    def __init__(self, in_features: int, out_features: int, rank: int, num_adapters: int,
+                 dtype: torch.dtype = torch.float16, device: Optional[torch.device] = None, dropout: float = 0.0,
+                 trainable: bool = False) -> None:
+        """``rank`` is a multiple of 8 up to 128: adapters of lower rank are filled up with zeros
+        (``load``).  ``dropout`` applies to the adapters' input while the module is in training
+        mode; its probability counts in steps of 2^-16."""
+        super().__init__()
+        if dtype not in _DTYPES:
+            raise TypeError("adapters are fp16 or bf16")
+        if rank < 8 or rank % 8 or rank > 128:
+            raise ValueError("the rank must be a multiple of 8 up to 128")
+        if in_features < 8 or in_features % 8 or out_features < 8 or out_features % 8:
+            raise ValueError("in_features and out_features must be multiples of 8")
+        if not 0 < num_adapters <= 1024:
+            raise ValueError("there are 1 to 1024 adapters")
+        self.in_features, self.out_features, self.rank, self.num_adapters = in_features, out_features, rank, num_adapters
+        self.dropout = dropout
+        self._dropped = _drop(dropout)
+        self.a = nn.Parameter(torch.randn(num_adapters, rank, in_features, dtype=torch.float32, device=device)
+                              .mul_(in_features ** -0.5).to(dtype), requires_grad=trainable)
+        self.b = nn.Parameter(torch.zeros(num_adapters, out_features, rank, dtype=dtype, device=device),
+                              requires_grad=trainable)
+        self.register_buffer("scaling", torch.ones(num_adapters, dtype=torch.float32, device=device))
+
+    @torch.no_grad()
+    def load(self, index: int, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: float) -> None:
+        """Adapter ``index`` from its matrices A [r, in_features] and B [out_features, r], r up to
+        the rank, and its scaling (alpha / r)."""
+        r = lora_a.shape[0]
+        if not 0 <= index < self.num_adapters:
+            raise IndexError(f"there are {self.num_adapters} adapters")
+        if r > self.rank or lora_a.shape != (r, self.in_features) or lora_b.shape != (self.out_features, r):
+            raise ValueError(f"A and B must be [r, {self.in_features}] and [{self.out_features}, r], r up to {self.rank}")
+        self.a[index].zero_()
+        self.b[index].zero_()
+        self.a[index, :r].copy_(lora_a)
+        self.b[index, :, :r].copy_(lora_b)
+        self.scaling[index] = scaling
+
+    def forward(self, x: torch.Tensor, base: torch.Tensor, rows: AdapterRows, seed: Optional[torch.Tensor] = None,
+                output: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [..., in_features] and the projection's output ``base`` [..., out_features] ->
+        base + each row's adapter's product.  ``seed``: int64 [2] on the device (seed and offset),
+        read where dropout applies; another step takes another offset, another projection another
+        seed.  Differentiable (once) in x, base, ``a`` and ``b``.  ``output``, without gradients:
+        where the result goes, which may be ``base``."""
+        if x.shape[-1] != self.in_features or base.shape != (*x.shape[:-1], self.out_features):
+            raise ValueError(f"x and base must be [..., {self.in_features}] and [..., {self.out_features}] of the same rows")
+        a, b, device = self.a, self.b, x.device
+        if x.dtype not in _DTYPES or any(t.dtype != x.dtype for t in (base, a, b)):
+            raise TypeError("x, base and the adapters must be of one type, fp16 or bf16")
+        if any(t.device != device for t in (base, a, self.scaling, rows)):
+            raise ValueError(f"x, base, the adapters and their rows must be on one device ({device})")
+        x2, base2 = x.reshape(-1, self.in_features), base.reshape(-1, self.out_features)
+        if x2.shape[0] != rows.num_rows or rows.num_adapters != self.num_adapters:
+            raise ValueError(f"rows were sorted for {rows.num_rows} rows of {rows.num_adapters} adapters, "
+                             f"not for {x2.shape[0]} of {self.num_adapters}")
+        drop = self._dropped if self.training else 0
+        seed = _seed(seed, device) if drop else None
+        scaling = self.scaling if self.scaling.dtype == torch.float32 else self.scaling.float()
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, base, a, b)):
+            if output is not None:
+                raise ValueError("output is for calls without gradients")
+            out2 = _LowRank.apply(x2, base2, a, b, scaling, rows, drop, seed)
+            return out2.view(base.shape)
+        if output is None:
+            return _forward(x2, base2, a, b, scaling, rows.plan, drop, seed, None, False)[0].view(base.shape)
+        if output.shape != base.shape or output.dtype != x.dtype or output.device != device or \
+                not output.is_contiguous() or output.data_ptr() % 16:
+            raise ValueError("output must be contiguous and 16-byte aligned, of base's shape, type and device")
+        _forward(x2, base2, a, b, scaling, rows.plan, drop, seed, output.view(-1, self.out_features), False)
+        increment_version(output)
+        return output
+
+
+def _shape(x, a, b):
+    return _DTYPES[x.dtype], x.shape[0], a.shape[0], x.shape[1], b.shape[1], a.shape[1]
+
+
+def _forward(x, base, a, b, scaling, plan, drop, seed, out, keep):
+    device = x.device
+    with _lib.on_device(device):
+        x, base = _matrix(x), _matrix(base)
+        a, b, scaling = a.contiguous(), b.contiguous(), scaling.contiguous()
+        if out is None:
+            out = torch.empty(base.shape, dtype=x.dtype, device=device)
+        shape = _shape(x, a, b)
+        nbytes, h_bytes = _lib.adapters_workspace_size(*shape[1:], False, device.index)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        h = torch.empty(h_bytes // 4, dtype=torch.float32, device=device) if keep else None
+        _lib.call("dw4_adapters", *shape, x.data_ptr(), _stride(x), base.data_ptr(), _stride(base), out.data_ptr(),
+                  _stride(out), a.data_ptr(), b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), drop,
+                  None if seed is None else seed.data_ptr(), None if h is None else h.data_ptr(), ws.data_ptr(), nbytes,
+                  _lib.current_stream(device.index))
+    return out, x, h
+
+
+class _LowRank(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, base, a, b, scaling, rows, drop, seed):
+        out, x, h = _forward(x, base, a, b, scaling, rows.plan, drop, seed, None, True)
+        ctx.drop = drop
+        ctx.save_for_backward(x, a, b, scaling, rows.plan, h, seed)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, a, b, scaling, plan, h, seed = ctx.saved_tensors
+        device = x.device
+        need_x, need_base, need_a, need_b = ctx.needs_input_grad[:4]
+        dbase = dout if need_base else None
+        if x.shape[0] == 0:
+            return (torch.zeros_like(x) if need_x else None, dbase, torch.zeros_like(a) if need_a else None,
+                    torch.zeros_like(b) if need_b else None, None, None, None, None)
+        if not (need_x or need_a or need_b):
+            return (None, dbase, None, None, None, None, None, None)
+        with _lib.on_device(device):
+            g = _matrix(dout)
+            a, b, scaling = a.contiguous(), b.contiguous(), scaling.contiguous()
+            dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
+            da = torch.empty(a.shape, dtype=x.dtype, device=device) if need_a else None
+            db = torch.empty(b.shape, dtype=x.dtype, device=device) if need_b else None
+            shape = _shape(x, a, b)
+            nbytes, _ = _lib.adapters_workspace_size(*shape[1:], True, device.index)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            _lib.call("dw4_adapters_backward", *shape, x.data_ptr(), _stride(x), g.data_ptr(), _stride(g), a.data_ptr(),
+                      b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), ctx.drop,
+                      None if seed is None else seed.data_ptr(), h.data_ptr(),
+                      None if dx is None else dx.data_ptr(), x.shape[1], None if da is None else da.data_ptr(),
+                      None if db is None else db.data_ptr(), ws.data_ptr(), nbytes, _lib.current_stream(device.index))
+        return dx, dbase, da, db, None, None, None, None
+
+
+class AdaptedLinear(Linear):
+    """A projection with the adapters of many requests: ``forward(x)`` is the projection's,
+    ``forward(x, rows)`` adds each row's adapter.  The projection's weight stays frozen (its input
+    gradient is its own); the adapters train where they were made trainable."""
+
+    def __init__(self, base: Linear, adapters: LowRankAdapters) -> None:
+        nn.Module.__init__(self)
+        self.base = base
+        self.adapters = adapters
+
+    def forward(self, x: torch.Tensor, rows: Optional[AdapterRows] = None,
+                seed: Optional[torch.Tensor] = None) -> torch.Tensor:
+        y = self.base(x)
+        if rows is None:
+            return y
+        bank = self.adapters
+        if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or bank.a.requires_grad or bank.b.requires_grad):
+            return bank(x, y, rows, seed)
+        return bank(x, y, rows, seed, output=y if y.is_contiguous() and y.data_ptr() % 16 == 0 else None)
+
+
+class CounterDropout(nn.Module):
+    """Dropout whose mask comes from a counter: element (row, column) of x [..., columns] is zero
+    with probability p (in steps of 2^-16), by its 16 bits of Philox 4x32 under the seed; the
+    others are scaled to keep the mean.  Nothing but the seed is kept for the backward pass."""
+
+    def __init__(self, p: float) -> None:
+        super().__init__()
+        self.p = p
+        self._dropped = _drop(p)
+
+    def forward(self, x: torch.Tensor, seed: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``seed``: int64 [2] on the device, seed and offset; another step takes another offset.
+        In evaluation mode, or with p 0, x itself."""
+        if x.dtype not in _DTYPES:
+            raise TypeError("dropout runs on fp16 or bf16")
+        if x.dim() < 1:
+            raise ValueError("x must have columns")
+        if not self.training or self._dropped == 0:
+            return x
+        return _Dropout.apply(x, _seed(seed, x.device), self._dropped)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def _run(x, seed, drop):
+        cols = x.shape[-1]
+        rows = x.numel() // cols if cols else 0
+        with _lib.on_device(x.device):
+            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            x2 = x.reshape(rows, cols)
+            if x2.stride(1) != 1 or (rows > 1 and x2.stride(0) < cols):
+                x2 = x2.contiguous()
+            _lib.call("dw4_dropout", _DTYPES[x.dtype], rows, cols, x2.data_ptr(), _stride(x2), y.data_ptr(), cols, drop,
+                      seed.data_ptr(), _lib.current_stream(x.device.index))
+        return y
+
+    @staticmethod
+    def forward(ctx, x, seed, drop):
+        ctx.drop = drop
+        ctx.save_for_backward(seed)
+        return _Dropout._run(x, seed, drop)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (seed,) = ctx.saved_tensors
+        return _Dropout._run(dy, seed, ctx.drop), None, None

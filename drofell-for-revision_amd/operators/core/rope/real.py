@@ -1,0 +1,186 @@
+"""Rotary positions on the HIP library.
+
+Stands beside ``attention_forward_rope_stage_v2_py`` (``hip_extends/w4a16.py``) and
+``LayerBlocksHolder.rope_and_cache``, which keep the reference's fp16 arithmetic over sin / cos
+tables (``cuda_extends/exllama/fuse_v2/rope.cu``, paths relative to
+``/root/reference/After-Revision-DROFELL``): here rows of any positions, fp16 or bf16, both pair
+layouts, a part of the head, scaled frequencies, angles computed from the position (no table, as
+exact at far positions as at near ones), and gradients.
+
+* ``forward``         queries and keys turned, differentiable;
+* ``forward_cached``  queries turned, keys turned and values as they are into their cache
+                      slots, in one launch, for ragged batches of prompts and single tokens.
+
+Every call runs on the current stream of its tensors' device, never synchronises, keeps nothing
+and may be captured into a graph.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from hip_extends import _lib
+
+from ... import flags
+from ..block.common import int32
+from ..block.real import LayerBlocksHolder
+from .common import RotaryScaling, rotary_frequencies
+
+_DTYPES = {torch.float16: _lib.DW4_F16, torch.bfloat16: _lib.DW4_BF16}
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x [rows, heads, dims] with its heads side by side and rows in 16-byte units; a copy
+    where it is not so."""
+    rows, heads, dims = x.shape
+    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != dims) or x.data_ptr() % 16 or \
+            (rows > 1 and (x.stride(0) % 8 or x.stride(0) < heads * dims)):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+
+
+class RotaryEmbedding:
+    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0,
+                 interleaved: bool = False, scaling: Optional[RotaryScaling] = None,
+                 device: Optional[torch.device] = None) -> None:
+        """The first ``rotary_dim`` dims of a head (an even number; all by default) turn, in
+        pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if ``interleaved``; pair i by
+        base^(-2 i / rotary_dim) radians a position, scaled as ``scaling`` says."""
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if head_dim < 8 or head_dim % 8 or head_dim > 512:
+            raise ValueError("head_dim must be a multiple of 8 up to 512")
+        if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > head_dim:
+            raise ValueError("rotary_dim must be even, at least 2 and at most head_dim")
+        if not (math.isfinite(base) and base > 1):
+            raise ValueError("the base must be above 1")
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ValueError("rotary positions run on a HIP device")
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, bool(interleaved)
+        self.frequencies, self.magnitude = rotary_frequencies(rotary_dim, base, scaling)
+        # turns per position as 64-bit fractions: their products with positions wrap at whole turns
+        turns = [int(math.ldexp(f / (2 * math.pi), 64)) % 2 ** 64 for f in self.frequencies]
+        self._turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns],
+                                   dtype=torch.int64).to(device)
+        self.device = self._turns.device
+
+    def _check(self, x: torch.Tensor, name: str) -> None:
+        if x.dim() != 3 or x.shape[2] != self.head_dim:
+            raise AssertionError(f"{name} must be [rows, heads, {self.head_dim}]")
+        if x.device != self.device:
+            raise ValueError(f"{name} must be on {self.device}")
+        if x.dtype not in _DTYPES:
+            raise TypeError("rotary positions run on fp16 or bf16")
+
+    def _positions(self, positions: torch.Tensor, rows: int) -> torch.Tensor:
+        if positions.shape != (rows,) or positions.device != self.device:
+            raise ValueError(f"positions must be {rows} integers on {self.device}")
+        return int32(positions, "positions")
+
+    def _turn(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+              inverse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+        with _lib.on_device(self.device):
+            q, k = _rows(q), _rows(k)
+            qo = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            ko = torch.empty(k.shape, dtype=q.dtype, device=self.device)
+            _lib.call("dw4_rotary", _DTYPES[q.dtype], q.shape[0], q.shape[1], k.shape[1], self.head_dim,
+                      self.rotary_dim, int(self.interleaved), int(inverse), q.data_ptr(), _stride(q),
+                      k.data_ptr(), _stride(k), qo.data_ptr(), _stride(qo), ko.data_ptr(), _stride(ko),
+                      positions.data_ptr(), self._turns.data_ptr(), self.magnitude,
+                      _lib.current_stream(self.device.index))
+        return qo, ko
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor,
+                positions: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """q [rows, heads, head_dim] and k [rows, kv heads, head_dim] turned by their rows'
+        ``positions`` (integers [rows]) -> new tensors.  Differentiable in q and k (once)."""
+        self._check(q, "q")
+        self._check(k, "k")
+        if k.shape[0] != q.shape[0]:
+            raise AssertionError("q and k must have the same rows")
+        if k.dtype != q.dtype:
+            raise TypeError("q and k must have one type")
+        pos = self._positions(positions, q.shape[0])
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+            return _Rotary.apply(q, k, pos, self)
+        return self._turn(q, k, pos, False)
+
+    def forward_cached(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                       slots: torch.Tensor, kv_cacher: LayerBlocksHolder,
+                       output: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q turned (returned, or written to ``output``, which may be q), k turned and v into
+        their cache ``slots`` (integers [rows]; -1: the row is not cached, and so is a slot outside the
+        cache's blocks).  k and v stay as they are.  No two rows may have one slot.  Without
+        gradients: a backward pass through it raises."""
+        self._check(q, "q")
+        self._check(k, "k")
+        self._check(v, "v")
+        rows, info = q.shape[0], kv_cacher.block_info
+        if k.shape != v.shape or k.shape[0] != rows:
+            raise AssertionError("k and v must have the same shape and q's rows")
+        if info.head_dim != self.head_dim or info.num_key_value_heads != k.shape[1]:
+            raise AssertionError("k and v do not match the cache's block geometry")
+        if k.dtype != q.dtype or v.dtype != q.dtype:
+            raise TypeError("q, k and v must have one type")
+        if kv_cacher.dtype != q.dtype:
+            raise TypeError(f"rows of {q.dtype} into a cache of {kv_cacher.dtype}")
+        if kv_cacher.device != self.device:
+            raise ValueError(f"the cache must be on {self.device}")
+        pos = self._positions(positions, rows)
+        if slots.shape != (rows,) or slots.device != self.device:
+            raise ValueError(f"slots must be {rows} integers on {self.device}")
+        if slots.dtype != torch.int64 and slots.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+            raise ValueError("slots must be integers")
+        slots = slots.to(torch.int64).contiguous()
+        if output is None:
+            output = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        elif output.shape != q.shape or output.dtype != q.dtype or output.device != self.device:
+            raise ValueError("output must have the queries' shape, type and device")
+        elif _rows(output) is not output:
+            raise ValueError("output rows must be contiguous and 16-byte aligned")
+        with _lib.on_device(self.device):
+            q2, k2, v2 = _rows(q), _rows(k), _rows(v)
+            _lib.call("dw4_rotary_and_cache", _DTYPES[q.dtype], rows, q.shape[1], k.shape[1], self.head_dim,
+                      self.rotary_dim, int(self.interleaved), q2.data_ptr(), _stride(q2), k2.data_ptr(),
+                      _stride(k2), v2.data_ptr(), _stride(v2), output.data_ptr(), _stride(output),
+                      pos.data_ptr(), self._turns.data_ptr(), self.magnitude, slots.data_ptr(),
+                      min(kv_cacher.layer_key_ptr_table_device.numel(),
+                          kv_cacher.layer_val_ptr_table_device.numel()), flags.BLOCK_SIZE,
+                      kv_cacher.layer_key_ptr_table_device.data_ptr(),
+                      kv_cacher.layer_val_ptr_table_device.data_ptr(), info.head_stride,
+                      _lib.current_stream(self.device.index))
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return _NoGradient.apply(output, q, k, v)
+        return output
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, rotary):
+        ctx.rotary = rotary
+        ctx.save_for_backward(positions)
+        return rotary._turn(q, k, positions, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        (positions,) = ctx.saved_tensors
+        return (*ctx.rotary._turn(dq, dk, positions, True), None, None)
+
+
+class _NoGradient(torch.autograd.Function):
+    """A backward pass that reaches the cached call fails instead of finding no gradient."""
+
+    @staticmethod
+    def forward(ctx, output, *inputs):
+        return output.detach()
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("rotary positions into a cache have no gradients (RotaryEmbedding.forward has)")

@@ -618,6 +618,100 @@ int dw4_compact_blocks(int num_layers, const int64_t* layer_key_ptrs,
                        int32_t* refs_out, int32_t* shortage, int32_t* live, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* Slots of rows' last tokens: row r has its last n_r = min(new_tokens[r], lens[r]) (0
+ * if negative) tokens among num_tokens, behind those of the rows before it.
+ * query_starts (int32 [num_rows + 1]): each row's first; and per token its position in
+ * the row, its cache slot (block number * block_size + slot in the block; -1 where the
+ * table has no block of the pool) and its row.  Tokens behind the last: position 0,
+ * slot and row -1.  excess (int32 [1]): how many tokens more than num_tokens the
+ * rows have; unless it is 0 no token is mapped and query_starts is zeros.  One
+ * launch; num_rows at most 8192. */
+int dw4_token_slots(int num_rows, int max_blocks, int num_blocks, int block_size,
+                    const int32_t* tables, const int32_t* lens, const int32_t* new_tokens,
+                    int num_tokens, int32_t* query_starts, int32_t* positions, int64_t* slots,
+                    int32_t* rows, int32_t* excess, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a shared projection:
+ *   out_t = base_t + scaling_a * B_a (A_a d(x_t)),   a = the row's adapter,
+ * d being dropout; a row without an adapter keeps base_t.  No counterpart in the reference,
+ * whose adapters are dense products (operators/core/lora).  x [num_rows][k],
+ * base and out [num_rows][n] with row strides (multiples of 8), 16-byte aligned;
+ * a [num_adapters][rank][k], b [num_adapters][n][rank], scaling float
+ * [num_adapters]; dtype DW4_F16 or DW4_BF16 of all 16-bit arrays.  k, n and
+ * rank are multiples of 8, rank at most 128, num_adapters at most 1024, num_rows
+ * at most 2^24.  Sums run in fp32; the product A x enters the second product
+ * in two 16-bit parts; out is rounded once.  Deterministic.
+ * ------------------------------------------------------------------------- */
+
+/* The rows of a batch in order of their adapters (int32 device [num_rows]; a number outside
+ * 0 .. num_adapters - 1: none), into plan (int32 device, dw4_adapter_plan_size bytes,
+ * 16-byte aligned), which every call over these rows takes: made once for all
+ * projections of all layers. */
+int dw4_adapter_plan_size(int num_rows, int num_adapters, size_t* plan_bytes);
+int dw4_adapter_plan(int num_rows, int num_adapters, const int32_t* adapters, int32_t* plan,
+                     size_t plan_bytes, void* stream);
+
+/* out may be base (with its stride).  drop: an element of x is zero with probability
+ * drop / 65536, by dw4_dropout's rule, and the others are scaled up; 0: no dropout, seed
+ * is not read.  h: float, h_bytes, what the backward pass needs, or NULL.
+ * workspace: dw4_adapters_workspace_size bytes (backward 0). */
+int dw4_adapters(int dtype, int num_rows, int num_adapters, int k, int n, int rank,
+                 const uint16_t* x, int64_t ldx, const uint16_t* base, int64_t ldb, uint16_t* out,
+                 int64_t ldo, const uint16_t* a, const uint16_t* b, const float* scaling,
+                 const int32_t* plan, int drop, const int64_t* seed, float* h, void* workspace,
+                 size_t workspace_bytes, void* stream);
+int dw4_adapters_workspace_size(int num_rows, int num_adapters, int k, int n, int rank, int backward,
+                                size_t* workspace_bytes, size_t* h_bytes);
+
+/* Gradients for the output gradient dout [num_rows][n], from the forward's inputs and h:
+ * dx [num_rows][k] (of the adapters alone; zeros in rows without one), da and db (shapes of a
+ * and b; zeros for adapters without rows); each may be NULL.  base's gradient is dout.
+ * num_rows at least 1.  workspace: dw4_adapters_workspace_size bytes (backward 1). */
+int dw4_adapters_backward(int dtype, int num_rows, int num_adapters, int k, int n, int rank,
+                          const uint16_t* x, int64_t ldx, const uint16_t* dout, int64_t ldd,
+                          const uint16_t* a, const uint16_t* b, const float* scaling,
+                          const int32_t* plan, int drop, const int64_t* seed, const float* h,
+                          uint16_t* dx, int64_t lddx, uint16_t* da, uint16_t* db, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Dropout whose mask is not stored: y = x * 65536 / (65536 - drop) for the elements kept,
+ * 0 for the others, whatever they hold.  Element (row, col) is kept if its 16 bits of
+ * Philox 4x32 (10 rounds) are at least drop (0 .. 65536): the counter's words are col / 8,
+ * row and the two halves of seed[1], the key's those of seed[0] (int64 device [2]), and of the
+ * four words of output the element has half col % 8, low halves first.  The gradient is the
+ * same call on the output's gradient.  Rows of any width, stride and alignment; y may be x. */
+int dw4_dropout(int dtype, int num_rows, int cols, const uint16_t* x, int64_t ldx, uint16_t* y,
+                int64_t ldy, int drop, const int64_t* seed, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Rotary positions: of every head's first rotary_size dims the pairs (i, i +
+ * rotary_size / 2), or interleaved (2 i, 2 i + 1), turned by positions[row] times
+ * the pair's frequency and scaled by magnitude; the other dims as they are.  turns (int64
+ * device [rotary_size / 2]): a frequency in turns per position, times 2^64 (modulo
+ * 2^64; angles keep that precision at any position).  Computed in fp32, rounded once.
+ * Beside dw4_rope (fp16 tables, half layout, in place).  q [num_rows][num_heads]
+ * [head_size], k (and v) [num_rows][num_kv_heads][head_size] with row strides
+ * (multiples of 8), 16-byte aligned; head_size a multiple of 8 up to 512, rotary_size
+ * even.  inverse: turned back, which is the gradient.  Outputs may be the inputs.
+ * ------------------------------------------------------------------------- */
+int dw4_rotary(int dtype, int num_rows, int num_heads, int num_kv_heads, int head_size,
+               int rotary_size, int interleaved, int inverse, const uint16_t* q, int64_t q_stride,
+               const uint16_t* k, int64_t k_stride, uint16_t* q_out, int64_t qo_stride,
+               uint16_t* k_out, int64_t ko_stride, const int32_t* positions, const int64_t* turns,
+               float magnitude, void* stream);
+
+/* q turned into q_out, k turned and v as it is into their cache slots (slots int64 device
+ * [num_rows], as in dw4_reshape_and_cache; a slot outside the num_blocks blocks is skipped;
+ * no two rows may have one slot), in one launch.  k and v are not changed. */
+int dw4_rotary_and_cache(int dtype, int num_rows, int num_heads, int num_kv_heads, int head_size,
+                         int rotary_size, int interleaved, const uint16_t* q, int64_t q_stride,
+                         const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
+                         uint16_t* q_out, int64_t qo_stride, const int32_t* positions,
+                         const int64_t* turns, float magnitude, const int64_t* slots, int num_blocks,
+                         int block_size, const int64_t* key_block_ptrs,
+                         const int64_t* value_block_ptrs, int kv_head_stride, void* stream);
+
 /* ------------------------------------------------------------------------
  * Decode chain: one launch over a list of projections at m <= 4 (no single
  * reference call: it runs the per-projection q4_matmul_cuda_v2 calls,

@@ -15,7 +15,7 @@ constexpr int kAdapterMaxRows = 1 << 24;
 
 // How the rows of a call are laid out by adapter: rows sorted by adapter (those
 // without one last), each adapter's from a tile of its own on.  A tile holds
-// `align` positions of one adapter, a chunk up to kChunkTiles(align) tiles of it.
+// `align` positions of one adapter, a chunk up to chunk_rows rows of it.
 // The counts are bounds that the host knows.
 struct AdapterLayout {
   int align, tiles, chunks, chunk_rows;
@@ -23,11 +23,12 @@ struct AdapterLayout {
   // offsets (int32) in the plan
   int64_t tile_adapter, chunk, chunk_start, order, ints;
 };
-constexpr int kFewRows = 256;  // rows up to which tiles hold 16 positions, above it 64
+constexpr int kChunkRows = 512;
+constexpr int kFewRows = 256;  // rows up to which tiles hold 32 positions, above it 64
 inline AdapterLayout adapter_layout(int rows, int adapters) {
   AdapterLayout l = {};
-  l.align = rows <= kFewRows ? 16 : 64;
-  l.chunk_rows = 256;
+  l.align = rows <= kFewRows ? 32 : 64;
+  l.chunk_rows = kChunkRows;
   const int segs = std::min(adapters + 1, rows);
   l.tiles = rows / l.align + segs;
   l.chunks = rows / l.chunk_rows + segs;
@@ -38,6 +39,33 @@ inline AdapterLayout adapter_layout(int rows, int adapters) {
   l.order = (l.chunk_start + adapters + 2 + 3) & ~(int64_t)3;
   l.ints = l.order + l.positions;
   return l;
+}
+
+// The rank that the matrix instructions see.
+inline int padded_rank(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
+
+// h (or dh) of every position as 16-bit operands in two parts (split16), in two forms:
+//   by row     [2][positions][padded rank], with an exponent per position;
+//   by column  [2][positions / 8][padded rank][8], the eight positions side by side, with an
+//              exponent per 32 positions and column.
+// bf16 operands have no exponents.
+struct AdapterPacks {
+  uint16_t* row;
+  int32_t* row_exp;
+  uint16_t* col;
+  int32_t* col_exp;
+};
+inline size_t row_pack_bytes(const AdapterLayout& l, int r) { return (size_t)l.positions * (4 * padded_rank(r) + 4); }
+inline size_t col_pack_bytes(const AdapterLayout& l, int r) {
+  return (size_t)l.positions * 4 * padded_rank(r) + (size_t)l.positions / 32 * padded_rank(r) * 4;
+}
+inline void place_row(AdapterPacks& p, const AdapterLayout& l, int r, void* at) {
+  p.row = static_cast<uint16_t*>(at);
+  p.row_exp = reinterpret_cast<int32_t*>(p.row + 2 * (size_t)l.positions * padded_rank(r));
+}
+inline void place_col(AdapterPacks& p, const AdapterLayout& l, int r, void* at) {
+  p.col = static_cast<uint16_t*>(at);
+  p.col_exp = reinterpret_cast<int32_t*>(p.col + 2 * (size_t)l.positions * padded_rank(r));
 }
 
 struct AdapterArgs {
@@ -58,7 +86,6 @@ struct AdapterArgs {
   int64_t ldb;
   uint16_t* out;
   int64_t ldo;
-  float* h;              // [positions][r], A x of the kept elements, or null
   // backward
   const uint16_t* g;     // [rows][n]
   int64_t ldg;
@@ -66,31 +93,63 @@ struct AdapterArgs {
   int64_t lddx;
   uint16_t* da;          // or null
   uint16_t* db;          // or null
-  float* ws;
+  void* h;               // h by column: written by a forward pass that keeps it, read by the backward pass
+  unsigned char* ws;
 };
 
-// Forward: the rows' products with A in `splits` parts of k.
-int adapter_splits(const AdapterLayout& l, int k, int cus);
-inline size_t adapter_ws_floats(const AdapterLayout& l, int splits, int r) { return (size_t)splits * l.positions * r; }
-// Backward: dH in a plane per slab of kSlab columns, its sum, and each chunk's share of dA and dB.
-constexpr int kSlab = 256;
-struct AdapterGradParts {
-  size_t dh, da, db, floats;  // offsets (floats) behind the planes, and the whole
+// Parts of the reduced axis in which rows are multiplied with A (or their gradients with B).
+int adapter_splits(const AdapterLayout& l, int width, int cus);
+
+// Workspaces: offsets in bytes.
+struct ForwardWs {
+  int splits;
+  size_t row, bytes;  // behind the planes [splits][positions][r]
 };
-inline AdapterGradParts adapter_grad_parts(const AdapterLayout& l, int k, int n, int r) {
-  AdapterGradParts p;
-  const size_t plane = (size_t)l.positions * r;
-  p.dh = (size_t)((n + kSlab - 1) / kSlab) * plane;
-  p.da = p.dh + plane;
-  p.db = p.da + (size_t)l.chunks * r * k;
-  p.floats = p.db + (size_t)l.chunks * r * n;
-  return p;
+inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+inline size_t plane_bytes(const AdapterLayout& l, int splits, int r) { return up256(sizeof(float) * splits * (size_t)l.positions * r); }
+inline ForwardWs forward_ws(const AdapterLayout& l, int k, int r, int cus) {
+  ForwardWs w;
+  w.splits = adapter_splits(l, k, cus);
+  w.row = plane_bytes(l, w.splits, r);
+  w.bytes = w.row + row_pack_bytes(l, r);
+  return w;
+}
+struct BackwardWs {
+  int splits;
+  size_t at, bt, row, col, da, db, bytes;
+};
+inline BackwardWs backward_ws(const AdapterLayout& l, int k, int n, int r, int adapters, int cus) {
+  BackwardWs w;
+  w.splits = adapter_splits(l, n, cus);
+  w.at = plane_bytes(l, w.splits, r);
+  w.bt = w.at + up256((size_t)2 * adapters * r * k);
+  w.row = w.bt + up256((size_t)2 * adapters * r * n);
+  w.col = w.row + up256(row_pack_bytes(l, r));
+  w.da = w.col + up256(col_pack_bytes(l, r));
+  w.db = w.da + up256(sizeof(float) * l.chunks * (size_t)r * k);
+  w.bytes = w.db + sizeof(float) * l.chunks * (size_t)r * n;
+  return w;
 }
 
+// What a kernel that multiplies rows with transposed weights reads: in [rows][width],
+// weights [adapters][r][width].
+struct ShrinkArgs {
+  AdapterLayout l;
+  const int32_t* plan;
+  const uint16_t* in;
+  int64_t ld;
+  const uint16_t* weights;
+  int width, r, adapters, drop;
+  const int64_t* seed;
+  float* planes;
+  bool again;  // the rows are read again soon
+};
+hipError_t launch_shrink(bool bf16, const ShrinkArgs& a, int splits, hipStream_t stream);
+hipError_t launch_join(const AdapterArgs& a, const float* planes, int splits, const AdapterPacks& p, hipStream_t stream);
 hipError_t launch_adapter_plan(const AdapterLayout& l, int rows, int adapters, const int32_t* index, int32_t* plan,
                                hipStream_t stream);
-hipError_t launch_adapters(const AdapterArgs& a, int splits, hipStream_t stream);
-hipError_t launch_adapters_grad(const AdapterArgs& a, hipStream_t stream);
+hipError_t launch_adapters(const AdapterArgs& a, const ForwardWs& w, hipStream_t stream);
+hipError_t launch_adapters_grad(const AdapterArgs& a, const BackwardWs& w, hipStream_t stream);
 hipError_t launch_dropout(bool bf16, int rows, int cols, const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int drop,
                           float keep_scale, const int64_t* seed, hipStream_t stream);
 

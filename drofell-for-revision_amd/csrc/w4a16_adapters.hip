@@ -4,9 +4,9 @@
 //
 // Rows are sorted by adapter once per batch (plan_kernel), so that a tile of 16 or 64
 // positions has one adapter and both its products run on 16 x 16 x 32 matrix
-// instructions, rows as their columns.  Two launches: the rows' products with A, in
-// parts of k over workgroups and waves (fp32 planes, joined in order), then the
-// products with B added to the projection's output, rounded once.
+// instructions, rows as their columns.  The rows' products with A are formed in parts of k
+// over workgroups and waves (fp32 planes), joined in order into 16-bit operands, and
+// multiplied with B on top of the projection's output, which is rounded once.
 
 #include <hip/hip_runtime.h>
 
@@ -18,7 +18,7 @@ namespace dw4 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kJoinThreads = 512;
 constexpr int kPlanThreads = 512, kPlanWaves = kPlanThreads / 64;
 
 // Exclusive sums of v[0 .. n) in LDS (n at most 1026), in place; v[n] becomes the total.
@@ -138,53 +138,80 @@ plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__
   }
 }
 
-// Rows' products with A: tile blockIdx.x's RT * 16 positions, part blockIdx.y of k, of
-// which each wave takes a part of its own.
-template <bool BF, int RT, int NT, bool DROP>
-__global__ void __launch_bounds__(kThreads) shrink_kernel(AdapterArgs p, int splits) {
+// Rows' products with A: a tile's RT * 16 positions, a part of the reduced axis, of which each wave takes a part of its own, 64 columns a step.
+template <bool BF, int RT, int NT, bool DROP, bool AGAIN>
+__global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int splits) {
+  constexpr int kAhead = NT <= 2 ? 2 : 1;  // steps whose loads are in flight together
   __shared__ __attribute__((aligned(16))) float red[4][RT * 16][20];
-  const int tile = blockIdx.x;
+  const int item = item_of_xcd(blockIdx.x, gridDim.x), tile = item / splits, split = item - tile * splits;
   const int ad = p.plan[p.l.tile_adapter + tile];
   if (ad < 0 || ad >= p.adapters) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+  const int lane = threadIdx.x & 63, wave = wave_index(), g = lane >> 4, c = lane & 15, unit = line_unit();
   const int32_t* order = p.plan + p.l.order + (int64_t)tile * (RT * 16);
-  const uint16_t* xr[RT];
-  int row[RT];
+  const uint16_t* xr[RT][2];
+  int row[RT][2];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    row[t] = max(order[t * 16 + c], 0);
-    xr[t] = p.x + row[t] * p.ldx;
-  }
-  const uint16_t* ar[NT];
+  for (int t = 0; t < RT; ++t)
 #pragma unroll
-  for (int t = 0; t < NT; ++t) ar[t] = p.a + ((int64_t)ad * p.r + min(t * 16 + c, p.r - 1)) * p.k;
+    for (int i = 0; i < 2; ++i) {
+      row[t][i] = max(order[t * 16 + 8 * i + (c & 7)], 0);
+      xr[t][i] = p.in + row[t][i] * p.ld;
+    }
+  const uint16_t* ar[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ar[t][i] = p.weights + ((int64_t)ad * p.r + min(t * 16 + 8 * i + (c & 7), p.r - 1)) * p.width;
   f4 acc[RT][NT] = {};
   const Philox philox(DROP ? p.seed : reinterpret_cast<const int64_t*>(p.plan));
-  const int steps = (p.k + 31) / 32, parts = splits * 4, part = blockIdx.y * 4 + wave;
+  const int steps = (p.width + 63) / 64, parts = splits * 4, part = split * 4 + wave;
   const int s0 = (int)((int64_t)steps * part / parts), s1 = (int)((int64_t)steps * (part + 1) / parts);
-  for (int s = s0; s < s1; ++s) {
-    const int k = s * 32 + 8 * g, kc = k < p.k ? k : 0;
-    u4 xv[RT], av[NT];
+  struct Step {
+    u4 x[RT][2], a[NT][2];
+  };
+  auto load = [&](int at, Step& v) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) xv[t] = *(const u4*)(xr[t] + kc);
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) av[t] = *(const u4*)(ar[t] + kc);
-    if (s * 32 + 32 > p.k) {
+      for (int t = 0; t < RT; ++t) v.x[t][i] = AGAIN ? *(const u4*)(xr[t][i] + at) : stream_load(xr[t][i] + at);
 #pragma unroll
-      for (int t = 0; t < RT; ++t) xv[t] = k < p.k ? xv[t] : u4{};
-#pragma unroll
-      for (int t = 0; t < NT; ++t) av[t] = k < p.k ? av[t] : u4{};
+      for (int t = 0; t < NT; ++t) v.a[t][i] = *(const u4*)(ar[t][i] + at);
     }
-    if constexpr (DROP) {
+  };
+  auto multiply = [&](int s, Step& v) {
 #pragma unroll
-      for (int t = 0; t < RT; ++t) xv[t] &= philox.mask(k >> 3, row[t], p.drop);
+    for (int t = 0; t < NT; ++t) exchange(v.a[t][0], v.a[t][1]);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if constexpr (DROP) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v.x[t][i] &= philox.mask(s * 8 + unit, row[t][i], p.drop);
+      }
+      exchange(v.x[t][0], v.x[t][1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) acc[t][u] = mfma16_of<BF>(v.a[u][i], v.x[t][i], acc[t][u]);
     }
+  };
+  const int whole = min(s1, p.width / 64);
+  int s = s0;
+  for (; s + kAhead <= whole; s += kAhead) {
+    Step v[kAhead];
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+    for (int i = 0; i < kAhead; ++i) load((s + i) * 64 + unit * 8, v[i]);
+    __builtin_amdgcn_sched_barrier(0);  // (else the loads sink to where they are used)
 #pragma unroll
-      for (int u = 0; u < NT; ++u) acc[t][u] = mfma16_of<BF>(av[u], xv[t], acc[t][u]);
+    for (int i = 0; i < kAhead; ++i) multiply(s + i, v[i]);
   }
-  float* plane = p.ws + ((int64_t)blockIdx.y * p.l.positions + (int64_t)tile * (RT * 16)) * p.r;
+  for (; s < s1; ++s) {  // (the last may be a part of a step)
+    const bool in = s * 64 + unit * 8 < p.width;
+    Step v;
+    load(in ? s * 64 + unit * 8 : 0, v);
+    if (!in) v = Step{};
+    multiply(s, v);
+  }
+  float* plane = p.planes + ((int64_t)split * p.l.positions + (int64_t)tile * (RT * 16)) * p.r;
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     if (u) __syncthreads();
@@ -202,112 +229,230 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(AdapterArgs p, int spl
   }
 }
 
-// The products with B, added to the projection's output: tile blockIdx.x, part
-// blockIdx.y of the columns.
-template <bool BF, int RT, int NT>
-__global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int splits) {
-  constexpr int kRows = RT * 16, kPitch = NT * 16 + 8, kJ = NT == 1 ? 1 : NT / 2;
-  __shared__ __attribute__((aligned(16))) uint16_t part[2][kRows][kPitch];
-  __shared__ int back[kRows];
-  const int tile = blockIdx.x;
+// The sum of a value's planes, in order, sixteen loads in flight.
+__device__ __forceinline__ f4 sum_planes(const float* at, int64_t plane, int splits) {
+  f4 v = {};
+  for (int s = 0; s < splits; s += 16) {
+    f4 x[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = *(const f4*)(at + min(s + e, splits - 1) * plane);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (s + e < splits) v += x[e];
+  }
+  return v;
+}
+
+// 32 positions' h (or dh): planes summed, times s_a / kept share, packed by row and by column.
+template <bool BF, int NT>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(AdapterArgs p, const float* planes, int splits, AdapterPacks packs) {
+  constexpr int kR = NT * 16;
+  __shared__ float v[32][kR + 1];
+  __shared__ int exps[32];
+  const int64_t first = (int64_t)blockIdx.x * 32;
+  const int ad = p.plan[p.l.tile_adapter + first / p.l.align];
+  if (ad < 0 || ad >= p.adapters) return;
+  const float scale = p.scaling[ad] * p.keep_scale;
+  for (int i = threadIdx.x; i < 32 * (kR / 4); i += kJoinThreads) {
+    const int at = i / (kR / 4), q = i % (kR / 4) * 4;
+    f4 s = {};
+    if (q < p.r) s = sum_planes(planes + (first + at) * p.r + q, p.l.positions * p.r, splits) * scale;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[at][q + e] = s[e];
+  }
+  __syncthreads();
+  if (packs.row != nullptr) {
+    if constexpr (!BF) {  // sixteen threads a row
+      const int at = threadIdx.x >> 4;
+      float m = 0.f;
+#pragma unroll
+      for (int e = 0; e < kR / 16; ++e) m = fmaxf(m, fabsf(v[at][(threadIdx.x & 15) + 16 * e]));
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+      if ((threadIdx.x & 15) == 0) {
+        exps[at] = range_exponent<BF>(m);
+        packs.row_exp[first + at] = -exps[at];
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < 32 * (kR / 8); i += kJoinThreads) {
+      const int at = i / (kR / 8), q = i % (kR / 8) * 8;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = BF ? v[at][q + e] : times_pow2(v[at][q + e], exps[at]);
+      u4 hi, lo;
+      split16<BF>(x, hi, lo);
+      uint16_t* to = packs.row + (first + at) * kR + q;
+      *(u4*)to = hi;
+      *(u4*)(to + p.l.positions * kR) = lo;
+    }
+  }
+  if (packs.col == nullptr) return;
+  for (int i = threadIdx.x; i < 4 * kR; i += kJoinThreads) {  // column i % kR, eight rows
+    const int col = i % kR, r0 = i / kR * 8;
+    int ex = 0;
+    if constexpr (!BF) {
+      float m = 0.f;
+      for (int e = 0; e < 32; ++e) m = fmaxf(m, fabsf(v[e][col]));
+      ex = range_exponent<BF>(m);
+      if (r0 == 0) packs.col_exp[first / 32 * kR + col] = -ex;
+    }
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = BF ? v[r0 + e][col] : times_pow2(v[r0 + e][col], ex);
+    u4 hi, lo;
+    split16<BF>(x, hi, lo);
+    uint16_t* to = packs.col + ((first + r0) * kR + col * 8);
+    *(u4*)to = hi;
+    *(u4*)(to + p.l.positions * kR) = lo;
+  }
+}
+
+// The products with B, added to the projection's output: a tile's rows, a part of the columns.  JOIN: the workgroup sums the planes itself (few rows: one launch
+// less); else the packed rows are read.
+template <bool BF, int RT, int NT, bool JOIN>
+__global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int splits, AdapterPacks packs, int wide) {
+  constexpr int kRows = RT * 16, kR = NT * 16, kPitch = kR + 8, kJ = NT == 1 ? 1 : NT / 2;
+  const int item = item_of_xcd(blockIdx.x, gridDim.x), tile = item / wide, column_part = item - tile * wide;
   const int ad = p.plan[p.l.tile_adapter + tile];
   if (ad < 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+  const int lane = threadIdx.x & 63, wave = wave_index(), g = lane >> 4, c = lane & 15;
   const int32_t* order = p.plan + p.l.order + (int64_t)tile * kRows;
-  const int groups = (p.n + 31) / 32;
-  const int g0 = (int)((int64_t)groups * blockIdx.y / gridDim.y), g1 = (int)((int64_t)groups * (blockIdx.y + 1) / gridDim.y);
+  const int groups = (p.n + 63) / 64;
+  const int g0 = (int)((int64_t)groups * column_part / wide), g1 = (int)((int64_t)groups * (column_part + 1) / wide);
   if (ad >= p.adapters) {  // rows without an adapter keep the projection's output
     if (p.out == p.base) return;
-    const int units = min(g1 * 4, p.n / 8) - g0 * 4;
+    const int units = min(g1 * 8, p.n / 8) - g0 * 8;
     for (int i = 0; i < kRows; ++i) {
       const int row = order[i];
       if (row < 0) break;
       for (int u = threadIdx.x; u < units; u += kThreads)
-        *(u4*)(p.out + row * p.ldo + (g0 * 4 + u) * 8) = *(const u4*)(p.base + row * p.ldb + (g0 * 4 + u) * 8);
+        *(u4*)(p.out + row * p.ldo + (g0 * 8 + u) * 8) = *(const u4*)(p.base + row * p.ldb + (g0 * 8 + u) * 8);
     }
     return;
   }
-  const float scale = p.scaling[ad] * p.keep_scale;
-  for (int i = threadIdx.x; i < kRows * NT * 4; i += kThreads) {
-    const int at = i / (NT * 4), q = i % (NT * 4) * 4;
-    f4 v = {};
-    if (q < p.r) {
-      const int64_t pos = ((int64_t)tile * kRows + at) * p.r + q;
-      for (int s = 0; s < splits; ++s) v += *(const f4*)(p.ws + (int64_t)s * p.l.positions * p.r + pos);
-      if (p.h != nullptr && blockIdx.y == 0) *(f4*)(p.h + pos) = v;
-      v *= scale;
-    }
-    int e = 0;
-    if constexpr (!BF) {
-      float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-#pragma unroll
-      for (int o = 1; o < NT * 4; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-      e = range_exponent<BF>(m);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = times_pow2(v[j], e);
-    }
-    if (q == 0) back[at] = -e;
-    uint2 hi, lo;
-    split16<BF>(v[0], v[1], hi.x, lo.x);
-    split16<BF>(v[2], v[3], hi.y, lo.y);
-    *(uint2*)&part[0][at][q] = hi;
-    *(uint2*)&part[1][at][q] = lo;
-  }
-  __syncthreads();
   // rank 16: both parts in one instruction, the second in the reduction's upper half
   u4 hv[RT][kJ], lv[RT][kJ];
-  int row[RT], scale_back[RT];
+  float back[RT];
+  if constexpr (JOIN) {
+    __shared__ __attribute__((aligned(16))) uint16_t part[2][kRows][kPitch];
+    __shared__ int back_s[kRows];
+    const float scale = p.scaling[ad] * p.keep_scale;
+    const float* planes = reinterpret_cast<const float*>(p.ws);
+    for (int i = threadIdx.x; i < kRows * NT * 4; i += kThreads) {
+      const int at = i / (NT * 4), q = i % (NT * 4) * 4;
+      f4 v = {};
+      if (q < p.r && order[at] >= 0)
+        v = sum_planes(planes + ((int64_t)tile * kRows + at) * p.r + q, p.l.positions * p.r, splits) * scale;
+      if constexpr (!BF) {
+        float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    row[t] = order[t * 16 + c];
-    scale_back[t] = back[t * 16 + c];
-    if constexpr (NT == 1) {
-      hv[t][0] = *(const u4*)&part[g >> 1][t * 16 + c][(g & 1) * 8];
-    } else {
+        for (int o = 1; o < NT * 4; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const int e = range_exponent<BF>(m);
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) {
-        hv[t][j] = *(const u4*)&part[0][t * 16 + c][32 * j + 8 * g];
-        lv[t][j] = *(const u4*)&part[1][t * 16 + c][32 * j + 8 * g];
+        for (int j = 0; j < 4; ++j) v[j] = times_pow2(v[j], e);
+        if (q == 0) back_s[at] = -e;
       }
+      uint2 hi, lo;
+      split16<BF>(v[0], v[1], hi.x, lo.x);
+      split16<BF>(v[2], v[3], hi.y, lo.y);
+      *(uint2*)&part[0][at][q] = hi;
+      *(uint2*)&part[1][at][q] = lo;
     }
-  }
-  for (int grp = g0 + wave; grp < g1; grp += 4) {
-    const int n = grp * 32 + 8 * g;  // the lane's eight output columns
-    const bool in = n < p.n;
-    u4 y[RT];
+    __syncthreads();
 #pragma unroll
-    for (int t = 0; t < RT; ++t) y[t] = *(const u4*)(p.base + max(row[t], 0) * p.ldb + (in ? n : 0));
-    f4 acc[RT][2] = {};
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int col = min(grp * 32 + (c >> 2) * 8 + u * 4 + (c & 3), p.n - 1);
-      const uint16_t* br = p.b + ((int64_t)ad * p.n + col) * p.r;
+    for (int t = 0; t < RT; ++t) {
+      if constexpr (!BF) back[t] = pow2(back_s[t * 16 + c]);
 #pragma unroll
       for (int j = 0; j < kJ; ++j) {
         const int r = NT == 1 ? (g & 1) * 8 : 32 * j + 8 * g;
-        u4 bv = *(const u4*)(br + (r < p.r ? r : 0));
-        if (r >= p.r) bv = u4{};
+        hv[t][j] = *(const u4*)&part[NT == 1 ? g >> 1 : 0][t * 16 + c][r];
+        if constexpr (NT > 1) lv[t][j] = *(const u4*)&part[1][t * 16 + c][r];
+      }
+    }
+  } else {
+    const int64_t half = p.l.positions * kR;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          acc[t][u] = mfma16_of<BF>(bv, hv[t][j], acc[t][u]);
-          if constexpr (NT > 1) acc[t][u] = mfma16_of<BF>(bv, lv[t][j], acc[t][u]);
-        }
+    for (int t = 0; t < RT; ++t) {
+      const int64_t pos = (int64_t)tile * kRows + t * 16 + c;
+      if constexpr (!BF) back[t] = pow2(packs.row_exp[pos]);
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) {
+        const uint16_t* at = packs.row + pos * kR + (NT == 1 ? (g >> 1) * half + (g & 1) * 8 : 32 * j + 8 * g);
+        hv[t][j] = *(const u4*)at;
+        if constexpr (NT > 1) lv[t][j] = *(const u4*)(at + half);
+      }
+    }
+  }
+  // rows as loads and stores take them (exchange())
+  int row[RT][2];
+  const uint16_t* from[RT][2];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      row[t][i] = order[t * 16 + 8 * i + (c & 7)];
+      from[t][i] = p.base + max(row[t][i], 0) * p.ldb;
+    }
+  const int unit = line_unit();
+  const uint16_t* const bw = p.b + (int64_t)ad * p.n * p.r;
+  struct Group {
+    u4 y[RT][2], b[4][kJ];
+  };
+  // the lane's eight columns of unit g (operands 0 and 1) and of unit 4 + g (2 and 3)
+  auto load = [&](int grp, Group& v) {
+    const int n = grp * 64 + unit * 8;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int col = min(grp * 64 + (u >> 1) * 32 + (c >> 2) * 8 + (u & 1) * 4 + (c & 3), p.n - 1);
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) {
+        const int r = NT == 1 ? (g & 1) * 8 : 32 * j + 8 * g;
+        v.b[u][j] = *(const u4*)(bw + (int64_t)col * p.r + (r < p.r ? r : 0));
       }
     }
 #pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v.y[t][i] = stream_load(from[t][i] + (n < p.n ? n : 0));
+  };
+  for (int grp = g0 + wave; grp < g1; grp += 4) {
+    Group v;
+    load(grp, v);
+    __builtin_amdgcn_sched_barrier(0);
+    const bool in = grp * 64 + unit * 8 < p.n;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+        if ((NT == 1 ? (g & 1) * 8 : 32 * j + 8 * g) >= p.r) v.b[u][j] = u4{};
+#pragma unroll
     for (int t = 0; t < RT; ++t) {
-      u4 o;
+      f4 acc[4] = {};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v[2];
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float d = acc[t][e >> 1][(e & 1) * 2 + j];
-          v[j] = unpack16<BF>(y[t][e], j) + (BF ? d : times_pow2(d, scale_back[t]));
+        for (int j = 0; j < kJ; ++j) {
+          acc[u] = mfma16_of<BF>(v.b[u][j], hv[t][j], acc[u]);
+          if constexpr (NT > 1) acc[u] = mfma16_of<BF>(v.b[u][j], lv[t][j], acc[u]);
         }
-        o[e] = pack16<BF>(v[0], v[1]);
-      }
-      if (in && row[t] >= 0) *(u4*)(p.out + row[t] * p.ldo + n) = o;
+      exchange(v.y[t][0], v.y[t][1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float w[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float d = acc[2 * i + (e >> 1)][(e & 1) * 2 + j];
+            w[j] = BF ? unpack16<BF>(v.y[t][i][e], j) + d : fmaf(d, back[t], unpack16<BF>(v.y[t][i][e], j));
+          }
+          v.y[t][i][e] = pack16<BF>(w[0], w[1]);
+        }
+      exchange(v.y[t][0], v.y[t][1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (in && row[t][i] >= 0) *(u4*)(p.out + row[t][i] * p.ldo + grp * 64 + unit * 8) = v.y[t][i];
     }
   }
 }
@@ -347,28 +492,43 @@ dropout_kernel(int rows, int cols, const uint16_t* __restrict__ x, int64_t ldx, 
 }
 
 template <bool BF, int RT, int NT>
-void launch_forward(const AdapterArgs& a, int splits, hipStream_t stream) {
-  const dim3 grid(a.l.tiles, splits);
-  if (a.drop) shrink_kernel<BF, RT, NT, true><<<grid, kThreads, 0, stream>>>(a, splits);
-  else shrink_kernel<BF, RT, NT, false><<<grid, kThreads, 0, stream>>>(a, splits);
-  const int groups = (a.n + 31) / 32;
-  const int wide = std::max(1, std::min((groups + 3) / 4, 1024 / a.l.tiles));
-  expand_kernel<BF, RT, NT><<<dim3(a.l.tiles, wide), kThreads, 0, stream>>>(a, splits);
+void shrink_of(const ShrinkArgs& a, int splits, hipStream_t stream) {
+  const unsigned grid = (unsigned)a.l.tiles * splits;
+  if (a.again) shrink_kernel<BF, RT, NT, false, true><<<grid, kThreads, 0, stream>>>(a, splits);
+  else if (a.drop) shrink_kernel<BF, RT, NT, true, false><<<grid, kThreads, 0, stream>>>(a, splits);
+  else shrink_kernel<BF, RT, NT, false, false><<<grid, kThreads, 0, stream>>>(a, splits);
 }
 template <bool BF, int RT>
-void launch_rank(const AdapterArgs& a, int splits, hipStream_t stream) {
-  if (a.r <= 16) launch_forward<BF, RT, 1>(a, splits, stream);
-  else if (a.r <= 32) launch_forward<BF, RT, 2>(a, splits, stream);
-  else if (a.r <= 64) launch_forward<BF, RT, 4>(a, splits, stream);
-  else launch_forward<BF, RT, 8>(a, splits, stream);
+void shrink_rank(const ShrinkArgs& a, int splits, hipStream_t stream) {
+  if (a.r <= 16) shrink_of<BF, RT, 1>(a, splits, stream);
+  else if (a.r <= 32) shrink_of<BF, RT, 2>(a, splits, stream);
+  else if (a.r <= 64) shrink_of<BF, RT, 4>(a, splits, stream);
+  else shrink_of<BF, RT, 8>(a, splits, stream);
+}
+
+template <bool BF, int NT>
+void expand_of(const AdapterArgs& a, int splits, bool join, const AdapterPacks& packs, hipStream_t stream) {
+  const int groups = (a.n + 63) / 64;
+  const int wide = std::max(1, std::min((groups + 3) / 4, 512 / a.l.tiles));
+  const unsigned grid = (unsigned)a.l.tiles * wide;
+  if (a.l.align == 64) expand_kernel<BF, 4, NT, false><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
+  else if (join) expand_kernel<BF, 2, NT, true><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
+  else expand_kernel<BF, 2, NT, false><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
+}
+template <bool BF>
+void expand_rank(const AdapterArgs& a, int splits, bool join, const AdapterPacks& packs, hipStream_t stream) {
+  if (a.r <= 16) expand_of<BF, 1>(a, splits, join, packs, stream);
+  else if (a.r <= 32) expand_of<BF, 2>(a, splits, join, packs, stream);
+  else if (a.r <= 64) expand_of<BF, 4>(a, splits, join, packs, stream);
+  else expand_of<BF, 8>(a, splits, join, packs, stream);
 }
 
 }  // namespace
 
-int adapter_splits(const AdapterLayout& l, int k, int cus) {
-  // about three workgroups per CU, parts of at least 64 values of k per wave
-  const int want = (3 * cus + l.tiles - 1) / l.tiles;
-  return std::max(1, std::min({want, k / 256, 32}));
+int adapter_splits(const AdapterLayout& l, int width, int cus) {
+  // about four workgroups per CU, parts of at least 64 values per wave
+  const int want = (4 * cus + l.tiles - 1) / l.tiles;
+  return std::max(1, std::min({want, width / 256, 32}));
 }
 
 hipError_t launch_adapter_plan(const AdapterLayout& l, int rows, int adapters, const int32_t* index, int32_t* plan,
@@ -378,9 +538,36 @@ hipError_t launch_adapter_plan(const AdapterLayout& l, int rows, int adapters, c
   return hipGetLastError();
 }
 
-hipError_t launch_adapters(const AdapterArgs& a, int splits, hipStream_t stream) {
-  if (a.l.align == 16) a.bf16 ? launch_rank<true, 1>(a, splits, stream) : launch_rank<false, 1>(a, splits, stream);
-  else a.bf16 ? launch_rank<true, 4>(a, splits, stream) : launch_rank<false, 4>(a, splits, stream);
+hipError_t launch_shrink(bool bf16, const ShrinkArgs& a, int splits, hipStream_t stream) {
+  if (a.l.align == 32) bf16 ? shrink_rank<true, 2>(a, splits, stream) : shrink_rank<false, 2>(a, splits, stream);
+  else bf16 ? shrink_rank<true, 4>(a, splits, stream) : shrink_rank<false, 4>(a, splits, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_join(const AdapterArgs& a, const float* planes, int splits, const AdapterPacks& p, hipStream_t stream) {
+  const unsigned grid = (unsigned)(a.l.positions / 32);
+  auto go = [&](auto kernel) { kernel<<<grid, kJoinThreads, 0, stream>>>(a, planes, splits, p); };
+  switch (padded_rank(a.r)) {
+    case 16: a.bf16 ? go(&join_kernel<true, 1>) : go(&join_kernel<false, 1>); break;
+    case 32: a.bf16 ? go(&join_kernel<true, 2>) : go(&join_kernel<false, 2>); break;
+    case 64: a.bf16 ? go(&join_kernel<true, 4>) : go(&join_kernel<false, 4>); break;
+    default: a.bf16 ? go(&join_kernel<true, 8>) : go(&join_kernel<false, 8>);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_adapters(const AdapterArgs& a, const ForwardWs& w, hipStream_t stream) {
+  float* const planes = reinterpret_cast<float*>(a.ws);
+  const ShrinkArgs s = {a.l, a.plan, a.x, a.ldx, a.a, a.k, a.r, a.adapters, a.drop, a.seed, planes, false};
+  hipError_t e = launch_shrink(a.bf16, s, w.splits, stream);
+  if (e != hipSuccess) return e;
+  // a batch of few rows whose h nobody keeps: the second launch joins the planes itself
+  const bool join = a.l.align == 32 && a.h == nullptr;
+  AdapterPacks packs = {};
+  place_row(packs, a.l, a.r, a.ws + w.row);
+  if (a.h != nullptr) place_col(packs, a.l, a.r, a.h);
+  if (!join && (e = launch_join(a, planes, w.splits, packs, stream)) != hipSuccess) return e;
+  a.bf16 ? expand_rank<true>(a, w.splits, join, packs, stream) : expand_rank<false>(a, w.splits, join, packs, stream);
   return hipGetLastError();
 }
 

@@ -57,7 +57,7 @@ float keep_scale(int drop) { return drop < 65536 ? 65536.f / (float)(65536 - dro
 
 dw4::AdapterArgs adapter_args(int dtype, int rows, int k, int n, int rank, int adapters, const uint16_t* x, int64_t ldx,
                               const uint16_t* a, const uint16_t* b, const float* scaling, const int32_t* plan, int drop,
-                              const int64_t* seed, float* h, void* ws) {
+                              const int64_t* seed, void* h, void* ws) {
   dw4::AdapterArgs p = {};
   p.l = dw4::adapter_layout(rows, adapters);
   p.bf16 = dtype == DW4_BF16;
@@ -76,7 +76,7 @@ dw4::AdapterArgs adapter_args(int dtype, int rows, int k, int n, int rank, int a
   p.seed = seed;
   p.keep_scale = keep_scale(drop);
   p.h = h;
-  p.ws = static_cast<float*>(ws);
+  p.ws = static_cast<unsigned char*>(ws);
   return p;
 }
 
@@ -120,18 +120,17 @@ int dw4_adapters_workspace_size(int num_rows, int num_adapters, int k, int n, in
   DW4_TRY(check_shape(num_rows, num_adapters, k, n, rank));
   if (workspace_bytes == nullptr) return DW4_ERR_INVALID_ARG;
   const dw4::AdapterLayout l = dw4::adapter_layout(num_rows, num_adapters);
-  if (h_bytes != nullptr) *h_bytes = num_rows ? sizeof(float) * (size_t)l.positions * rank : 0;
-  size_t floats = 0;
+  if (h_bytes != nullptr) *h_bytes = num_rows ? dw4::col_pack_bytes(l, rank) : 0;
+  *workspace_bytes = 0;
   if (num_rows > 0)
-    floats = backward ? dw4::adapter_grad_parts(l, k, n, rank).floats
-                      : dw4::adapter_ws_floats(l, dw4::adapter_splits(l, k, dw4::cu_count()), rank);
-  *workspace_bytes = sizeof(float) * floats;
+    *workspace_bytes = backward ? dw4::backward_ws(l, k, n, rank, num_adapters, dw4::cu_count()).bytes
+                                : dw4::forward_ws(l, k, rank, dw4::cu_count()).bytes;
   return DW4_OK;
 }
 
 int dw4_adapters(int dtype, int num_rows, int num_adapters, int k, int n, int rank, const uint16_t* x, int64_t ldx,
                  const uint16_t* base, int64_t ldb, uint16_t* out, int64_t ldo, const uint16_t* a, const uint16_t* b,
-                 const float* scaling, const int32_t* plan, int drop, const int64_t* seed, float* h, void* workspace,
+                 const float* scaling, const int32_t* plan, int drop, const int64_t* seed, void* h, void* workspace,
                  size_t workspace_bytes, void* stream) {
   if (!good_dtype(dtype)) return DW4_ERR_UNSUPPORTED;
   DW4_TRY(check_shape(num_rows, num_adapters, k, n, rank));
@@ -148,15 +147,15 @@ int dw4_adapters(int dtype, int num_rows, int num_adapters, int k, int n, int ra
   p.ldb = ldb;
   p.out = out;
   p.ldo = ldo;
-  const int splits = dw4::adapter_splits(p.l, k, dw4::cu_count());
-  if (workspace == nullptr || workspace_bytes < sizeof(float) * dw4::adapter_ws_floats(p.l, splits, rank)) return DW4_ERR_WORKSPACE;
+  const dw4::ForwardWs w = dw4::forward_ws(p.l, k, rank, dw4::cu_count());
+  if (workspace == nullptr || workspace_bytes < w.bytes) return DW4_ERR_WORKSPACE;
   if (!aligned16(workspace)) return DW4_ERR_MISALIGNED;
-  return status_of(dw4::launch_adapters(p, splits, static_cast<hipStream_t>(stream)));
+  return status_of(dw4::launch_adapters(p, w, static_cast<hipStream_t>(stream)));
 }
 
 int dw4_adapters_backward(int dtype, int num_rows, int num_adapters, int k, int n, int rank, const uint16_t* x, int64_t ldx,
                           const uint16_t* dout, int64_t ldd, const uint16_t* a, const uint16_t* b, const float* scaling,
-                          const int32_t* plan, int drop, const int64_t* seed, const float* h, uint16_t* dx, int64_t lddx,
+                          const int32_t* plan, int drop, const int64_t* seed, const void* h, uint16_t* dx, int64_t lddx,
                           uint16_t* da, uint16_t* db, void* workspace, size_t workspace_bytes, void* stream) {
   if (!good_dtype(dtype)) return DW4_ERR_UNSUPPORTED;
   DW4_TRY(check_shape(num_rows, num_adapters, k, n, rank));
@@ -171,17 +170,17 @@ int dw4_adapters_backward(int dtype, int num_rows, int num_adapters, int k, int 
     return DW4_ERR_MISALIGNED;
   if (dx == nullptr && da == nullptr && db == nullptr) return DW4_OK;
   dw4::AdapterArgs p = adapter_args(dtype, num_rows, k, n, rank, num_adapters, x, ldx, a, b, scaling, plan, drop, seed,
-                                    const_cast<float*>(h), workspace);
+                                    const_cast<void*>(h), workspace);
   p.g = dout;
   p.ldg = ldd;
   p.dx = dx;
   p.lddx = lddx;
   p.da = num_adapters ? da : nullptr;
   p.db = num_adapters ? db : nullptr;
-  if (workspace == nullptr || workspace_bytes < sizeof(float) * dw4::adapter_grad_parts(p.l, k, n, rank).floats)
-    return DW4_ERR_WORKSPACE;
+  const dw4::BackwardWs w = dw4::backward_ws(p.l, k, n, rank, num_adapters, dw4::cu_count());
+  if (workspace == nullptr || workspace_bytes < w.bytes) return DW4_ERR_WORKSPACE;
   if (!aligned16(workspace)) return DW4_ERR_MISALIGNED;
-  return status_of(dw4::launch_adapters_grad(p, static_cast<hipStream_t>(stream)));
+  return status_of(dw4::launch_adapters_grad(p, w, static_cast<hipStream_t>(stream)));
 }
 
 int dw4_dropout(int dtype, int num_rows, int cols, const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int drop,

@@ -36,8 +36,14 @@ from .real import Linear
 _DTYPES = {torch.float16: _lib.DW4_F16, torch.bfloat16: _lib.DW4_BF16}
 
 
+def _whole(x: torch.Tensor) -> torch.Tensor:
+    return x if x.is_contiguous() else x.contiguous()
+
+
 def _matrix(x: torch.Tensor) -> torch.Tensor:
     """x [rows, width] as the kernels read it, in 16-byte units of its rows; a copy where it is not so."""
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x
     if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < x.shape[1])):
         return x.clone(memory_format=torch.contiguous_format)
     return x
@@ -134,28 +140,34 @@ class LowRankAdapters(nn.Module):
         read where dropout applies; another step takes another offset, another projection another
         seed.  Differentiable (once) in x, base, ``a`` and ``b``.  ``output``, without gradients:
         where the result goes, which may be ``base``."""
-        if x.shape[-1] != self.in_features or base.shape != (*x.shape[:-1], self.out_features):
+        params = self._parameters  # (attribute look-up on a module takes 0.4 us each)
+        a, b, scaling = params["a"], params["b"], self._buffers["scaling"]
+        device, dtype = x.device, x.dtype
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        base2 = base if base.dim() == 2 else base.reshape(-1, base.shape[-1])
+        num_rows, width = x2.shape
+        if width != self.in_features or base2.shape != (num_rows, self.out_features) or x.shape[:-1] != base.shape[:-1]:
             raise ValueError(f"x and base must be [..., {self.in_features}] and [..., {self.out_features}] of the same rows")
-        a, b, device = self.a, self.b, x.device
-        if x.dtype not in _DTYPES or any(t.dtype != x.dtype for t in (base, a, b)):
+        if dtype not in _DTYPES or base.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
             raise TypeError("x, base and the adapters must be of one type, fp16 or bf16")
-        if any(t.device != device for t in (base, a, self.scaling, rows)):
+        if base.device != device or a.device != device or scaling.device != device or rows.device != device:
             raise ValueError(f"x, base, the adapters and their rows must be on one device ({device})")
-        x2, base2 = x.reshape(-1, self.in_features), base.reshape(-1, self.out_features)
-        if x2.shape[0] != rows.num_rows or rows.num_adapters != self.num_adapters:
+        if num_rows != rows.num_rows or rows.num_adapters != self.num_adapters:
             raise ValueError(f"rows were sorted for {rows.num_rows} rows of {rows.num_adapters} adapters, "
-                             f"not for {x2.shape[0]} of {self.num_adapters}")
+                             f"not for {num_rows} of {self.num_adapters}")
         drop = self._dropped if self.training else 0
         seed = _seed(seed, device) if drop else None
-        scaling = self.scaling if self.scaling.dtype == torch.float32 else self.scaling.float()
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, base, a, b)):
+        if scaling.dtype != torch.float32:  # (of a module that was made half)
+            scaling = scaling.float()
+        if torch.is_grad_enabled() and (a.requires_grad or x.requires_grad or b.requires_grad or base.requires_grad):
             if output is not None:
                 raise ValueError("output is for calls without gradients")
-            out2 = _LowRank.apply(x2, base2, a, b, scaling, rows, drop, seed)
-            return out2.view(base.shape)
+            out2 = _LowRank.apply(x2, base2, a, b, scaling, rows.plan, drop, seed)
+            return out2 if base.dim() == 2 else out2.view(base.shape)
         if output is None:
-            return _forward(x2, base2, a, b, scaling, rows.plan, drop, seed, None, False)[0].view(base.shape)
-        if output.shape != base.shape or output.dtype != x.dtype or output.device != device or \
+            out2 = _forward(x2, base2, a, b, scaling, rows.plan, drop, seed, None, False)[0]
+            return out2 if base.dim() == 2 else out2.view(base.shape)
+        if output.shape != base.shape or output.dtype != dtype or output.device != device or \
                 not output.is_contiguous() or output.data_ptr() % 16:
             raise ValueError("output must be contiguous and 16-byte aligned, of base's shape, type and device")
         _forward(x2, base2, a, b, scaling, rows.plan, drop, seed, output.view(-1, self.out_features), False)
@@ -163,61 +175,61 @@ class LowRankAdapters(nn.Module):
         return output
 
 
-def _shape(x, a, b):
-    return _DTYPES[x.dtype], x.shape[0], a.shape[0], x.shape[1], b.shape[1], a.shape[1]
-
-
 def _forward(x, base, a, b, scaling, plan, drop, seed, out, keep):
+    """The call itself -> (out, x as the kernels read it, h or None, its shape)."""
     device = x.device
     with _lib.on_device(device):
         x, base = _matrix(x), _matrix(base)
-        a, b, scaling = a.contiguous(), b.contiguous(), scaling.contiguous()
+        a, b, scaling = _whole(a), _whole(b), _whole(scaling)
+        shape = (_DTYPES[x.dtype], x.shape[0], a.shape[0], x.shape[1], b.shape[1], a.shape[1])
+        nbytes, h_bytes = _lib.adapters_workspace_size(*shape[1:], False, device.index)
         if out is None:
             out = torch.empty(base.shape, dtype=x.dtype, device=device)
-        shape = _shape(x, a, b)
-        nbytes, h_bytes = _lib.adapters_workspace_size(*shape[1:], False, device.index)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        h = torch.empty(h_bytes // 4, dtype=torch.float32, device=device) if keep else None
+        h = torch.empty(h_bytes, dtype=torch.uint8, device=device) if keep else None
         _lib.call("dw4_adapters", *shape, x.data_ptr(), _stride(x), base.data_ptr(), _stride(base), out.data_ptr(),
                   _stride(out), a.data_ptr(), b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), drop,
                   None if seed is None else seed.data_ptr(), None if h is None else h.data_ptr(), ws.data_ptr(), nbytes,
                   _lib.current_stream(device.index))
-    return out, x, h
+    return out, x, h, shape
 
 
 class _LowRank(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, base, a, b, scaling, rows, drop, seed):
-        out, x, h = _forward(x, base, a, b, scaling, rows.plan, drop, seed, None, True)
-        ctx.drop = drop
-        ctx.save_for_backward(x, a, b, scaling, rows.plan, h, seed)
+    def forward(ctx, x, base, a, b, scaling, plan, drop, seed):
+        a, b, scaling = _whole(a), _whole(b), _whole(scaling)
+        out, x, h, shape = _forward(x, base, a, b, scaling, plan, drop, seed, None, True)
+        # what the backward pass needs, worked out here: it runs in a thread of autograd's, where
+        # the same Python takes twice as long
+        index = x.device.index
+        nbytes = _lib.adapters_workspace_size(*shape[1:], True, index)[0] if shape[1] else 0
+        ctx.call = shape, drop, nbytes, x.device, _stride(x)
+        ctx.save_for_backward(x, a, b, scaling, plan, h, seed)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         x, a, b, scaling, plan, h, seed = ctx.saved_tensors
-        device = x.device
+        shape, drop, nbytes, device, ldx = ctx.call
         need_x, need_base, need_a, need_b = ctx.needs_input_grad[:4]
         dbase = dout if need_base else None
-        if x.shape[0] == 0:
+        if shape[1] == 0:
             return (torch.zeros_like(x) if need_x else None, dbase, torch.zeros_like(a) if need_a else None,
                     torch.zeros_like(b) if need_b else None, None, None, None, None)
         if not (need_x or need_a or need_b):
-            return (None, dbase, None, None, None, None, None, None)
+            return None, dbase, None, None, None, None, None, None
         with _lib.on_device(device):
             g = _matrix(dout)
-            a, b, scaling = a.contiguous(), b.contiguous(), scaling.contiguous()
-            dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
-            da = torch.empty(a.shape, dtype=x.dtype, device=device) if need_a else None
-            db = torch.empty(b.shape, dtype=x.dtype, device=device) if need_b else None
-            shape = _shape(x, a, b)
-            nbytes, _ = _lib.adapters_workspace_size(*shape[1:], True, device.index)
+            dtype = x.dtype
+            dx = torch.empty(x.shape, dtype=dtype, device=device) if need_x else None
+            da = torch.empty(a.shape, dtype=dtype, device=device) if need_a else None
+            db = torch.empty(b.shape, dtype=dtype, device=device) if need_b else None
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-            _lib.call("dw4_adapters_backward", *shape, x.data_ptr(), _stride(x), g.data_ptr(), _stride(g), a.data_ptr(),
-                      b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), ctx.drop,
+            _lib.call("dw4_adapters_backward", *shape, x.data_ptr(), ldx, g.data_ptr(), _stride(g), a.data_ptr(),
+                      b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), drop,
                       None if seed is None else seed.data_ptr(), h.data_ptr(),
-                      None if dx is None else dx.data_ptr(), x.shape[1], None if da is None else da.data_ptr(),
+                      None if dx is None else dx.data_ptr(), shape[3], None if da is None else da.data_ptr(),
                       None if db is None else db.data_ptr(), ws.data_ptr(), nbytes, _lib.current_stream(device.index))
         return dx, dbase, da, db, None, None, None, None
 

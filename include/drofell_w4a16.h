@@ -654,12 +654,12 @@ int dw4_adapter_plan(int num_rows, int num_adapters, const int32_t* adapters, in
 
 /* out may be base (with its stride).  drop: an element of x is zero with probability
  * drop / 65536, by dw4_dropout's rule, and the others are scaled up; 0: no dropout, seed
- * is not read.  h: float, h_bytes, what the backward pass needs, or NULL.
+ * is not read.  h: h_bytes, 16-byte aligned, what the backward pass needs, or NULL.
  * workspace: dw4_adapters_workspace_size bytes (backward 0). */
 int dw4_adapters(int dtype, int num_rows, int num_adapters, int k, int n, int rank,
                  const uint16_t* x, int64_t ldx, const uint16_t* base, int64_t ldb, uint16_t* out,
                  int64_t ldo, const uint16_t* a, const uint16_t* b, const float* scaling,
-                 const int32_t* plan, int drop, const int64_t* seed, float* h, void* workspace,
+                 const int32_t* plan, int drop, const int64_t* seed, void* h, void* workspace,
                  size_t workspace_bytes, void* stream);
 int dw4_adapters_workspace_size(int num_rows, int num_adapters, int k, int n, int rank, int backward,
                                 size_t* workspace_bytes, size_t* h_bytes);
@@ -671,7 +671,7 @@ int dw4_adapters_workspace_size(int num_rows, int num_adapters, int k, int n, in
 int dw4_adapters_backward(int dtype, int num_rows, int num_adapters, int k, int n, int rank,
                           const uint16_t* x, int64_t ldx, const uint16_t* dout, int64_t ldd,
                           const uint16_t* a, const uint16_t* b, const float* scaling,
-                          const int32_t* plan, int drop, const int64_t* seed, const float* h,
+                          const int32_t* plan, int drop, const int64_t* seed, const void* h,
                           uint16_t* dx, int64_t lddx, uint16_t* da, uint16_t* db, void* workspace,
                           size_t workspace_bytes, void* stream);
 

@@ -473,7 +473,7 @@ dropout_kernel(int rows, int cols, const uint16_t* __restrict__ x, int64_t ldx, 
     const int n = min(8, cols - unit * 8);
     u4 v = {};
     if constexpr (VEC) {
-      v = *(const u4*)xr;
+      v = stream_load(xr);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -574,7 +574,7 @@ hipError_t launch_adapters(const AdapterArgs& a, const ForwardWs& w, hipStream_t
 hipError_t launch_dropout(bool bf16, int rows, int cols, const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int drop,
                           float keep_scale, const int64_t* seed, hipStream_t stream) {
   const int64_t items = (int64_t)rows * ((cols + 7) / 8);
-  const unsigned grid = (unsigned)std::min<int64_t>((items + kThreads - 1) / kThreads, 1 << 16);
+  const unsigned grid = (unsigned)std::min<int64_t>((items + kThreads - 1) / kThreads, 8192);
   const bool vec = cols % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(y) % 16 == 0;
   auto kernel = bf16 ? (vec ? &dropout_kernel<true, true> : &dropout_kernel<true, false>)

@@ -65,8 +65,9 @@ __device__ __forceinline__ int item_of_xcd(int b, int items) {
   const int each = items / 8, more = items % 8, xcd = b & 7;
   return xcd * each + min(xcd, more) + (b >> 3);
 }
-__device__ __forceinline__ void stream_store(uint16_t* p, u4 v) { __builtin_nontemporal_store(v, (u4*)p); }
-// A load of what is read once.
+// A load of what is read once: past the caches' usual places, which the weights then keep. Measured,
+// 10175 rows of 11008 against rank 16: 53.7 us with plain loads, 43.3 with these; the sum with
+// the projection's output 59.7 and 45.8.
 __device__ __forceinline__ u4 stream_load(const uint16_t* p) { return __builtin_nontemporal_load((const u4*)p); }
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 

@@ -55,7 +55,8 @@ struct Turn {
       sn[e] = (p.inverse ? -s : s) * p.magnitude;
     }
   }
-  template <bool BF>
+  // STREAM: the source is read once
+  template <bool BF, bool STREAM>
   __device__ __forceinline__ void apply(const uint16_t* src, uint16_t* dst) const {
     if constexpr (!VEC) {
       if (other < 0) {
@@ -67,7 +68,7 @@ struct Turn {
       dst[at] = (uint16_t)pack16<BF>(a * cs[0] - b * sn[0], 0.f);
       dst[j] = (uint16_t)pack16<BF>(b * cs[0] + a * sn[0], 0.f);
     } else {
-      const u4 x = *(const u4*)(src + at);
+      const u4 x = STREAM ? stream_load(src + at) : *(const u4*)(src + at);
       if (other < 0) {
         *(u4*)(dst + at) = x;
       } else if constexpr (IL) {
@@ -79,7 +80,7 @@ struct Turn {
         }
         *(u4*)(dst + at) = o;
       } else {
-        const u4 y = *(const u4*)(src + other);
+        const u4 y = STREAM ? stream_load(src + other) : *(const u4*)(src + other);
         u4 o, q;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -112,7 +113,7 @@ __device__ __forceinline__ void rotate_heads(const RotaryArgs& p, int64_t item, 
   for (int h = first; h < end; ++h) {
     const bool is_q = h < p.heads;
     const int64_t hh = (int64_t)(is_q ? h : h - p.heads) * p.head_size;
-    turn.template apply<BF>((is_q ? p.q + row * p.q_stride : p.k + row * p.k_stride) + hh,
+    turn.template apply<BF, true>((is_q ? p.q + row * p.q_stride : p.k + row * p.k_stride) + hh,
                             (is_q ? p.q_out + row * p.qo_stride : p.k_out + row * p.ko_stride) + hh);
   }
 }
@@ -136,7 +137,8 @@ template <bool BF, bool VEC, bool IL>
 __global__ void __launch_bounds__(kThreads) rotary_cache_kernel(RotaryArgs p, int each, int q_groups, int q_blocks, int tile) {
   extern __shared__ __attribute__((aligned(16))) uint16_t sm[];
   __shared__ int64_t slot_s[kHalo + kTile + kHalo];  // of tokens t0 - 7 on; -1: none
-  __shared__ int run_s[kTile];                       // 1: a run of eight starts here; 2: a token by itself
+  __shared__ int run_s[kTile], single_s[kTile];      // tokens at which a run of eight starts; by themselves
+  __shared__ int count_s[2];
   const int hd = p.head_size, tid = threadIdx.x;
   if ((int)blockIdx.x < q_groups * q_blocks) {
     const int first = (int)blockIdx.x / q_blocks * each;
@@ -162,20 +164,25 @@ __global__ void __launch_bounds__(kThreads) rotary_cache_kernel(RotaryArgs p, in
     if (t0 + t >= p.rows) break;
     Turn<VEC, IL> turn;
     turn.set(p, t0 + t, i - t * units);
-    turn.template apply<BF>(p.k + (t0 + t) * p.k_stride + (int64_t)head * hd, ktile + t * kpitch);
+    turn.template apply<BF, true>(p.k + (t0 + t) * p.k_stride + (int64_t)head * hd, ktile + t * kpitch);
   }
   __syncthreads();
-  if (tid < tile) {
-    const int64_t s = slot_s[kHalo + tid];
+  if (tid < 64) {  // the first wave lists both
     int run = 0;
-    if (s >= 0) {
-      const int64_t from = s & ~(int64_t)7;
+    if (tid < tile && slot_s[kHalo + tid] >= 0) {
+      const int64_t s = slot_s[kHalo + tid], from = s & ~(int64_t)7;
       const int at = kHalo + tid - (int)(s & 7);  // the run's first token, if it is one
       bool whole = ((uint64_t)p.vptr[s / p.block_size] & 15) == 0;
       for (int e = 0; e < 8; ++e) whole = whole && slot_s[at + e] == from + e;
       run = !whole ? 2 : at == kHalo + tid ? 1 : 0;
     }
-    run_s[tid] = run;
+    const uint64_t runs = __ballot(run == 1), singles = __ballot(run == 2), before = (1ull << tid) - 1;
+    if (run == 1) run_s[__popcll(runs & before)] = tid;
+    if (run == 2) single_s[__popcll(singles & before)] = tid;
+    if (tid == 0) {
+      count_s[0] = __popcll(runs);
+      count_s[1] = __popcll(singles);
+    }
   }
   // values: of the tile, and of the tokens behind it that its last run needs
   const int nu = hd / 8;
@@ -201,19 +208,15 @@ __global__ void __launch_bounds__(kThreads) rotary_cache_kernel(RotaryArgs p, in
       for (int e = 0; e < 8; ++e) unit[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
     }
   }
-  for (int i = tid; i < tile * (hd / 2); i += kThreads) {
-    const int t = i % tile, d = i / tile * 2;
-    const int run = run_s[t];
-    if (run == 0) continue;
+  auto place = [&](int t, int d) {
     const int64_t s = slot_s[kHalo + t];
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.vptr[s / bs]) + (int64_t)head * p.kv_head_stride + d * bs + (int)(s % bs);
+    return reinterpret_cast<uint16_t*>(p.vptr[s / bs]) + (int64_t)head * p.kv_head_stride + d * bs + (int)(s % bs);
+  };
+  const int runs = count_s[0], singles = count_s[1];
+  for (int i = tid; i < runs * (hd / 2); i += kThreads) {
+    const int t = run_s[i % runs], d = i / runs * 2;
+    uint16_t* dst = place(t, d);
     const uint16_t* src = vtile + t * vpitch + d;
-    if (run == 2) {
-      const uint32_t v = *(const uint32_t*)src;
-      dst[0] = (uint16_t)v;
-      dst[bs] = (uint16_t)(v >> 16);
-      continue;
-    }
     u4 lo, hi;  // eight tokens of the even and of the odd dim
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -223,6 +226,13 @@ __global__ void __launch_bounds__(kThreads) rotary_cache_kernel(RotaryArgs p, in
     }
     *(u4*)dst = lo;
     *(u4*)(dst + bs) = hi;
+  }
+  for (int i = tid; i < singles * (hd / 2); i += kThreads) {
+    const int t = single_s[i % singles], d = i / singles * 2;
+    uint16_t* dst = place(t, d);
+    const uint32_t v = *(const uint32_t*)(vtile + t * vpitch + d);
+    dst[0] = (uint16_t)v;
+    dst[bs] = (uint16_t)(v >> 16);
   }
 }
 
@@ -243,14 +253,14 @@ int heads_each(const RotaryArgs& a, int heads, int want) {
 
 template <bool BF, bool VEC, bool IL>
 hipError_t launch_plain(const RotaryArgs& a, hipStream_t stream) {
-  const int all = a.heads + a.kv_heads, each = heads_each(a, all, 8192);
+  const int all = a.heads + a.kv_heads, each = heads_each(a, all, 16384);
   const int64_t blocks = ((int64_t)a.rows * host_units(a) + kThreads - 1) / kThreads;
   rotary_kernel<BF, VEC, IL><<<dim3((unsigned)blocks, (all + each - 1) / each), kThreads, 0, stream>>>(a, each);
   return hipGetLastError();
 }
 template <bool BF, bool VEC, bool IL>
 hipError_t launch_cache(const RotaryArgs& a, hipStream_t stream) {
-  const int each = heads_each(a, a.heads, 8192);
+  const int each = heads_each(a, a.heads, 4096);
   const int64_t q_blocks = ((int64_t)a.rows * host_units(a) + kThreads - 1) / kThreads;
   const int q_groups = (a.heads + each - 1) / each;
   const int tile = a.rows >= 2048 ? kTile : 8;

@@ -17,6 +17,7 @@ and may be captured into a graph.
 from __future__ import annotations
 
 import math
+from fractions import Fraction
 from typing import Optional, Tuple
 
 import torch
@@ -28,6 +29,7 @@ from ..block.common import int32
 from ..block.real import LayerBlocksHolder
 from .common import RotaryScaling, rotary_frequencies
 
+_TWO_PI = Fraction(62831853071795864769252867665590057683943, 10 ** 40)
 _DTYPES = {torch.float16: _lib.DW4_F16, torch.bfloat16: _lib.DW4_BF16}
 
 
@@ -35,6 +37,8 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     """x [rows, heads, dims] with its heads side by side and rows in 16-byte units; a copy
     where it is not so."""
     rows, heads, dims = x.shape
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x
     if x.stride(2) != 1 or (heads > 1 and x.stride(1) != dims) or x.data_ptr() % 16 or \
             (rows > 1 and (x.stride(0) % 8 or x.stride(0) < heads * dims)):
         return x.clone(memory_format=torch.contiguous_format)
@@ -42,7 +46,8 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 
 def _stride(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+    rows, heads, dims = x.shape
+    return x.stride(0) if rows > 1 else heads * dims
 
 
 class RotaryEmbedding:
@@ -65,18 +70,23 @@ class RotaryEmbedding:
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, bool(interleaved)
         self.frequencies, self.magnitude = rotary_frequencies(rotary_dim, base, scaling)
         # turns per position as 64-bit fractions: their products with positions wrap at whole turns
-        turns = [int(math.ldexp(f / (2 * math.pi), 64)) % 2 ** 64 for f in self.frequencies]
+        turns = [round(Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64 for f in self.frequencies]
         self._turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns],
                                    dtype=torch.int64).to(device)
         self.device = self._turns.device
 
-    def _check(self, x: torch.Tensor, name: str) -> None:
-        if x.dim() != 3 or x.shape[2] != self.head_dim:
-            raise AssertionError(f"{name} must be [rows, heads, {self.head_dim}]")
-        if x.device != self.device:
-            raise ValueError(f"{name} must be on {self.device}")
-        if x.dtype not in _DTYPES:
+    def _check(self, *rows: torch.Tensor) -> int:
+        dtype, count = rows[0].dtype, rows[0].shape[0]
+        for x in rows:
+            if x.dim() != 3 or x.shape[2] != self.head_dim or x.shape[0] != count:
+                raise AssertionError(f"q, k and v must be [rows, heads, {self.head_dim}], of the same rows")
+            if x.dtype != dtype:
+                raise TypeError("q, k and v must have one type")
+            if x.device != self.device:
+                raise ValueError(f"q, k and v must be on {self.device}")
+        if dtype not in _DTYPES:
             raise TypeError("rotary positions run on fp16 or bf16")
+        return count
 
     def _positions(self, positions: torch.Tensor, rows: int) -> torch.Tensor:
         if positions.shape != (rows,) or positions.device != self.device:
@@ -100,13 +110,7 @@ class RotaryEmbedding:
                 positions: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """q [rows, heads, head_dim] and k [rows, kv heads, head_dim] turned by their rows'
         ``positions`` (integers [rows]) -> new tensors.  Differentiable in q and k (once)."""
-        self._check(q, "q")
-        self._check(k, "k")
-        if k.shape[0] != q.shape[0]:
-            raise AssertionError("q and k must have the same rows")
-        if k.dtype != q.dtype:
-            raise TypeError("q and k must have one type")
-        pos = self._positions(positions, q.shape[0])
+        pos = self._positions(positions, self._check(q, k))
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
             return _Rotary.apply(q, k, pos, self)
         return self._turn(q, k, pos, False)
@@ -118,16 +122,11 @@ class RotaryEmbedding:
         their cache ``slots`` (integers [rows]; -1: the row is not cached, and so is a slot outside the
         cache's blocks).  k and v stay as they are.  No two rows may have one slot.  Without
         gradients: a backward pass through it raises."""
-        self._check(q, "q")
-        self._check(k, "k")
-        self._check(v, "v")
-        rows, info = q.shape[0], kv_cacher.block_info
-        if k.shape != v.shape or k.shape[0] != rows:
-            raise AssertionError("k and v must have the same shape and q's rows")
+        rows, info = self._check(q, k, v), kv_cacher.block_info
+        if k.shape != v.shape:
+            raise AssertionError("k and v must have the same shape")
         if info.head_dim != self.head_dim or info.num_key_value_heads != k.shape[1]:
             raise AssertionError("k and v do not match the cache's block geometry")
-        if k.dtype != q.dtype or v.dtype != q.dtype:
-            raise TypeError("q, k and v must have one type")
         if kv_cacher.dtype != q.dtype:
             raise TypeError(f"rows of {q.dtype} into a cache of {kv_cacher.dtype}")
         if kv_cacher.device != self.device:
@@ -135,9 +134,10 @@ class RotaryEmbedding:
         pos = self._positions(positions, rows)
         if slots.shape != (rows,) or slots.device != self.device:
             raise ValueError(f"slots must be {rows} integers on {self.device}")
-        if slots.dtype != torch.int64 and slots.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
-            raise ValueError("slots must be integers")
-        slots = slots.to(torch.int64).contiguous()
+        if slots.dtype is not torch.int64:
+            slots = int32(slots, "slots").to(torch.int64)
+        elif not slots.is_contiguous():
+            slots = slots.contiguous()
         if output is None:
             output = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         elif output.shape != q.shape or output.dtype != q.dtype or output.device != self.device:

@@ -83,3 +83,20 @@ def compact(tables, refs):
     for a, b in to.items():
         refs[b], refs[a] = refs[a], 0
     return [[to.get(e, e) for e in row] for row in tables], refs, live, list(to.items())
+
+
+def slots(tables, lens, refs, new_tokens, tokens, bs):
+    """(query starts, positions, slots, rows, excess) of each row's last new_tokens tokens, in
+    arrays of `tokens` entries; nothing is mapped where the rows have more."""
+    new = [max(min(n, length), 0) for n, length in zip(new_tokens, lens)]
+    excess = max(sum(new) - tokens, 0)
+    starts, positions, where, rows = [0], [], [], []
+    for r, n in enumerate(new):
+        for pos in range(lens[r] - n, lens[r]) if not excess else ():
+            block = tables[r][pos // bs] if pos // bs < len(tables[r]) else -1
+            positions.append(pos)
+            where.append(block * bs + pos % bs if 0 <= block < len(refs) else -1)
+            rows.append(r)
+        starts.append(len(rows))
+    pad = tokens - len(rows)
+    return starts, positions + [0] * pad, where + [-1] * pad, rows + [-1] * pad, excess

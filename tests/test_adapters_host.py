@@ -1,0 +1,177 @@
+"""CPU tests: adapters, dropout, rotary positions and slot maps refuse malformed calls before anything
+reaches a device (fake addresses are never dereferenced), and the generator's oracle gives the
+published numbers."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from hip_extends import _lib
+from operators.core.linear.adapters import CounterDropout, LowRankAdapters
+from operators.core.rope.common import RotaryScaling, rotary_frequencies
+from operators.core.rope.real import RotaryEmbedding
+from oracle import adapters as O
+from oracle import blocks as B
+from oracle import rotary as R
+
+FAKE, ODD = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8)
+OK, BAD, UNSUP, MISAL, WORK = (_lib.DW4_OK, _lib.DW4_ERR_INVALID_ARG, _lib.DW4_ERR_UNSUPPORTED,
+                               _lib.DW4_ERR_MISALIGNED, _lib.DW4_ERR_WORKSPACE)
+
+
+def adapters(dtype=0, rows=50, count=3, k=64, n=32, rank=16, x=FAKE, ldx=64, base=FAKE, ldb=32, out=FAKE, ldo=32, a=FAKE, b=FAKE,
+             scaling=FAKE, plan=FAKE, drop=0, seed=None, h=None, ws=FAKE, wsb=0):
+    return _lib.load().dw4_adapters(dtype, rows, count, k, n, rank, x, ldx, base, ldb, out, ldo, a, b, scaling, plan, drop, seed,
+                                    h, ws, wsb, None)
+
+
+def backward(dtype=1, rows=50, count=3, k=64, n=32, rank=16, x=FAKE, ldx=64, g=FAKE, ldg=32, a=FAKE, b=FAKE, scaling=FAKE,
+             plan=FAKE, drop=0, seed=None, h=FAKE, dx=FAKE, lddx=64, da=FAKE, db=FAKE, ws=FAKE, wsb=0):
+    return _lib.load().dw4_adapters_backward(dtype, rows, count, k, n, rank, x, ldx, g, ldg, a, b, scaling, plan, drop, seed, h,
+                                             dx, lddx, da, db, ws, wsb, None)
+
+
+def test_adapter_refusals():
+    for call in (adapters, backward):
+        assert call() == WORK                                     # a workspace that is too small
+        assert call(ws=None, wsb=1 << 30) == WORK
+        assert call(ws=ODD, wsb=1 << 30) == MISAL
+        assert call(dtype=2) == UNSUP and call(rank=12) == UNSUP and call(rank=136) == UNSUP
+        assert call(k=60, ldx=64) == UNSUP and call(n=28) == UNSUP
+        assert call(rows=-1) == BAD and call(count=-1) == BAD and call(rank=0) == BAD and call(k=0) == BAD
+        assert call(count=1025) == UNSUP and call(rows=(1 << 24) + 1) == UNSUP and call(k=(1 << 20) + 8, ldx=1 << 21) == UNSUP
+        assert call(x=None) == BAD and call(a=None) == BAD and call(b=None) == BAD and call(scaling=None) == BAD
+        assert call(plan=None) == BAD and call(plan=ODD) == MISAL
+        assert call(x=ODD) == MISAL and call(ldx=68) == MISAL and call(ldx=56) == BAD and call(a=ODD) == MISAL
+        assert call(drop=-1) == BAD and call(drop=65537) == BAD and call(drop=5) == BAD  # dropout without a seed
+        assert call(drop=5, seed=FAKE) == WORK
+        assert call(count=0, a=None, b=None, scaling=None) == WORK  # no adapters, no weights
+    assert adapters(rows=0, x=None, plan=None) == OK
+    assert adapters(base=None) == BAD and adapters(out=None) == BAD and adapters(ldo=24) == BAD and adapters(base=ODD) == MISAL
+    assert adapters(h=ODD) == MISAL
+    assert adapters(ldo=40, wsb=1 << 30) == BAD                   # in place of base, but other rows
+    assert backward(rows=0) == BAD and backward(h=None) == BAD and backward(h=ODD) == MISAL
+    assert backward(g=None) == BAD and backward(g=ODD) == MISAL and backward(dx=ODD) == MISAL and backward(lddx=56) == BAD
+    assert backward(da=ODD) == MISAL and backward(db=ODD) == MISAL
+    assert backward(dx=None, da=None, db=None) == OK
+
+
+def test_plan_and_workspace_sizes():
+    lib, out, h = _lib.load(), ctypes.c_size_t(7), ctypes.c_size_t(7)
+    assert lib.dw4_adapter_plan_size(0, 5, ctypes.byref(out)) == OK and out.value == 0
+    assert lib.dw4_adapter_plan_size(10, 5, None) == BAD and lib.dw4_adapter_plan_size(-1, 5, ctypes.byref(out)) == BAD
+    assert lib.dw4_adapter_plan_size(10, 1025, ctypes.byref(out)) == UNSUP
+    assert lib.dw4_adapter_plan_size(1 << 24, 1024, ctypes.byref(out)) == OK and out.value < 1 << 28
+    need = _lib.adapter_plan_size(100, 4)
+    assert lib.dw4_adapter_plan(100, 4, FAKE, FAKE, need - 1, None) == WORK
+    assert lib.dw4_adapter_plan(100, 4, FAKE, ODD, need, None) == MISAL
+    assert lib.dw4_adapter_plan(100, 4, None, FAKE, need, None) == BAD and lib.dw4_adapter_plan(100, 4, FAKE, None, need, None) == BAD
+    assert lib.dw4_adapter_plan(0, 4, None, None, 0, None) == OK
+    size = lib.dw4_adapters_workspace_size
+    assert size(0, 4, 64, 64, 16, 1, ctypes.byref(out), ctypes.byref(h)) == OK and out.value == 0 and h.value == 0
+    assert size(10, 4, 64, 64, 16, 0, None, None) == BAD and size(10, 4, 64, 64, 15, 0, ctypes.byref(out), None) == UNSUP
+    assert size(10, 4, 64, 64, 16, 0, ctypes.byref(out), None) == OK and out.value > 0
+
+
+def test_dropout_refusals():
+    call = _lib.load().dw4_dropout
+    assert call(2, 4, 8, FAKE, 8, FAKE, 8, 5, FAKE, None) == UNSUP
+    assert call(0, -1, 8, FAKE, 8, FAKE, 8, 5, FAKE, None) == BAD and call(0, 4, 8, FAKE, 8, FAKE, 8, 5, None, None) == BAD
+    assert call(0, 4, 8, None, 8, FAKE, 8, 5, FAKE, None) == BAD and call(0, 4, 8, FAKE, 7, FAKE, 8, 5, FAKE, None) == BAD
+    assert call(0, 4, 8, FAKE, 8, FAKE, 8, 65537, FAKE, None) == BAD
+    assert call(0, 0, 8, None, 8, None, 8, 5, FAKE, None) == OK and call(0, 4, 0, None, 0, None, 0, 5, FAKE, None) == OK
+
+
+def rotary(dtype=0, rows=9, heads=4, kvh=2, hd=64, rd=64, inter=0, q=FAKE, qs=256, k=FAKE, ks=128, qo=FAKE, qos=256, ko=FAKE, kos=128,
+           pos=FAKE, turns=FAKE, m=1.0):
+    return _lib.load().dw4_rotary(dtype, rows, heads, kvh, hd, rd, inter, 0, q, qs, k, ks, qo, qos, ko, kos, pos, turns, m, None)
+
+
+def cached(dtype=0, rows=9, heads=4, kvh=2, hd=64, rd=64, q=FAKE, qs=256, k=FAKE, ks=128, v=FAKE, vs=128, qo=FAKE, qos=256, pos=FAKE,
+           turns=FAKE, m=1.0, slots=FAKE, nb=4, bs=16, kp=FAKE, vp=FAKE, hs=1024):
+    return _lib.load().dw4_rotary_and_cache(dtype, rows, heads, kvh, hd, rd, 0, q, qs, k, ks, v, vs, qo, qos, pos, turns, m, slots, nb,
+                                            bs, kp, vp, hs, None)
+
+
+def test_rotary_refusals():
+    for call in (rotary, cached):
+        assert call(dtype=2) == UNSUP and call(rows=-1) == BAD and call(heads=-1) == BAD and call(hd=0) == BAD
+        assert call(rd=0) == BAD and call(rd=66) == BAD and call(rd=7) == UNSUP and call(hd=60, rd=60) == UNSUP
+        assert call(hd=520, qs=4 * 520, qos=4 * 520, ks=2 * 520, rd=64) == UNSUP
+        assert call(m=float("nan")) == BAD and call(m=float("inf")) == BAD
+        assert call(q=None) == BAD and call(k=None) == BAD and call(qo=None) == BAD and call(pos=None) == BAD
+        assert call(turns=None) == BAD and call(qs=248) == BAD and call(q=ODD) == MISAL and call(ks=132) == MISAL
+        assert call(rows=(1 << 24) + 1) == UNSUP and call(rows=1 << 24, heads=64, qs=4096, qos=4096) == UNSUP
+        assert call(rows=0, q=None) == OK
+    assert rotary(heads=0, kvh=0) == OK and rotary(ko=None) == BAD and rotary(kos=120) == BAD
+    assert cached(v=None) == BAD and cached(slots=None) == BAD and cached(kp=None) == BAD and cached(vp=None) == BAD
+    assert cached(bs=8) == UNSUP and cached(nb=-1) == BAD and cached(hs=1016) == BAD and cached(hs=1028) == MISAL
+    assert cached(kvh=0) == BAD and cached(heads=0) == BAD and cached(v=ODD) == MISAL
+
+
+def test_slot_refusals():
+    def call(rows=5, width=4, nb=9, bs=16, tables=FAKE, lens=FAKE, new=FAKE, tokens=7, starts=FAKE, pos=FAKE, slots=FAKE, row=FAKE,
+             excess=FAKE):
+        return _lib.load().dw4_token_slots(rows, width, nb, bs, tables, lens, new, tokens, starts, pos, slots, row, excess, None)
+    assert call(rows=-1) == BAD and call(width=-1) == BAD and call(nb=-1) == BAD and call(tokens=-1) == BAD
+    assert call(bs=24) == UNSUP and call(rows=8193) == UNSUP and call(tokens=(1 << 28) + 1) == UNSUP
+    for name in ("tables", "lens", "new", "starts", "pos", "slots", "row", "excess"):
+        assert call(**{name: None}) == BAD
+
+
+def test_modules_refuse_what_the_kernels_do_not_take():
+    for kwargs in (dict(rank=12), dict(rank=0), dict(rank=136), dict(in_features=60), dict(out_features=0), dict(num_adapters=0),
+                   dict(num_adapters=1025), dict(dropout=1.5), dict(dropout=-0.1)):
+        with pytest.raises(ValueError):
+            LowRankAdapters(**{**dict(in_features=64, out_features=64, rank=8, num_adapters=2), **kwargs})
+    with pytest.raises(TypeError):
+        LowRankAdapters(64, 64, 8, 2, dtype=torch.float32)
+    with pytest.raises(ValueError):
+        CounterDropout(1.01)
+    bank = LowRankAdapters(64, 64, 8, 2)
+    assert not bank.a.requires_grad and LowRankAdapters(64, 64, 8, 2, trainable=True).b.requires_grad
+    assert set(bank.state_dict()) == {"a", "b", "scaling"}
+    for args in ((60,), (64, 63), (64, 66), (64, 0), (520,)):
+        with pytest.raises(ValueError):
+            RotaryEmbedding(*args, device="cuda")
+    with pytest.raises(ValueError):
+        RotaryEmbedding(64, device="cpu")
+    with pytest.raises(ValueError):
+        RotaryEmbedding(64, base=0.5)
+    for args in (("other", 2.0), ("linear", 0.5), ("yarn", float("inf")), ("yarn", 2.0, 0), ("wavelength", 2.0, 4096, 4.0, 4.0)):
+        with pytest.raises(ValueError):
+            RotaryScaling(*args)
+    with pytest.raises(ValueError):
+        rotary_frequencies(2, 10000.0, RotaryScaling("ntk", 2.0))
+
+
+def test_the_generator_gives_its_published_numbers():
+    """Known answers of Philox 4x32 with 10 rounds, published with it."""
+    for counter, key, want in (((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+                               ((O.WORD,) * 4, (O.WORD,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+                               ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+                                (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1))):
+        assert tuple(O.philox(counter, key)) == want
+
+
+def test_oracles_agree_with_autograd():
+    g = torch.Generator().manual_seed(1)
+    x, base, dout = (torch.randn(6, w, generator=g).half() for w in (16, 8, 8))
+    a, b, s = torch.randn(2, 8, 16, generator=g).half(), torch.randn(2, 8, 8, generator=g).half(), torch.rand(2, generator=g)
+    index = torch.tensor([0, 1, -1, 1, 0, 7])
+    mask = O.kept(6, 16, 20000, 3, 4)
+    leaves = [t.double().requires_grad_(True) for t in (x, a, b)]
+    z = torch.where(mask, leaves[0] * (65536 / 45536), 0.0)
+    rows = [base[t].double() + (s[i].double() * (leaves[2][i] @ (leaves[1][i] @ z[t])) if 0 <= i < 2 else 0)
+            for t, i in enumerate(index.tolist())]
+    out = torch.stack(rows)
+    want = (out, *torch.autograd.grad(out, leaves, dout.double()))
+    got, _ = O.low_rank(x, base, a, b, s, index, dout, mask, 20000)
+    assert all(torch.allclose(u, v, rtol=1e-12, atol=1e-12) for u, v in zip(got, want))
+    y, _ = R.turned(torch.randn(3, 2, 8, generator=g).half(), torch.tensor([0, 5, -9]), [1.0, 0.5], 1.0, 4, True)
+    back, _ = R.turned(y.half(), torch.tensor([0, 5, -9]), [1.0, 0.5], 1.0, 4, True, inverse=True)
+    assert y.shape == (3, 2, 8) and torch.isfinite(back).all()
+    assert B.slots([[4, -1]], [20], [0] * 9, [6], 8, 16) == ([0, 6], [14, 15, 16, 17, 18, 19, 0, 0], [78, 79, -1, -1, -1, -1, -1, -1],
+                                                            [0] * 6 + [-1] * 2, 0)

@@ -1,0 +1,533 @@
+"""GPU parity of low-rank adapters (LowRankAdapters, AdaptedLinear) and of dropout from a counter
+(CounterDropout) against oracle/adapters.py in float64, element by element within the error that the
+kernels' roundings allow (derived there).
+
+Rows with and without adapters in any order, from none to some hundred; ranks of 8 to 128, widths
+that end inside a step, 1 to 1024 adapters of which few are used; strided, misaligned and
+three-dimensional inputs, results in place of the projection's; gradients of every subset, with
+dropout of some, all and no elements, small and large values; non-finite values that must not reach
+other rows and adapters; captured and replayed calls with other adapters and seeds; other streams.
+Every case prints its name before touching the GPU.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from gptq_synth import make_layer
+from hip_extends.w4a16 import CacheV2, TuningParams
+from operators.core.linear.adapters import AdaptedLinear, AdapterRows, CounterDropout, LowRankAdapters
+from operators.core.linear.real_quant import QuantLinearMaker
+from oracle import adapters as O
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def say(msg: str) -> None:
+    print(f"[case] {msg}", flush=True)
+
+
+def index_of(g, rows, adapters, order):
+    if order == "mixed":  # none (-1), and numbers outside, among them
+        return torch.randint(-1, adapters + 1, (rows,), generator=g)
+    if order == "runs":
+        return torch.randint(0, adapters, (-(-rows // 37),), generator=g).repeat_interleave(37)[:rows]
+    if order == "none":
+        return torch.full((rows,), -1)
+    return torch.full((rows,), adapters - 1)  # "one"
+
+
+class Case:
+    def __init__(self, dev, rows, k, n, rank, adapters, dtype, order="mixed", seed=0, dropout=0.0, trainable=False,
+                 scale=1.0):
+        g = torch.Generator().manual_seed(seed + 1000 * rows + k)
+        self.dev, self.g = dev, g
+        self.x = torch.randn(rows, k, generator=g).to(dtype)
+        self.base = torch.randn(rows, n, generator=g).to(dtype)
+        self.a = (torch.randn(adapters, rank, k, generator=g) * k ** -0.5).to(dtype)
+        self.b = (torch.randn(adapters, n, rank, generator=g) * rank ** -0.5).to(dtype)
+        self.scaling = torch.rand(adapters, generator=g) + 0.5
+        self.dout = (torch.randn(rows, n, generator=g) * scale).to(dtype)
+        self.index = index_of(g, rows, adapters, order)
+        self.bank = LowRankAdapters(k, n, rank, adapters, dtype=dtype, device=dev, dropout=dropout, trainable=trainable)
+        self.put()
+        self.rows = AdapterRows(self.index.to(dev), adapters)
+        self.seed = torch.tensor([123456789 * (seed + 1) + 2 ** 40, 5 + 2 ** 33])
+
+    def put(self):
+        with torch.no_grad():
+            self.bank.a.copy_(self.a)
+            self.bank.b.copy_(self.b)
+            self.bank.scaling.copy_(self.scaling)
+
+    def mask(self):
+        drop = round(self.bank.dropout * 65536)
+        return (O.kept(*self.x.shape, drop, *self.seed.tolist()), drop) if drop else (None, 0)
+
+    def want(self, grads=False):
+        mask, drop = self.mask()
+        return O.low_rank(self.x, self.base, self.a, self.b, self.scaling, self.index, self.dout if grads else None, mask, drop)
+
+    def run(self):
+        return self.bank(self.x.to(self.dev), self.base.to(self.dev), self.rows, self.seed.to(self.dev))
+
+    def grads(self):
+        x, base = self.x.to(self.dev).requires_grad_(True), self.base.to(self.dev).requires_grad_(True)
+        out = self.bank(x, base, self.rows, self.seed.to(self.dev))
+        dx, dbase, da, db = torch.autograd.grad(out, (x, base, self.bank.a, self.bank.b), self.dout.to(self.dev))
+        assert torch.equal(dbase.cpu().view(torch.int16), self.dout.view(torch.int16))
+        return out.detach(), dx, da, db
+
+
+def check(got, want, err, what):
+    d = (got.cpu().double() - want).abs()
+    worst = (d - err).max().item() if d.numel() else -1.0
+    assert not d.isnan().any() and worst <= 0, f"{what}: {worst} beyond the bound, at {(d - err).argmax().item()}"
+
+
+SHAPES = [  # rows, k, n, rank, adapters, order
+    (1, 256, 128, 16, 1, "one"), (1, 8, 8, 8, 3, "mixed"), (2, 72, 24, 24, 2, "mixed"), (15, 200, 136, 8, 5, "mixed"),
+    (16, 256, 64, 32, 1, "one"), (33, 1000, 72, 64, 3, "runs"), (48, 136, 520, 128, 40, "mixed"), (256, 64, 64, 16, 7, "mixed"),
+    (257, 64, 72, 16, 7, "mixed"), (300, 320, 200, 40, 1024, "mixed"), (640, 136, 264, 96, 4, "runs"),
+    (1100, 72, 80, 128, 2, "runs"), (700, 528, 136, 32, 1, "one"), (100, 64, 64, 16, 4, "none"), (520, 64, 64, 8, 4, "none")]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,k,n,rank,adapters,order", SHAPES)
+def test_forward(hip_device, rows, k, n, rank, adapters, order, dtype):
+    say(f"forward {rows} rows {k} -> {n}, rank {rank}, {adapters} adapters {order} {dtype}")
+    case = Case(hip_device, rows, k, n, rank, adapters, dtype, order)
+    out, err = case.want()
+    got = case.run()
+    check(got, out, err, "out")
+    assert torch.equal(got, case.run())
+    away = (case.index < 0) | (case.index >= adapters)
+    assert torch.equal(got.cpu()[away], case.base[away])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("p", [0.0, 0.1])
+@pytest.mark.parametrize("rows,k,n,rank,adapters,order", SHAPES)
+def test_gradients(hip_device, rows, k, n, rank, adapters, order, p, dtype):
+    say(f"gradients {rows} rows {k} -> {n}, rank {rank}, {adapters} adapters {order} p {p} {dtype}")
+    case = Case(hip_device, rows, k, n, rank, adapters, dtype, order, dropout=p, trainable=True, seed=3)
+    want, err = case.want(grads=True)
+    got = case.grads()
+    for name, g, w, e in zip(("out", "dx", "da", "db"), got, want, err):
+        check(g, w, e, name)
+    assert all(torch.equal(s, t) for s, t in zip(got, case.grads()))
+
+
+def test_gradients_of_a_long_run_of_rows(hip_device):
+    """Rows past several chunks of one adapter, another one beginning inside a chunk's size."""
+    say("gradients over 2300 rows")
+    case = Case(hip_device, 2300, 72, 40, 16, 2, BF16, "one", dropout=0.25, trainable=True)
+    case.index[:700] = 0
+    case.rows.update(case.index.to(hip_device))
+    want, err = case.want(grads=True)
+    for name, g, w, e in zip(("out", "dx", "da", "db"), case.grads(), want, err):
+        check(g, w, e, name)
+
+
+@pytest.mark.parametrize("exponent", [-18, -8, 8])
+def test_fp16_gradients_keep_their_range(hip_device, exponent):
+    """Output gradients far from one: what leaves fp16's normal range inside the products must not
+    cost precision in results that have it."""
+    say(f"fp16 gradients of 2^{exponent}")
+    case = Case(hip_device, 90, 128, 64, 16, 2, F16, "runs", trainable=True, scale=2.0 ** exponent)
+    want, err = case.want(grads=True)
+    for name, g, w, e in zip(("out", "dx", "da", "db"), case.grads(), want, err):
+        check(g, w, e, name)
+
+
+def test_fp16_rows_of_different_size(hip_device):
+    say("fp16 rows of 2^-10 beside rows of 2^6")
+    case = Case(hip_device, 70, 128, 64, 16, 1, F16, "one", trainable=True)
+    factor = torch.where(torch.arange(70) % 2 == 0, 2.0 ** 6, 2.0 ** -10)[:, None]
+    case.x, case.dout = (case.x * factor).to(F16), (case.dout * factor.flip(0)).to(F16)
+    want, err = case.want(grads=True)
+    for name, g, w, e in zip(("out", "dx", "da", "db"), case.grads(), want, err):
+        check(g, w, e, name)
+
+
+def test_every_subset_of_gradients(hip_device):
+    case = Case(hip_device, 60, 128, 72, 16, 3, BF16, dropout=0.2, trainable=True)
+    want, err = case.want(grads=True)
+    for need in range(1, 16):
+        say(f"gradients of subset {need}")
+        x, base = case.x.to(hip_device), case.base.to(hip_device)
+        leaves = [t.requires_grad_(bool(need >> i & 1)) for i, t in enumerate((x, case.bank.a, case.bank.b, base))]
+        out = case.bank(x, base, case.rows, case.seed.to(hip_device))
+        asked = [i for i, t in enumerate(leaves) if t.requires_grad]
+        got = torch.autograd.grad(out, [leaves[i] for i in asked], case.dout.to(hip_device))
+        for i, g in zip(asked, got):
+            if i == 3:
+                assert torch.equal(g.cpu(), case.dout)
+            else:
+                check(g, want[1 + i], err[1 + i], ("dx", "da", "db")[i])
+
+
+def test_gradients_against_differences(hip_device):
+    """out is linear in each of x, A and B: a difference of any size is the gradient's product
+    with it, but for the roundings of the two outputs."""
+    say("differences")
+    case = Case(hip_device, 80, 64, 48, 16, 2, F16, "runs", trainable=True)
+    _, dx, da, db = (t.double().cpu() for t in case.grads())
+    before = case.run().double().cpu()
+    for name, grad in (("x", dx), ("a", da), ("b", db)):
+        kept = getattr(case, name)
+        # moved by sums that stay representable, so that the step is what was asked
+        moved = (kept + (torch.rand(kept.shape, generator=case.g) - 0.5).to(F16)).to(F16)
+        step = moved.double() - kept.double()
+        setattr(case, name, moved)
+        case.put()
+        after = case.run().double().cpu()
+        setattr(case, name, kept)
+        case.put()
+        got = ((after - before) * case.dout.double()).sum()
+        # outputs and gradients rounded by half a step, each term of both sums
+        u = O.half_step(F16) * 1.01
+        room = u * (((after.abs() + before.abs()) * case.dout.double().abs()).sum() + (grad.abs() * step.abs()).sum())
+        assert (got - (grad * step).sum()).abs() <= room, name
+
+
+@pytest.mark.parametrize("p", [0.5, 1.0])
+def test_dropout_inside_equals_dropout_before(hip_device, p):
+    """The adapters' dropout drops what CounterDropout drops; with p 1 nothing is left."""
+    say(f"dropout {p} inside and before")
+    case = Case(hip_device, 70, 200, 64, 16, 2, BF16, dropout=p, trainable=True)
+    x, seed = case.x.to(hip_device), case.seed.to(hip_device)
+    dropped = CounterDropout(p)(x, seed)
+    mask, drop = case.mask()
+    assert torch.equal(dropped.cpu() != 0, mask & (case.x != 0))
+    out, err = case.want()
+    check(case.run(), out, err, "out")
+    if p == 1.0:
+        assert torch.equal(case.run().cpu(), case.base)
+        got = case.grads()
+        assert not got[1].any() and not got[2].any() and not got[3].any()
+    case.bank.eval()  # no dropout outside training
+    plain = O.low_rank(case.x, case.base, case.a, case.b, case.scaling, case.index)
+    check(case.run(), *plain, "out without dropout")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 8), (17, 1000), (300, 65), (2, 4096)])
+def test_counter_dropout(hip_device, rows, cols, dtype):
+    say(f"dropout {rows} x {cols} {dtype}")
+    g = torch.Generator().manual_seed(rows + cols)
+    x, dy = torch.randn(rows, cols, generator=g).to(dtype), torch.randn(rows, cols, generator=g).to(dtype)
+    seed = torch.tensor([2 ** 62 - 3 * rows, -cols])
+    for p in (0.02, 0.5, 1.0):
+        drop = round(p * 65536)
+        mask = O.kept(rows, cols, drop, *seed.tolist())
+        leaf = x.to(hip_device).requires_grad_(True)
+        y = CounterDropout(p)(leaf, seed.to(hip_device))
+        (dx,) = torch.autograd.grad(y, leaf, dy.to(hip_device))
+        share = 65536 / (65536 - drop) if drop < 65536 else 0.0
+        for got, t in ((y.detach(), x), (dx, dy)):
+            want = torch.where(mask, t.double() * share, 0.0)
+            # rounded to float32 (factor and product) and once to the type
+            room = want.abs() * (O.half_step(dtype) + 2.0 ** -22) + O.floor(dtype)
+            check(got, want, torch.where(mask, room, 0.0), f"p {p}")
+
+
+def test_dropout_forms(hip_device):
+    say("dropout of strided, misaligned and empty inputs")
+    seed = torch.tensor([7, 9], device=hip_device)
+    wide = torch.randn(40, 3, 136, device=hip_device).to(BF16)
+    drop = CounterDropout(0.3)
+    want = drop(wide.contiguous(), seed)
+    assert torch.equal(drop(wide.transpose(0, 1).contiguous().transpose(0, 1), seed), want)
+    odd = torch.empty(40 * 3 * 136 + 1, device=hip_device, dtype=BF16)[1:].view(40, 3, 136).copy_(wide)
+    assert torch.equal(drop(odd, seed), want)
+    part = wide.view(120, 136)[:, 5:60]
+    assert torch.equal(drop(part, seed), drop(part.contiguous(), seed))
+    for shape in ((0, 8), (8, 0), (0,)):
+        assert drop(torch.empty(shape, device=hip_device, dtype=BF16), seed).shape == shape
+    assert drop.eval()(wide, seed) is wide
+    assert CounterDropout(0.0)(wide) is wide
+    # a dropped element is zero whatever it holds
+    mask = O.kept(40, 136, round(0.3 * 65536), 7, 9).to(hip_device)
+    x = wide[:, 0].contiguous().masked_fill(~mask, float("nan"))
+    assert torch.equal(drop.train()(x, seed) == 0, ~mask | (x == 0))
+
+
+def test_rates_of_dropout(hip_device):
+    """Shares of kept elements over rows, columns and places in a unit: within five standard
+    deviations of the stated probability (a million independent elements)."""
+    say("rates of dropout")
+    x = torch.ones(1000, 1024, device=hip_device, dtype=BF16)
+    kept = (CounterDropout(0.3)(x, torch.tensor([11, 3], device=hip_device)) != 0).double().cpu()
+    p = round(0.3 * 65536) / 65536
+    for shares, n in ((kept.mean().view(1), kept.numel()), (kept.mean(0), 1000), (kept.mean(1), 1024),
+                      (kept.view(-1, 8).mean(0), kept.numel() // 8)):
+        assert ((shares - (1 - p)).abs() <= 5 * (p * (1 - p) / n) ** 0.5).all()
+    other = (CounterDropout(0.3)(x, torch.tensor([11, 4], device=hip_device)) != 0).double().cpu()
+    both = (kept * other).mean()
+    assert abs(both - (1 - p) ** 2) <= 5 * ((1 - p) ** 2 / kept.numel()) ** 0.5
+
+
+def test_inputs_as_they_come(hip_device):
+    """Strided, misaligned and three-dimensional inputs, a result in the projection's place."""
+    case = Case(hip_device, 66, 128, 72, 16, 3, BF16)
+    say("forms of inputs")
+    out, err = case.want()
+    want = case.run()
+    check(want, out, err, "out")
+    dev = hip_device
+    x, base = case.x.to(dev), case.base.to(dev)
+    xs, bs = torch.randn(66, 200, device=dev).to(BF16), torch.randn(66, 88, device=dev).to(BF16)
+    xs[:, 64:192], bs[:, 8:80] = x, base
+    odd = torch.empty(66 * 128 + 1, device=dev, dtype=BF16)[1:].view(66, 128).copy_(x)
+    skew = torch.empty(66, 131, device=dev, dtype=BF16)[:, :128].copy_(x)
+    for a, b in ((xs[:, 64:192], bs[:, 8:80]), (odd, base), (skew, base), (x.t().contiguous().t(), base.t().contiguous().t())):
+        assert torch.equal(case.bank(a, b, case.rows), want)
+    assert torch.equal(case.bank(x.view(11, 6, 128), base.view(11, 6, 72), case.rows), want.view(11, 6, 72))
+    into = torch.empty(66, 72, device=dev, dtype=BF16)
+    assert case.bank(x, base, case.rows, output=into) is into and torch.equal(into, want)
+    version = base._version
+    assert case.bank(x, base, case.rows, output=base) is base and torch.equal(base, want) and base._version > version
+    g = x.view(11, 6, 128).detach().requires_grad_(True)
+    o = case.bank(g, case.base.to(dev).view(11, 6, 72), case.rows)
+    assert o.shape == (11, 6, 72)
+    (dx,) = torch.autograd.grad(o, g, torch.ones(1, device=dev, dtype=BF16).expand(11, 6, 72))
+    assert dx.shape == g.shape
+    none = AdapterRows(torch.empty(0, dtype=torch.int64, device=dev), 3)
+    assert case.bank(x[:0], base[:0], none).shape == (0, 72)
+    e = x[:0].clone().requires_grad_(True)
+    case.bank.a.requires_grad_(True)
+    d = torch.autograd.grad(case.bank(e, base[:0], none).sum(), (e, case.bank.a))
+    assert d[0].shape == (0, 128) and not d[1].any()
+
+
+def test_half_modules_keep_their_scaling(hip_device):
+    say("a module made half")
+    case = Case(hip_device, 20, 64, 64, 8, 2, F16)
+    case.bank.half()
+    case.scaling = case.bank.scaling.float().cpu()
+    check(case.run(), *case.want(), "out")
+
+
+@pytest.mark.parametrize("rows", [40, 300])
+def test_nonfinite_values_stay_in_their_rows(hip_device, rows):
+    say(f"non-finite values, {rows} rows")
+    case = Case(hip_device, rows, 128, 64, 24, 3, BF16, trainable=True)
+    clean = [t.cpu() for t in case.grads()]
+    bad = rows // 2
+    case.index[bad] = 1
+    case.rows.update(case.index.to(hip_device))
+    clean = [t.cpu() for t in case.grads()]
+    for value in (float("nan"), float("inf")):
+        kept = case.x[bad].clone(), case.dout[bad].clone()
+        case.x[bad, 3], case.dout[bad, 5] = value, value
+        got = [t.cpu() for t in case.grads()]
+        case.x[bad], case.dout[bad] = kept
+        rest = torch.arange(rows) != bad
+        for i in (0, 1):
+            assert torch.equal(got[i][rest], clean[i][rest])
+            assert not got[i][bad].isfinite().all()
+        other = torch.tensor([0, 2])
+        for i in (2, 3):
+            assert torch.equal(got[i][other], clean[i][other]) and not got[i][1].isfinite().all()
+    # an adapter's weights reach its own rows alone
+    case.a[1, 0, 7] = float("inf")
+    case.b[1, 9, 1] = float("nan")
+    case.put()
+    got = [t.cpu() for t in case.grads()]
+    away = case.index != 1
+    assert torch.equal(got[0][away], clean[0][away]) and torch.equal(got[1][away], clean[1][away])
+    assert torch.equal(got[2][[0, 2]], clean[2][[0, 2]]) and torch.equal(got[3][[0, 2]], clean[3][[0, 2]])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_infinite_products_are_infinite(hip_device, dtype):
+    """An infinite h with finite weights gives infinities, as the sum of its products is."""
+    say(f"infinite h {dtype}")
+    case = Case(hip_device, 4, 64, 32, 8, 1, dtype, "one")
+    case.x[1], case.a[0, 2] = 1.0, 1.0
+    case.x[1, 5] = float("inf")
+    case.a[0, :, 5] = torch.tensor([1.0] * 8).to(dtype)
+    case.b[0] = 1.0
+    case.put()
+    got = case.run().cpu()
+    assert (got[1] == float("inf")).all() and got[[0, 2, 3]].isfinite().all()
+
+
+def test_loading_adapters(hip_device):
+    say("loading adapters of lower rank")
+    g = torch.Generator().manual_seed(5)
+    bank = LowRankAdapters(96, 40, 16, 3, dtype=BF16, device=hip_device)
+    x, base = torch.randn(12, 96, generator=g).to(BF16), torch.randn(12, 40, generator=g).to(BF16)
+    index = torch.arange(12) % 3
+    rows = AdapterRows(index.to(hip_device), 3)
+    assert torch.equal(bank(x.to(hip_device), base.to(hip_device), rows).cpu(), base)  # B is zero at first
+    for i, r in enumerate((4, 16, 1)):
+        bank.load(i, torch.randn(r, 96, generator=g), torch.randn(40, r, generator=g), 2.0 / r)
+    assert not bank.a[0, 4:].any() and not bank.b[2, :, 1:].any()
+    want, err = O.low_rank(x, base, bank.a.detach().cpu(), bank.b.detach().cpu(), bank.scaling.cpu(), index)
+    check(bank(x.to(hip_device), base.to(hip_device), rows), want, err, "out")
+    with pytest.raises(IndexError):
+        bank.load(3, torch.zeros(4, 96), torch.zeros(40, 4), 1.0)
+    with pytest.raises(ValueError):
+        bank.load(0, torch.zeros(17, 96), torch.zeros(40, 17), 1.0)
+
+
+def test_changed_inputs_fail_the_backward_pass(hip_device):
+    say("rows, weights or seed changed before the backward pass")
+    case = Case(hip_device, 30, 64, 64, 8, 2, BF16, dropout=0.1, trainable=True)
+    seed = case.seed.to(hip_device)
+
+    def after(change):
+        x = case.x.to(hip_device).requires_grad_(True)
+        out = case.bank(x, case.base.to(hip_device), case.rows, seed)
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+
+    after(lambda: case.rows.update(case.index.to(hip_device)))
+    after(lambda: seed.add_(1))
+    after(case.put)
+    x = case.x.to(hip_device).requires_grad_(True)
+    (dx,) = torch.autograd.grad(case.bank(x, case.base.to(hip_device), case.rows, seed).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+def test_captured_serving_step(hip_device):
+    """One capture, replayed for other inputs and adapters (re-sorted outside the graph)."""
+    say("captured serving step")
+    case = Case(hip_device, 40, 256, 136, 16, 5, BF16)
+    x, base = case.x.to(hip_device), case.base.to(hip_device)
+    case.bank(x, base, case.rows)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = case.bank(x, base, case.rows)
+    for i in range(4):
+        case.x = torch.randn(40, 256, generator=case.g).to(BF16)
+        case.index = torch.randint(-1, 5, (40,), generator=case.g)
+        x.copy_(case.x)
+        case.rows.update(case.index.to(hip_device))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, *case.want(), f"replay {i}")
+        assert torch.equal(out, case.bank(x, base, case.rows))
+
+
+def test_captured_plan_and_training_step(hip_device):
+    """Sorting, forward and backward in one graph; seeds and rows change between replays."""
+    say("captured training step")
+    case = Case(hip_device, 90, 136, 72, 16, 3, BF16, dropout=0.25, trainable=True)
+    dev = hip_device
+    x, base, dout = case.x.to(dev).requires_grad_(True), case.base.to(dev), case.dout.to(dev)
+    index, seed = case.index.to(dev), case.seed.to(dev)
+
+    def step():
+        out = case.bank(x, base, AdapterRows(index, 3), seed)
+        return out.detach(), *torch.autograd.grad(out, (x, case.bank.a, case.bank.b), dout)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        case.seed = torch.tensor([99 + i, i])
+        case.index = torch.randint(-1, 3, (90,), generator=case.g)
+        seed.copy_(case.seed)
+        index.copy_(case.index)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, err = case.want(grads=True)
+        for name, g, w, e in zip(("out", "dx", "da", "db"), got, want, err):
+            check(g, w, e, f"replay {i} {name}")
+
+
+def test_another_stream(hip_device):
+    say("another stream than the default")
+    case = Case(hip_device, 64, 128, 128, 16, 3, F16, trainable=True, dropout=0.1)
+    want = case.grads()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        rows = AdapterRows(case.index.to(hip_device), 3)
+        case.rows = rows
+        got = case.grads()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def quant(dev, k, n, seed):
+    lay = make_layer(k, n, 128, seed=seed)
+    maker = QuantLinearMaker(quantization_group_size=128, use_act_order=False)
+    with torch.device(dev):
+        lin = maker.make_linear(k, n, bias=False)
+    lin.load_state_dict({"qweight": lay.qweight, "qzeros": lay.qzeros, "scales": lay.scales, "g_idx": lay.g_idx})
+    c = CacheV2(dev)
+    maker.post_init(TuningParams(), c)
+    c.init_cache()
+    return lin
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_adapted_linear(hip_device, dtype):
+    """A quantised projection with adapters: its own output and input gradient, and the adapters'
+    beside them; the adapters' part against the oracle on top of what the projection gives."""
+    say(f"adapted linear {dtype}")
+    lin = quant(hip_device, 256, 128, seed=4)
+    case = Case(hip_device, 50, 256, 128, 16, 3, dtype, trainable=True)
+    adapted = AdaptedLinear(lin, case.bank)
+    x = case.x.to(hip_device)
+    with torch.no_grad():
+        case.base = lin(x).cpu()
+        assert torch.equal(adapted(x).cpu(), case.base)
+        out, err = case.want()
+        check(adapted(x, case.rows), out, err, "out")
+    leaf = x.clone().requires_grad_(True)
+    y = adapted(leaf, case.rows)
+    case.base = lin(leaf).detach().cpu()  # (bf16 rows whose gradient is wanted take another product)
+    check(y.detach(), *case.want(), "out with gradients")
+    dx, da, db = torch.autograd.grad(y, (leaf, case.bank.a, case.bank.b), case.dout.to(hip_device))
+    want, errs = case.want(grads=True)
+    check(da, want[2], errs[2], "da")
+    check(db, want[3], errs[3], "db")
+    other = x.clone().requires_grad_(True)
+    (own,) = torch.autograd.grad(lin(other), other, case.dout.to(hip_device))
+    total = want[1] + own.cpu().double()  # two 16-bit gradients added in that type
+    check(dx, total, errs[1] + O.half_step(dtype) * (total.abs() + errs[1]), "dx")
+
+
+def test_refusals(hip_device):
+    say("refusals")
+    dev = hip_device
+    case = Case(dev, 10, 64, 64, 8, 2, F16, dropout=0.1)
+    x, base = case.x.to(dev), case.base.to(dev)
+    seed = case.seed.to(dev)
+    for args, kind in (((x[:, :32], base, case.rows, seed), ValueError), ((x, base[:5], case.rows, seed), ValueError),
+                       ((x.bfloat16(), base, case.rows, seed), TypeError), ((x.float(), base.float(), case.rows, seed), TypeError),
+                       ((x[:5], base[:5], case.rows, seed), ValueError), ((x, base, case.rows), ValueError),
+                       ((x, base, case.rows, seed.float()), ValueError), ((x, base, case.rows, seed[:1]), ValueError),
+                       ((x, base, case.rows, seed.cpu()), ValueError), ((x.cpu(), base, case.rows, seed), ValueError),
+                       ((x, base, AdapterRows(case.index.to(dev), 3), seed), ValueError)):
+        with pytest.raises(kind):
+            case.bank(*args)
+    with pytest.raises(ValueError):
+        case.bank(x, base, case.rows, seed, output=torch.empty(10, 128, device=dev, dtype=F16)[:, ::2])
+    with pytest.raises(ValueError):
+        case.bank(x.requires_grad_(True), base, case.rows, seed, output=torch.empty_like(base))
+    with pytest.raises(ValueError):
+        AdapterRows(torch.zeros(4, 2, dtype=torch.int64, device=dev), 2)
+    with pytest.raises(ValueError):
+        AdapterRows(torch.zeros(4, device=dev), 2)
+    with pytest.raises(ValueError):
+        case.rows.update(case.index[:4].to(dev))
+    with pytest.raises(TypeError):
+        CounterDropout(0.5)(torch.zeros(4, 4, device=dev), seed)
+    with pytest.raises(ValueError):
+        CounterDropout(0.5)(torch.zeros(4, 4, device=dev, dtype=F16))

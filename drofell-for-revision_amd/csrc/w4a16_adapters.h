@@ -33,8 +33,8 @@ inline AdapterLayout adapter_layout(int rows, int adapters) {
   l.tiles = rows / l.align + segs;
   l.chunks = rows / l.chunk_rows + segs;
   l.positions = (int64_t)l.tiles * l.align;
-  l.tile_adapter = 0;
-  l.chunk = (l.tiles + 3) & ~3;
+  l.tile_adapter = 4;  // behind the head: [0] tiles that hold rows
+  l.chunk = l.tile_adapter + ((l.tiles + 3) & ~3);
   l.chunk_start = l.chunk + 4 * (int64_t)l.chunks;
   l.order = (l.chunk_start + adapters + 2 + 3) & ~(int64_t)3;
   l.ints = l.order + l.positions;

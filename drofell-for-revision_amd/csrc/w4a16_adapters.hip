@@ -103,6 +103,7 @@ plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__
       at += n;
     }
   }
+  if (t == 0) plan[0] = tile0[segs];
   for (int s = t; s <= segs; s += kPlanThreads) plan[l.chunk_start + s] = chunk0[s];
   for (int i = t; i < l.tiles; i += kPlanThreads)
     plan[l.tile_adapter + i] = i < tile0[segs] ? segment_of(tile0, segs, i) : -1;
@@ -143,9 +144,11 @@ template <bool BF, int RT, int NT, bool DROP, bool AGAIN>
 __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int splits) {
   constexpr int kAhead = NT <= 2 ? 2 : 1;  // steps whose loads are in flight together
   __shared__ __attribute__((aligned(16))) float red[4][RT * 16][20];
-  const int item = item_of_xcd(blockIdx.x, gridDim.x), tile = item / splits, split = item - tile * splits;
+  const int item = item_of_xcd(blockIdx.x, p.plan[0] * splits);
+  if (item < 0) return;
+  const int tile = item / splits, split = item - tile * splits;
   const int ad = p.plan[p.l.tile_adapter + tile];
-  if (ad < 0 || ad >= p.adapters) return;
+  if (ad >= p.adapters) return;
   const int lane = threadIdx.x & 63, wave = wave_index(), g = lane >> 4, c = lane & 15, unit = line_unit();
   const int32_t* order = p.plan + p.l.order + (int64_t)tile * (RT * 16);
   const uint16_t* xr[RT][2];
@@ -313,9 +316,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AdapterArgs p, const
 template <bool BF, int RT, int NT, bool JOIN>
 __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int splits, AdapterPacks packs, int wide) {
   constexpr int kRows = RT * 16, kR = NT * 16, kPitch = kR + 8, kJ = NT == 1 ? 1 : NT / 2;
-  const int item = item_of_xcd(blockIdx.x, gridDim.x), tile = item / wide, column_part = item - tile * wide;
+  const int item = item_of_xcd(blockIdx.x, p.plan[0] * wide);
+  if (item < 0) return;
+  const int tile = item / wide, column_part = item - tile * wide;
   const int ad = p.plan[p.l.tile_adapter + tile];
-  if (ad < 0) return;
   const int lane = threadIdx.x & 63, wave = wave_index(), g = lane >> 4, c = lane & 15;
   const int32_t* order = p.plan + p.l.order + (int64_t)tile * kRows;
   const int groups = (p.n + 63) / 64;
@@ -509,6 +513,8 @@ void shrink_rank(const ShrinkArgs& a, int splits, hipStream_t stream) {
 template <bool BF, int NT>
 void expand_of(const AdapterArgs& a, int splits, bool join, const AdapterPacks& packs, hipStream_t stream) {
   const int groups = (a.n + 63) / 64;
+  // (up to two workgroups per CU with four waves each: more read the packed rows too often; half as many
+  // left 54 us of 46 at 10175 rows)
   const int wide = std::max(1, std::min((groups + 3) / 4, 512 / a.l.tiles));
   const unsigned grid = (unsigned)a.l.tiles * wide;
   if (a.l.align == 64) expand_kernel<BF, 4, NT, false><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
@@ -528,7 +534,7 @@ void expand_rank(const AdapterArgs& a, int splits, bool join, const AdapterPacks
 int adapter_splits(const AdapterLayout& l, int width, int cus) {
   // about four workgroups per CU, parts of at least 64 values per wave
   const int want = (4 * cus + l.tiles - 1) / l.tiles;
-  return std::max(1, std::min({want, width / 256, 32}));
+  return std::max(1, std::min({want, width / 256, l.align == 32 ? 16 : 8}));
 }
 
 hipError_t launch_adapter_plan(const AdapterLayout& l, int rows, int adapters, const int32_t* index, int32_t* plan,

@@ -59,11 +59,12 @@ __device__ __forceinline__ void exchange(u4& p, u4& q) {
     q[e] = (uint32_t)__builtin_amdgcn_update_dpp(b, a, kRotate8, 0xF, 0x3, false);  // lanes 0 .. 7: a of 8 .. 15
   }
 }
-// Workgroup b of a launch of `items` of them: the item it works on.  Workgroups go round-robin to
-// the eight XCDs, each with an L2 of its own: neighbouring items, which read the same weights, go to one.
+// The item (of `items`) that workgroup b of at least as many works on, or -1.  Workgroups go round-robin
+// to the eight XCDs, each with an L2 of its own: neighbouring items, which read the same
+// weights, go to one, equally many to each.
 __device__ __forceinline__ int item_of_xcd(int b, int items) {
-  const int each = items / 8, more = items % 8, xcd = b & 7;
-  return xcd * each + min(xcd, more) + (b >> 3);
+  const int each = items / 8, more = items % 8, xcd = b & 7, slot = b >> 3;
+  return slot < each + (xcd < more) ? xcd * each + min(xcd, more) + slot : -1;
 }
 // A load of what is read once: past the caches' usual places, which the weights then keep. Measured,
 // 10175 rows of 11008 against rank 16: 53.7 us with plain loads, 43.3 with these; the sum with

@@ -5,7 +5,7 @@
 // Five launches.  The weights are turned around, so that dh is the forward's first product
 // over g and B; beside that, in the same launch, g h^T, which needs neither.  Then dh, and dh x^T
 // with dx.  The sums over rows (outer()) come from tiles of 32 rows by 64 columns turned around by
-// way of LDS (rows as the matrix instruction's reduction), a chunk of 512 rows of one adapter per
+// way of LDS (rows as the matrix instruction's reduction), a chunk of 1024 rows of one adapter per
 // workgroup; dx comes from the same tile of x and its dropout mask.  The chunks' shares of
 // dA and dB are added up in order: no float atomics.
 
@@ -19,7 +19,7 @@ namespace dw4 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kOuterThreads = 256, kOuterWaves = kOuterThreads / 64;
 constexpr int kStep = 32;    // rows a step
 constexpr int kTurn = 72;    // halfs per row of a wave's tile of 64 columns in LDS
 
@@ -40,19 +40,19 @@ __device__ __forceinline__ u4 turned(const uint16_t* tile, int ct) {
 
 // out[c][r] = in[r][c], 16-bit: 64 x 64 at a time.
 __device__ __forceinline__ void turn_tile(const uint16_t* in, uint16_t* out, int rows, int cols, int r0, int c0, uint16_t* tile) {
-  constexpr int kPitch = 66;
+  constexpr int kPitch = 66, kRows = kOuterThreads / 32;
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + y + 8 * i, c = c0 + 2 * x;
-    if (r < rows && c < cols) *(uint32_t*)(tile + (y + 8 * i) * kPitch + 2 * x) = *(const uint32_t*)(in + (int64_t)r * cols + c);
+  for (int i = 0; i < 64 / kRows; ++i) {
+    const int r = r0 + y + kRows * i, c = c0 + 2 * x;
+    if (r < rows && c < cols) *(uint32_t*)(tile + (y + kRows * i) * kPitch + 2 * x) = *(const uint32_t*)(in + (int64_t)r * cols + c);
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = c0 + y + 8 * i, r = r0 + 2 * x;
+  for (int i = 0; i < 64 / kRows; ++i) {
+    const int c = c0 + y + kRows * i, r = r0 + 2 * x;
     if (c < cols && r < rows)
-      *(uint32_t*)(out + (int64_t)c * rows + r) = (uint32_t)tile[2 * x * kPitch + y + 8 * i] | (uint32_t)tile[(2 * x + 1) * kPitch + y + 8 * i] << 16;
+      *(uint32_t*)(out + (int64_t)c * rows + r) = (uint32_t)tile[2 * x * kPitch + y + kRows * i] | (uint32_t)tile[(2 * x + 1) * kPitch + y + kRows * i] << 16;
   }
 }
 
@@ -62,18 +62,19 @@ struct OuterArgs {
   int width;
   AdapterPacks packs;
   float* share;          // [chunks][r * width], or null
+  uint16_t* grad;        // [adapters][r * width], with share
   const uint16_t* at;    // DX: [adapters][width][r]
 };
-constexpr int kOuterLds = sizeof(uint16_t) * 4 * kStep * kTurn;
+constexpr int kOuterLds = sizeof(uint16_t) * kOuterWaves * kStep * kTurn;
 constexpr int kSumPitch = 68;
-static_assert(sizeof(float) * 4 * 16 * kSumPitch <= kOuterLds, "the waves' sums take the tiles' place");
+static_assert(sizeof(float) * kOuterWaves * 16 * kSumPitch <= kOuterLds, "the waves' sums take the tiles' place");
 
 // A chunk's rows of in, columns k0 .. k0 + 63, of which each wave takes every fourth step of 32 rows: the
-// chunk's share of sum of in_t h_t^T (COLS: stored [width][r], else [r][width]), and with DX
-// dx of the same places.
+// chunk's share of sum of in_t h_t^T (COLS: stored [width][r], else [r][width]), which is the gradient
+// itself where the adapter has no other chunk, and with DX dx of the same places.
 template <bool BF, int NT, bool DX, bool DROP, bool COLS>
 __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, int chunk_index, int k0, unsigned char* lds) {
-  constexpr int kR = NT * 16, kJ = NT == 1 ? 1 : NT / 2, kSteps = kChunkRows / kStep / 4;
+  constexpr int kR = NT * 16, kJ = NT == 1 ? 1 : NT / 2;
   const int4 chunk = *(const int4*)(p.plan + p.l.chunk + 4 * chunk_index);
   const int ad = chunk.x;
   if (ad < 0) return;
@@ -82,24 +83,24 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
   if (ad >= p.adapters) {  // rows without an adapter
     if (!DX) return;
     const int units = min(64, o.width - k0) / 8;
-    for (int i = threadIdx.x; i < chunk.z * units; i += kThreads)
+    for (int i = threadIdx.x; i < chunk.z * units; i += kOuterThreads)
       *(u4*)(p.dx + order[i / units] * p.lddx + k0 + i % units * 8) = u4{};
     return;
   }
   uint16_t* const tile = reinterpret_cast<uint16_t*>(lds) + wave * (kStep * kTurn);
   // rows as loads and stores take them (exchange()), -1 behind the chunk and the width
   const int unit = line_unit(), k = k0 + unit * 8;
-  int row[kSteps][2][2];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s)
+  int row[2][2], row2[2][2], row3[2][2];  // this step's, the next two's
+  auto rows_of = [&](int first, int (&r)[2][2]) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int at = (wave + 4 * s) * kStep + t * 16 + 8 * i + (c & 7);
-        row[s][t][i] = order[at < chunk.z ? at : 0];
-        if (at >= chunk.z || k >= o.width) row[s][t][i] = -1;
+        const int at = first + t * 16 + 8 * i + (c & 7);
+        r[t][i] = order[at < chunk.z ? at : 0];
+        if (at >= chunk.z || k >= o.width) r[t][i] = -1;
       }
+  };
   // A turned around: the operand's row is a column of x, eight values of r
   u4 at[2][2][DX ? kJ : 1];
   if constexpr (DX) {
@@ -125,35 +126,51 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
 #pragma unroll
       for (int i = 0; i < 2; ++i) x[t][i] = stream_load(o.in + (r[t][i] >= 0 ? r[t][i] * o.ld + k : 0));
   };
-  u4 v[2][2][2];
-  load(row[0], v[0]);
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int first = (wave + 4 * s) * kStep;
-    if (first >= chunk.z) break;
-    if (s + 1 < kSteps) load(row[s + 1], v[(s + 1) & 1]);
-    u4 (&x)[2][2] = v[s & 1];
+  constexpr int kStride = kOuterWaves * kStep;
+  u4 x[2][2], x2[2][2];
+  rows_of(wave * kStep, row);
+  rows_of(wave * kStep + kStride, row2);
+  load(row, x);
+  for (int first = wave * kStep; first < chunk.z; first += kStride) {
+    // h (or dh) first, the next step's rows last: loads return in order, and a wait for the former
+    // then leaves the latter in flight
     const int64_t pos = chunk.y + first;
-    u4 hi[NT], lo[NT];
+    u4 hi[NT], lo[NT], rhi[2][DX ? kJ : 1], rlo[2][DX ? kJ : 1];
+    int col_exp[NT], row_exp[2];
     if (o.share != nullptr) {
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         const uint16_t* from = o.packs.col + (pos + 8 * g) * kR + (u * 16 + c) * 8;
         hi[u] = *(const u4*)from;
         lo[u] = *(const u4*)(from + half);
+        if constexpr (!BF) col_exp[u] = o.packs.col_exp[pos / 32 * kR + u * 16 + c];
       }
     }
-    __builtin_amdgcn_sched_barrier(0);  // (else the loads sink to where they are used)
+    if constexpr (DX) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint16_t* from = o.packs.row + (pos + t * 16 + c) * kR;
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          rhi[t][j] = *(const u4*)(from + (NT == 1 ? (g >> 1) * half + (g & 1) * 8 : 32 * j + 8 * g));
+          if constexpr (NT > 1) rlo[t][j] = *(const u4*)(from + 32 * j + 8 * g + half);
+        }
+        if constexpr (!BF) row_exp[t] = o.packs.row_exp[pos + t * 16 + c];
+      }
+    }
+    rows_of(first + 2 * kStride, row3);
+    load(row2, x2);
+    if constexpr (NT < 8) __builtin_amdgcn_sched_barrier(0);  // (else the loads sink to where they are used)
     u4 keep[2][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if constexpr (DROP) {
-          keep[t][i] = philox.mask(k >> 3, row[s][t][i], p.drop);
+          keep[t][i] = philox.mask(k >> 3, row[t][i], p.drop);
           x[t][i] &= keep[t][i];
         }
-        if (row[s][t][i] < 0) x[t][i] = u4{};
+        if (row[t][i] < 0) x[t][i] = u4{};
         *(u4*)(tile + (t * 16 + 8 * i + (c & 7)) * kTurn + unit * 8) = x[t][i];
       }
     if constexpr (DX) {
@@ -162,21 +179,18 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
         f4 d[2][2] = {};
 #pragma unroll
         for (int j = 0; j < kJ; ++j) {
-          const uint16_t* from = o.packs.row + (pos + t * 16 + c) * kR + (NT == 1 ? (g >> 1) * half + (g & 1) * 8 : 32 * j + 8 * g);
-          const u4 first_part = *(const u4*)from;
 #pragma unroll
           for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) d[q][u] = mfma16_of<BF>(at[q][u][j], first_part, d[q][u]);
+            for (int u = 0; u < 2; ++u) d[q][u] = mfma16_of<BF>(at[q][u][j], rhi[t][j], d[q][u]);
           if constexpr (NT > 1) {
-            const u4 rest = *(const u4*)(from + half);
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
-              for (int u = 0; u < 2; ++u) d[q][u] = mfma16_of<BF>(at[q][u][j], rest, d[q][u]);
+              for (int u = 0; u < 2; ++u) d[q][u] = mfma16_of<BF>(at[q][u][j], rlo[t][j], d[q][u]);
           }
         }
-        const float back = BF ? 1.f : pow2(o.packs.row_exp[pos + t * 16 + c]);
+        const float back = BF ? 1.f : pow2(row_exp[t]);
         u4 w[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q)
@@ -193,11 +207,11 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if constexpr (DROP) w[i] &= keep[t][i];
-          if (row[s][t][i] >= 0) *(u4*)(p.dx + row[s][t][i] * p.lddx + k) = w[i];
+          if (row[t][i] >= 0) *(u4*)(p.dx + row[t][i] * p.lddx + k) = w[i];
         }
       }
     }
-    if (o.share == nullptr) continue;
+    if (o.share != nullptr) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     u4 xt[4];
 #pragma unroll
@@ -211,7 +225,7 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
           acc[t][u] = mfma16_of<BF>(xt[t], lo[u], acc[t][u]);
         }
       } else {
-        const float back = pow2(o.packs.col_exp[pos / 32 * kR + u * 16 + c]);
+        const float back = pow2(col_exp[u]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           f4 d = mfma16_of<BF>(xt[t], hi[u], f4{});
@@ -222,39 +236,53 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        row[t][i] = row2[t][i];
+        row2[t][i] = row3[t][i];
+        x[t][i] = x2[t][i];
+      }
   }
   if (o.share == nullptr) return;
   // the waves' sums, 16 columns of h at a time
-  float* const sums = reinterpret_cast<float*>(lds);  // [4][16][kSumPitch]
+  float* const sums = reinterpret_cast<float*>(lds);  // [waves][16][kSumPitch]
+  const bool alone = p.plan[p.l.chunk_start + ad + 1] - p.plan[p.l.chunk_start + ad] == 1;
   float* share = o.share + (int64_t)chunk_index * o.width * p.r;
+  uint16_t* grad = o.grad + (int64_t)ad * o.width * p.r;
+  auto store = [&](int64_t at, f4 v) {
+    if (alone) *(uint2*)(grad + at) = make_uint2(pack16<BF>(v[0], v[1]), pack16<BF>(v[2], v[3]));
+    else *(f4*)(share + at) = v;
+  };
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < 4; ++t) *(f4*)(sums + (wave * 16 + c) * kSumPitch + t * 16 + 4 * g) = acc[t][u];
     __syncthreads();
+    f4 v = {};
     if constexpr (COLS) {
       const int col = threadIdx.x >> 2, r = (threadIdx.x & 3) * 4;
-      f4 v = {};
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
+      for (int w = 0; w < kOuterWaves; ++w)
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += sums[(w * 16 + r + e) * kSumPitch + col];
-      if (k0 + col < o.width && u * 16 + r < p.r) *(f4*)(share + (int64_t)(k0 + col) * p.r + u * 16 + r) = v;
+      if (k0 + col < o.width && u * 16 + r < p.r) store((int64_t)(k0 + col) * p.r + u * 16 + r, v);
     } else {
       const int r = threadIdx.x >> 4, col = (threadIdx.x & 15) * 4;
-      f4 v = {};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) v += *(const f4*)(sums + (w * 16 + r) * kSumPitch + col);
-      if (k0 + col < o.width && u * 16 + r < p.r) *(f4*)(share + (int64_t)(u * 16 + r) * o.width + k0 + col) = v;
+      for (int w = 0; w < kOuterWaves; ++w) v += *(const f4*)(sums + (w * 16 + r) * kSumPitch + col);
+      if (k0 + col < o.width && u * 16 + r < p.r) store((int64_t)(u * 16 + r) * o.width + k0 + col, v);
     }
   }
 }
 
 // The first launch of a backward pass: A [r][k] turned to [k][r] and B [n][r] to [r][n], and g h^T.
 template <bool BF, int NT>
-__global__ void __launch_bounds__(kThreads)
-first_kernel(AdapterArgs p, OuterArgs o, uint16_t* at, uint16_t* bt, int a_tiles, int b_tiles, int outer_items) {
+__global__ void __launch_bounds__(kOuterThreads)
+first_kernel(AdapterArgs p, OuterArgs o, uint16_t* at, uint16_t* bt, int a_tiles, int b_tiles) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[kOuterLds];
   int i = blockIdx.x;
   const int rt = (p.r + 63) / 64, turns = (a_tiles + b_tiles) * p.adapters;
@@ -272,18 +300,19 @@ first_kernel(AdapterArgs p, OuterArgs o, uint16_t* at, uint16_t* bt, int a_tiles
     }
     return;
   }
-  i = item_of_xcd(i - turns, outer_items);
+  i -= turns;
   const int cols = (o.width + 63) / 64;
   outer<BF, NT, false, false, true>(p, o, i / cols, i % cols * 64, lds);
 }
 template <bool BF, int NT, bool DX, bool DROP>
-__global__ void __launch_bounds__(kThreads) outer_kernel(AdapterArgs p, OuterArgs o) {
+__global__ void __launch_bounds__(kOuterThreads) outer_kernel(AdapterArgs p, OuterArgs o) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[kOuterLds];
-  const int i = item_of_xcd(blockIdx.x, gridDim.x), cols = (o.width + 63) / 64;
+  const int i = blockIdx.x, cols = (o.width + 63) / 64;
   outer<BF, NT, DX, DROP, false>(p, o, i / cols, i % cols * 64, lds);
 }
 
-// dA and dB of each adapter: its chunks' shares summed in order; four elements a thread.
+// dA and dB of the adapters of several chunks, whose shares are summed in order, and of none; four
+// elements a thread.
 template <bool BF>
 __global__ void __launch_bounds__(kThreads) reduce_kernel(AdapterArgs p, const float* share_a, const float* share_b) {
   const int64_t each_a = p.da ? (int64_t)p.r * p.k / 4 : 0, each_b = p.db ? (int64_t)p.r * p.n / 4 : 0;
@@ -295,6 +324,7 @@ __global__ void __launch_bounds__(kThreads) reduce_kernel(AdapterArgs p, const f
     const int64_t q = is_a ? at : at - each_a, each = is_a ? each_a : each_b;
     const float* share = (is_a ? share_a : share_b) + q * 4;
     const int c0 = p.plan[p.l.chunk_start + ad], c1 = p.plan[p.l.chunk_start + ad + 1];
+    if (c1 - c0 == 1) continue;  // stored already
     f4 v = {};
     for (int c = c0; c < c1; c += 4) {  // four loads in flight
       f4 x[4];
@@ -318,10 +348,10 @@ hipError_t launch_grad(const AdapterArgs& a, const BackwardWs& w, hipStream_t st
   const int rt = (a.r + 63) / 64;
   const int a_tiles = a.dx ? rt * ((a.k + 63) / 64) : 0, b_tiles = inner ? rt * ((a.n + 63) / 64) : 0;
   const int outer_items = a.db ? a.l.chunks * ((a.n + 63) / 64) : 0;
-  OuterArgs g = {a.g, a.ldg, a.n, {}, share_b, nullptr};
+  OuterArgs g = {a.g, a.ldg, a.n, {}, share_b, a.db, nullptr};
   place_col(g.packs, a.l, a.r, a.h);
   const unsigned first = (unsigned)((a_tiles + b_tiles) * a.adapters + outer_items);
-  if (first) first_kernel<BF, NT><<<first, kThreads, 0, stream>>>(a, g, at, bt, a_tiles, b_tiles, outer_items);
+  if (first) first_kernel<BF, NT><<<first, kOuterThreads, 0, stream>>>(a, g, at, bt, a_tiles, b_tiles);
   if (inner) {
     AdapterPacks packs = {};
     hipError_t e;
@@ -333,14 +363,14 @@ hipError_t launch_grad(const AdapterArgs& a, const BackwardWs& w, hipStream_t st
       if (a.da != nullptr) place_col(packs, a.l, a.r, a.ws + w.col);
       if ((e = launch_join(a, planes, w.splits, packs, stream)) != hipSuccess) return e;
     }
-    const OuterArgs x = {a.x, a.ldx, a.k, packs, a.da ? share_a : nullptr, at};
+    const OuterArgs x = {a.x, a.ldx, a.k, packs, a.da ? share_a : nullptr, a.da, at};
     const unsigned grid = (unsigned)(a.l.chunks * ((a.k + 63) / 64));
     if (a.dx != nullptr) {
-      if (a.drop) outer_kernel<BF, NT, true, true><<<grid, kThreads, 0, stream>>>(a, x);
-      else outer_kernel<BF, NT, true, false><<<grid, kThreads, 0, stream>>>(a, x);
+      if (a.drop) outer_kernel<BF, NT, true, true><<<grid, kOuterThreads, 0, stream>>>(a, x);
+      else outer_kernel<BF, NT, true, false><<<grid, kOuterThreads, 0, stream>>>(a, x);
     } else {
-      if (a.drop) outer_kernel<BF, NT, false, true><<<grid, kThreads, 0, stream>>>(a, x);
-      else outer_kernel<BF, NT, false, false><<<grid, kThreads, 0, stream>>>(a, x);
+      if (a.drop) outer_kernel<BF, NT, false, true><<<grid, kOuterThreads, 0, stream>>>(a, x);
+      else outer_kernel<BF, NT, false, false><<<grid, kOuterThreads, 0, stream>>>(a, x);
     }
   }
   if (a.da != nullptr || a.db != nullptr) {

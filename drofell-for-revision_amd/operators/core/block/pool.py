@@ -169,7 +169,7 @@ class BlockPool:
         if tokens < 0:
             raise ValueError("tokens must not be negative")
         ints = torch.empty(rows + 2 + 2 * tokens, dtype=torch.int32, device=self.device)
-        excess, starts, positions, row_of = ints.split([1, rows + 1, tokens, tokens])
+        excess, starts, positions, row_of = torch.split_with_sizes(ints, (1, rows + 1, tokens, tokens))
         slots = torch.empty(tokens, dtype=torch.int64, device=self.device)
         self._call("dw4_token_slots", rows, width, self.num_blocks, flags.BLOCK_SIZE,
                    state.block_tables.data_ptr(), state.context_lens.data_ptr(), n.data_ptr(), tokens,

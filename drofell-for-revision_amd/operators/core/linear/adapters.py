@@ -201,15 +201,18 @@ class _LowRank(torch.autograd.Function):
         out, x, h, shape = _forward(x, base, a, b, scaling, plan, drop, seed, None, True)
         # what the backward pass needs, worked out here: it runs in a thread of autograd's, where
         # the same Python takes twice as long
-        index = x.device.index
-        nbytes = _lib.adapters_workspace_size(*shape[1:], True, index)[0] if shape[1] else 0
+        nbytes = _lib.adapters_workspace_size(*shape[1:], True, x.device.index)[0] if shape[1] else 0
         ctx.call = shape, drop, nbytes, x.device, _stride(x)
         ctx.save_for_backward(x, a, b, scaling, plan, h, seed)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        # (the wrapper that refuses a second derivative takes 3 us, and is needed where one may follow)
+        return _LowRank._once(ctx, dout) if torch.is_grad_enabled() else _LowRank._gradients(ctx, dout)
+
+    @staticmethod
+    def _gradients(ctx, dout):
         x, a, b, scaling, plan, h, seed = ctx.saved_tensors
         shape, drop, nbytes, device, ldx = ctx.call
         need_x, need_base, need_a, need_b = ctx.needs_input_grad[:4]
@@ -221,10 +224,9 @@ class _LowRank(torch.autograd.Function):
             return None, dbase, None, None, None, None, None, None
         with _lib.on_device(device):
             g = _matrix(dout)
-            dtype = x.dtype
-            dx = torch.empty(x.shape, dtype=dtype, device=device) if need_x else None
-            da = torch.empty(a.shape, dtype=dtype, device=device) if need_a else None
-            db = torch.empty(b.shape, dtype=dtype, device=device) if need_b else None
+            dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+            da = torch.empty_like(a) if need_a else None
+            db = torch.empty_like(b) if need_b else None
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
             _lib.call("dw4_adapters_backward", *shape, x.data_ptr(), ldx, g.data_ptr(), _stride(g), a.data_ptr(),
                       b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), drop,
@@ -232,6 +234,8 @@ class _LowRank(torch.autograd.Function):
                       None if dx is None else dx.data_ptr(), shape[3], None if da is None else da.data_ptr(),
                       None if db is None else db.data_ptr(), ws.data_ptr(), nbytes, _lib.current_stream(device.index))
         return dx, dbase, da, db, None, None, None, None
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_gradients.__func__))
 
 
 class AdaptedLinear(Linear):
@@ -280,15 +284,16 @@ class CounterDropout(nn.Module):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def _run(x, seed, drop):
+        device = x.device
         cols = x.shape[-1]
         rows = x.numel() // cols if cols else 0
-        with _lib.on_device(x.device):
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            x2 = x.reshape(rows, cols)
-            if x2.stride(1) != 1 or (rows > 1 and x2.stride(0) < cols):
-                x2 = x2.contiguous()
+        x2 = x if x.dim() == 2 else x.reshape(rows, cols)
+        if not x2.is_contiguous() and (x2.stride(1) != 1 or (rows > 1 and x2.stride(0) < cols)):
+            x2 = x2.contiguous()
+        with _lib.on_device(device):
+            y = torch.empty_like(x, memory_format=torch.contiguous_format)
             _lib.call("dw4_dropout", _DTYPES[x.dtype], rows, cols, x2.data_ptr(), _stride(x2), y.data_ptr(), cols, drop,
-                      seed.data_ptr(), _lib.current_stream(x.device.index))
+                      seed.data_ptr(), _lib.current_stream(device.index))
         return y
 
     @staticmethod
@@ -298,7 +303,12 @@ class _Dropout(torch.autograd.Function):
         return _Dropout._run(x, seed, drop)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        return _Dropout._once(ctx, dy) if torch.is_grad_enabled() else _Dropout._gradient(ctx, dy)
+
+    @staticmethod
+    def _gradient(ctx, dy):
         (seed,) = ctx.saved_tensors
         return _Dropout._run(dy, seed, ctx.drop), None, None
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_gradient.__func__))

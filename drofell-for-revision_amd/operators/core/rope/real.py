@@ -97,8 +97,8 @@ class RotaryEmbedding:
               inverse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
         with _lib.on_device(self.device):
             q, k = _rows(q), _rows(k)
-            qo = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-            ko = torch.empty(k.shape, dtype=q.dtype, device=self.device)
+            qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+            ko = torch.empty_like(k, memory_format=torch.contiguous_format)
             _lib.call("dw4_rotary", _DTYPES[q.dtype], q.shape[0], q.shape[1], k.shape[1], self.head_dim,
                       self.rotary_dim, int(self.interleaved), int(inverse), q.data_ptr(), _stride(q),
                       k.data_ptr(), _stride(k), qo.data_ptr(), _stride(qo), ko.data_ptr(), _stride(ko),
@@ -139,7 +139,7 @@ class RotaryEmbedding:
         elif not slots.is_contiguous():
             slots = slots.contiguous()
         if output is None:
-            output = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            output = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif output.shape != q.shape or output.dtype != q.dtype or output.device != self.device:
             raise ValueError("output must have the queries' shape, type and device")
         elif _rows(output) is not output:
@@ -168,10 +168,16 @@ class _Rotary(torch.autograd.Function):
         return rotary._turn(q, k, positions, False)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
+        # (the wrapper that refuses a second derivative takes 3 us, and is needed where one may follow)
+        return _Rotary._once(ctx, dq, dk) if torch.is_grad_enabled() else _Rotary._gradients(ctx, dq, dk)
+
+    @staticmethod
+    def _gradients(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
         return (*ctx.rotary._turn(dq, dk, positions, True), None, None)
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_gradients.__func__))
 
 
 class _NoGradient(torch.autograd.Function):

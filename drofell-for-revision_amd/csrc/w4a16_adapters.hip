@@ -165,6 +165,8 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int i = 0; i < 2; ++i) ar[t][i] = p.weights + ((int64_t)ad * p.r + min(t * 16 + 8 * i + (c & 7), p.r - 1)) * p.width;
+  // a tile of few rows: its second half may hold none
+  const bool two = RT != 2 || __builtin_amdgcn_readfirstlane(order[16]) >= 0;
   f4 acc[RT][NT] = {};
   const Philox philox(DROP ? p.seed : reinterpret_cast<const int64_t*>(p.plan));
   const int steps = (p.width + 63) / 64, parts = splits * 4, part = split * 4 + wave;
@@ -176,7 +178,8 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int t = 0; t < RT; ++t) v.x[t][i] = AGAIN ? *(const u4*)(xr[t][i] + at) : stream_load(xr[t][i] + at);
+      for (int t = 0; t < RT; ++t)
+        if (t == 0 || two) v.x[t][i] = AGAIN ? *(const u4*)(xr[t][i] + at) : stream_load(xr[t][i] + at);
 #pragma unroll
       for (int t = 0; t < NT; ++t) v.a[t][i] = *(const u4*)(ar[t][i] + at);
     }
@@ -186,6 +189,7 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
     for (int t = 0; t < NT; ++t) exchange(v.a[t][0], v.a[t][1]);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
+      if (t > 0 && !two) break;
       if constexpr (DROP) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) v.x[t][i] &= philox.mask(s * 8 + unit, row[t][i], p.drop);
@@ -398,6 +402,8 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
       row[t][i] = order[t * 16 + 8 * i + (c & 7)];
       from[t][i] = p.base + max(row[t][i], 0) * p.ldb;
     }
+  // a tile of few rows: its second half may hold none
+  const bool two = RT != 2 || __builtin_amdgcn_readfirstlane(order[16]) >= 0;
   const int unit = line_unit();
   const uint16_t* const bw = p.b + (int64_t)ad * p.n * p.r;
   struct Group {
@@ -418,7 +424,8 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) v.y[t][i] = stream_load(from[t][i] + (n < p.n ? n : 0));
+      for (int i = 0; i < 2; ++i)
+        if (t == 0 || two) v.y[t][i] = stream_load(from[t][i] + (n < p.n ? n : 0));
   };
   for (int grp = g0 + wave; grp < g1; grp += 4) {
     Group v;
@@ -432,6 +439,7 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
         if ((NT == 1 ? (g & 1) * 8 : 32 * j + 8 * g) >= p.r) v.b[u][j] = u4{};
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
+      if (t > 0 && !two) break;
       f4 acc[4] = {};
 #pragma unroll
       for (int u = 0; u < 4; ++u)

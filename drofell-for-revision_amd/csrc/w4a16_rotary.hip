@@ -263,7 +263,7 @@ hipError_t launch_cache(const RotaryArgs& a, hipStream_t stream) {
   const int each = heads_each(a, a.heads, 4096);
   const int64_t q_blocks = ((int64_t)a.rows * host_units(a) + kThreads - 1) / kThreads;
   const int q_groups = (a.heads + each - 1) / each;
-  const int tile = a.rows >= 2048 ? kTile : 8;
+  const int tile = a.rows < 2048 ? 8 : a.head_size > 256 ? kTile / 2 : kTile;  // (LDS: 37 KiB at heads of 256)
   const int64_t kv = (int64_t)((a.rows + tile - 1) / tile) * a.kv_heads;
   const size_t smem = 2 * ((size_t)tile * (a.head_size + 8) + (size_t)(tile + kHalo) * (a.head_size + 2));
   rotary_cache_kernel<BF, VEC, IL><<<(unsigned)(q_blocks * q_groups + kv), kThreads, smem, stream>>>(a, each, q_groups, (int)q_blocks, tile);

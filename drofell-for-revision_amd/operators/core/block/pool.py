@@ -168,9 +168,9 @@ class BlockPool:
         n, tokens = self._by_row(new_tokens, rows, "new_tokens"), int(tokens)
         if tokens < 0:
             raise ValueError("tokens must not be negative")
-        ints = torch.empty(rows + 2 + 2 * tokens, dtype=torch.int32, device=self.device)
+        ints = n.new_empty(rows + 2 + 2 * tokens)
         excess, starts, positions, row_of = torch.split_with_sizes(ints, (1, rows + 1, tokens, tokens))
-        slots = torch.empty(tokens, dtype=torch.int64, device=self.device)
+        slots = n.new_empty(tokens, dtype=torch.int64)
         self._call("dw4_token_slots", rows, width, self.num_blocks, flags.BLOCK_SIZE,
                    state.block_tables.data_ptr(), state.context_lens.data_ptr(), n.data_ptr(), tokens,
                    starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), row_of.data_ptr(),

@@ -184,9 +184,9 @@ def _forward(x, base, a, b, scaling, plan, drop, seed, out, keep):
         shape = (_DTYPES[x.dtype], x.shape[0], a.shape[0], x.shape[1], b.shape[1], a.shape[1])
         nbytes, h_bytes = _lib.adapters_workspace_size(*shape[1:], False, device.index)
         if out is None:
-            out = torch.empty(base.shape, dtype=x.dtype, device=device)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        h = torch.empty(h_bytes, dtype=torch.uint8, device=device) if keep else None
+            out = torch.empty_like(base, memory_format=torch.contiguous_format)
+        ws = x.new_empty(nbytes // 2)  # (16-bit elements; torch.empty takes 0.6 us more)
+        h = x.new_empty(h_bytes // 2) if keep else None
         _lib.call("dw4_adapters", *shape, x.data_ptr(), _stride(x), base.data_ptr(), _stride(base), out.data_ptr(),
                   _stride(out), a.data_ptr(), b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), drop,
                   None if seed is None else seed.data_ptr(), None if h is None else h.data_ptr(), ws.data_ptr(), nbytes,
@@ -227,7 +227,7 @@ class _LowRank(torch.autograd.Function):
             dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
             da = torch.empty_like(a) if need_a else None
             db = torch.empty_like(b) if need_b else None
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            ws = x.new_empty(nbytes // 2)
             _lib.call("dw4_adapters_backward", *shape, x.data_ptr(), ldx, g.data_ptr(), _stride(g), a.data_ptr(),
                       b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), drop,
                       None if seed is None else seed.data_ptr(), h.data_ptr(),

@@ -21,6 +21,7 @@ from fractions import Fraction
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from hip_extends import _lib
 
@@ -109,7 +110,8 @@ class RotaryEmbedding:
     def forward(self, q: torch.Tensor, k: torch.Tensor,
                 positions: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """q [rows, heads, head_dim] and k [rows, kv heads, head_dim] turned by their rows'
-        ``positions`` (integers [rows]) -> new tensors.  Differentiable in q and k (once)."""
+        ``positions`` (integers [rows] within 32 bits) -> new tensors.  Differentiable in q and k
+        (once)."""
         pos = self._positions(positions, self._check(q, k))
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
             return _Rotary.apply(q, k, pos, self)
@@ -138,7 +140,8 @@ class RotaryEmbedding:
             slots = int32(slots, "slots").to(torch.int64)
         elif not slots.is_contiguous():
             slots = slots.contiguous()
-        if output is None:
+        given = output is not None
+        if not given:
             output = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif output.shape != q.shape or output.dtype != q.dtype or output.device != self.device:
             raise ValueError("output must have the queries' shape, type and device")
@@ -155,6 +158,8 @@ class RotaryEmbedding:
                       kv_cacher.layer_key_ptr_table_device.data_ptr(),
                       kv_cacher.layer_val_ptr_table_device.data_ptr(), info.head_stride,
                       _lib.current_stream(self.device.index))
+        if given:
+            increment_version(output)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
             return _NoGradient.apply(output, q, k, v)
         return output

@@ -154,7 +154,7 @@ def slots_of(g, rows, blocks, bs, kind):
 @pytest.mark.parametrize("hd,rd,interleaved,bs,kvh,rows,kind", [
     (128, 128, False, 16, 2, 1, "runs"), (128, 128, False, 32, 2, 45, "scattered"), (64, 64, True, 16, 1, 333, "runs"),
     (80, 20, False, 32, 3, 100, "runs"), (112, 50, True, 16, 2, 70, "scattered"), (256, 256, False, 32, 1, 90, "runs"),
-    (64, 64, False, 16, 1, 2500, "runs"), (96, 48, True, 32, 2, 2100, "runs"), (128, 2, False, 16, 1, 2049, "scattered")])
+    (64, 64, False, 16, 1, 2500, "runs"), (96, 48, True, 32, 2, 2100, "runs"), (512, 512, False, 16, 1, 2100, "runs"), (512, 40, True, 32, 1, 9, "scattered"), (128, 2, False, 16, 1, 2049, "scattered")])
 def test_into_the_cache(hip_device, hd, rd, interleaved, bs, kvh, rows, kind, dtype):
     say(f"rotary into the cache: {rows} rows, {kvh} heads of {hd}, {rd} turning, blocks of {bs}, {kind} {dtype}")
     g = torch.Generator().manual_seed(rows + hd)

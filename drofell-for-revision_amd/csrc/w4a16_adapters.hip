@@ -144,12 +144,13 @@ template <bool BF, int RT, int NT, bool DROP, bool AGAIN>
 __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int splits) {
   constexpr int kAhead = NT <= 2 ? 2 : 1;  // steps whose loads are in flight together
   __shared__ __attribute__((aligned(16))) float red[4][RT * 16][20];
+  __shared__ u4 lines[4][128];
   const int item = item_of_xcd(blockIdx.x, p.plan[0] * splits);
   if (item < 0) return;
   const int tile = item / splits, split = item - tile * splits;
   const int ad = p.plan[p.l.tile_adapter + tile];
   if (ad >= p.adapters) return;
-  const int lane = threadIdx.x & 63, wave = wave_index(), g = lane >> 4, c = lane & 15, unit = line_unit();
+  const int lane = threadIdx.x & 63, wave = wave_index(), g = lane >> 4, c = lane & 15, unit = lane & 7, line = lane >> 3;
   const int32_t* order = p.plan + p.l.order + (int64_t)tile * (RT * 16);
   const uint16_t* xr[RT][2];
   int row[RT][2];
@@ -157,14 +158,14 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
   for (int t = 0; t < RT; ++t)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      row[t][i] = max(order[t * 16 + 8 * i + (c & 7)], 0);
+      row[t][i] = max(order[t * 16 + 8 * i + line], 0);
       xr[t][i] = p.in + row[t][i] * p.ld;
     }
   const uint16_t* ar[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) ar[t][i] = p.weights + ((int64_t)ad * p.r + min(t * 16 + 8 * i + (c & 7), p.r - 1)) * p.width;
+    for (int i = 0; i < 2; ++i) ar[t][i] = p.weights + ((int64_t)ad * p.r + min(t * 16 + 8 * i + line, p.r - 1)) * p.width;
   // a tile of few rows: its second half may hold none
   const bool two = RT != 2 || __builtin_amdgcn_readfirstlane(order[16]) >= 0;
   f4 acc[RT][NT] = {};
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
   };
   auto multiply = [&](int s, Step& v) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) exchange(v.a[t][0], v.a[t][1]);
+    for (int t = 0; t < NT; ++t) to_operands(v.a[t][0], v.a[t][1], lines[wave]);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       if (t > 0 && !two) break;
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
 #pragma unroll
         for (int i = 0; i < 2; ++i) v.x[t][i] &= philox.mask(s * 8 + unit, row[t][i], p.drop);
       }
-      exchange(v.x[t][0], v.x[t][1]);
+      to_operands(v.x[t][0], v.x[t][1], lines[wave]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -392,19 +393,21 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
       }
     }
   }
-  // rows as loads and stores take them (exchange())
+  // rows as loads and stores take them (to_operands())
   int row[RT][2];
   const uint16_t* from[RT][2];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      row[t][i] = order[t * 16 + 8 * i + (c & 7)];
+      row[t][i] = order[t * 16 + 8 * i + (lane >> 3)];
       from[t][i] = p.base + max(row[t][i], 0) * p.ldb;
     }
   // a tile of few rows: its second half may hold none
   const bool two = RT != 2 || __builtin_amdgcn_readfirstlane(order[16]) >= 0;
-  const int unit = line_unit();
+  const int unit = lane & 7;
+  __shared__ __attribute__((aligned(16))) float sums[4][16 * 68];
+  float* const own = sums[wave];
   const uint16_t* const bw = p.b + (int64_t)ad * p.n * p.r;
   struct Group {
     u4 y[RT][2], b[4][kJ];
@@ -448,20 +451,23 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
           acc[u] = mfma16_of<BF>(v.b[u][j], hv[t][j], acc[u]);
           if constexpr (NT > 1) acc[u] = mfma16_of<BF>(v.b[u][j], lv[t][j], acc[u]);
         }
-      exchange(v.y[t][0], v.y[t][1]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int u = 0; u < 4; ++u) {
+        if constexpr (!BF) acc[u] *= back[t];
+        *(f4*)(own + c * 68 + (4 * (u >> 1) + g) * 8 + (u & 1) * 4) = acc[u];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float* at = own + (8 * i + (lane >> 3)) * 68 + unit * 8;
+        const f4 lo = *(const f4*)at, hi = *(const f4*)(at + 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float w[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float d = acc[2 * i + (e >> 1)][(e & 1) * 2 + j];
-            w[j] = BF ? unpack16<BF>(v.y[t][i][e], j) + d : fmaf(d, back[t], unpack16<BF>(v.y[t][i][e], j));
-          }
-          v.y[t][i][e] = pack16<BF>(w[0], w[1]);
+          const f4& d = e < 2 ? lo : hi;
+          v.y[t][i][e] = pack16<BF>(unpack16<BF>(v.y[t][i][e], 0) + d[(e & 1) * 2], unpack16<BF>(v.y[t][i][e], 1) + d[(e & 1) * 2 + 1]);
         }
-      exchange(v.y[t][0], v.y[t][1]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (in && row[t][i] >= 0) *(u4*)(p.out + row[t][i] * p.ldo + grp * 64 + unit * 8) = v.y[t][i];
@@ -523,7 +529,7 @@ void expand_of(const AdapterArgs& a, int splits, bool join, const AdapterPacks& 
   const int groups = (a.n + 63) / 64;
   // (up to two workgroups per CU with four waves each: more read the packed rows too often; half as many
   // left 54 us of 46 at 10175 rows)
-  const int wide = std::max(1, std::min((groups + 3) / 4, 512 / a.l.tiles));
+  const int wide = std::max(1, std::min((groups + 3) / 4, (a.l.align == 32 ? 1024 : 512) / a.l.tiles));
   const unsigned grid = (unsigned)a.l.tiles * wide;
   if (a.l.align == 64) expand_kernel<BF, 4, NT, false><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
   else if (join) expand_kernel<BF, 2, NT, true><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);

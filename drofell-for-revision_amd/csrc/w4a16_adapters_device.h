@@ -44,21 +44,33 @@ struct Philox {
 };
 
 // Rows in memory and rows as operands.  A 16 x 16 x 32 operand holds four 16-byte units of 16
-// rows (lane 16 g + c: unit g of row c), so that a load in that layout takes 64 bytes of
-// each row, half a line.  Loads and stores take 128 instead: of a pair, the first instruction has
-// rows 0 .. 7 and the second rows 8 .. 15, lane 16 g + c unit g (c below 8) or 4 + g (else) of
-// row c % 8.  exchange() turns such a pair into the operands of units g and 4 + g of row c, and
-// back: two moves a register within each 16 lanes.  Measured, 10240 rows of 16 KiB copied by tiles
-// of 64 rows: 3.4 TB/s by 64 bytes a row, 4.6 by 128 or 256.
-__device__ __forceinline__ void exchange(u4& p, u4& q) {
-  constexpr int kRotate8 = 0x128;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int a = (int)p[e], b = (int)q[e];
-    p[e] = (uint32_t)__builtin_amdgcn_update_dpp(a, b, kRotate8, 0xF, 0xC, false);  // lanes 8 .. 15: b of 0 .. 7
-    q[e] = (uint32_t)__builtin_amdgcn_update_dpp(b, a, kRotate8, 0xF, 0x3, false);  // lanes 0 .. 7: a of 8 .. 15
-  }
+// rows, lane 16 g + c unit g of row c: loaded in that layout, neighbouring lanes touch different rows, half a
+// line of each, one 16-byte access after the other.  Loads and stores take whole lines in consecutive lanes
+// instead, a pair of instructions 16 rows of 128 bytes (lane l: unit l % 8 of rows l / 8 and 8 + l / 8), and
+// 2 KiB of LDS of the wave's own turn the pair into the operands of units g and 4 + g of row c, and
+// back; the units' places are exchanged by row so that the accesses spread over the banks.  Measured: 10240
+// rows of 16 KiB copied by tiles of 64 rows 3.4 TB/s by 64 bytes a row, 4.6 by 128 or 256; 10175 rows
+// of 11008 against rank 16 43.4 us with the lanes of a row 16 apart, 40.4 in consecutive lanes.
+__device__ __forceinline__ void to_operands(u4& p, u4& q, u4* own) {
+  const int lane = threadIdx.x & 63, r = lane >> 3, u = lane & 7, g = lane >> 4, c = lane & 15;
+  own[r * 8 + (u ^ r)] = p;
+  own[(8 + r) * 8 + (u ^ r)] = q;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  p = own[c * 8 + (g ^ (c & 7))];
+  q = own[c * 8 + ((4 + g) ^ (c & 7))];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
+__device__ __forceinline__ void from_operands(u4& p, u4& q, u4* own) {
+  const int lane = threadIdx.x & 63, r = lane >> 3, u = lane & 7, g = lane >> 4, c = lane & 15;
+  own[c * 8 + (g ^ (c & 7))] = p;
+  own[c * 8 + ((4 + g) ^ (c & 7))] = q;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  p = own[r * 8 + (u ^ r)];
+  q = own[(8 + r) * 8 + (u ^ r)];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // The item (of `items`) that workgroup b of at least as many works on, or -1.  Workgroups go round-robin
 // to the eight XCDs, each with an L2 of its own: neighbouring items, which read the same
 // weights, go to one, equally many to each.
@@ -70,13 +82,6 @@ __device__ __forceinline__ int item_of_xcd(int b, int items) {
 // 10175 rows of 11008 against rank 16: 53.7 us with plain loads, 43.3 with these; the sum with
 // the projection's output 59.7 and 45.8.
 __device__ __forceinline__ u4 stream_load(const uint16_t* p) { return __builtin_nontemporal_load((const u4*)p); }
-__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
-
-// The lane's unit (of eight) in the memory layout.
-__device__ __forceinline__ int line_unit() {
-  const int lane = threadIdx.x & 63;
-  return (lane >> 4) + ((lane & 8) >> 1);
-}
 
 template <bool BF>
 __device__ __forceinline__ f4 mfma16_of(u4 a, u4 b, f4 c) {

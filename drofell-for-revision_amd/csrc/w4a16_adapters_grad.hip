@@ -88,15 +88,16 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
     return;
   }
   uint16_t* const tile = reinterpret_cast<uint16_t*>(lds) + wave * (kStep * kTurn);
-  // rows as loads and stores take them (exchange()), -1 behind the chunk and the width
-  const int unit = line_unit(), k = k0 + unit * 8;
+  // rows as loads and stores take them (to_operands()), -1 behind the chunk and the width
+  const int unit = lane & 7, line = lane >> 3, k = k0 + unit * 8;
+  __shared__ u4 lines[4][128];
   int row[2][2], row2[2][2], row3[2][2];  // this step's, the next two's
   auto rows_of = [&](int first, int (&r)[2][2]) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int at = first + t * 16 + 8 * i + (c & 7);
+        const int at = first + t * 16 + 8 * i + line;
         r[t][i] = order[at < chunk.z ? at : 0];
         if (at >= chunk.z || k >= o.width) r[t][i] = -1;
       }
@@ -171,7 +172,7 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
           x[t][i] &= keep[t][i];
         }
         if (row[t][i] < 0) x[t][i] = u4{};
-        *(u4*)(tile + (t * 16 + 8 * i + (c & 7)) * kTurn + unit * 8) = x[t][i];
+        *(u4*)(tile + (t * 16 + 8 * i + line) * kTurn + unit * 8) = x[t][i];
       }
     if constexpr (DX) {
 #pragma unroll
@@ -203,7 +204,7 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
             }
             w[q][i] = pack16<BF>(a, b);
           }
-        exchange(w[0], w[1]);
+        from_operands(w[0], w[1], lines[wave]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if constexpr (DROP) w[i] &= keep[t][i];

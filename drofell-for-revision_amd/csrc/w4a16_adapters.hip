@@ -2,7 +2,7 @@
 //   out_t = base_t + s_a B_a A_a d(x_t),   a = the row's adapter (or none),
 // with d dropout whose mask comes from a counter; and that dropout by itself.
 //
-// Rows are sorted by adapter once per batch (plan_kernel), so that a tile of 16 or 64
+// Rows are sorted by adapter once per batch (plan_kernel), so that a tile of 32
 // positions has one adapter and both its products run on 16 x 16 x 32 matrix
 // instructions, rows as their columns.  The rows' products with A are formed in parts of k
 // over workgroups and waves (fp32 planes), joined in order into 16-bit operands, and
@@ -19,6 +19,7 @@ namespace dw4 {
 namespace {
 
 constexpr int kThreads = 256, kJoinThreads = 512;
+constexpr int kHalves = kTileRows / 16;
 constexpr int kPlanThreads = 512, kPlanWaves = kPlanThreads / 64;
 
 // Exclusive sums of v[0 .. n) in LDS (n at most 1026), in place; v[n] becomes the total.
@@ -89,14 +90,14 @@ plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__
     int n = 0;
     for (int w = 0; w < kPlanWaves; ++w) n += count[w * segs + s];
     total[s] = n;
-    tile0[s] = (n + l.align - 1) / l.align;
-    chunk0[s] = (n + l.chunk_rows - 1) / l.chunk_rows;
+    tile0[s] = (n + kTileRows - 1) / kTileRows;
+    chunk0[s] = (n + kChunkRows - 1) / kChunkRows;
   }
   __syncthreads();
   scan_ints(tile0, segs, wave_sum);
   scan_ints(chunk0, segs, wave_sum);
   for (int s = t; s < segs; s += kPlanThreads) {
-    int at = tile0[s] * l.align;
+    int at = tile0[s] * kTileRows;
     for (int w = 0; w < kPlanWaves; ++w) {
       const int n = count[w * segs + s];
       count[w * segs + s] = at;
@@ -110,15 +111,15 @@ plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__
   for (int i = t; i < l.chunks; i += kPlanThreads) {
     int4 c = make_int4(-1, 0, 0, 0);  // adapter, first position, rows, none
     if (i < chunk0[segs]) {
-      const int s = segment_of(chunk0, segs, i), at = (i - chunk0[s]) * l.chunk_rows;
-      c = make_int4(s, tile0[s] * l.align + at, min(l.chunk_rows, total[s] - at), 0);
+      const int s = segment_of(chunk0, segs, i), at = (i - chunk0[s]) * kChunkRows;
+      c = make_int4(s, tile0[s] * kTileRows + at, min(kChunkRows, total[s] - at), 0);
     }
     *(int4*)(plan + l.chunk + 4 * i) = c;
   }
   for (int i = t; i < l.positions; i += kPlanThreads) {  // positions without a row
-    const int tile = i / l.align;
+    const int tile = i / kTileRows;
     const int s = tile < tile0[segs] ? segment_of(tile0, segs, tile) : -1;
-    if (s < 0 || i - tile0[s] * l.align >= total[s]) plan[l.order + i] = -1;
+    if (s < 0 || i - tile0[s] * kTileRows >= total[s]) plan[l.order + i] = -1;
   }
   __syncthreads();
   for (int first = from; first < to; first += 64) {
@@ -139,11 +140,15 @@ plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__
   }
 }
 
-// Rows' products with A: a tile's RT * 16 positions, a part of the reduced axis, of which each wave takes a part of its own, 64 columns a step.
-template <bool BF, int RT, int NT, bool DROP, bool AGAIN>
+// Rows' products with A (or gradients' with B): a tile's positions and a part of the reduced axis, of which
+// each wave takes a part of its own, 64 columns a step.  What bounds it is the rows, read once (nontemporal,
+// whole lines); A stays in the XCD's L2, and neighbouring items share it.  Two steps' loads are in flight
+// where the registers allow it.  10175 rows of 11008 against rank 16: 42 us for 224 MB, 5.3 TB/s; 1 row of
+// 4096 3.8 us, a launch and two trips to memory.
+template <bool BF, int NT, bool DROP>
 __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int splits) {
   constexpr int kAhead = NT <= 2 ? 2 : 1;  // steps whose loads are in flight together
-  __shared__ __attribute__((aligned(16))) float red[4][RT * 16][20];
+  __shared__ __attribute__((aligned(16))) float red[4][kTileRows][20];
   __shared__ u4 lines[4][128];
   const int item = item_of_xcd(blockIdx.x, p.plan[0] * splits);
   if (item < 0) return;
@@ -151,11 +156,11 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
   const int ad = p.plan[p.l.tile_adapter + tile];
   if (ad >= p.adapters) return;
   const int lane = threadIdx.x & 63, wave = wave_index(), g = lane >> 4, c = lane & 15, unit = lane & 7, line = lane >> 3;
-  const int32_t* order = p.plan + p.l.order + (int64_t)tile * (RT * 16);
-  const uint16_t* xr[RT][2];
-  int row[RT][2];
+  const int32_t* order = p.plan + p.l.order + (int64_t)tile * kTileRows;
+  const uint16_t* xr[kHalves][2];
+  int row[kHalves][2];
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+  for (int t = 0; t < kHalves; ++t)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       row[t][i] = max(order[t * 16 + 8 * i + line], 0);
@@ -167,20 +172,20 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
 #pragma unroll
     for (int i = 0; i < 2; ++i) ar[t][i] = p.weights + ((int64_t)ad * p.r + min(t * 16 + 8 * i + line, p.r - 1)) * p.width;
   // a tile of few rows: its second half may hold none
-  const bool two = RT != 2 || __builtin_amdgcn_readfirstlane(order[16]) >= 0;
-  f4 acc[RT][NT] = {};
+  const bool two = __builtin_amdgcn_readfirstlane(order[16]) >= 0;
+  f4 acc[kHalves][NT] = {};
   const Philox philox(DROP ? p.seed : reinterpret_cast<const int64_t*>(p.plan));
   const int steps = (p.width + 63) / 64, parts = splits * 4, part = split * 4 + wave;
   const int s0 = (int)((int64_t)steps * part / parts), s1 = (int)((int64_t)steps * (part + 1) / parts);
   struct Step {
-    u4 x[RT][2], a[NT][2];
+    u4 x[kHalves][2], a[NT][2];
   };
   auto load = [&](int at, Step& v) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
-        if (t == 0 || two) v.x[t][i] = AGAIN ? *(const u4*)(xr[t][i] + at) : stream_load(xr[t][i] + at);
+      for (int t = 0; t < kHalves; ++t)
+        if (t == 0 || two) v.x[t][i] = stream_load(xr[t][i] + at);
 #pragma unroll
       for (int t = 0; t < NT; ++t) v.a[t][i] = *(const u4*)(ar[t][i] + at);
     }
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
 #pragma unroll
     for (int t = 0; t < NT; ++t) to_operands(v.a[t][0], v.a[t][1], lines[wave]);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
+    for (int t = 0; t < kHalves; ++t) {
       if (t > 0 && !two) break;
       if constexpr (DROP) {
 #pragma unroll
@@ -219,15 +224,15 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int spli
     if (!in) v = Step{};
     multiply(s, v);
   }
-  float* plane = p.planes + ((int64_t)split * p.l.positions + (int64_t)tile * (RT * 16)) * p.r;
+  float* plane = p.planes + ((int64_t)split * p.l.positions + (int64_t)tile * kTileRows) * p.r;
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     if (u) __syncthreads();
 #pragma unroll
-    for (int t = 0; t < RT; ++t) *(f4*)&red[wave][t * 16 + c][4 * g] = acc[t][u];
+    for (int t = 0; t < kHalves; ++t) *(f4*)&red[wave][t * 16 + c][4 * g] = acc[t][u];
     __syncthreads();
     const int i = threadIdx.x >> 2, q = (threadIdx.x & 3) * 4;
-    if (i < RT * 16 && u * 16 + q < p.r) {
+    if (i < kTileRows && u * 16 + q < p.r) {
       f4 v = *(const f4*)&red[0][i][q];
 #pragma unroll
       for (int w = 1; w < 4; ++w) v += *(const f4*)&red[w][i][q];
@@ -251,14 +256,15 @@ __device__ __forceinline__ f4 sum_planes(const float* at, int64_t plane, int spl
   return v;
 }
 
-// 32 positions' h (or dh): planes summed, times s_a / kept share, packed by row and by column.
+// 32 positions' h (or dh): planes summed in order, times s_a / kept share, packed by row and by column.  Bound
+// by its launch and the trip to the planes: 5325 rows of rank 16 4.2 us, 1762 of rank 64 4.9.
 template <bool BF, int NT>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(AdapterArgs p, const float* planes, int splits, AdapterPacks packs) {
   constexpr int kR = NT * 16;
   __shared__ float v[32][kR + 1];
   __shared__ int exps[32];
   const int64_t first = (int64_t)blockIdx.x * 32;
-  const int ad = p.plan[p.l.tile_adapter + first / p.l.align];
+  const int ad = p.plan[p.l.tile_adapter + first / kTileRows];
   if (ad < 0 || ad >= p.adapters) return;
   const float scale = p.scaling[ad] * p.keep_scale;
   for (int i = threadIdx.x; i < 32 * (kR / 4); i += kJoinThreads) {
@@ -316,43 +322,44 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AdapterArgs p, const
   }
 }
 
-// The products with B, added to the projection's output: a tile's rows, a part of the columns.  JOIN: the workgroup sums the planes itself (few rows: one launch
-// less); else the packed rows are read.
-template <bool BF, int RT, int NT, bool JOIN>
+// The products with B, added in 32 bits to the projection's output: a tile's rows, a part of the columns, of
+// which each wave takes every fourth group of 64.  h goes in as two 16-bit parts, so that nothing but the
+// result is rounded to 16 bits.  Bound by the output, read and written once as whole lines: 10175 rows of
+// 4096 by rank 16 40 us for 169 MB, 4.2 TB/s, with the sum of the planes (JOIN); rank 64 by 11008 is bound
+// by B's way from the L2 to every tile (1762 rows 30 us for 91 MB).
+template <bool BF, int NT, bool JOIN>
 __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int splits, AdapterPacks packs, int wide) {
-  constexpr int kRows = RT * 16, kR = NT * 16, kPitch = kR + 8, kJ = NT == 1 ? 1 : NT / 2;
+  constexpr int kR = NT * 16, kPitch = kR + 8, kJ = NT == 1 ? 1 : NT / 2;
   const int item = item_of_xcd(blockIdx.x, p.plan[0] * wide);
   if (item < 0) return;
   const int tile = item / wide, column_part = item - tile * wide;
   const int ad = p.plan[p.l.tile_adapter + tile];
   const int lane = threadIdx.x & 63, wave = wave_index(), g = lane >> 4, c = lane & 15;
-  const int32_t* order = p.plan + p.l.order + (int64_t)tile * kRows;
+  const int32_t* order = p.plan + p.l.order + (int64_t)tile * kTileRows;
   const int groups = (p.n + 63) / 64;
   const int g0 = (int)((int64_t)groups * column_part / wide), g1 = (int)((int64_t)groups * (column_part + 1) / wide);
   if (ad >= p.adapters) {  // rows without an adapter keep the projection's output
     if (p.out == p.base) return;
     const int units = min(g1 * 8, p.n / 8) - g0 * 8;
-    for (int i = 0; i < kRows; ++i) {
-      const int row = order[i];
-      if (row < 0) break;
-      for (int u = threadIdx.x; u < units; u += kThreads)
-        *(u4*)(p.out + row * p.ldo + (g0 * 8 + u) * 8) = *(const u4*)(p.base + row * p.ldb + (g0 * 8 + u) * 8);
+    for (int i = threadIdx.x; i < kTileRows * units; i += kThreads) {
+      const int row = order[i / units], at = (g0 * 8 + i % units) * 8;
+      if (row >= 0) *(u4*)(p.out + row * p.ldo + at) = stream_load(p.base + row * p.ldb + at);
     }
     return;
   }
   // rank 16: both parts in one instruction, the second in the reduction's upper half
-  u4 hv[RT][kJ], lv[RT][kJ];
-  float back[RT];
+  u4 hv[kHalves][kJ], lv[kHalves][kJ];
+  float back[kHalves];
   if constexpr (JOIN) {
-    __shared__ __attribute__((aligned(16))) uint16_t part[2][kRows][kPitch];
-    __shared__ int back_s[kRows];
+    __shared__ __attribute__((aligned(16))) uint16_t part[2][kTileRows][kPitch];
+    __shared__ int back_s[kTileRows];
     const float scale = p.scaling[ad] * p.keep_scale;
     const float* planes = reinterpret_cast<const float*>(p.ws);
-    for (int i = threadIdx.x; i < kRows * NT * 4; i += kThreads) {
+    for (int i = threadIdx.x; i < kTileRows * NT * 4; i += kThreads) {
       const int at = i / (NT * 4), q = i % (NT * 4) * 4;
       f4 v = {};
       if (q < p.r && order[at] >= 0)
-        v = sum_planes(planes + ((int64_t)tile * kRows + at) * p.r + q, p.l.positions * p.r, splits) * scale;
+        v = sum_planes(planes + ((int64_t)tile * kTileRows + at) * p.r + q, p.l.positions * p.r, splits) * scale;
       if constexpr (!BF) {
         float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
@@ -370,7 +377,7 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
     }
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
+    for (int t = 0; t < kHalves; ++t) {
       if constexpr (!BF) back[t] = pow2(back_s[t * 16 + c]);
 #pragma unroll
       for (int j = 0; j < kJ; ++j) {
@@ -382,8 +389,8 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
   } else {
     const int64_t half = p.l.positions * kR;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int64_t pos = (int64_t)tile * kRows + t * 16 + c;
+    for (int t = 0; t < kHalves; ++t) {
+      const int64_t pos = (int64_t)tile * kTileRows + t * 16 + c;
       if constexpr (!BF) back[t] = pow2(packs.row_exp[pos]);
 #pragma unroll
       for (int j = 0; j < kJ; ++j) {
@@ -394,23 +401,23 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
     }
   }
   // rows as loads and stores take them (to_operands())
-  int row[RT][2];
-  const uint16_t* from[RT][2];
+  int row[kHalves][2];
+  const uint16_t* from[kHalves][2];
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+  for (int t = 0; t < kHalves; ++t)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       row[t][i] = order[t * 16 + 8 * i + (lane >> 3)];
       from[t][i] = p.base + max(row[t][i], 0) * p.ldb;
     }
   // a tile of few rows: its second half may hold none
-  const bool two = RT != 2 || __builtin_amdgcn_readfirstlane(order[16]) >= 0;
+  const bool two = __builtin_amdgcn_readfirstlane(order[16]) >= 0;
   const int unit = lane & 7;
   __shared__ __attribute__((aligned(16))) float sums[4][16 * 68];
   float* const own = sums[wave];
   const uint16_t* const bw = p.b + (int64_t)ad * p.n * p.r;
   struct Group {
-    u4 y[RT][2], b[4][kJ];
+    u4 y[kHalves][2], b[4][kJ];
   };
   // the lane's eight columns of unit g (operands 0 and 1) and of unit 4 + g (2 and 3)
   auto load = [&](int grp, Group& v) {
@@ -425,7 +432,7 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
       }
     }
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+    for (int t = 0; t < kHalves; ++t)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (t == 0 || two) v.y[t][i] = stream_load(from[t][i] + (n < p.n ? n : 0));
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
       for (int j = 0; j < kJ; ++j)
         if ((NT == 1 ? (g & 1) * 8 : 32 * j + 8 * g) >= p.r) v.b[u][j] = u4{};
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
+    for (int t = 0; t < kHalves; ++t) {
       if (t > 0 && !two) break;
       f4 acc[4] = {};
 #pragma unroll
@@ -475,7 +482,9 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
   }
 }
 
-// y = x of the kept elements times keep_scale: eight elements a thread.
+// y = x of the kept elements times keep_scale: eight elements a thread, one counter.  9001 rows of 4096 (bf16)
+// 27.2 us for 147 MB, 5.4 TB/s; the counter's ten rounds take 54 % of the vector units' time and hide
+// behind the loads.
 template <bool BF, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 dropout_kernel(int rows, int cols, const uint16_t* __restrict__ x, int64_t ldx, uint16_t* __restrict__ y, int64_t ldy, int drop,
@@ -509,31 +518,29 @@ dropout_kernel(int rows, int cols, const uint16_t* __restrict__ x, int64_t ldx, 
   }
 }
 
-template <bool BF, int RT, int NT>
+template <bool BF, int NT>
 void shrink_of(const ShrinkArgs& a, int splits, hipStream_t stream) {
   const unsigned grid = (unsigned)a.l.tiles * splits;
-  if (a.again) shrink_kernel<BF, RT, NT, false, true><<<grid, kThreads, 0, stream>>>(a, splits);
-  else if (a.drop) shrink_kernel<BF, RT, NT, true, false><<<grid, kThreads, 0, stream>>>(a, splits);
-  else shrink_kernel<BF, RT, NT, false, false><<<grid, kThreads, 0, stream>>>(a, splits);
+  if (a.drop) shrink_kernel<BF, NT, true><<<grid, kThreads, 0, stream>>>(a, splits);
+  else shrink_kernel<BF, NT, false><<<grid, kThreads, 0, stream>>>(a, splits);
 }
-template <bool BF, int RT>
+template <bool BF>
 void shrink_rank(const ShrinkArgs& a, int splits, hipStream_t stream) {
-  if (a.r <= 16) shrink_of<BF, RT, 1>(a, splits, stream);
-  else if (a.r <= 32) shrink_of<BF, RT, 2>(a, splits, stream);
-  else if (a.r <= 64) shrink_of<BF, RT, 4>(a, splits, stream);
-  else shrink_of<BF, RT, 8>(a, splits, stream);
+  if (a.r <= 16) shrink_of<BF, 1>(a, splits, stream);
+  else if (a.r <= 32) shrink_of<BF, 2>(a, splits, stream);
+  else if (a.r <= 64) shrink_of<BF, 4>(a, splits, stream);
+  else shrink_of<BF, 8>(a, splits, stream);
 }
 
 template <bool BF, int NT>
 void expand_of(const AdapterArgs& a, int splits, bool join, const AdapterPacks& packs, hipStream_t stream) {
   const int groups = (a.n + 63) / 64;
-  // (up to two workgroups per CU with four waves each: more read the packed rows too often; half as many
-  // left 54 us of 46 at 10175 rows)
-  const int wide = std::max(1, std::min((groups + 3) / 4, (a.l.align == 32 ? 1024 : 512) / a.l.tiles));
+  // About four workgroups per CU of four waves each.  Half as many: 10175 rows against rank 16 76 us for 40;
+  // twice as many 39.6, but each sums the planes anew.
+  const int wide = std::max(1, std::min((groups + 3) / 4, 1024 / a.l.tiles));
   const unsigned grid = (unsigned)a.l.tiles * wide;
-  if (a.l.align == 64) expand_kernel<BF, 4, NT, false><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
-  else if (join) expand_kernel<BF, 2, NT, true><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
-  else expand_kernel<BF, 2, NT, false><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
+  if (join) expand_kernel<BF, NT, true><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
+  else expand_kernel<BF, NT, false><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
 }
 template <bool BF>
 void expand_rank(const AdapterArgs& a, int splits, bool join, const AdapterPacks& packs, hipStream_t stream) {
@@ -548,7 +555,7 @@ void expand_rank(const AdapterArgs& a, int splits, bool join, const AdapterPacks
 int adapter_splits(const AdapterLayout& l, int width, int cus) {
   // about four workgroups per CU, parts of at least 64 values per wave
   const int want = (4 * cus + l.tiles - 1) / l.tiles;
-  return std::max(1, std::min({want, width / 256, l.align == 32 ? 16 : 8}));
+  return std::max(1, std::min({want, width / 256, 16}));
 }
 
 hipError_t launch_adapter_plan(const AdapterLayout& l, int rows, int adapters, const int32_t* index, int32_t* plan,
@@ -559,8 +566,7 @@ hipError_t launch_adapter_plan(const AdapterLayout& l, int rows, int adapters, c
 }
 
 hipError_t launch_shrink(bool bf16, const ShrinkArgs& a, int splits, hipStream_t stream) {
-  if (a.l.align == 32) bf16 ? shrink_rank<true, 2>(a, splits, stream) : shrink_rank<false, 2>(a, splits, stream);
-  else bf16 ? shrink_rank<true, 4>(a, splits, stream) : shrink_rank<false, 4>(a, splits, stream);
+  bf16 ? shrink_rank<true>(a, splits, stream) : shrink_rank<false>(a, splits, stream);
   return hipGetLastError();
 }
 
@@ -578,15 +584,17 @@ hipError_t launch_join(const AdapterArgs& a, const float* planes, int splits, co
 
 hipError_t launch_adapters(const AdapterArgs& a, const ForwardWs& w, hipStream_t stream) {
   float* const planes = reinterpret_cast<float*>(a.ws);
-  const ShrinkArgs s = {a.l, a.plan, a.x, a.ldx, a.a, a.k, a.r, a.adapters, a.drop, a.seed, planes, false};
+  const ShrinkArgs s = {a.l, a.plan, a.x, a.ldx, a.a, a.k, a.r, a.adapters, a.drop, a.seed, planes};
   hipError_t e = launch_shrink(a.bf16, s, w.splits, stream);
   if (e != hipSuccess) return e;
-  // a batch of few rows whose h nobody keeps: the second launch joins the planes itself
-  const bool join = a.l.align == 32 && a.h == nullptr;
+  // Where nobody keeps h the second launch joins the planes itself: 10175 rows of 11008 against rank 16 in two
+  // launches 82.7 us, 87.2 in three.  Where h is kept, join_kernel packs it for the products with g as well,
+  // and the second launch reads its rows: 5325 rows, rank 16 19.5 us that way, 21.4 by the planes.
+  const bool join = a.h == nullptr;
   AdapterPacks packs = {};
-  place_row(packs, a.l, a.r, a.ws + w.row);
+  if (!join) place_row(packs, a.l, a.r, a.ws + w.row);
   if (a.h != nullptr) place_col(packs, a.l, a.r, a.h);
-  if (!join && (e = launch_join(a, planes, w.splits, packs, stream)) != hipSuccess) return e;
+  if (a.h && (e = launch_join(a, planes, w.splits, packs, stream)) != hipSuccess) return e;
   a.bf16 ? expand_rank<true>(a, w.splits, join, packs, stream) : expand_rank<false>(a, w.splits, join, packs, stream);
   return hipGetLastError();
 }

@@ -358,7 +358,7 @@ hipError_t launch_grad(const AdapterArgs& a, const BackwardWs& w, hipStream_t st
     hipError_t e;
     if (a.adapters > 0) {
       float* const planes = reinterpret_cast<float*>(a.ws);
-      const ShrinkArgs s = {a.l, a.plan, a.g, a.ldg, bt, a.n, a.r, a.adapters, 0, nullptr, planes, false};
+      const ShrinkArgs s = {a.l, a.plan, a.g, a.ldg, bt, a.n, a.r, a.adapters, 0, nullptr, planes};
       if ((e = launch_shrink(a.bf16, s, w.splits, stream)) != hipSuccess) return e;
       if (a.dx != nullptr) place_row(packs, a.l, a.r, a.ws + w.row);
       if (a.da != nullptr) place_col(packs, a.l, a.r, a.ws + w.col);

@@ -263,7 +263,12 @@ hipError_t launch_cache(const RotaryArgs& a, hipStream_t stream) {
   const int each = heads_each(a, a.heads, 4096);
   const int64_t q_blocks = ((int64_t)a.rows * host_units(a) + kThreads - 1) / kThreads;
   const int q_groups = (a.heads + each - 1) / each;
-  const int tile = a.rows < 2048 ? 8 : a.head_size > 256 ? kTile / 2 : kTile;  // (LDS: 37 KiB at heads of 256)
+  // Tiles of 32 rows write whole lines of the value cache; of 8 where those would leave fewer than two
+  // workgroups per CU.  Measured, heads of 128: 48 rows of 8 kv heads 5.3 us by 8 and 8.3 by 32, 1024 of 8
+  // 11.1 and 11.6, 512 of 32 12.3 and 11.4, 2048 of 8 16.6 and 14.1, 4096 of 32 66.5 and 45.9.  Heads above
+  // 256 halve the tile: LDS, 37 KiB at heads of 256.
+  const bool few = (int64_t)a.rows / kTile * a.kv_heads < 512;
+  const int tile = few ? kTile / 4 : a.head_size > 256 ? kTile / 2 : kTile;
   const int64_t kv = (int64_t)((a.rows + tile - 1) / tile) * a.kv_heads;
   const size_t smem = 2 * ((size_t)tile * (a.head_size + 8) + (size_t)(tile + kHalo) * (a.head_size + 2));
   rotary_cache_kernel<BF, VEC, IL><<<(unsigned)(q_blocks * q_groups + kv), kThreads, smem, stream>>>(a, each, q_groups, (int)q_blocks, tile);

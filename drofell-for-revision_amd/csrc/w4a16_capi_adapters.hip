@@ -88,8 +88,8 @@ int check_rotary(int dtype, int rows, int heads, int kv_heads, int head_size, in
       !std::isfinite(magnitude))
     return DW4_ERR_INVALID_ARG;
   if (head_size % 8 != 0 || head_size > 512 || rotary_size % 2 != 0) return DW4_ERR_UNSUPPORTED;
-  // workgroups are counted in 32 bits
-  if (rows > 1 << 24 || heads > 1 << 14 || kv_heads > 1 << 14 || (int64_t)rows * (heads + kv_heads) > (int64_t)1 << 28)
+  // a launch counts its threads in 32 bits, up to one a dim of every row
+  if (rows > 1 << 22 || heads > 1 << 14 || kv_heads > 1 << 14 || (int64_t)rows * (heads + kv_heads) > (int64_t)1 << 27)
     return DW4_ERR_UNSUPPORTED;
   return DW4_OK;
 }
@@ -187,6 +187,7 @@ int dw4_dropout(int dtype, int num_rows, int cols, const uint16_t* x, int64_t ld
                 const int64_t* seed, void* stream) {
   if (!good_dtype(dtype)) return DW4_ERR_UNSUPPORTED;
   if (num_rows < 0 || cols < 0 || seed == nullptr) return DW4_ERR_INVALID_ARG;
+  if (cols > 1 << 30) return DW4_ERR_UNSUPPORTED;
   DW4_TRY(check_drop(drop, seed));
   if (num_rows == 0 || cols == 0) return DW4_OK;
   if (x == nullptr || y == nullptr || (num_rows > 1 && (ldx < cols || ldy < cols))) return DW4_ERR_INVALID_ARG;

@@ -166,8 +166,8 @@ class BlockPool:
         mapped.  Up to 8192 rows."""
         rows, width = self._check(state)
         n, tokens = self._by_row(new_tokens, rows, "new_tokens"), int(tokens)
-        if tokens < 0:
-            raise ValueError("tokens must not be negative")
+        if not 0 <= tokens <= 1 << 28:
+            raise ValueError("tokens lies between 0 and 2^28")
         ints = n.new_empty(rows + 2 + 2 * tokens)
         excess, starts, positions, row_of = torch.split_with_sizes(ints, (1, rows + 1, tokens, tokens))
         slots = n.new_empty(tokens, dtype=torch.int64)

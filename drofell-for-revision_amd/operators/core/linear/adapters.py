@@ -76,6 +76,8 @@ class AdapterRows:
     def __init__(self, adapters: torch.Tensor, num_adapters: int) -> None:
         if adapters.dim() != 1:
             raise ValueError("adapters must hold one integer per row")
+        if adapters.shape[0] > 1 << 24 or not 0 <= num_adapters <= 1024:
+            raise ValueError("a batch has up to 2^24 rows and 1024 adapters")
         self.num_rows, self.num_adapters, self.device = adapters.shape[0], int(num_adapters), adapters.device
         with _lib.on_device(self.device):
             self.plan = torch.empty(_lib.adapter_plan_size(self.num_rows, self.num_adapters) // 4, dtype=torch.int32,
@@ -105,8 +107,8 @@ class LowRankAdapters(nn.Module):
             raise TypeError("adapters are fp16 or bf16")
         if rank < 8 or rank % 8 or rank > 128:
             raise ValueError("the rank must be a multiple of 8 up to 128")
-        if in_features < 8 or in_features % 8 or out_features < 8 or out_features % 8:
-            raise ValueError("in_features and out_features must be multiples of 8")
+        if any(width < 8 or width % 8 or width > 1 << 20 for width in (in_features, out_features)):
+            raise ValueError("in_features and out_features must be multiples of 8 up to 2^20")
         if not 0 < num_adapters <= 1024:
             raise ValueError("there are 1 to 1024 adapters")
         self.in_features, self.out_features, self.rank, self.num_adapters = in_features, out_features, rank, num_adapters
@@ -141,7 +143,10 @@ class LowRankAdapters(nn.Module):
         seed.  Differentiable (once) in x, base, ``a`` and ``b``.  ``output``, without gradients:
         where the result goes, which may be ``base``."""
         params = self._parameters  # (attribute look-up on a module takes 0.4 us each)
-        a, b, scaling = params["a"], params["b"], self._buffers["scaling"]
+        try:
+            a, b, scaling = params["a"], params["b"], self._buffers["scaling"]
+        except KeyError:  # (parametrized)
+            a, b, scaling = self.a, self.b, self.scaling
         device, dtype = x.device, x.dtype
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         base2 = base if base.dim() == 2 else base.reshape(-1, base.shape[-1])
@@ -256,7 +261,8 @@ class AdaptedLinear(Linear):
         bank = self.adapters
         if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or bank.a.requires_grad or bank.b.requires_grad):
             return bank(x, y, rows, seed)
-        return bank(x, y, rows, seed, output=y if y.is_contiguous() and y.data_ptr() % 16 == 0 else None)
+        own = y.is_contiguous() and y.data_ptr() % 16 == 0 and y.data_ptr() != x.data_ptr()
+        return bank(x, y, rows, seed, output=y if own else None)
 
 
 class CounterDropout(nn.Module):
@@ -274,8 +280,8 @@ class CounterDropout(nn.Module):
         In evaluation mode, or with p 0, x itself."""
         if x.dtype not in _DTYPES:
             raise TypeError("dropout runs on fp16 or bf16")
-        if x.dim() < 1:
-            raise ValueError("x must have columns")
+        if x.dim() < 1 or x.shape[-1] > 1 << 30 or x.numel() >= x.shape[-1] << 31 > 0:
+            raise ValueError("x must have columns, up to 2^30, and fewer than 2^31 rows of them")
         if not self.training or self._dropped == 0:
             return x
         return _Dropout.apply(x, _seed(seed, x.device), self._dropped)

@@ -87,6 +87,8 @@ class RotaryEmbedding:
                 raise ValueError(f"q, k and v must be on {self.device}")
         if dtype not in _DTYPES:
             raise TypeError("rotary positions run on fp16 or bf16")
+        if count > 1 << 22 or rows[0].shape[1] > 1 << 14 or rows[1].shape[1] > 1 << 14:
+            raise ValueError("a call turns up to 2^22 rows and 2^14 heads")
         return count
 
     def _positions(self, positions: torch.Tensor, rows: int) -> torch.Tensor:

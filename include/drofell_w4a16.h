@@ -680,7 +680,8 @@ int dw4_adapters_backward(int dtype, int num_rows, int num_adapters, int k, int 
  * Philox 4x32 (10 rounds) are at least drop (0 .. 65536): the counter's words are col / 8,
  * row and the two halves of seed[1], the key's those of seed[0] (int64 device [2]), and of the
  * four words of output the element has half col % 8, low halves first.  The gradient is the
- * same call on the output's gradient.  Rows of any width, stride and alignment; y may be x. */
+ * same call on the output's gradient.  Rows of any stride and alignment, up to 2^30 wide; y may
+ * be x. */
 int dw4_dropout(int dtype, int num_rows, int cols, const uint16_t* x, int64_t ldx, uint16_t* y,
                 int64_t ldy, int drop, const int64_t* seed, void* stream);
 
@@ -693,7 +694,8 @@ int dw4_dropout(int dtype, int num_rows, int cols, const uint16_t* x, int64_t ld
  * Beside dw4_rope (fp16 tables, half layout, in place).  q [num_rows][num_heads]
  * [head_size], k (and v) [num_rows][num_kv_heads][head_size] with row strides
  * (multiples of 8), 16-byte aligned; head_size a multiple of 8 up to 512, rotary_size
- * even.  inverse: turned back, which is the gradient.  Outputs may be the inputs.
+ * even; num_rows at most 2^22, num_rows * (num_heads + num_kv_heads) at most 2^27.  inverse:
+ * turned back, which is the gradient.  Outputs may be the inputs.
  * ------------------------------------------------------------------------- */
 int dw4_rotary(int dtype, int num_rows, int num_heads, int num_kv_heads, int head_size,
                int rotary_size, int interleaved, int inverse, const uint16_t* q, int64_t q_stride,

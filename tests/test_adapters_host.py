@@ -9,7 +9,8 @@ import pytest
 import torch
 
 from hip_extends import _lib
-from operators.core.linear.adapters import CounterDropout, LowRankAdapters
+from operators.core.linear.adapters import AdaptedLinear, AdapterRows, CounterDropout, LowRankAdapters
+from operators.core.linear.real import Linear
 from operators.core.rope.common import RotaryScaling, rotary_frequencies
 from operators.core.rope.real import RotaryEmbedding
 from oracle import adapters as O
@@ -175,3 +176,46 @@ def test_oracles_agree_with_autograd():
     assert y.shape == (3, 2, 8) and torch.isfinite(back).all()
     assert B.slots([[4, -1]], [20], [0] * 9, [6], 8, 16) == ([0, 6], [14, 15, 16, 17, 18, 19, 0, 0], [78, 79, -1, -1, -1, -1, -1, -1],
                                                             [0] * 6 + [-1] * 2, 0)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Sizes that a 32-bit argument would wrap around to small ones."""
+    one = torch.zeros(1, dtype=torch.int32)
+    for rows, count in (((1 << 24) + 1, 4), ((1 << 32) + 5, 4), (9, 1025), (9, -1)):
+        with pytest.raises(ValueError):
+            AdapterRows(one.expand(rows), count)
+    for kwargs in (dict(in_features=(1 << 20) + 8), dict(out_features=(1 << 32) + 8)):
+        with pytest.raises(ValueError):
+            LowRankAdapters(**{**dict(in_features=64, out_features=64, rank=8, num_adapters=2), **kwargs})
+    x, seed = torch.zeros(1, dtype=torch.float16), torch.zeros(2, dtype=torch.int64)
+    for shape in (((1 << 32) + 8,), (3, (1 << 30) + 1), ((1 << 31), 1), ((1 << 32) + 1, 8)):
+        with pytest.raises(ValueError):
+            CounterDropout(0.5)(x.expand(shape), seed)
+    call = _lib.load().dw4_dropout
+    assert call(0, 1, (1 << 30) + 1, FAKE, 1 << 31, FAKE, 1 << 31, 5, FAKE, None) == UNSUP
+    for test in (rotary, cached):
+        assert test(rows=(1 << 22) + 1) == UNSUP and test(rows=1 << 22, heads=32, qs=2048, qos=2048) == UNSUP
+
+
+class _Passes(Linear):
+    def __init__(self):
+        torch.nn.Module.__init__(self)
+
+    def forward(self, x):
+        return x
+
+
+def test_a_projection_that_returns_its_input_keeps_it():
+    """The adapters' sum goes into the projection's output unless that is the caller's input."""
+    seen = []
+
+    class Bank(torch.nn.Module):
+        a = b = torch.zeros(1)
+
+        def forward(self, x, y, rows, seed=None, output=None):
+            seen.append(output)
+            return y
+
+    x = torch.zeros(4, 64, dtype=torch.float16)
+    AdaptedLinear(_Passes(), Bank())(x, rows=object())
+    assert seen == [None]

@@ -107,7 +107,9 @@ struct ForwardWs {
   size_t row, bytes;  // behind the planes [splits][positions][r]
 };
 inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-inline size_t plane_bytes(const AdapterLayout& l, int splits, int r) { return up256(sizeof(float) * splits * (size_t)l.positions * r); }
+inline size_t plane_bytes(const AdapterLayout& l, int splits, int r) {
+  return up256(sizeof(float) * splits * (size_t)l.positions * r);
+}
 inline ForwardWs forward_ws(const AdapterLayout& l, int k, int r, int cus) {
   ForwardWs w;
   w.splits = adapter_splits(l, k, cus);

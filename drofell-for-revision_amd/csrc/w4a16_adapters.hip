@@ -65,7 +65,9 @@ __device__ __forceinline__ int segment_of(const int* start, int n, int t) {
 }
 
 // One workgroup: rows counted by adapter (each wave a run of them), the adapters'
-// first tiles and chunks by a scan, then each row to its place, in order within its adapter.
+// first tiles and chunks by a scan, then each row to its place, in order within its adapter.  Bound by
+// one CU's passes over the rows' numbers: 1 row 4.8 us, 5325 rows 15, 10175 rows 27, once per batch for
+// all projections of all layers.
 __global__ void __launch_bounds__(kPlanThreads)
 plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__ index, int32_t* __restrict__ plan) {
   extern __shared__ int sm[];
@@ -143,7 +145,7 @@ plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__
 // Rows' products with A (or gradients' with B): a tile's positions and a part of the reduced axis, of which
 // each wave takes a part of its own, 64 columns a step.  What bounds it is the rows, read once (nontemporal,
 // whole lines); A stays in the XCD's L2, and neighbouring items share it.  Two steps' loads are in flight
-// where the registers allow it.  10175 rows of 11008 against rank 16: 42 us for 224 MB, 5.3 TB/s; 1 row of
+// where the registers allow it.  10175 rows of 11008 against rank 16: 42 us for 222 MB, 5.3 TB/s; 1 row of
 // 4096 3.8 us, a launch and two trips to memory.
 template <bool BF, int NT, bool DROP>
 __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs p, int splits) {
@@ -257,9 +259,10 @@ __device__ __forceinline__ f4 sum_planes(const float* at, int64_t plane, int spl
 }
 
 // 32 positions' h (or dh): planes summed in order, times s_a / kept share, packed by row and by column.  Bound
-// by its launch and the trip to the planes: 5325 rows of rank 16 4.2 us, 1762 of rank 64 4.9.
+// by its launch and the trip to the planes: 5325 rows of rank 16 4.2 us, 1763 of rank 64 4.9.
 template <bool BF, int NT>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(AdapterArgs p, const float* planes, int splits, AdapterPacks packs) {
+__global__ void __launch_bounds__(kJoinThreads)
+join_kernel(AdapterArgs p, const float* planes, int splits, AdapterPacks packs) {
   constexpr int kR = NT * 16;
   __shared__ float v[32][kR + 1];
   __shared__ int exps[32];
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AdapterArgs p, const
 // which each wave takes every fourth group of 64.  h goes in as two 16-bit parts, so that nothing but the
 // result is rounded to 16 bits.  Bound by the output, read and written once as whole lines: 10175 rows of
 // 4096 by rank 16 40 us for 169 MB, 4.2 TB/s, with the sum of the planes (JOIN); rank 64 by 11008 is bound
-// by B's way from the L2 to every tile (1762 rows 30 us for 91 MB).
+// by B's way from the L2 to every tile (1763 rows 30 us for 91 MB).
 template <bool BF, int NT, bool JOIN>
 __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int splits, AdapterPacks packs, int wide) {
   constexpr int kR = NT * 16, kPitch = kR + 8, kJ = NT == 1 ? 1 : NT / 2;
@@ -471,7 +474,8 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const f4& d = e < 2 ? lo : hi;
-          v.y[t][i][e] = pack16<BF>(unpack16<BF>(v.y[t][i][e], 0) + d[(e & 1) * 2], unpack16<BF>(v.y[t][i][e], 1) + d[(e & 1) * 2 + 1]);
+          const uint32_t y = v.y[t][i][e];
+          v.y[t][i][e] = pack16<BF>(unpack16<BF>(y, 0) + d[(e & 1) * 2], unpack16<BF>(y, 1) + d[(e & 1) * 2 + 1]);
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -507,7 +511,8 @@ dropout_kernel(int rows, int cols, const uint16_t* __restrict__ x, int64_t ldx, 
         if (e < n) v[e >> 1] |= (uint32_t)xr[e] << (16 * (e & 1));
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = pack16<BF>(unpack16<BF>(v[e], 0) * keep_scale, unpack16<BF>(v[e], 1) * keep_scale) & m[e];
+    for (int e = 0; e < 4; ++e)
+      v[e] = pack16<BF>(unpack16<BF>(v[e], 0) * keep_scale, unpack16<BF>(v[e], 1) * keep_scale) & m[e];
     if constexpr (VEC) {
       *(u4*)yr = v;
     } else {

@@ -5,9 +5,12 @@
 // Five launches.  The weights are turned around, so that dh is the forward's first product
 // over g and B; beside that, in the same launch, g h^T, which needs neither.  Then dh, and dh x^T
 // with dx.  The sums over rows (outer()) come from tiles of 32 rows by 64 columns turned around by
-// way of LDS (rows as the matrix instruction's reduction), a chunk of 1024 rows of one adapter per
+// way of LDS (rows as the matrix instruction's reduction), a chunk of 512 rows of one adapter per
 // workgroup; dx comes from the same tile of x and its dropout mask.  The chunks' shares of
 // dA and dB are added up in order: no float atomics.
+//
+// Bound by memory: x, g and dx pass once, g a second time on its way to dh.  Chunks of 256 rows took longer
+// for their shares, chunks of 1024 left CUs idle; workgroups of eight waves were slower than of four.
 
 #include <hip/hip_runtime.h>
 
@@ -39,20 +42,23 @@ __device__ __forceinline__ u4 turned(const uint16_t* tile, int ct) {
 }
 
 // out[c][r] = in[r][c], 16-bit: 64 x 64 at a time.
-__device__ __forceinline__ void turn_tile(const uint16_t* in, uint16_t* out, int rows, int cols, int r0, int c0, uint16_t* tile) {
+__device__ __forceinline__ void turn_tile(const uint16_t* in, uint16_t* out, int rows, int cols, int r0, int c0,
+                                          uint16_t* tile) {
   constexpr int kPitch = 66, kRows = kOuterThreads / 32;
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
 #pragma unroll
   for (int i = 0; i < 64 / kRows; ++i) {
     const int r = r0 + y + kRows * i, c = c0 + 2 * x;
-    if (r < rows && c < cols) *(uint32_t*)(tile + (y + kRows * i) * kPitch + 2 * x) = *(const uint32_t*)(in + (int64_t)r * cols + c);
+    if (r < rows && c < cols)
+      *(uint32_t*)(tile + (y + kRows * i) * kPitch + 2 * x) = *(const uint32_t*)(in + (int64_t)r * cols + c);
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 64 / kRows; ++i) {
     const int c = c0 + y + kRows * i, r = r0 + 2 * x;
     if (c < cols && r < rows)
-      *(uint32_t*)(out + (int64_t)c * rows + r) = (uint32_t)tile[2 * x * kPitch + y + kRows * i] | (uint32_t)tile[(2 * x + 1) * kPitch + y + kRows * i] << 16;
+      *(uint32_t*)(out + (int64_t)c * rows + r) = (uint32_t)tile[2 * x * kPitch + y + kRows * i] |
+                                                  (uint32_t)tile[(2 * x + 1) * kPitch + y + kRows * i] << 16;
   }
 }
 
@@ -213,30 +219,30 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
       }
     }
     if (o.share != nullptr) {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    u4 xt[4];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      u4 xt[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) xt[t] = turned(tile, t);
+      for (int t = 0; t < 4; ++t) xt[t] = turned(tile, t);
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      if constexpr (BF) {
+      for (int u = 0; u < NT; ++u) {
+        if constexpr (BF) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          acc[t][u] = mfma16_of<BF>(xt[t], hi[u], acc[t][u]);
-          acc[t][u] = mfma16_of<BF>(xt[t], lo[u], acc[t][u]);
-        }
-      } else {
-        const float back = pow2(col_exp[u]);
+          for (int t = 0; t < 4; ++t) {
+            acc[t][u] = mfma16_of<BF>(xt[t], hi[u], acc[t][u]);
+            acc[t][u] = mfma16_of<BF>(xt[t], lo[u], acc[t][u]);
+          }
+        } else {
+          const float back = pow2(col_exp[u]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          f4 d = mfma16_of<BF>(xt[t], hi[u], f4{});
-          d = mfma16_of<BF>(xt[t], lo[u], d);
+          for (int t = 0; t < 4; ++t) {
+            f4 d = mfma16_of<BF>(xt[t], hi[u], f4{});
+            d = mfma16_of<BF>(xt[t], lo[u], d);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][u][i] = fmaf(d[i], back, acc[t][u][i]);
+            for (int i = 0; i < 4; ++i) acc[t][u][i] = fmaf(d[i], back, acc[t][u][i]);
+          }
         }
       }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -280,7 +286,8 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
   }
 }
 
-// The first launch of a backward pass: A [r][k] turned to [k][r] and B [n][r] to [r][n], and g h^T.
+// The first launch of a backward pass: A [r][k] turned to [k][r] and B [n][r] to [r][n], and g h^T.  5325 rows
+// of 4096 by rank 16 14.6 us for 51 MB (3.5 TB/s), 1763 of 11008 by rank 64 22.2 us for 63 MB (2.8 TB/s).
 template <bool BF, int NT>
 __global__ void __launch_bounds__(kOuterThreads)
 first_kernel(AdapterArgs p, OuterArgs o, uint16_t* at, uint16_t* bt, int a_tiles, int b_tiles) {
@@ -305,6 +312,8 @@ first_kernel(AdapterArgs p, OuterArgs o, uint16_t* at, uint16_t* bt, int a_tiles
   const int cols = (o.width + 63) / 64;
   outer<BF, NT, false, false, true>(p, o, i / cols, i % cols * 64, lds);
 }
+// dh x^T and dx, of the same tiles of x.  5325 rows of 4096 by rank 16 with dropout 27.1 us for 96 MB
+// (3.5 TB/s), 1763 by rank 64 15.8 us for 41 MB (2.6 TB/s).
 template <bool BF, int NT, bool DX, bool DROP>
 __global__ void __launch_bounds__(kOuterThreads) outer_kernel(AdapterArgs p, OuterArgs o) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[kOuterLds];
@@ -313,7 +322,7 @@ __global__ void __launch_bounds__(kOuterThreads) outer_kernel(AdapterArgs p, Out
 }
 
 // dA and dB of the adapters of several chunks, whose shares are summed in order, and of none; four
-// elements a thread.
+// elements a thread.  4.0 us, a launch and two trips to memory.
 template <bool BF>
 __global__ void __launch_bounds__(kThreads) reduce_kernel(AdapterArgs p, const float* share_a, const float* share_b) {
   const int64_t each_a = p.da ? (int64_t)p.r * p.k / 4 : 0, each_b = p.db ? (int64_t)p.r * p.n / 4 : 0;

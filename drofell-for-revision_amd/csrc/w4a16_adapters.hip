@@ -329,7 +329,7 @@ join_kernel(AdapterArgs p, const float* planes, int splits, AdapterPacks packs) 
 // which each wave takes every fourth group of 64.  h goes in as two 16-bit parts, so that nothing but the
 // result is rounded to 16 bits.  Bound by the output, read and written once as whole lines: 10175 rows of
 // 4096 by rank 16 40 us for 169 MB, 4.2 TB/s, with the sum of the planes (JOIN); rank 64 by 11008 is bound
-// by B's way from the L2 to every tile (1763 rows 30 us for 91 MB).
+// by B's way from the L2 to every tile (1763 rows 28.6 us for 91 MB).
 template <bool BF, int NT, bool JOIN>
 __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int splits, AdapterPacks packs, int wide) {
   constexpr int kR = NT * 16, kPitch = kR + 8, kJ = NT == 1 ? 1 : NT / 2;
@@ -350,6 +350,47 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
     }
     return;
   }
+  // rows as loads and stores take them (to_operands())
+  int row[kHalves][2];
+  const uint16_t* from[kHalves][2];
+#pragma unroll
+  for (int t = 0; t < kHalves; ++t)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      row[t][i] = order[t * 16 + 8 * i + (lane >> 3)];
+      from[t][i] = p.base + max(row[t][i], 0) * p.ldb;
+    }
+  // a tile of few rows: its second half may hold none
+  const bool two = __builtin_amdgcn_readfirstlane(order[16]) >= 0;
+  const int unit = lane & 7;
+  __shared__ __attribute__((aligned(16))) float sums[4][16 * 68];
+  float* const own = sums[wave];
+  const uint16_t* const bw = p.b + (int64_t)ad * p.n * p.r;
+  struct Group {
+    u4 y[kHalves][2], b[4][kJ];
+  };
+  // the lane's eight columns of unit g (operands 0 and 1) and of unit 4 + g (2 and 3)
+  auto load = [&](int grp, Group& v) {
+    const int n = grp * 64 + unit * 8;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int col = min(grp * 64 + (u >> 1) * 32 + (c >> 2) * 8 + (u & 1) * 4 + (c & 3), p.n - 1);
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) {
+        const int r = NT == 1 ? (g & 1) * 8 : 32 * j + 8 * g;
+        v.b[u][j] = *(const u4*)(bw + (int64_t)col * p.r + (r < p.r ? r : 0));
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kHalves; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (t == 0 || two) v.y[t][i] = stream_load(from[t][i] + (n < p.n ? n : 0));
+  };
+  // The first group's loads before the packed rows' (rank 64, 1763 rows: 28.3 us, 30.3 behind them); the planes'
+  // sums need the registers (10175 rows, rank 16: 40.2 us, 50.5 with the group before them).
+  Group v;
+  if constexpr (!JOIN) load(min(g0 + wave, g1 - 1), v);
   // rank 16: both parts in one instruction, the second in the reduction's upper half
   u4 hv[kHalves][kJ], lv[kHalves][kJ];
   float back[kHalves];
@@ -403,46 +444,8 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
       }
     }
   }
-  // rows as loads and stores take them (to_operands())
-  int row[kHalves][2];
-  const uint16_t* from[kHalves][2];
-#pragma unroll
-  for (int t = 0; t < kHalves; ++t)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      row[t][i] = order[t * 16 + 8 * i + (lane >> 3)];
-      from[t][i] = p.base + max(row[t][i], 0) * p.ldb;
-    }
-  // a tile of few rows: its second half may hold none
-  const bool two = __builtin_amdgcn_readfirstlane(order[16]) >= 0;
-  const int unit = lane & 7;
-  __shared__ __attribute__((aligned(16))) float sums[4][16 * 68];
-  float* const own = sums[wave];
-  const uint16_t* const bw = p.b + (int64_t)ad * p.n * p.r;
-  struct Group {
-    u4 y[kHalves][2], b[4][kJ];
-  };
-  // the lane's eight columns of unit g (operands 0 and 1) and of unit 4 + g (2 and 3)
-  auto load = [&](int grp, Group& v) {
-    const int n = grp * 64 + unit * 8;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int col = min(grp * 64 + (u >> 1) * 32 + (c >> 2) * 8 + (u & 1) * 4 + (c & 3), p.n - 1);
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) {
-        const int r = NT == 1 ? (g & 1) * 8 : 32 * j + 8 * g;
-        v.b[u][j] = *(const u4*)(bw + (int64_t)col * p.r + (r < p.r ? r : 0));
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < kHalves; ++t)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (t == 0 || two) v.y[t][i] = stream_load(from[t][i] + (n < p.n ? n : 0));
-  };
   for (int grp = g0 + wave; grp < g1; grp += 4) {
-    Group v;
-    load(grp, v);
+    if (JOIN || grp != g0 + wave) load(grp, v);
     __builtin_amdgcn_sched_barrier(0);
     const bool in = grp * 64 + unit * 8 < p.n;
 #pragma unroll
@@ -594,7 +597,7 @@ hipError_t launch_adapters(const AdapterArgs& a, const ForwardWs& w, hipStream_t
   if (e != hipSuccess) return e;
   // Where nobody keeps h the second launch joins the planes itself: 10175 rows of 11008 against rank 16 in two
   // launches 82.7 us, 87.2 in three.  Where h is kept, join_kernel packs it for the products with g as well,
-  // and the second launch reads its rows: 5325 rows, rank 16 19.5 us that way, 21.4 by the planes.
+  // and the second launch reads its rows: 5325 rows, rank 16 18.7 us that way, 21.4 by the planes.
   const bool join = a.h == nullptr;
   AdapterPacks packs = {};
   if (!join) place_row(packs, a.l, a.r, a.ws + w.row);

@@ -99,6 +99,7 @@ struct AdapterArgs {
 };
 
 // Parts of the reduced axis in which rows are multiplied with A (or their gradients with B).
+constexpr int kMaxSplits = 16;
 int adapter_splits(const AdapterLayout& l, int width, int cus);
 
 // Workspaces: offsets in bytes.

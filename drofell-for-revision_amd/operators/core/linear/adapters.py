@@ -141,7 +141,7 @@ class LowRankAdapters(nn.Module):
         base + each row's adapter's product.  ``seed``: int64 [2] on the device (seed and offset),
         read where dropout applies; another step takes another offset, another projection another
         seed.  Differentiable (once) in x, base, ``a`` and ``b``.  ``output``, without gradients:
-        where the result goes, which may be ``base``."""
+        where the result goes: ``base`` itself, or memory apart from it."""
         params = self._parameters  # (attribute look-up on a module takes 0.4 us each)
         try:
             a, b, scaling = params["a"], params["b"], self._buffers["scaling"]

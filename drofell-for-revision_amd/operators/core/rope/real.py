@@ -122,10 +122,10 @@ class RotaryEmbedding:
     def forward_cached(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
                        slots: torch.Tensor, kv_cacher: LayerBlocksHolder,
                        output: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """q turned (returned, or written to ``output``, which may be q), k turned and v into
-        their cache ``slots`` (integers [rows]; -1: the row is not cached, and so is a slot outside the
-        cache's blocks).  k and v stay as they are.  No two rows may have one slot.  Without
-        gradients: a backward pass through it raises."""
+        """q turned (returned, or written to ``output``: q itself, or memory apart from q, k and
+        v), k turned and v into their cache ``slots`` (integers [rows]; -1: the row is not cached,
+        and so is a slot outside the cache's blocks).  k and v stay as they are.  No two rows may
+        have one slot.  Without gradients: a backward pass through it raises."""
         rows, info = self._check(q, k, v), kv_cacher.block_info
         if k.shape != v.shape:
             raise AssertionError("k and v must have the same shape")

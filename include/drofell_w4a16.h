@@ -652,7 +652,7 @@ int dw4_adapter_plan_size(int num_rows, int num_adapters, size_t* plan_bytes);
 int dw4_adapter_plan(int num_rows, int num_adapters, const int32_t* adapters, int32_t* plan,
                      size_t plan_bytes, void* stream);
 
-/* out may be base (with its stride).  drop: an element of x is zero with probability
+/* out may be base (with its stride), else it lies apart from it.  drop: an element of x is zero with probability
  * drop / 65536, by dw4_dropout's rule, and the others are scaled up; 0: no dropout, seed
  * is not read.  h: h_bytes, 16-byte aligned, what the backward pass needs, or NULL.
  * workspace: dw4_adapters_workspace_size bytes (backward 0). */

@@ -119,6 +119,20 @@ def test_gradients(hip_device, rows, k, n, rank, adapters, order, p, dtype):
     assert all(torch.equal(s, t) for s, t in zip(got, case.grads()))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,k,n,rank,adapters,order", [
+    (1, 4096, 64, 16, 1, "one"), (31, 4168, 1096, 8, 3, "mixed"), (65, 8200, 520, 72, 2, "runs"), (96, 64, 4360, 128, 3, "runs")])
+def test_wide_features(hip_device, rows, k, n, rank, adapters, order, dtype):
+    """As many parts of the reduced axis as there may be, and columns over many workgroups, in both directions."""
+    say(f"wide features {rows} rows {k} -> {n}, rank {rank}, {adapters} adapters {order} {dtype}")
+    case = Case(hip_device, rows, k, n, rank, adapters, dtype, order, dropout=0.1, trainable=True, seed=11)
+    want, err = case.want(grads=True)
+    for name, g, w, e in zip(("out", "dx", "da", "db"), case.grads(), want, err):
+        check(g, w, e, name)
+    with torch.no_grad():
+        check(case.run(), want[0], err[0], "out, served")
+
+
 def test_gradients_of_a_long_run_of_rows(hip_device):
     """Rows past several chunks of one adapter, another one beginning inside a chunk's size."""
     say("gradients over 2300 rows")
@@ -308,6 +322,22 @@ def test_half_modules_keep_their_scaling(hip_device):
     case.bank.half()
     case.scaling = case.bank.scaling.float().cpu()
     check(case.run(), *case.want(), "out")
+
+
+def test_parametrized_adapters(hip_device):
+    say("a parametrized A")
+    case = Case(hip_device, 20, 64, 64, 8, 2, F16, trainable=True)
+    want = case.grads()
+
+    class Same(torch.nn.Module):
+        def forward(self, a):
+            return a * 1
+
+    torch.nn.utils.parametrize.register_parametrization(case.bank, "a", Same())
+    x = case.x.to(hip_device).requires_grad_(True)
+    out = case.bank(x, case.base.to(hip_device), case.rows)
+    da, = torch.autograd.grad(out, case.bank.parametrizations.a.original, case.dout.to(hip_device))
+    assert torch.equal(out, want[0]) and torch.equal(da, want[2])
 
 
 @pytest.mark.parametrize("rows", [40, 300])

@@ -22,7 +22,7 @@ same leaves is alive.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 from torch import nn
@@ -40,17 +40,15 @@ def _whole(x: torch.Tensor) -> torch.Tensor:
     return x if x.is_contiguous() else x.contiguous()
 
 
-def _matrix(x: torch.Tensor) -> torch.Tensor:
-    """x [rows, width] as the kernels read it, in 16-byte units of its rows; a copy where it is not so."""
-    if x.is_contiguous() and x.data_ptr() % 16 == 0:
-        return x
-    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < x.shape[1])):
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
-def _stride(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+def _matrix(x: torch.Tensor, width: int) -> Tuple[torch.Tensor, int]:
+    """x [rows, width] as the kernels read it, in 16-byte units of its rows (a copy where it is not so),
+    and its row stride."""
+    aligned = x.data_ptr() % 16 == 0
+    if aligned and x.is_contiguous():
+        return x, width
+    if not aligned or x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < width:
+        return x.clone(memory_format=torch.contiguous_format), width
+    return x, x.stride(0)
 
 
 def _drop(p: float) -> int:
@@ -79,19 +77,21 @@ class AdapterRows:
         if adapters.shape[0] > 1 << 24 or not 0 <= num_adapters <= 1024:
             raise ValueError("a batch has up to 2^24 rows and 1024 adapters")
         self.num_rows, self.num_adapters, self.device = adapters.shape[0], int(num_adapters), adapters.device
-        with _lib.on_device(self.device):
-            self.plan = torch.empty(_lib.adapter_plan_size(self.num_rows, self.num_adapters) // 4, dtype=torch.int32,
-                                    device=self.device)
+        _lib.is_current(self.device)  # (raises where it is no HIP device)
+        self.plan = torch.empty(_lib.adapter_plan_size(self.num_rows, self.num_adapters) // 4, dtype=torch.int32,
+                                device=self.device)
         self.update(adapters)
 
     def update(self, adapters: torch.Tensor) -> None:
         """The same rows with other adapters, in the memory that captured calls read."""
         if adapters.shape != (self.num_rows,) or adapters.device != self.device:
             raise ValueError(f"adapters must be {self.num_rows} integers on {self.device}")
+        if not _lib.is_current(self.device):
+            with torch.cuda.device(self.device):
+                return self.update(adapters)
         index = int32(adapters, "adapters")
-        with _lib.on_device(self.device):
-            _lib.call("dw4_adapter_plan", self.num_rows, self.num_adapters, index.data_ptr(), self.plan.data_ptr(),
-                      self.plan.numel() * 4, _lib.current_stream(self.device.index))
+        _lib.call("dw4_adapter_plan", self.num_rows, self.num_adapters, index.data_ptr(), self.plan.data_ptr(),
+                  self.plan.numel() * 4, _lib.current_stream(self.device.index))
         increment_version(self.plan)  # a backward pass that was to read the old one fails
 
 
@@ -148,10 +148,11 @@ class LowRankAdapters(nn.Module):
         except KeyError:  # (parametrized)
             a, b, scaling = self.a, self.b, self.scaling
         device, dtype = x.device, x.dtype
-        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-        base2 = base if base.dim() == 2 else base.reshape(-1, base.shape[-1])
+        flat = x.dim() == 2 and base.dim() == 2
+        x2, base2 = (x, base) if flat else (x.reshape(-1, x.shape[-1]), base.reshape(-1, base.shape[-1]))
         num_rows, width = x2.shape
-        if width != self.in_features or base2.shape != (num_rows, self.out_features) or x.shape[:-1] != base.shape[:-1]:
+        if width != self.in_features or base2.shape != (num_rows, self.out_features) or \
+                not (flat or x.shape[:-1] == base.shape[:-1]):
             raise ValueError(f"x and base must be [..., {self.in_features}] and [..., {self.out_features}] of the same rows")
         if dtype not in _DTYPES or base.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
             raise TypeError("x, base and the adapters must be of one type, fp16 or bf16")
@@ -168,10 +169,10 @@ class LowRankAdapters(nn.Module):
             if output is not None:
                 raise ValueError("output is for calls without gradients")
             out2 = _LowRank.apply(x2, base2, a, b, scaling, rows.plan, drop, seed)
-            return out2 if base.dim() == 2 else out2.view(base.shape)
+            return out2 if flat else out2.view(base.shape)
         if output is None:
             out2 = _forward(x2, base2, a, b, scaling, rows.plan, drop, seed, None, False)[0]
-            return out2 if base.dim() == 2 else out2.view(base.shape)
+            return out2 if flat else out2.view(base.shape)
         if output.shape != base.shape or output.dtype != dtype or output.device != device or \
                 not output.is_contiguous() or output.data_ptr() % 16:
             raise ValueError("output must be contiguous and 16-byte aligned, of base's shape, type and device")
@@ -181,33 +182,38 @@ class LowRankAdapters(nn.Module):
 
 
 def _forward(x, base, a, b, scaling, plan, drop, seed, out, keep):
-    """The call itself -> (out, x as the kernels read it, h or None, its shape)."""
+    """The call itself -> (out, x as the kernels read it, h or None, what the backward pass's call takes).
+    (Each property of a tensor takes 0.1 to 0.2 us: they are read once.)"""
     device = x.device
-    with _lib.on_device(device):
-        x, base = _matrix(x), _matrix(base)
-        a, b, scaling = _whole(a), _whole(b), _whole(scaling)
-        shape = (_DTYPES[x.dtype], x.shape[0], a.shape[0], x.shape[1], b.shape[1], a.shape[1])
-        nbytes, h_bytes = _lib.adapters_workspace_size(*shape[1:], False, device.index)
-        if out is None:
-            out = torch.empty_like(base, memory_format=torch.contiguous_format)
-        ws = x.new_empty(nbytes // 2)  # (16-bit elements; torch.empty takes 0.6 us more)
-        h = x.new_empty(h_bytes // 2) if keep else None
-        _lib.call("dw4_adapters", *shape, x.data_ptr(), _stride(x), base.data_ptr(), _stride(base), out.data_ptr(),
-                  _stride(out), a.data_ptr(), b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), drop,
-                  None if seed is None else seed.data_ptr(), None if h is None else h.data_ptr(), ws.data_ptr(), nbytes,
-                  _lib.current_stream(device.index))
-    return out, x, h, shape
+    if not _lib.is_current(device):
+        with torch.cuda.device(device):
+            return _forward(x, base, a, b, scaling, plan, drop, seed, out, keep)
+    rows, k = x.shape
+    adapters, n, rank = b.shape
+    x, ldx = _matrix(x, k)
+    base, ldb = _matrix(base, n)
+    a, b, scaling = _whole(a), _whole(b), _whole(scaling)
+    nbytes, h_bytes = _lib.adapters_workspace_size(rows, adapters, k, n, rank, False, device.index)
+    if out is None:
+        out = torch.empty_like(base) if ldb == n else torch.empty_like(base, memory_format=torch.contiguous_format)
+    ws = x.new_empty(nbytes // 2)  # (16-bit elements; torch.empty takes 0.6 us more)
+    h = x.new_empty(h_bytes // 2) if keep else None
+    shape = (_DTYPES[x.dtype], rows, adapters, k, n, rank)
+    _lib.call("dw4_adapters", *shape, x.data_ptr(), ldx, base.data_ptr(), ldb, out.data_ptr(), n, a.data_ptr(),
+              b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), drop, None if seed is None else seed.data_ptr(),
+              None if h is None else h.data_ptr(), ws.data_ptr(), nbytes, _lib.current_stream(device.index))
+    if not keep:
+        return out, x, h, None
+    # worked out here: the backward pass runs in a thread of autograd's, where Python takes twice as long
+    nbytes = _lib.adapters_workspace_size(rows, adapters, k, n, rank, True, device.index)[0] if rows else 0
+    return out, x, h, (shape, drop, nbytes, device, ldx)
 
 
 class _LowRank(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, base, a, b, scaling, plan, drop, seed):
         a, b, scaling = _whole(a), _whole(b), _whole(scaling)
-        out, x, h, shape = _forward(x, base, a, b, scaling, plan, drop, seed, None, True)
-        # what the backward pass needs, worked out here: it runs in a thread of autograd's, where
-        # the same Python takes twice as long
-        nbytes = _lib.adapters_workspace_size(*shape[1:], True, x.device.index)[0] if shape[1] else 0
-        ctx.call = shape, drop, nbytes, x.device, _stride(x)
+        out, x, h, ctx.call = _forward(x, base, a, b, scaling, plan, drop, seed, None, True)
         ctx.save_for_backward(x, a, b, scaling, plan, h, seed)
         return out
 
@@ -227,17 +233,18 @@ class _LowRank(torch.autograd.Function):
                     torch.zeros_like(b) if need_b else None, None, None, None, None)
         if not (need_x or need_a or need_b):
             return None, dbase, None, None, None, None, None, None
-        with _lib.on_device(device):
-            g = _matrix(dout)
-            dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
-            da = torch.empty_like(a) if need_a else None
-            db = torch.empty_like(b) if need_b else None
-            ws = x.new_empty(nbytes // 2)
-            _lib.call("dw4_adapters_backward", *shape, x.data_ptr(), ldx, g.data_ptr(), _stride(g), a.data_ptr(),
-                      b.data_ptr(), scaling.data_ptr(), plan.data_ptr(), drop,
-                      None if seed is None else seed.data_ptr(), h.data_ptr(),
-                      None if dx is None else dx.data_ptr(), shape[3], None if da is None else da.data_ptr(),
-                      None if db is None else db.data_ptr(), ws.data_ptr(), nbytes, _lib.current_stream(device.index))
+        if not _lib.is_current(device):
+            with torch.cuda.device(device):
+                return _LowRank._gradients(ctx, dout)
+        g, ldg = _matrix(dout, shape[4])
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+        da = torch.empty_like(a) if need_a else None
+        db = torch.empty_like(b) if need_b else None
+        ws = x.new_empty(nbytes // 2)
+        _lib.call("dw4_adapters_backward", *shape, x.data_ptr(), ldx, g.data_ptr(), ldg, a.data_ptr(), b.data_ptr(),
+                  scaling.data_ptr(), plan.data_ptr(), drop, None if seed is None else seed.data_ptr(), h.data_ptr(),
+                  None if dx is None else dx.data_ptr(), shape[3], None if da is None else da.data_ptr(),
+                  None if db is None else db.data_ptr(), ws.data_ptr(), nbytes, _lib.current_stream(device.index))
         return dx, dbase, da, db, None, None, None, None
 
     _once = staticmethod(torch.autograd.function.once_differentiable(_gradients.__func__))
@@ -291,15 +298,21 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def _run(x, seed, drop):
         device = x.device
+        if not _lib.is_current(device):
+            with torch.cuda.device(device):
+                return _Dropout._run(x, seed, drop)
         cols = x.shape[-1]
         rows = x.numel() // cols if cols else 0
         x2 = x if x.dim() == 2 else x.reshape(rows, cols)
-        if not x2.is_contiguous() and (x2.stride(1) != 1 or (rows > 1 and x2.stride(0) < cols)):
-            x2 = x2.contiguous()
-        with _lib.on_device(device):
-            y = torch.empty_like(x, memory_format=torch.contiguous_format)
-            _lib.call("dw4_dropout", _DTYPES[x.dtype], rows, cols, x2.data_ptr(), _stride(x2), y.data_ptr(), cols, drop,
-                      seed.data_ptr(), _lib.current_stream(device.index))
+        ldx = cols
+        if not x2.is_contiguous():
+            if x2.stride(1) != 1 or x2.stride(0) < cols:
+                x2 = x2.contiguous()
+            else:
+                ldx = x2.stride(0)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        _lib.call("dw4_dropout", _DTYPES[x.dtype], rows, cols, x2.data_ptr(), ldx, y.data_ptr(), cols, drop,
+                  seed.data_ptr(), _lib.current_stream(device.index))
         return y
 
     @staticmethod

@@ -34,21 +34,17 @@ _TWO_PI = Fraction(62831853071795864769252867665590057683943, 10 ** 40)
 _DTYPES = {torch.float16: _lib.DW4_F16, torch.bfloat16: _lib.DW4_BF16}
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x [rows, heads, dims] with its heads side by side and rows in 16-byte units; a copy
-    where it is not so."""
+def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """x [rows, heads, dims] with its heads side by side and rows in 16-byte units (a copy
+    where it is not so), and its row stride."""
     rows, heads, dims = x.shape
-    if x.is_contiguous() and x.data_ptr() % 16 == 0:
-        return x
-    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != dims) or x.data_ptr() % 16 or \
-            (rows > 1 and (x.stride(0) % 8 or x.stride(0) < heads * dims)):
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
-def _stride(x: torch.Tensor) -> int:
-    rows, heads, dims = x.shape
-    return x.stride(0) if rows > 1 else heads * dims
+    width, aligned = heads * dims, x.data_ptr() % 16 == 0
+    if aligned and x.is_contiguous():
+        return x, width
+    if not aligned or x.stride(2) != 1 or (heads > 1 and x.stride(1) != dims) or \
+            (rows > 1 and (x.stride(0) % 8 or x.stride(0) < width)):
+        return x.clone(memory_format=torch.contiguous_format), width
+    return x, x.stride(0) if rows > 1 else width
 
 
 class RotaryEmbedding:
@@ -77,10 +73,11 @@ class RotaryEmbedding:
         self.device = self._turns.device
 
     def _check(self, *rows: torch.Tensor) -> int:
-        dtype, count = rows[0].dtype, rows[0].shape[0]
+        dtype, count, dims = rows[0].dtype, rows[0].shape[0], self.head_dim
         for x in rows:
-            if x.dim() != 3 or x.shape[2] != self.head_dim or x.shape[0] != count:
-                raise AssertionError(f"q, k and v must be [rows, heads, {self.head_dim}], of the same rows")
+            shape = x.shape
+            if len(shape) != 3 or shape[2] != dims or shape[0] != count:
+                raise AssertionError(f"q, k and v must be [rows, heads, {dims}], of the same rows")
             if x.dtype != dtype:
                 raise TypeError("q, k and v must have one type")
             if x.device != self.device:
@@ -98,15 +95,18 @@ class RotaryEmbedding:
 
     def _turn(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
               inverse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-        with _lib.on_device(self.device):
-            q, k = _rows(q), _rows(k)
-            qo = torch.empty_like(q, memory_format=torch.contiguous_format)
-            ko = torch.empty_like(k, memory_format=torch.contiguous_format)
-            _lib.call("dw4_rotary", _DTYPES[q.dtype], q.shape[0], q.shape[1], k.shape[1], self.head_dim,
-                      self.rotary_dim, int(self.interleaved), int(inverse), q.data_ptr(), _stride(q),
-                      k.data_ptr(), _stride(k), qo.data_ptr(), _stride(qo), ko.data_ptr(), _stride(ko),
-                      positions.data_ptr(), self._turns.data_ptr(), self.magnitude,
-                      _lib.current_stream(self.device.index))
+        if not _lib.is_current(self.device):
+            with torch.cuda.device(self.device):
+                return self._turn(q, k, positions, inverse)
+        (q, ldq), (k, ldk) = _rows(q), _rows(k)
+        rows, heads, dims = q.shape
+        kv_heads = k.shape[1]
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        _lib.call("dw4_rotary", _DTYPES[q.dtype], rows, heads, kv_heads, dims, self.rotary_dim, int(self.interleaved),
+                  int(inverse), q.data_ptr(), ldq, k.data_ptr(), ldk, qo.data_ptr(), heads * dims, ko.data_ptr(),
+                  kv_heads * dims, positions.data_ptr(), self._turns.data_ptr(), self.magnitude,
+                  _lib.current_stream(self.device.index))
         return qo, ko
 
     def forward(self, q: torch.Tensor, k: torch.Tensor,
@@ -126,10 +126,14 @@ class RotaryEmbedding:
         v), k turned and v into their cache ``slots`` (integers [rows]; -1: the row is not cached,
         and so is a slot outside the cache's blocks).  k and v stay as they are.  No two rows may
         have one slot.  Without gradients: a backward pass through it raises."""
+        if not _lib.is_current(self.device):
+            with torch.cuda.device(self.device):
+                return self.forward_cached(q, k, v, positions, slots, kv_cacher, output)
         rows, info = self._check(q, k, v), kv_cacher.block_info
-        if k.shape != v.shape:
+        heads, kv_heads, dims = q.shape[1], k.shape[1], self.head_dim
+        if v.shape[1] != kv_heads:
             raise AssertionError("k and v must have the same shape")
-        if info.head_dim != self.head_dim or info.num_key_value_heads != k.shape[1]:
+        if info.head_dim != dims or info.num_key_value_heads != kv_heads:
             raise AssertionError("k and v do not match the cache's block geometry")
         if kv_cacher.dtype != q.dtype:
             raise TypeError(f"rows of {q.dtype} into a cache of {kv_cacher.dtype}")
@@ -142,24 +146,22 @@ class RotaryEmbedding:
             slots = int32(slots, "slots").to(torch.int64)
         elif not slots.is_contiguous():
             slots = slots.contiguous()
-        given = output is not None
+        given, ldo = output is not None, heads * dims
         if not given:
             output = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif output.shape != q.shape or output.dtype != q.dtype or output.device != self.device:
             raise ValueError("output must have the queries' shape, type and device")
-        elif _rows(output) is not output:
-            raise ValueError("output rows must be contiguous and 16-byte aligned")
-        with _lib.on_device(self.device):
-            q2, k2, v2 = _rows(q), _rows(k), _rows(v)
-            _lib.call("dw4_rotary_and_cache", _DTYPES[q.dtype], rows, q.shape[1], k.shape[1], self.head_dim,
-                      self.rotary_dim, int(self.interleaved), q2.data_ptr(), _stride(q2), k2.data_ptr(),
-                      _stride(k2), v2.data_ptr(), _stride(v2), output.data_ptr(), _stride(output),
-                      pos.data_ptr(), self._turns.data_ptr(), self.magnitude, slots.data_ptr(),
-                      min(kv_cacher.layer_key_ptr_table_device.numel(),
-                          kv_cacher.layer_val_ptr_table_device.numel()), flags.BLOCK_SIZE,
-                      kv_cacher.layer_key_ptr_table_device.data_ptr(),
-                      kv_cacher.layer_val_ptr_table_device.data_ptr(), info.head_stride,
-                      _lib.current_stream(self.device.index))
+        else:
+            same, ldo = _rows(output)
+            if same is not output:
+                raise ValueError("output rows must be contiguous and 16-byte aligned")
+        (q2, ldq), (k2, ldk), (v2, ldv) = _rows(q), _rows(k), _rows(v)
+        keys, values = kv_cacher.layer_key_ptr_table_device, kv_cacher.layer_val_ptr_table_device
+        _lib.call("dw4_rotary_and_cache", _DTYPES[q.dtype], rows, heads, kv_heads, dims, self.rotary_dim,
+                  int(self.interleaved), q2.data_ptr(), ldq, k2.data_ptr(), ldk, v2.data_ptr(), ldv, output.data_ptr(),
+                  ldo, pos.data_ptr(), self._turns.data_ptr(), self.magnitude, slots.data_ptr(),
+                  min(keys.numel(), values.numel()), flags.BLOCK_SIZE, keys.data_ptr(), values.data_ptr(),
+                  info.head_stride, _lib.current_stream(self.device.index))
         if given:
             increment_version(output)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

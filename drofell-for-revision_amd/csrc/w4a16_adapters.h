@@ -105,7 +105,7 @@ int adapter_splits(const AdapterLayout& l, int width, int cus);
 // Workspaces: offsets in bytes.
 struct ForwardWs {
   int splits;
-  size_t row, bytes;  // behind the planes [splits][positions][r]
+  size_t bytes;  // planes [splits][positions][r]
 };
 inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 inline size_t plane_bytes(const AdapterLayout& l, int splits, int r) {
@@ -114,8 +114,7 @@ inline size_t plane_bytes(const AdapterLayout& l, int splits, int r) {
 inline ForwardWs forward_ws(const AdapterLayout& l, int k, int r, int cus) {
   ForwardWs w;
   w.splits = adapter_splits(l, k, cus);
-  w.row = plane_bytes(l, w.splits, r);
-  w.bytes = w.row + row_pack_bytes(l, r);
+  w.bytes = plane_bytes(l, w.splits, r);
   return w;
 }
 struct BackwardWs {

@@ -255,8 +255,32 @@ __device__ __forceinline__ f4 sum_planes(const float* at, int64_t plane, int spl
   return v;
 }
 
-// 32 positions' h (or dh): planes summed in order, times s_a / kept share, packed by row and by column.  Bound
-// by its launch and the trip to the planes: 5325 rows of rank 16 4.2 us, 1763 of rank 64 4.9.
+// 32 positions' h (or dh) v [32][kR + 1], from position `first` on, by column (AdapterPacks).
+template <bool BF, int kR>
+__device__ __forceinline__ void pack_columns(const float* v, const AdapterPacks& packs, int64_t first, int64_t positions,
+                                             int threads) {
+  for (int i = threadIdx.x; i < 4 * kR; i += threads) {  // column i % kR, eight rows
+    const int col = i % kR, r0 = i / kR * 8;
+    int ex = 0;
+    if constexpr (!BF) {
+      float m = 0.f;
+      for (int e = 0; e < 32; ++e) m = fmaxf(m, fabsf(v[e * (kR + 1) + col]));
+      ex = range_exponent<BF>(m);
+      if (r0 == 0) packs.col_exp[first / 32 * kR + col] = -ex;
+    }
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = BF ? v[(r0 + e) * (kR + 1) + col] : times_pow2(v[(r0 + e) * (kR + 1) + col], ex);
+    u4 hi, lo;
+    split16<BF>(x, hi, lo);
+    uint16_t* to = packs.col + ((first + r0) * kR + col * 8);
+    *(u4*)to = hi;
+    *(u4*)(to + positions * kR) = lo;
+  }
+}
+
+// 32 positions' dh: planes summed in order, times s_a / kept share, packed by row and by column.  Bound
+// by its launch and the trip to the planes: 5325 rows of rank 16 3.6 us, 1763 of rank 64 5.2.
 template <bool BF, int NT>
 __global__ void __launch_bounds__(kJoinThreads)
 join_kernel(AdapterArgs p, const float* planes, int splits, AdapterPacks packs) {
@@ -301,33 +325,18 @@ join_kernel(AdapterArgs p, const float* planes, int splits, AdapterPacks packs) 
       *(u4*)(to + p.l.positions * kR) = lo;
     }
   }
-  if (packs.col == nullptr) return;
-  for (int i = threadIdx.x; i < 4 * kR; i += kJoinThreads) {  // column i % kR, eight rows
-    const int col = i % kR, r0 = i / kR * 8;
-    int ex = 0;
-    if constexpr (!BF) {
-      float m = 0.f;
-      for (int e = 0; e < 32; ++e) m = fmaxf(m, fabsf(v[e][col]));
-      ex = range_exponent<BF>(m);
-      if (r0 == 0) packs.col_exp[first / 32 * kR + col] = -ex;
-    }
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = BF ? v[r0 + e][col] : times_pow2(v[r0 + e][col], ex);
-    u4 hi, lo;
-    split16<BF>(x, hi, lo);
-    uint16_t* to = packs.col + ((first + r0) * kR + col * 8);
-    *(u4*)to = hi;
-    *(u4*)(to + p.l.positions * kR) = lo;
-  }
+  if (packs.col != nullptr) pack_columns<BF, kR>(&v[0][0], packs, first, p.l.positions, kJoinThreads);
 }
 
 // The products with B, added in 32 bits to the projection's output: a tile's rows, a part of the columns, of
-// which each wave takes every fourth group of 64.  h goes in as two 16-bit parts, so that nothing but the
-// result is rounded to 16 bits.  Bound by the output, read and written once as whole lines: 10175 rows of
-// 4096 by rank 16 40 us for 169 MB, 4.2 TB/s, with the sum of the planes (JOIN); rank 64 by 11008 is bound
-// by B's way from the L2 to every tile (1763 rows 28.6 us for 91 MB).
-template <bool BF, int NT, bool JOIN>
+// which each wave takes every fourth group of 64.  A workgroup sums the tile's planes itself; h goes into the
+// product as two 16-bit parts, so that nothing but the result is rounded to 16 bits.  Where h is kept, the tile's
+// first workgroup packs it by column: 5325 rows of rank 16 20.2 us that way, 18.7 by rows that a launch of
+// 4.1 had packed before; 1763 of rank 64 35.1, and 28.5 behind 5.1.
+// Bound by the output, read and written once as whole lines: 10175 rows of 4096 by rank 16 40 us for 169 MB,
+// 4.2 TB/s; rank 64 by 11008 is bound by B's way from the L2 to every tile (1763 rows 35 us for 91 MB).
+// The first group's loads before the planes' sums take the registers of a wave (10175 rows 50.5 us for 40.2).
+template <bool BF, int NT>
 __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int splits, AdapterPacks packs, int wide) {
   constexpr int kR = NT * 16, kPitch = kR + 8, kJ = NT == 1 ? 1 : NT / 2;
   const int item = item_of_xcd(blockIdx.x, p.plan[0] * wide);
@@ -360,8 +369,6 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
   // a tile of few rows: its second half may hold none
   const bool two = __builtin_amdgcn_readfirstlane(order[16]) >= 0;
   const int unit = lane & 7;
-  __shared__ __attribute__((aligned(16))) float sums[4][16 * 68];
-  float* const own = sums[wave];
   const uint16_t* const bw = p.b + (int64_t)ad * p.n * p.r;
   struct Group {
     u4 y[kHalves][2], b[4][kJ];
@@ -384,65 +391,60 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
       for (int i = 0; i < 2; ++i)
         if (t == 0 || two) v.y[t][i] = stream_load(from[t][i] + (n < p.n ? n : 0));
   };
-  // The first group's loads before the packed rows' (rank 64, 1763 rows: 28.3 us, 30.3 behind them); the planes'
-  // sums need the registers (10175 rows, rank 16: 40.2 us, 50.5 with the group before them).
-  Group v;
-  if constexpr (!JOIN) load(min(g0 + wave, g1 - 1), v);
+  // the waves' own parts of the sums below; before them, where h is kept, its 32-bit values
+  __shared__ __attribute__((aligned(16))) float sums[4][16 * 68];
+  static_assert(kTileRows * (kR + 1) <= 4 * 16 * 68, "h takes the sums' place");
+  const bool keep = packs.col != nullptr && column_part == 0;
   // rank 16: both parts in one instruction, the second in the reduction's upper half
   u4 hv[kHalves][kJ], lv[kHalves][kJ];
   float back[kHalves];
-  if constexpr (JOIN) {
-    __shared__ __attribute__((aligned(16))) uint16_t part[2][kTileRows][kPitch];
-    __shared__ int back_s[kTileRows];
-    const float scale = p.scaling[ad] * p.keep_scale;
-    const float* planes = reinterpret_cast<const float*>(p.ws);
-    for (int i = threadIdx.x; i < kTileRows * NT * 4; i += kThreads) {
-      const int at = i / (NT * 4), q = i % (NT * 4) * 4;
-      f4 v = {};
-      if (q < p.r && order[at] >= 0)
-        v = sum_planes(planes + ((int64_t)tile * kTileRows + at) * p.r + q, p.l.positions * p.r, splits) * scale;
-      if constexpr (!BF) {
-        float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+  __shared__ __attribute__((aligned(16))) uint16_t part[2][kTileRows][kPitch];
+  __shared__ int back_s[kTileRows];
+  const float scale = p.scaling[ad] * p.keep_scale;
+  const float* planes = reinterpret_cast<const float*>(p.ws);
+  for (int i = threadIdx.x; i < kTileRows * NT * 4; i += kThreads) {
+    const int at = i / (NT * 4), q = i % (NT * 4) * 4;
+    f4 v = {};
+    if (q < p.r && order[at] >= 0)
+      v = sum_planes(planes + ((int64_t)tile * kTileRows + at) * p.r + q, p.l.positions * p.r, splits) * scale;
+    if (keep) {
 #pragma unroll
-        for (int o = 1; o < NT * 4; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        const int e = range_exponent<BF>(m);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = times_pow2(v[j], e);
-        if (q == 0) back_s[at] = -e;
-      }
-      uint2 hi, lo;
-      split16<BF>(v[0], v[1], hi.x, lo.x);
-      split16<BF>(v[2], v[3], hi.y, lo.y);
-      *(uint2*)&part[0][at][q] = hi;
-      *(uint2*)&part[1][at][q] = lo;
+      for (int e = 0; e < 4; ++e) (&sums[0][0])[at * (kR + 1) + q + e] = v[e];
     }
+    if constexpr (!BF) {
+      float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+      for (int o = 1; o < NT * 4; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+      const int e = range_exponent<BF>(m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = times_pow2(v[j], e);
+      if (q == 0) back_s[at] = -e;
+    }
+    uint2 hi, lo;
+    split16<BF>(v[0], v[1], hi.x, lo.x);
+    split16<BF>(v[2], v[3], hi.y, lo.y);
+    *(uint2*)&part[0][at][q] = hi;
+    *(uint2*)&part[1][at][q] = lo;
+  }
+  __syncthreads();
+  if (keep) {
+    pack_columns<BF, kR>(&sums[0][0], packs, (int64_t)tile * kTileRows, p.l.positions, kThreads);
     __syncthreads();
+  }
 #pragma unroll
-    for (int t = 0; t < kHalves; ++t) {
-      if constexpr (!BF) back[t] = pow2(back_s[t * 16 + c]);
+  for (int t = 0; t < kHalves; ++t) {
+    if constexpr (!BF) back[t] = pow2(back_s[t * 16 + c]);
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) {
-        const int r = NT == 1 ? (g & 1) * 8 : 32 * j + 8 * g;
-        hv[t][j] = *(const u4*)&part[NT == 1 ? g >> 1 : 0][t * 16 + c][r];
-        if constexpr (NT > 1) lv[t][j] = *(const u4*)&part[1][t * 16 + c][r];
-      }
-    }
-  } else {
-    const int64_t half = p.l.positions * kR;
-#pragma unroll
-    for (int t = 0; t < kHalves; ++t) {
-      const int64_t pos = (int64_t)tile * kTileRows + t * 16 + c;
-      if constexpr (!BF) back[t] = pow2(packs.row_exp[pos]);
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) {
-        const uint16_t* at = packs.row + pos * kR + (NT == 1 ? (g >> 1) * half + (g & 1) * 8 : 32 * j + 8 * g);
-        hv[t][j] = *(const u4*)at;
-        if constexpr (NT > 1) lv[t][j] = *(const u4*)(at + half);
-      }
+    for (int j = 0; j < kJ; ++j) {
+      const int r = NT == 1 ? (g & 1) * 8 : 32 * j + 8 * g;
+      hv[t][j] = *(const u4*)&part[NT == 1 ? g >> 1 : 0][t * 16 + c][r];
+      if constexpr (NT > 1) lv[t][j] = *(const u4*)&part[1][t * 16 + c][r];
     }
   }
+  float* const own = sums[wave];
   for (int grp = g0 + wave; grp < g1; grp += 4) {
-    if (JOIN || grp != g0 + wave) load(grp, v);
+    Group v;
+    load(grp, v);
     __builtin_amdgcn_sched_barrier(0);
     const bool in = grp * 64 + unit * 8 < p.n;
 #pragma unroll
@@ -538,21 +540,19 @@ void shrink_rank(const ShrinkArgs& a, int splits, hipStream_t stream) {
 }
 
 template <bool BF, int NT>
-void expand_of(const AdapterArgs& a, int splits, bool join, const AdapterPacks& packs, hipStream_t stream) {
+void expand_of(const AdapterArgs& a, int splits, const AdapterPacks& packs, hipStream_t stream) {
   const int groups = (a.n + 63) / 64;
   // About four workgroups per CU of four waves each.  Half as many: 10175 rows against rank 16 76 us for 40;
   // twice as many 39.6, but each sums the planes anew.
   const int wide = std::max(1, std::min((groups + 3) / 4, 1024 / a.l.tiles));
-  const unsigned grid = (unsigned)a.l.tiles * wide;
-  if (join) expand_kernel<BF, NT, true><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
-  else expand_kernel<BF, NT, false><<<grid, kThreads, 0, stream>>>(a, splits, packs, wide);
+  expand_kernel<BF, NT><<<(unsigned)a.l.tiles * wide, kThreads, 0, stream>>>(a, splits, packs, wide);
 }
 template <bool BF>
-void expand_rank(const AdapterArgs& a, int splits, bool join, const AdapterPacks& packs, hipStream_t stream) {
-  if (a.r <= 16) expand_of<BF, 1>(a, splits, join, packs, stream);
-  else if (a.r <= 32) expand_of<BF, 2>(a, splits, join, packs, stream);
-  else if (a.r <= 64) expand_of<BF, 4>(a, splits, join, packs, stream);
-  else expand_of<BF, 8>(a, splits, join, packs, stream);
+void expand_rank(const AdapterArgs& a, int splits, const AdapterPacks& packs, hipStream_t stream) {
+  if (a.r <= 16) expand_of<BF, 1>(a, splits, packs, stream);
+  else if (a.r <= 32) expand_of<BF, 2>(a, splits, packs, stream);
+  else if (a.r <= 64) expand_of<BF, 4>(a, splits, packs, stream);
+  else expand_of<BF, 8>(a, splits, packs, stream);
 }
 
 }  // namespace
@@ -593,15 +593,9 @@ hipError_t launch_adapters(const AdapterArgs& a, const ForwardWs& w, hipStream_t
   const ShrinkArgs s = {a.l, a.plan, a.x, a.ldx, a.a, a.k, a.r, a.adapters, a.drop, a.seed, planes};
   hipError_t e = launch_shrink(a.bf16, s, w.splits, stream);
   if (e != hipSuccess) return e;
-  // Where nobody keeps h the second launch joins the planes itself: 10175 rows of 11008 against rank 16 in two
-  // launches 82.7 us, 87.2 in three.  Where h is kept, join_kernel packs it for the products with g as well,
-  // and the second launch reads its rows: 5325 rows, rank 16 18.7 us that way, 21.4 by the planes.
-  const bool join = a.h == nullptr;
   AdapterPacks packs = {};
-  if (!join) place_row(packs, a.l, a.r, a.ws + w.row);
   if (a.h != nullptr) place_col(packs, a.l, a.r, a.h);
-  if (a.h && (e = launch_join(a, planes, w.splits, packs, stream)) != hipSuccess) return e;
-  a.bf16 ? expand_rank<true>(a, w.splits, join, packs, stream) : expand_rank<false>(a, w.splits, join, packs, stream);
+  a.bf16 ? expand_rank<true>(a, w.splits, packs, stream) : expand_rank<false>(a, w.splits, packs, stream);
   return hipGetLastError();
 }
 

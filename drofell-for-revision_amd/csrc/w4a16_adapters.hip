@@ -264,7 +264,7 @@ __device__ __forceinline__ void pack_columns(const float* v, const AdapterPacks&
     int ex = 0;
     if constexpr (!BF) {
       float m = 0.f;
-      for (int e = 0; e < 32; ++e) m = fmaxf(m, fabsf(v[e * (kR + 1) + col]));
+      for (int e = 0; e < 32; ++e) m = fmaxf(m, finite_magnitude(v[e * (kR + 1) + col]));
       ex = range_exponent<BF>(m);
       if (r0 == 0) packs.col_exp[first / 32 * kR + col] = -ex;
     }
@@ -304,7 +304,7 @@ join_kernel(AdapterArgs p, const float* planes, int splits, AdapterPacks packs) 
       const int at = threadIdx.x >> 4;
       float m = 0.f;
 #pragma unroll
-      for (int e = 0; e < kR / 16; ++e) m = fmaxf(m, fabsf(v[at][(threadIdx.x & 15) + 16 * e]));
+      for (int e = 0; e < kR / 16; ++e) m = fmaxf(m, finite_magnitude(v[at][(threadIdx.x & 15) + 16 * e]));
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
       if ((threadIdx.x & 15) == 0) {
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
       for (int e = 0; e < 4; ++e) (&sums[0][0])[at * (kR + 1) + q + e] = v[e];
     }
     if constexpr (!BF) {
-      float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+      float m = fmaxf(fmaxf(finite_magnitude(v[0]), finite_magnitude(v[1])), fmaxf(finite_magnitude(v[2]), finite_magnitude(v[3])));
 #pragma unroll
       for (int o = 1; o < NT * 4; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
       const int e = range_exponent<BF>(m);
@@ -463,6 +463,18 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
           acc[u] = mfma16_of<BF>(v.b[u][j], hv[t][j], acc[u]);
           if constexpr (NT > 1) acc[u] = mfma16_of<BF>(v.b[u][j], lv[t][j], acc[u]);
         }
+      if (nan_among(acc)) {  // an infinite B, or h
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          acc[u] = f4{};
+#pragma unroll
+          for (int j = 0; j < kJ; ++j) {
+            const u4 b = finite_only<BF>(v.b[u][j]);
+            acc[u] = mfma16_of<BF>(NT == 1 && g >= 2 ? b : v.b[u][j], hv[t][j], acc[u]);
+            if constexpr (NT > 1) acc[u] = mfma16_of<BF>(b, lv[t][j], acc[u]);
+          }
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if constexpr (!BF) acc[u] *= back[t];
@@ -482,8 +494,11 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int spl
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (in && row[t][i] >= 0) *(u4*)(p.out + row[t][i] * p.ldo + grp * 64 + unit * 8) = v.y[t][i];
+      for (int i = 0; i < 2; ++i) {
+        int to = row[t][i];
+        asm volatile("" : "+v"(to));  // (addresses kept over the groups took 8 registers)
+        if (in && to >= 0) *(u4*)(p.out + to * p.ldo + grp * 64 + unit * 8) = v.y[t][i];
+      }
     }
   }
 }

@@ -120,13 +120,39 @@ __device__ __forceinline__ void split16(const float (&v)[8], u4& hi, u4& lo) {
     lo[e] = y;
   }
 }
+// An infinite value's product with a first part is what the sum comes to, infinite or NaN; its product with a
+// second part of zero, or of the other sign, would make the sum NaN in any case.  What a second part is multiplied
+// with where infinities are about: the finite values, zeros for the others.
+template <bool BF>
+__device__ __forceinline__ u4 finite_only(u4 v) {
+  constexpr uint32_t kExp = BF ? 0x7F80u : 0x7C00u;
+  asm volatile("" : "+v"(v));  // made where it is used: kept for several products it took 60 registers
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    v[e] = ((v[e] & kExp) == kExp ? 0u : v[e] & 0xFFFFu) | ((v[e] & (kExp << 16)) == kExp << 16 ? 0u : v[e] & 0xFFFF0000u);
+  return v;
+}
+// Adds to `bits` whether a value of v is not finite (the exponent's carry into bits 15 and 31; other bits mean nothing).
+template <bool BF>
+__device__ __forceinline__ void add_nonfinite(u4 v, uint32_t& bits) {
+  constexpr uint32_t kExp = BF ? 0x7F807F80u : 0x7C007C00u, kLow = BF ? 0x00800080u : 0x04000400u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bits |= (v[e] & kExp) + kLow;
+}
+// Whether a lane of the wave holds NaN in v (infinities of both signs count too).
+__device__ __forceinline__ bool nan_among(const f4 (&v)[4]) {
+  const f4 s = v[0] + v[1] + v[2] + v[3];
+  const float x = (s[0] + s[1]) + (s[2] + s[3]);
+  return __ballot(x != x) != 0;
+}
 // fp16's range is small: its operands are brought to below 2^14 by the power of two that
-// this gives for their largest magnitude, and the product back by its inverse.  bf16 needs none.
+// this gives for their largest finite magnitude, and the product back by its inverse.  bf16 needs none.
 template <bool BF>
 __device__ __forceinline__ int range_exponent(float largest) {
-  if (BF || !(largest > 0.f) || isinf(largest)) return 0;
+  if (BF || !(largest > 0.f)) return 0;
   return min(13 - ilogbf(largest), 120);
 }
+__device__ __forceinline__ float finite_magnitude(float v) { return isfinite(v) ? fabsf(v) : 0.f; }
 __device__ __forceinline__ float times_pow2(float v, int e) { return __builtin_ldexpf(v, e); }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }  // |e| below 127
 

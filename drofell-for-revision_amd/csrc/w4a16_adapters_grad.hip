@@ -124,6 +124,17 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
           if (!in) at[q][u][j] = u4{};
         }
   }
+  bool odd_a = false;  // whether A has values that are not finite
+  if constexpr (DX) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) add_nonfinite<BF>(at[q][u][j], bits);
+    odd_a = __ballot((bits & 0x80008000u) != 0) != 0;
+  }
   const Philox philox(DROP ? p.seed : reinterpret_cast<const int64_t*>(p.plan));
   const int64_t half = p.l.positions * kR;
   f4 acc[4][NT] = {};
@@ -253,12 +264,45 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
         x[t][i] = x2[t][i];
       }
   }
+  // Infinities (finite_only()): a sum that is NaN may be so by its second parts alone.  It is formed once more, by
+  // itself, from the first parts, beside which nothing finite counts.  dx: where A holds some, by the lanes that
+  // stored it.
+  if constexpr (DX) {
+    if (odd_a) {
+#pragma unroll 1
+      for (int i = 0; wave * kStep + i / 4 * kStride < chunk.z; ++i) {
+        const int from = wave * kStep + i / 4 * kStride + i % 4 * 8 + line;
+        if (from >= chunk.z) continue;
+        const int to = order[from];
+        const uint16_t* dh = o.packs.row + (int64_t)(chunk.y + from) * kR;
+        const u4 kept = DROP ? philox.mask(k >> 3, to, p.drop) : ~u4{};
+#pragma unroll 1
+        for (int e = 0; e < 8 && k + e < o.width; ++e) {
+          const uint16_t* a = o.at + ((int64_t)ad * o.width + k + e) * p.r;
+          float s = 0.f;
+          for (int r = 0; r < p.r; ++r) s += unpack16<BF>(a[r], 0) * unpack16<BF>(dh[r], 0);
+          if (!isfinite(s) && (kept[e >> 1] >> (16 * (e & 1)) & 1)) p.dx[to * p.lddx + k + e] = (uint16_t)pack16<BF>(s, 0.f);
+        }
+      }
+    }
+  }
   if (o.share == nullptr) return;
   // the waves' sums, 16 columns of h at a time
   float* const sums = reinterpret_cast<float*>(lds);  // [waves][16][kSumPitch]
   const bool alone = p.plan[p.l.chunk_start + ad + 1] - p.plan[p.l.chunk_start + ad] == 1;
   float* share = o.share + (int64_t)chunk_index * o.width * p.r;
   uint16_t* grad = o.grad + (int64_t)ad * o.width * p.r;
+  auto first_parts = [&](int r, int col, float sum) {
+    float s = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < chunk.z; ++i) {
+      const int from = order[i], pos = chunk.y + i;
+      uint32_t v = o.in[from * o.ld + k0 + col];
+      if constexpr (DROP) v &= philox.mask((k0 + col) >> 3, from, p.drop)[(col & 7) >> 1] >> (16 * (col & 1));
+      s += unpack16<BF>(v, 0) * unpack16<BF>(o.packs.col[(int64_t)(pos & ~7) * kR + r * 8 + (pos & 7)], 0);
+    }
+    return isfinite(s) ? sum : s;
+  };
   auto store = [&](int64_t at, f4 v) {
     if (alone) *(uint2*)(grad + at) = make_uint2(pack16<BF>(v[0], v[1]), pack16<BF>(v[2], v[3]));
     else *(f4*)(share + at) = v;
@@ -276,12 +320,22 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
       for (int w = 0; w < kOuterWaves; ++w)
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += sums[(w * 16 + r + e) * kSumPitch + col];
-      if (k0 + col < o.width && u * 16 + r < p.r) store((int64_t)(k0 + col) * p.r + u * 16 + r, v);
+      if (k0 + col < o.width && u * 16 + r < p.r) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (isnan(v[e])) v[e] = first_parts(u * 16 + r + e, col, v[e]);
+        store((int64_t)(k0 + col) * p.r + u * 16 + r, v);
+      }
     } else {
       const int r = threadIdx.x >> 4, col = (threadIdx.x & 15) * 4;
 #pragma unroll
       for (int w = 0; w < kOuterWaves; ++w) v += *(const f4*)(sums + (w * 16 + r) * kSumPitch + col);
-      if (k0 + col < o.width && u * 16 + r < p.r) store((int64_t)(u * 16 + r) * o.width + k0 + col, v);
+      if (k0 + col < o.width && u * 16 + r < p.r) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (isnan(v[e])) v[e] = first_parts(u * 16 + r, col + e, v[e]);
+        store((int64_t)(u * 16 + r) * o.width + k0 + col, v);
+      }
     }
   }
 }

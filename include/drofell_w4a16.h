@@ -666,7 +666,8 @@ int dw4_adapters_workspace_size(int num_rows, int num_adapters, int k, int n, in
 
 /* Gradients for the output gradient dout [num_rows][n], from the forward's inputs and h:
  * dx [num_rows][k] (of the adapters alone; zeros in rows without one), da and db (shapes of a
- * and b; zeros for adapters without rows); each may be NULL.  base's gradient is dout.
+ * and b; zeros for adapters without rows); each may be NULL, and lies apart from the inputs.
+ * base's gradient is dout.
  * num_rows at least 1.  workspace: dw4_adapters_workspace_size bytes (backward 1). */
 int dw4_adapters_backward(int dtype, int num_rows, int num_adapters, int k, int n, int rank,
                           const uint16_t* x, int64_t ldx, const uint16_t* dout, int64_t ldd,

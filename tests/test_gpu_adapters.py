@@ -561,3 +561,34 @@ def test_refusals(hip_device):
         CounterDropout(0.5)(torch.zeros(4, 4, device=dev), seed)
     with pytest.raises(ValueError):
         CounterDropout(0.5)(torch.zeros(4, 4, device=dev, dtype=F16))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("p", [0.0, 0.1])
+@pytest.mark.parametrize("rank", [8, 24, 64, 128])
+def test_infinities_are_those_of_the_sums(hip_device, rank, p, dtype):
+    """An infinity in x, in the output's gradient, in A or in B makes the results infinite or NaN where
+    it makes the formulas' sums so, with their signs, and leaves the others."""
+    case = Case(hip_device, 600, 72, 80, rank, 2, dtype, "one", dropout=p, trainable=True, seed=7)
+    case.index[:20] = 0
+    case.rows.update(case.index.to(hip_device))
+    keep = case.mask()[0]
+    row = next(t for t in range(300, 600) if keep is None or keep[t, 11])
+    for name, place in (("x", (row, 11)), ("x", (3, 70)), ("dout", (590, 33)), ("dout", (4, 0)), ("a", (1, rank - 1, 71)),
+                        ("b", (1, 13, rank // 2))):
+        for value in (float("inf"), -float("inf")):
+            say(f"infinity {value} in {name} {place}, rank {rank} p {p} {dtype}")
+            held = getattr(case, name)
+            was = held[place].clone()
+            held[place] = value
+            case.put()
+            want, err = case.want(grads=True)
+            got = case.grads()
+            held[place] = was
+            for what, g, w, e in zip(("out", "dx", "da", "db"), got, want, err):
+                g = g.cpu().double()
+                odd = ~w.isfinite()
+                assert torch.equal(g[odd].nan_to_num(7.0), w[odd].nan_to_num(7.0)), what
+                close = ~odd & e.isfinite()
+                assert ((g - w).abs() <= e)[close].all() and g[~odd].isfinite().all(), what
+    case.put()

@@ -12,6 +12,7 @@ from dataclasses import dataclass
 from typing import Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import flags
 
@@ -26,6 +27,13 @@ def int32(x: torch.Tensor, name: str) -> torch.Tensor:
     elif x.dtype not in (torch.int16, torch.int8, torch.uint8, torch.bool):
         raise ValueError(f"{name} must be integers")
     return x.to(torch.int32).contiguous()
+
+
+def no_tangents(*inputs: torch.Tensor) -> None:
+    """A call has no forward-mode derivative: one whose inputs carry a tangent is refused, where its
+    result would come without."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in inputs):
+        raise NotImplementedError("this call has no forward-mode derivative")
 
 
 @dataclass

@@ -30,7 +30,7 @@ from torch.autograd.graph import increment_version
 
 from hip_extends import _lib
 
-from ..block.common import int32
+from ..block.common import int32, no_tangents
 from .real import Linear
 
 _DTYPES = {torch.float16: _lib.DW4_F16, torch.bfloat16: _lib.DW4_BF16}
@@ -140,7 +140,7 @@ class LowRankAdapters(nn.Module):
         """x [..., in_features] and the projection's output ``base`` [..., out_features] ->
         base + each row's adapter's product.  ``seed``: int64 [2] on the device (seed and offset),
         read where dropout applies; another step takes another offset, another projection another
-        seed.  Differentiable (once) in x, base, ``a`` and ``b``.  ``output``, without gradients:
+        seed.  Differentiable (once, backward) in x, base, ``a`` and ``b``.  ``output``, without gradients:
         where the result goes: ``base`` itself, or memory apart from it."""
         params = self._parameters  # (attribute look-up on a module takes 0.4 us each)
         try:
@@ -161,6 +161,7 @@ class LowRankAdapters(nn.Module):
         if num_rows != rows.num_rows or rows.num_adapters != self.num_adapters:
             raise ValueError(f"rows were sorted for {rows.num_rows} rows of {rows.num_adapters} adapters, "
                              f"not for {num_rows} of {self.num_adapters}")
+        no_tangents(x, base, a, b, scaling)
         drop = self._dropped if self.training else 0
         seed = _seed(seed, device) if drop else None
         if scaling.dtype != torch.float32:  # (of a module that was made half)

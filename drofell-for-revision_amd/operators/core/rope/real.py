@@ -26,7 +26,7 @@ from torch.autograd.graph import increment_version
 from hip_extends import _lib
 
 from ... import flags
-from ..block.common import int32
+from ..block.common import int32, no_tangents
 from ..block.real import LayerBlocksHolder
 from .common import RotaryScaling, rotary_frequencies
 
@@ -84,6 +84,7 @@ class RotaryEmbedding:
                 raise ValueError(f"q, k and v must be on {self.device}")
         if dtype not in _DTYPES:
             raise TypeError("rotary positions run on fp16 or bf16")
+        no_tangents(*rows)
         if count > 1 << 22 or rows[0].shape[1] > 1 << 14 or rows[1].shape[1] > 1 << 14:
             raise ValueError("a call turns up to 2^22 rows and 2^14 heads")
         return count
@@ -113,7 +114,7 @@ class RotaryEmbedding:
                 positions: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """q [rows, heads, head_dim] and k [rows, kv heads, head_dim] turned by their rows'
         ``positions`` (integers [rows] within 32 bits) -> new tensors.  Differentiable in q and k
-        (once)."""
+        (once, backward)."""
         pos = self._positions(positions, self._check(q, k))
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
             return _Rotary.apply(q, k, pos, self)

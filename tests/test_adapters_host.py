@@ -4,9 +4,11 @@ published numbers."""
 from __future__ import annotations
 
 import ctypes
+from types import SimpleNamespace
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from hip_extends import _lib
 from operators.core.linear.adapters import AdaptedLinear, AdapterRows, CounterDropout, LowRankAdapters
@@ -219,3 +221,41 @@ def test_a_projection_that_returns_its_input_keeps_it():
     x = torch.zeros(4, 64, dtype=torch.float16)
     AdaptedLinear(_Passes(), Bank())(x, rows=object())
     assert seen == [None]
+
+
+def cpu_rotary(head_dim):
+    """A RotaryEmbedding whose checks run on the CPU."""
+    r = object.__new__(RotaryEmbedding)
+    r.device, r.head_dim, r.rotary_dim, r.interleaved, r.magnitude = torch.device("cpu"), head_dim, head_dim, False, 1.0
+    return r
+
+
+class _Doubles(_Passes):
+    def forward(self, x):
+        return x * 2
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A result without its tangent would be a wrong derivative, and one written into the projection's
+    output would keep the projection's tangent alone."""
+    rows = SimpleNamespace(device=torch.device("cpu"), num_rows=4, num_adapters=2, plan=None)
+    x, t = torch.randn(4, 64).half(), torch.randn(4, 64).half()
+    rotary, pos = cpu_rotary(8), torch.arange(4)
+    for trainable in (False, True):
+        bank = LowRankAdapters(64, 64, 8, 2, trainable=trainable)
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, t)
+            for args in ((dual, x), (x, dual)):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    bank(*args, rows)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                AdaptedLinear(_Doubles(), bank)(dual, rows)
+            turned = forward_ad.make_dual(bank.a.detach(), torch.ones_like(bank.a))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.func.functional_call(bank, {"a": turned}, (x, x, rows))
+            q, plain = dual.view(4, 8, 8), x.view(4, 8, 8)
+            for pair in ((q, plain), (plain, q)):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    rotary.forward(*pair, pos)
+            with pytest.raises(ValueError):  # without tangents: no HIP device
+                bank(x, x, rows)

@@ -361,3 +361,20 @@ def test_requests_with_adapters_through_a_stage(hip_device):
                 # the bound of windowed attention's own tests is finer; here the wiring is what counts
                 assert (out[at + i].double().cpu() - want).abs().max() <= 2.0 ** -9 * values.abs().max()
             at += n
+
+
+def test_forward_mode_derivatives_are_refused(hip_device):
+    say("forward-mode derivatives")
+    g = torch.Generator().manual_seed(4)
+    holder, pages = cache(hip_device, 4, 2, 64, 16, F16, g)
+    rotary = RotaryEmbedding(64, device=hip_device)
+    q, k = torch.randn(6, 4, 64, generator=g).to(hip_device, F16), torch.randn(6, 2, 64, generator=g).to(hip_device, F16)
+    pos = torch.arange(6, device=hip_device)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(k, torch.ones_like(k))
+        for call in (lambda: rotary.forward(q, dual, pos), lambda: rotary.forward_cached(q, k, dual, pos, pos, holder),
+                     lambda: rotary.forward_cached(q, dual, k, pos, pos, holder, output=q)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        rotary.forward(q, k, pos)
+    assert all(torch.equal(t.cpu(), p) for t, p in zip(holder.contigious_kv_tenosr, pages))

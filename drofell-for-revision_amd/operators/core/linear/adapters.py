@@ -129,6 +129,8 @@ class LowRankAdapters(nn.Module):
             raise IndexError(f"there are {self.num_adapters} adapters")
         if r > self.rank or lora_a.shape != (r, self.in_features) or lora_b.shape != (self.out_features, r):
             raise ValueError(f"A and B must be [r, {self.in_features}] and [{self.out_features}, r], r up to {self.rank}")
+        if "a" not in self._parameters or "b" not in self._parameters:
+            raise RuntimeError("A or B is parametrized: load into what it is made of")
         self.a[index].zero_()
         self.b[index].zero_()
         self.a[index, :r].copy_(lora_a)

@@ -259,3 +259,14 @@ def test_forward_mode_derivatives_are_refused():
                     rotary.forward(*pair, pos)
             with pytest.raises(ValueError):  # without tangents: no HIP device
                 bank(x, x, rows)
+
+
+@pytest.mark.parametrize("name", ["a", "b"])
+def test_loading_into_parametrized_adapters_is_refused(name):
+    """What a parametrization gives is a tensor of the moment: matrices copied there are lost."""
+    bank = LowRankAdapters(64, 32, 8, 2)
+    torch.nn.utils.parametrize.register_parametrization(bank, name, torch.nn.Identity())
+    before = {k: t.clone() for k, t in bank.state_dict().items()}
+    with pytest.raises(RuntimeError, match="parametrized"):
+        bank.load(0, torch.ones(8, 64), torch.ones(32, 8), 2.0)
+    assert all(torch.equal(t, before[k]) for k, t in bank.state_dict().items())

@@ -131,10 +131,11 @@ class LowRankAdapters(nn.Module):
             raise ValueError(f"A and B must be [r, {self.in_features}] and [{self.out_features}, r], r up to {self.rank}")
         if "a" not in self._parameters or "b" not in self._parameters:
             raise RuntimeError("A or B is parametrized: load into what it is made of")
-        self.a[index].zero_()
-        self.b[index].zero_()
-        self.a[index, :r].copy_(lora_a)
-        self.b[index, :, :r].copy_(lora_b)
+        a, b = torch.zeros_like(self.a[index]), torch.zeros_like(self.b[index])  # (the matrices may be parts of the bank)
+        a[:r].copy_(lora_a)
+        b[:, :r].copy_(lora_b)
+        self.a[index].copy_(a)
+        self.b[index].copy_(b)
         self.scaling[index] = scaling
 
     def forward(self, x: torch.Tensor, base: torch.Tensor, rows: AdapterRows, seed: Optional[torch.Tensor] = None,

@@ -270,3 +270,19 @@ def test_loading_into_parametrized_adapters_is_refused(name):
     with pytest.raises(RuntimeError, match="parametrized"):
         bank.load(0, torch.ones(8, 64), torch.ones(32, 8), 2.0)
     assert all(torch.equal(t, before[k]) for k, t in bank.state_dict().items())
+
+
+def test_loading_parts_of_the_bank():
+    """An adapter from the bank itself, in its own place with another scaling or moved up in rank, and
+    from another's place."""
+    bank = LowRankAdapters(64, 32, 16, 2)
+    with torch.no_grad():
+        bank.b.normal_()
+    a, b = bank.a.detach().clone(), bank.b.detach().clone()
+    bank.load(0, bank.a[0], bank.b[0], 3.0)
+    assert torch.equal(bank.a, a) and torch.equal(bank.b, b) and bank.scaling.tolist() == [3.0, 1.0]
+    bank.load(0, bank.a[0, 5:], bank.b[0, :, 5:], 2.0)
+    assert torch.equal(bank.a[0, :11], a[0, 5:]) and torch.equal(bank.b[0, :, :11], b[0, :, 5:])
+    assert not bank.a[0, 11:].any() and not bank.b[0, :, 11:].any()
+    bank.load(1, bank.a[0, :11], bank.b[0, :, :11], 2.0)
+    assert torch.equal(bank.a[1], bank.a[0]) and torch.equal(bank.b[1], bank.b[0])

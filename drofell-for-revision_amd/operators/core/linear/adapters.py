@@ -27,11 +27,14 @@ from typing import Optional, Tuple
 import torch
 from torch import nn
 from torch.autograd.graph import increment_version
+from torch.nn.modules import module as _modules
 
 from hip_extends import _lib
 
 from ..block.common import int32, no_tangents
 from .real import Linear
+from .real_marlin import MarlinQuantLinear
+from .real_quant import QuantLinear
 
 _DTYPES = {torch.float16: _lib.DW4_F16, torch.bfloat16: _lib.DW4_BF16}
 
@@ -272,8 +275,16 @@ class AdaptedLinear(Linear):
         bank = self.adapters
         if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or bank.a.requires_grad or bank.b.requires_grad):
             return bank(x, y, rows, seed)
-        own = y.is_contiguous() and y.data_ptr() % 16 == 0 and y.data_ptr() != x.data_ptr()
-        return bank(x, y, rows, seed, output=y if own else None)
+        return bank(x, y, rows, seed, output=y if self._own(y) else None)
+
+    def _own(self, y: torch.Tensor) -> bool:
+        """Whether the projection's output is this call's alone, so that the sum may take its place: these
+        projections return new memory; of any other, of a hook that saw the output and of a ``forward``
+        put in its place nobody knows."""
+        base = self.base
+        return type(base) in (QuantLinear, MarlinQuantLinear) and not base._forward_hooks and \
+            not _modules._global_forward_hooks and "forward" not in base.__dict__ and \
+            y.is_contiguous() and y.data_ptr() % 16 == 0
 
 
 class CounterDropout(nn.Module):

@@ -13,6 +13,7 @@ from torch.autograd import forward_ad
 from hip_extends import _lib
 from operators.core.linear.adapters import AdaptedLinear, AdapterRows, CounterDropout, LowRankAdapters
 from operators.core.linear.real import Linear
+from operators.core.linear.real_quant import QuantLinear
 from operators.core.rope.common import RotaryScaling, rotary_frequencies
 from operators.core.rope.real import RotaryEmbedding
 from oracle import adapters as O
@@ -286,3 +287,52 @@ def test_loading_parts_of_the_bank():
     assert not bank.a[0, 11:].any() and not bank.b[0, :, 11:].any()
     bank.load(1, bank.a[0, :11], bank.b[0, :, :11], 2.0)
     assert torch.equal(bank.a[1], bank.a[0]) and torch.equal(bank.b[1], bank.b[0])
+
+
+class _Slice(_Passes):
+    def forward(self, x):
+        return x.flatten()[64:192].view(2, 64)  # begins inside x
+
+
+class _Keeps(_Passes):
+    def __init__(self):
+        super().__init__()
+        self.kept = torch.zeros(2, 64, dtype=torch.float16)
+
+    def forward(self, x):
+        return self.kept
+
+
+def test_sums_take_the_place_of_new_outputs_alone(monkeypatch):
+    """A projection's output is overwritten where it is known to be the call's own: not where it lies in
+    the input, where the projection keeps it, or where a hook has seen it."""
+    seen = []
+
+    class Bank(torch.nn.Module):
+        a = b = torch.zeros(1)
+
+        def forward(self, x, y, rows, seed=None, output=None):
+            seen.append(output is y)
+            return y
+
+    x = torch.zeros(4, 64, dtype=torch.float16)
+
+    def taken(base):
+        AdaptedLinear(base, Bank())(x, rows=object())
+        return seen.pop()
+
+    assert not taken(_Slice()) and not taken(_Keeps()) and not taken(_Doubles())
+    monkeypatch.setattr(QuantLinear, "forward", lambda self, x: x * 2)
+    quant = QuantLinear(64, 64, 64, False, False)
+    assert taken(quant)
+    hook = quant.register_forward_hook(lambda module, args, y: None)
+    assert not taken(quant)
+    hook.remove()
+    assert taken(quant)
+    hook = torch.nn.modules.module.register_module_forward_hook(lambda module, args, y: None)
+    try:
+        assert not taken(quant)
+    finally:
+        hook.remove()
+    quant.forward = lambda x: x
+    assert not taken(quant)

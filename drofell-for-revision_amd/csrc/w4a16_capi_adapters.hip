@@ -82,8 +82,9 @@ dw4::AdapterArgs adapter_args(int dtype, int rows, int k, int n, int rank, int a
 
 bool good_dtype(int dtype) { return dtype == DW4_F16 || dtype == DW4_BF16; }
 
-int check_rotary(int dtype, int rows, int heads, int kv_heads, int head_size, int rotary_size, float magnitude) {
+int check_rotary(int dtype, int rows, int heads, int kv_heads, int head_size, int rotary_size, int form, float magnitude) {
   if (!good_dtype(dtype)) return DW4_ERR_UNSUPPORTED;
+  if (form & ~(DW4_ROTARY_INTERLEAVED | DW4_ROTARY_POSITIONS64)) return DW4_ERR_INVALID_ARG;
   if (rows < 0 || heads < 0 || kv_heads < 0 || head_size <= 0 || rotary_size <= 0 || rotary_size > head_size ||
       !std::isfinite(magnitude))
     return DW4_ERR_INVALID_ARG;
@@ -195,11 +196,11 @@ int dw4_dropout(int dtype, int num_rows, int cols, const uint16_t* x, int64_t ld
                                        static_cast<hipStream_t>(stream)));
 }
 
-int dw4_rotary(int dtype, int num_rows, int num_heads, int num_kv_heads, int head_size, int rotary_size, int interleaved,
+int dw4_rotary(int dtype, int num_rows, int num_heads, int num_kv_heads, int head_size, int rotary_size, int form,
                int inverse, const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, uint16_t* q_out,
-               int64_t qo_stride, uint16_t* k_out, int64_t ko_stride, const int32_t* positions, const int64_t* turns,
+               int64_t qo_stride, uint16_t* k_out, int64_t ko_stride, const void* positions, const int64_t* turns,
                float magnitude, void* stream) {
-  DW4_TRY(check_rotary(dtype, num_rows, num_heads, num_kv_heads, head_size, rotary_size, magnitude));
+  DW4_TRY(check_rotary(dtype, num_rows, num_heads, num_kv_heads, head_size, rotary_size, form, magnitude));
   if (num_rows == 0 || num_heads + num_kv_heads == 0) return DW4_OK;
   if (positions == nullptr || turns == nullptr) return DW4_ERR_INVALID_ARG;
   if (num_heads > 0) {
@@ -212,7 +213,8 @@ int dw4_rotary(int dtype, int num_rows, int num_heads, int num_kv_heads, int hea
   }
   dw4::RotaryArgs a = {};
   a.bf16 = dtype == DW4_BF16;
-  a.interleaved = interleaved != 0;
+  a.interleaved = (form & DW4_ROTARY_INTERLEAVED) != 0;
+  a.positions64 = (form & DW4_ROTARY_POSITIONS64) != 0;
   a.inverse = inverse != 0;
   a.rows = num_rows;
   a.heads = num_heads;
@@ -234,11 +236,11 @@ int dw4_rotary(int dtype, int num_rows, int num_heads, int num_kv_heads, int hea
 }
 
 int dw4_rotary_and_cache(int dtype, int num_rows, int num_heads, int num_kv_heads, int head_size, int rotary_size,
-                         int interleaved, const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
-                         const uint16_t* v, int64_t v_stride, uint16_t* q_out, int64_t qo_stride, const int32_t* positions,
+                         int form, const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride,
+                         const uint16_t* v, int64_t v_stride, uint16_t* q_out, int64_t qo_stride, const void* positions,
                          const int64_t* turns, float magnitude, const int64_t* slots, int num_blocks, int block_size,
                          const int64_t* key_block_ptrs, const int64_t* value_block_ptrs, int kv_head_stride, void* stream) {
-  DW4_TRY(check_rotary(dtype, num_rows, num_heads, num_kv_heads, head_size, rotary_size, magnitude));
+  DW4_TRY(check_rotary(dtype, num_rows, num_heads, num_kv_heads, head_size, rotary_size, form, magnitude));
   if (block_size != 16 && block_size != 32) return DW4_ERR_UNSUPPORTED;
   if (num_blocks < 0 || num_kv_heads == 0 || num_heads == 0 || kv_head_stride < head_size * block_size) return DW4_ERR_INVALID_ARG;
   if (num_rows == 0) return DW4_OK;
@@ -251,7 +253,8 @@ int dw4_rotary_and_cache(int dtype, int num_rows, int num_heads, int num_kv_head
   if (kv_head_stride % 8 != 0) return DW4_ERR_MISALIGNED;
   dw4::RotaryArgs a = {};
   a.bf16 = dtype == DW4_BF16;
-  a.interleaved = interleaved != 0;
+  a.interleaved = (form & DW4_ROTARY_INTERLEAVED) != 0;
+  a.positions64 = (form & DW4_ROTARY_POSITIONS64) != 0;
   a.rows = num_rows;
   a.heads = num_heads;
   a.kv_heads = num_kv_heads;

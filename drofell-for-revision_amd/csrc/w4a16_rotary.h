@@ -7,7 +7,7 @@
 namespace dw4 {
 
 struct RotaryArgs {
-  bool bf16, interleaved, inverse;
+  bool bf16, interleaved, inverse, positions64;
   int rows, heads, kv_heads, head_size, rotary_size;
   const uint16_t* q;
   int64_t q_stride;
@@ -17,7 +17,7 @@ struct RotaryArgs {
   int64_t qo_stride;
   uint16_t* k_out;          // not with a cache
   int64_t ko_stride;
-  const int32_t* positions;
+  const void* positions;    // int32, or int64
   const int64_t* turns;     // [rotary_size / 2]: turns per position, times 2^64
   float magnitude;
   // cache

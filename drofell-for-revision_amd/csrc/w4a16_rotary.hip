@@ -5,7 +5,8 @@
 // same with the keys, and the values as they are, going to their cache slots.
 //
 // A frequency comes as a 64-bit fraction of a turn, so that its product with a position
-// wraps around at whole turns without rounding: angles are as exact at position 2^30 as at 2.
+// wraps around at whole turns without rounding: angles are as exact at position 2^30 as at 2 (the fraction's
+// own rounding, 2^-65 of a turn, reaches fp32's beyond position 2^38).
 //
 // Bound by memory: every element is read and written once.  A thread holds the sines and
 // cosines of eight pairs (four, interleaved) of a row and turns them in one head after the other.
@@ -46,7 +47,8 @@ struct Turn {
     const int pair = unit * kPairs;
     at = IL ? 2 * pair : pair;
     other = IL ? at : at + rd / 2;
-    const int64_t pos = p.positions[row];
+    const int64_t pos = p.positions64 ? static_cast<const int64_t*>(p.positions)[row]
+                                      : static_cast<const int32_t*>(p.positions)[row];
 #pragma unroll
     for (int e = 0; e < kPairs; ++e) {
       const uint64_t turns = (uint64_t)p.turns[pair + e] * (uint64_t)pos + (1u << 31);

@@ -29,6 +29,9 @@ NOALLOC_SCRATCH_BYTES = 64 << 20
 DW4_F16 = 0
 DW4_BF16 = 1
 
+DW4_ROTARY_INTERLEAVED = 1
+DW4_ROTARY_POSITIONS64 = 2
+
 DW4_PATH_AUTO = 0
 DW4_PATH_DECODE = 1
 DW4_PATH_PREFILL = 2

@@ -92,7 +92,12 @@ class RotaryEmbedding:
     def _positions(self, positions: torch.Tensor, rows: int) -> torch.Tensor:
         if positions.shape != (rows,) or positions.device != self.device:
             raise ValueError(f"positions must be {rows} integers on {self.device}")
-        return int32(positions, "positions")
+        # (every 64-bit number is a position)
+        return positions.contiguous() if positions.dtype is torch.int64 else int32(positions, "positions")
+
+    def _form(self, positions: torch.Tensor) -> int:
+        return (_lib.DW4_ROTARY_INTERLEAVED if self.interleaved else 0) | \
+            (_lib.DW4_ROTARY_POSITIONS64 if positions.dtype is torch.int64 else 0)
 
     def _turn(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
               inverse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -104,7 +109,7 @@ class RotaryEmbedding:
         kv_heads = k.shape[1]
         qo = torch.empty_like(q, memory_format=torch.contiguous_format)
         ko = torch.empty_like(k, memory_format=torch.contiguous_format)
-        _lib.call("dw4_rotary", _DTYPES[q.dtype], rows, heads, kv_heads, dims, self.rotary_dim, int(self.interleaved),
+        _lib.call("dw4_rotary", _DTYPES[q.dtype], rows, heads, kv_heads, dims, self.rotary_dim, self._form(positions),
                   int(inverse), q.data_ptr(), ldq, k.data_ptr(), ldk, qo.data_ptr(), heads * dims, ko.data_ptr(),
                   kv_heads * dims, positions.data_ptr(), self._turns.data_ptr(), self.magnitude,
                   _lib.current_stream(self.device.index))
@@ -113,11 +118,12 @@ class RotaryEmbedding:
     def forward(self, q: torch.Tensor, k: torch.Tensor,
                 positions: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """q [rows, heads, head_dim] and k [rows, kv heads, head_dim] turned by their rows'
-        ``positions`` (integers [rows] within 32 bits) -> new tensors.  Differentiable in q and k
+        ``positions`` (integers [rows]; angles are as exact as fp32's up to 2^38) -> new tensors.  Differentiable in q and k
         (once, backward)."""
         pos = self._positions(positions, self._check(q, k))
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-            return _Rotary.apply(q, k, pos, self)
+            # (64-bit positions may be counted on before the backward pass)
+            return _Rotary.apply(q, k, pos.clone() if pos is positions and pos.dtype is torch.int64 else pos, self)
         return self._turn(q, k, pos, False)
 
     def forward_cached(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -159,7 +165,7 @@ class RotaryEmbedding:
         (q2, ldq), (k2, ldk), (v2, ldv) = _rows(q), _rows(k), _rows(v)
         keys, values = kv_cacher.layer_key_ptr_table_device, kv_cacher.layer_val_ptr_table_device
         _lib.call("dw4_rotary_and_cache", _DTYPES[q.dtype], rows, heads, kv_heads, dims, self.rotary_dim,
-                  int(self.interleaved), q2.data_ptr(), ldq, k2.data_ptr(), ldk, v2.data_ptr(), ldv, output.data_ptr(),
+                  self._form(pos), q2.data_ptr(), ldq, k2.data_ptr(), ldk, v2.data_ptr(), ldv, output.data_ptr(),
                   ldo, pos.data_ptr(), self._turns.data_ptr(), self.magnitude, slots.data_ptr(),
                   min(keys.numel(), values.numel()), flags.BLOCK_SIZE, keys.data_ptr(), values.data_ptr(),
                   info.head_stride, _lib.current_stream(self.device.index))

@@ -688,29 +688,31 @@ int dw4_dropout(int dtype, int num_rows, int cols, const uint16_t* x, int64_t ld
 
 /* ---------------------------------------------------------------------------
  * Rotary positions: of every head's first rotary_size dims the pairs (i, i +
- * rotary_size / 2), or interleaved (2 i, 2 i + 1), turned by positions[row] times
- * the pair's frequency and scaled by magnitude; the other dims as they are.  turns (int64
+ * rotary_size / 2), or with DW4_ROTARY_INTERLEAVED in form (2 i, 2 i + 1), turned by
+ * positions[row] (int32, or with DW4_ROTARY_POSITIONS64 int64) times the pair's frequency and scaled by magnitude; the other dims as they are.  turns (int64
  * device [rotary_size / 2]): a frequency in turns per position, times 2^64 (modulo
- * 2^64; angles keep that precision at any position).  Computed in fp32, rounded once.
+ * 2^64; angles are as exact as fp32's up to positions of 2^38).  Computed in fp32, rounded once.
  * Beside dw4_rope (fp16 tables, half layout, in place).  q [num_rows][num_heads]
  * [head_size], k (and v) [num_rows][num_kv_heads][head_size] with row strides
  * (multiples of 8), 16-byte aligned; head_size a multiple of 8 up to 512, rotary_size
  * even; num_rows at most 2^22, num_rows * (num_heads + num_kv_heads) at most 2^27.  inverse:
  * turned back, which is the gradient.  Outputs may be the inputs.
  * ------------------------------------------------------------------------- */
+#define DW4_ROTARY_INTERLEAVED 1
+#define DW4_ROTARY_POSITIONS64 2
 int dw4_rotary(int dtype, int num_rows, int num_heads, int num_kv_heads, int head_size,
-               int rotary_size, int interleaved, int inverse, const uint16_t* q, int64_t q_stride,
+               int rotary_size, int form, int inverse, const uint16_t* q, int64_t q_stride,
                const uint16_t* k, int64_t k_stride, uint16_t* q_out, int64_t qo_stride,
-               uint16_t* k_out, int64_t ko_stride, const int32_t* positions, const int64_t* turns,
+               uint16_t* k_out, int64_t ko_stride, const void* positions, const int64_t* turns,
                float magnitude, void* stream);
 
 /* q turned into q_out, k turned and v as it is into their cache slots (slots int64 device
  * [num_rows], as in dw4_reshape_and_cache; a slot outside the num_blocks blocks is skipped;
  * no two rows may have one slot), in one launch.  k and v are not changed. */
 int dw4_rotary_and_cache(int dtype, int num_rows, int num_heads, int num_kv_heads, int head_size,
-                         int rotary_size, int interleaved, const uint16_t* q, int64_t q_stride,
+                         int rotary_size, int form, const uint16_t* q, int64_t q_stride,
                          const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
-                         uint16_t* q_out, int64_t qo_stride, const int32_t* positions,
+                         uint16_t* q_out, int64_t qo_stride, const void* positions,
                          const int64_t* turns, float magnitude, const int64_t* slots, int num_blocks,
                          int block_size, const int64_t* key_block_ptrs,
                          const int64_t* value_block_ptrs, int kv_head_stride, void* stream);

@@ -336,3 +336,13 @@ def test_sums_take_the_place_of_new_outputs_alone(monkeypatch):
         hook.remove()
     quant.forward = lambda x: x
     assert not taken(quant)
+
+
+def test_forms_of_rotary_calls():
+    lib = _lib.load()
+    for form in (4, -1, 1 << 20):
+        assert rotary(inter=form) == BAD
+        assert lib.dw4_rotary_and_cache(0, 9, 4, 2, 64, 64, form, FAKE, 256, FAKE, 128, FAKE, 128, FAKE, 256, FAKE, FAKE, 1.0, FAKE, 4, 16,
+                                        FAKE, FAKE, 1024, None) == BAD
+    for form in range(4):
+        assert rotary(rows=0, inter=form) == OK

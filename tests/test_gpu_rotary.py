@@ -378,3 +378,28 @@ def test_forward_mode_derivatives_are_refused(hip_device):
                 call()
         rotary.forward(q, k, pos)
     assert all(torch.equal(t.cpu(), p) for t, p in zip(holder.contigious_kv_tenosr, pages))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,rd,interleaved", [(128, 128, False), (64, 32, True), (64, 50, False)])
+def test_positions_of_64_bits(hip_device, hd, rd, interleaved, dtype):
+    """64-bit positions are what they are, also those that 32 bits do not hold."""
+    say(f"64-bit positions, heads of {hd}, {rd} turning, interleaved {interleaved} {dtype}")
+    g = torch.Generator().manual_seed(hd)
+    wide = [2 ** 31, 2 ** 31 + 4097, -2 ** 31 - 1, 2 ** 32, 2 ** 33 + 5, -2 ** 35 - 7, 2 ** 38 - 1, 2 ** 31 - 1, 0]
+    pos = torch.tensor(wide)
+    rotary = RotaryEmbedding(hd, rd, interleaved=interleaved, scaling=SCALINGS[4], device=hip_device)
+    q, k, v, dq, dk = (torch.randn(9, h, hd, generator=g).to(dtype) for h in (4, 2, 2, 4, 2))
+    there = pos.to(hip_device)
+    a, b = q.to(hip_device).requires_grad_(True), k.to(hip_device).requires_grad_(True)
+    qo, ko = rotary.forward(a, b, there)
+    there += 1  # (the next step's, before the backward pass)
+    grads = torch.autograd.grad((qo, ko), (a, b), (dq.to(hip_device), dk.to(hip_device)))
+    for name, got, x, inverse in (("q", qo, q, False), ("k", ko, k, False), ("dq", grads[0], dq, True), ("dk", grads[1], dk, True)):
+        check(got.detach(), *turned(x, pos, rotary, inverse), name)
+    holder, pages = cache(hip_device, 2, 2, hd, 16, dtype, g)
+    every_other = torch.stack([pos, pos * 0], 1).to(hip_device)[:, 0]
+    out = rotary.forward_cached(a.detach(), b.detach(), v.to(hip_device), every_other, torch.arange(9, device=hip_device), holder)
+    assert torch.equal(out, qo)
+    got = holder.contigious_kv_tenosr[0].cpu()[0, :, :, :9].permute(2, 0, 1, 3).reshape(9, 2, hd)
+    assert torch.equal(got, ko.detach().cpu())

@@ -132,7 +132,8 @@ class RotaryEmbedding:
         """q turned (returned, or written to ``output``: q itself, or memory apart from q, k and
         v), k turned and v into their cache ``slots`` (integers [rows]; -1: the row is not cached,
         and so is a slot outside the cache's blocks).  k and v stay as they are.  No two rows may
-        have one slot.  Without gradients: a backward pass through it raises."""
+        have one slot.  Without gradients: a backward pass through it, or through an ``output`` that
+        required a gradient, raises."""
         if not _lib.is_current(self.device):
             with torch.cuda.device(self.device):
                 return self.forward_cached(q, k, v, positions, slots, kv_cacher, output)
@@ -162,6 +163,8 @@ class RotaryEmbedding:
             same, ldo = _rows(output)
             if same is not output:
                 raise ValueError("output rows must be contiguous and 16-byte aligned")
+            if output.requires_grad and output.is_leaf and torch.is_grad_enabled():
+                raise RuntimeError("output is a leaf that requires a gradient")
         (q2, ldq), (k2, ldk), (v2, ldv) = _rows(q), _rows(k), _rows(v)
         keys, values = kv_cacher.layer_key_ptr_table_device, kv_cacher.layer_val_ptr_table_device
         _lib.call("dw4_rotary_and_cache", _DTYPES[q.dtype], rows, heads, kv_heads, dims, self.rotary_dim,
@@ -171,8 +174,8 @@ class RotaryEmbedding:
                   info.head_stride, _lib.current_stream(self.device.index))
         if given:
             increment_version(output)
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-            return _NoGradient.apply(output, q, k, v)
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or output.requires_grad):
+            return _NoGradient.apply(output, output.requires_grad, q, k, v)
         return output
 
 
@@ -197,10 +200,14 @@ class _Rotary(torch.autograd.Function):
 
 
 class _NoGradient(torch.autograd.Function):
-    """A backward pass that reaches the cached call fails instead of finding no gradient."""
+    """A backward pass that reaches the cached call fails instead of finding no gradient, or by way of
+    an output with a history of its own (the queries) that of what was there before."""
 
     @staticmethod
-    def forward(ctx, output, *inputs):
+    def forward(ctx, output, in_place, *inputs):
+        if in_place:
+            ctx.mark_dirty(output)
+            return output
         return output.detach()
 
     @staticmethod

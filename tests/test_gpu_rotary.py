@@ -403,3 +403,34 @@ def test_positions_of_64_bits(hip_device, hd, rd, interleaved, dtype):
     assert torch.equal(out, qo)
     got = holder.contigious_kv_tenosr[0].cpu()[0, :, :, :9].permute(2, 0, 1, 3).reshape(9, 2, hd)
     assert torch.equal(got, ko.detach().cpu())
+
+
+def test_turned_in_place_of_queries_with_a_gradient(hip_device):
+    """Queries that were overwritten no longer lead to what they were made of."""
+    say("in place of queries that require a gradient")
+    g = torch.Generator().manual_seed(6)
+    holder, _ = cache(hip_device, 4, 2, 64, 16, F16, g)
+    rotary = RotaryEmbedding(64, device=hip_device)
+    leaf = torch.randn(6, 4, 64, generator=g).to(hip_device, F16).requires_grad_(True)
+    k = torch.randn(6, 2, 64, generator=g).to(hip_device, F16)
+    pos = torch.arange(6, device=hip_device)
+    want = rotary.forward(leaf.detach(), k, pos)[0]
+    for made in (lambda: leaf * 1, lambda: (leaf.view(6, 256) * 1).view(6, 4, 64)):
+        q = made()
+        out = rotary.forward_cached(q, k, k, pos, pos, holder, output=q)
+        assert torch.equal(out, want) and torch.equal(q, want)
+        for t in (out, q):
+            with pytest.raises(RuntimeError, match="no gradients"):
+                t.sum().backward()
+    into = torch.empty_like(want)
+    out = rotary.forward_cached(leaf * 1, k, k, pos, pos, holder, output=into)
+    assert torch.equal(into, want) and not into.requires_grad
+    with pytest.raises(RuntimeError, match="no gradients"):
+        out.sum().backward()
+    other = leaf * 1
+    rotary.forward_cached(want.clone(), k, k, pos, pos, holder, output=other)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        other.sum().backward()
+    with pytest.raises(RuntimeError, match="leaf"):
+        rotary.forward_cached(leaf, k, k, pos, pos, holder, output=leaf)
+    assert torch.equal(rotary.forward(leaf.detach(), k, pos)[0], want)

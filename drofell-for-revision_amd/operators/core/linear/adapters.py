@@ -162,7 +162,11 @@ class LowRankAdapters(nn.Module):
             raise ValueError(f"x and base must be [..., {self.in_features}] and [..., {self.out_features}] of the same rows")
         if dtype not in _DTYPES or base.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
             raise TypeError("x, base and the adapters must be of one type, fp16 or bf16")
-        if base.device != device or a.device != device or scaling.device != device or rows.device != device:
+        if a.shape != (self.num_adapters, self.rank, width) or scaling.shape != (self.num_adapters,) or \
+                b.shape != (self.num_adapters, self.out_features, self.rank):
+            raise ValueError(f"A, B and the scaling must keep the shapes of {self.num_adapters} adapters of rank {self.rank}")
+        if base.device != device or a.device != device or b.device != device or scaling.device != device or \
+                rows.device != device:
             raise ValueError(f"x, base, the adapters and their rows must be on one device ({device})")
         if num_rows != rows.num_rows or rows.num_adapters != self.num_adapters:
             raise ValueError(f"rows were sorted for {rows.num_rows} rows of {rows.num_adapters} adapters, "

@@ -346,3 +346,19 @@ def test_forms_of_rotary_calls():
                                         FAKE, FAKE, 1024, None) == BAD
     for form in range(4):
         assert rotary(rows=0, inter=form) == OK
+
+
+def test_replaced_adapters_keep_their_shapes():
+    """A parametrization, a functional call or an assignment may bring other tensors than the module was
+    made with: the kernels would read past them."""
+    rows = SimpleNamespace(device=torch.device("cpu"), num_rows=4, num_adapters=2, plan=None)
+    bank, x = LowRankAdapters(64, 32, 8, 2), torch.zeros(4, 64).half()
+    base = torch.zeros(4, 32).half()
+    for name, shape in (("a", (1, 8, 64)), ("a", (2, 8, 32)), ("a", (2, 16, 64)), ("a", (8, 64)), ("b", (1, 32, 8)), ("b", (2, 32, 16)),
+                        ("b", (2, 24, 8)), ("scaling", (1,)), ("scaling", (2, 1))):
+        other = torch.zeros(shape, dtype=torch.float32 if name == "scaling" else torch.float16)
+        with pytest.raises(ValueError, match="shapes"):
+            torch.func.functional_call(bank, {name: other}, (x, base, rows))
+    for name in ("a", "b", "scaling"):
+        with pytest.raises(ValueError, match="one device"):
+            torch.func.functional_call(bank, {name: getattr(bank, name).detach().to("meta")}, (x, base, rows))

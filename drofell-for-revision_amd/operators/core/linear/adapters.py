@@ -187,6 +187,8 @@ class LowRankAdapters(nn.Module):
         if output.shape != base.shape or output.dtype != dtype or output.device != device or \
                 not output.is_contiguous() or output.data_ptr() % 16:
             raise ValueError("output must be contiguous and 16-byte aligned, of base's shape, type and device")
+        if output.requires_grad and torch.is_grad_enabled():
+            raise ValueError("output is for calls without gradients, and has one")
         _forward(x2, base2, a, b, scaling, rows.plan, drop, seed, output.view(-1, self.out_features), False)
         increment_version(output)
         return output

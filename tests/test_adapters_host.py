@@ -362,3 +362,13 @@ def test_replaced_adapters_keep_their_shapes():
     for name in ("a", "b", "scaling"):
         with pytest.raises(ValueError, match="one device"):
             torch.func.functional_call(bank, {name: getattr(bank, name).detach().to("meta")}, (x, base, rows))
+
+
+def test_an_output_with_a_gradient_is_refused():
+    """What is written over would keep the gradient of what was there."""
+    rows = SimpleNamespace(device=torch.device("cpu"), num_rows=4, num_adapters=2, plan=None)
+    bank, x = LowRankAdapters(64, 32, 8, 2), torch.zeros(4, 64).half()
+    base, into = torch.zeros(4, 32).half(), torch.zeros(4, 32).half().requires_grad_(True)
+    for output in (into, into * 1):
+        with pytest.raises(ValueError, match="without gradients"):
+            bank(x, base, rows, output=output)

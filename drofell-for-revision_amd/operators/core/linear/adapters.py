@@ -116,12 +116,19 @@ class LowRankAdapters(nn.Module):
             raise ValueError("there are 1 to 1024 adapters")
         self.in_features, self.out_features, self.rank, self.num_adapters = in_features, out_features, rank, num_adapters
         self.dropout = dropout
-        self._dropped = _drop(dropout)
         self.a = nn.Parameter(torch.randn(num_adapters, rank, in_features, dtype=torch.float32, device=device)
                               .mul_(in_features ** -0.5).to(dtype), requires_grad=trainable)
         self.b = nn.Parameter(torch.zeros(num_adapters, out_features, rank, dtype=dtype, device=device),
                               requires_grad=trainable)
         self.register_buffer("scaling", torch.ones(num_adapters, dtype=torch.float32, device=device))
+
+    @property
+    def dropout(self) -> float:
+        return self._dropout
+
+    @dropout.setter
+    def dropout(self, p: float) -> None:
+        self._dropout, self._dropped = p, _drop(p)
 
     @torch.no_grad()
     def load(self, index: int, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: float) -> None:
@@ -301,7 +308,14 @@ class CounterDropout(nn.Module):
     def __init__(self, p: float) -> None:
         super().__init__()
         self.p = p
-        self._dropped = _drop(p)
+
+    @property
+    def p(self) -> float:
+        return self._p
+
+    @p.setter
+    def p(self, p: float) -> None:
+        self._p, self._dropped = p, _drop(p)
 
     def forward(self, x: torch.Tensor, seed: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``seed``: int64 [2] on the device, seed and offset; another step takes another offset.

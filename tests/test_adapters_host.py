@@ -372,3 +372,16 @@ def test_an_output_with_a_gradient_is_refused():
     for output in (into, into * 1):
         with pytest.raises(ValueError, match="without gradients"):
             bank(x, base, rows, output=output)
+
+
+def test_the_probability_of_dropout_may_change():
+    drop, bank = CounterDropout(0.5), LowRankAdapters(64, 32, 8, 2, dropout=0.5)
+    x = torch.zeros(4, 64).half()
+    drop.p = 0.0
+    assert drop(x) is x and drop.p == 0.0  # no seed is read
+    bank.dropout = 0.25
+    assert bank.dropout == 0.25 and bank._dropped == 16384
+    for change in (lambda: setattr(drop, "p", 1.5), lambda: setattr(bank, "dropout", -0.5)):
+        with pytest.raises(ValueError):
+            change()
+    assert drop.p == 0.0 and bank.dropout == 0.25

@@ -16,14 +16,15 @@ constexpr int kAdapterMaxRows = 1 << 24;
 // How the rows of a call are laid out by adapter: rows sorted by adapter (those
 // without one last), each adapter's from a tile of its own on.  A tile holds
 // kTileRows positions of one adapter, a chunk up to kChunkRows rows of it.
-// The counts are bounds that the host knows.
+// Chunks of an adapter that has several leave a share of its gradients each.
+// The counts are bounds that the host knows: an adapter has several chunks from kChunkRows + 1 rows on.
 //
 // Measured against tiles of 64 positions (both products of a serving call, 4096 x 4096, rank 16): 256 rows of
 // 32 adapters 9.9 us against 12.1, 2048 rows of 8 18.4 against 24.5, 8192 of 8 51 against 73; only
 // rank 64 with all rows on one adapter had gained from 64 (4096 rows 58 against 65).
 constexpr int kTileRows = 32, kChunkRows = 512;
 struct AdapterLayout {
-  int tiles, chunks;
+  int tiles, chunks, shares;
   int64_t positions;
   // offsets (int32) in the plan
   int64_t tile_adapter, chunk, chunk_start, order, ints;
@@ -33,6 +34,8 @@ inline AdapterLayout adapter_layout(int rows, int adapters) {
   const int segs = std::min(adapters + 1, rows);
   l.tiles = rows / kTileRows + segs;
   l.chunks = rows / kChunkRows + segs;
+  l.shares = rows / kChunkRows + std::min(adapters, rows / (kChunkRows + 1));
+  if (rows <= kChunkRows) l.shares = 0;
   l.positions = (int64_t)l.tiles * kTileRows;
   l.tile_adapter = 4;  // behind the head: [0] tiles that hold rows
   l.chunk = l.tile_adapter + ((l.tiles + 3) & ~3);
@@ -129,8 +132,8 @@ inline BackwardWs backward_ws(const AdapterLayout& l, int k, int n, int r, int a
   w.row = w.bt + up256((size_t)2 * adapters * r * n);
   w.col = w.row + up256(row_pack_bytes(l, r));
   w.da = w.col + up256(col_pack_bytes(l, r));
-  w.db = w.da + up256(sizeof(float) * l.chunks * (size_t)r * k);
-  w.bytes = w.db + sizeof(float) * l.chunks * (size_t)r * n;
+  w.db = w.da + up256(sizeof(float) * l.shares * (size_t)r * k);
+  w.bytes = w.db + sizeof(float) * l.shares * (size_t)r * n;
   return w;
 }
 

@@ -76,7 +76,8 @@ plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__
   int* const total = count + kPlanWaves * segs;  // [segs]
   int* const tile0 = total + segs;               // [segs + 1]
   int* const chunk0 = tile0 + segs + 1;          // [segs + 1]
-  int* const wave_sum = chunk0 + segs + 1;
+  int* const share0 = chunk0 + segs + 1;         // [segs + 1]
+  int* const wave_sum = share0 + segs + 1;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   for (int i = t; i < kPlanWaves * segs; i += kPlanThreads) count[i] = 0;
   __syncthreads();
@@ -94,10 +95,12 @@ plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__
     total[s] = n;
     tile0[s] = (n + kTileRows - 1) / kTileRows;
     chunk0[s] = (n + kChunkRows - 1) / kChunkRows;
+    share0[s] = s < adapters && n > kChunkRows ? chunk0[s] : 0;
   }
   __syncthreads();
   scan_ints(tile0, segs, wave_sum);
   scan_ints(chunk0, segs, wave_sum);
+  scan_ints(share0, segs, wave_sum);
   for (int s = t; s < segs; s += kPlanThreads) {
     int at = tile0[s] * kTileRows;
     for (int w = 0; w < kPlanWaves; ++w) {
@@ -111,10 +114,10 @@ plan_kernel(AdapterLayout l, int rows, int adapters, const int32_t* __restrict__
   for (int i = t; i < l.tiles; i += kPlanThreads)
     plan[l.tile_adapter + i] = i < tile0[segs] ? segment_of(tile0, segs, i) : -1;
   for (int i = t; i < l.chunks; i += kPlanThreads) {
-    int4 c = make_int4(-1, 0, 0, 0);  // adapter, first position, rows, none
+    int4 c = make_int4(-1, 0, 0, -1);  // adapter, first position, rows, share or -1
     if (i < chunk0[segs]) {
-      const int s = segment_of(chunk0, segs, i), at = (i - chunk0[s]) * kChunkRows;
-      c = make_int4(s, tile0[s] * kTileRows + at, min(kChunkRows, total[s] - at), 0);
+      const int s = segment_of(chunk0, segs, i), j = i - chunk0[s], at = j * kChunkRows;
+      c = make_int4(s, tile0[s] * kTileRows + at, min(kChunkRows, total[s] - at), share0[s] < share0[s + 1] ? share0[s] + j : -1);
     }
     *(int4*)(plan + l.chunk + 4 * i) = c;
   }
@@ -581,7 +584,7 @@ int adapter_splits(const AdapterLayout& l, int width, int cus) {
 
 hipError_t launch_adapter_plan(const AdapterLayout& l, int rows, int adapters, const int32_t* index, int32_t* plan,
                                hipStream_t stream) {
-  const size_t smem = sizeof(int) * ((kPlanWaves + 3) * (size_t)(adapters + 1) + 2 + kPlanWaves);
+  const size_t smem = sizeof(int) * ((kPlanWaves + 4) * (size_t)(adapters + 1) + 3 + kPlanWaves);
   plan_kernel<<<1, kPlanThreads, smem, stream>>>(l, rows, adapters, index, plan);
   return hipGetLastError();
 }

@@ -67,7 +67,7 @@ struct OuterArgs {
   int64_t ld;
   int width;
   AdapterPacks packs;
-  float* share;          // [chunks][r * width], or null
+  float* share;          // [shares][r * width], or null: no such gradient
   uint16_t* grad;        // [adapters][r * width], with share
   const uint16_t* at;    // DX: [adapters][width][r]
 };
@@ -289,8 +289,8 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
   if (o.share == nullptr) return;
   // the waves' sums, 16 columns of h at a time
   float* const sums = reinterpret_cast<float*>(lds);  // [waves][16][kSumPitch]
-  const bool alone = p.plan[p.l.chunk_start + ad + 1] - p.plan[p.l.chunk_start + ad] == 1;
-  float* share = o.share + (int64_t)chunk_index * o.width * p.r;
+  const bool alone = chunk.w < 0;
+  float* share = o.share + (int64_t)max(chunk.w, 0) * o.width * p.r;
   uint16_t* grad = o.grad + (int64_t)ad * o.width * p.r;
   auto first_parts = [&](int r, int col, float sum) {
     float s = 0.f;
@@ -390,13 +390,14 @@ __global__ void __launch_bounds__(kThreads) reduce_kernel(AdapterArgs p, const f
     const int c0 = p.plan[p.l.chunk_start + ad], c1 = p.plan[p.l.chunk_start + ad + 1];
     if (c1 - c0 == 1) continue;  // stored already
     f4 v = {};
-    for (int c = c0; c < c1; c += 4) {  // four loads in flight
+    if (c0 < c1) share += p.plan[p.l.chunk + 4 * c0 + 3] * each * 4;
+    for (int c = 0; c < c1 - c0; c += 4) {  // four loads in flight
       f4 x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = *(const f4*)(share + min(c + e, c1 - 1) * each * 4);
+      for (int e = 0; e < 4; ++e) x[e] = *(const f4*)(share + min(c + e, c1 - c0 - 1) * each * 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < c1) v += x[e];
+        if (c + e < c1 - c0) v += x[e];
     }
     *(uint2*)((is_a ? p.da : p.db) + (ad * each + q) * 4) = make_uint2(pack16<BF>(v[0], v[1]), pack16<BF>(v[2], v[3]));
   }

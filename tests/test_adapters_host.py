@@ -385,3 +385,15 @@ def test_the_probability_of_dropout_may_change():
         with pytest.raises(ValueError):
             change()
     assert drop.p == 0.0 and bank.dropout == 0.25
+
+
+def test_backward_workspaces_hold_what_is_written():
+    """Shares of gradients are for adapters of more than 512 rows: beside the turned weights a batch of few rows
+    an adapter needs little."""
+    for rows, count, rank, k, n in ((1024, 1024, 64, 4096, 11008), (512, 2, 128, 4096, 4096), (1, 1024, 8, 64, 64)):
+        turned = 2 * count * rank * (k + n)
+        need, _ = _lib.adapters_workspace_size(rows, count, k, n, rank, True)
+        several = rows // 512 + min(count, rows // 513) if rows > 512 else 0
+        # beside them: planes and packed operands, some 16 planes of 32 rows an adapter with rows
+        positions = 32 * (rows // 32 + min(count + 1, rows))
+        assert turned <= need <= turned + 4 * several * rank * (k + n) + positions * max(rank, 16) * (16 * 4 + 12) + 4096

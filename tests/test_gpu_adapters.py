@@ -592,3 +592,19 @@ def test_infinities_are_those_of_the_sums(hip_device, rank, p, dtype):
                 close = ~odd & e.isfinite()
                 assert ((g - w).abs() <= e)[close].all() and g[~odd].isfinite().all(), what
     case.put()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gradients_of_adapters_with_and_without_shares(hip_device, dtype):
+    """Adapters of one chunk of rows (their gradients are stored directly) between some of several, as many
+    as the rows allow, in any order of rows."""
+    counts = [513, 512, 0, 513, 1, 1025, 513]
+    rows = sum(counts) + 40
+    say(f"gradients of {counts} rows and 40 without adapter {dtype}")
+    case = Case(hip_device, rows, 72, 40, 24, len(counts), dtype, "one", trainable=True)
+    index = torch.cat([torch.full((n,), i) for i, n in enumerate(counts)] + [torch.full((40,), -1)])
+    for case.index in (index, index[torch.randperm(rows, generator=case.g)]):
+        case.rows.update(case.index.to(hip_device))
+        want, err = case.want(grads=True)
+        for name, g, w, e in zip(("out", "dx", "da", "db"), case.grads(), want, err):
+            check(g, w, e, name)

@@ -149,6 +149,12 @@ struct ShrinkArgs {
   const int64_t* seed;
   float* planes;
 };
+// Workgroups of the gradients' largest launches (w4a16_adapters_grad.hip): the weights turned around with g h^T, and
+// dh x^T with dx.
+inline int64_t grad_workgroups(const AdapterLayout& l, int k, int n, int r, int adapters) {
+  const int64_t kt = (k + 63) / 64, nt = (n + 63) / 64;
+  return std::max((r + 63) / 64 * (kt + nt) * adapters + l.chunks * nt, l.chunks * kt);
+}
 hipError_t launch_shrink(bool bf16, const ShrinkArgs& a, int splits, hipStream_t stream);
 hipError_t launch_join(const AdapterArgs& a, const float* planes, int splits, const AdapterPacks& p, hipStream_t stream);
 hipError_t launch_adapter_plan(const AdapterLayout& l, int rows, int adapters, const int32_t* index, int32_t* plan,

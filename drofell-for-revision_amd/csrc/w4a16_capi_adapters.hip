@@ -34,6 +34,12 @@ int check_shape(int rows, int adapters, int k, int n, int rank) {
   return DW4_OK;
 }
 
+// A launch counts its threads, 256 a workgroup, in 32 bits.
+int check_grad(int rows, int adapters, int k, int n, int rank) {
+  const dw4::AdapterLayout l = dw4::adapter_layout(rows, adapters);
+  return dw4::grad_workgroups(l, k, n, rank, adapters) < (int64_t)1 << 24 ? DW4_OK : DW4_ERR_UNSUPPORTED;
+}
+
 // A matrix [rows][width] of 16-bit values that kernels read or write in 16-byte units.
 int check_matrix(const void* p, int64_t stride, int rows, int width) {
   if (p == nullptr) return DW4_ERR_INVALID_ARG;
@@ -120,6 +126,7 @@ int dw4_adapters_workspace_size(int num_rows, int num_adapters, int k, int n, in
                                 size_t* h_bytes) {
   DW4_TRY(check_shape(num_rows, num_adapters, k, n, rank));
   if (workspace_bytes == nullptr) return DW4_ERR_INVALID_ARG;
+  if (backward) DW4_TRY(check_grad(num_rows, num_adapters, k, n, rank));
   const dw4::AdapterLayout l = dw4::adapter_layout(num_rows, num_adapters);
   if (h_bytes != nullptr) *h_bytes = num_rows ? dw4::col_pack_bytes(l, rank) : 0;
   *workspace_bytes = 0;
@@ -162,6 +169,7 @@ int dw4_adapters_backward(int dtype, int num_rows, int num_adapters, int k, int 
   DW4_TRY(check_shape(num_rows, num_adapters, k, n, rank));
   DW4_TRY(check_drop(drop, seed));
   if (num_rows == 0) return DW4_ERR_INVALID_ARG;  // nothing to reduce: the caller's zeros
+  DW4_TRY(check_grad(num_rows, num_adapters, k, n, rank));
   if (plan == nullptr || h == nullptr || (num_adapters > 0 && (a == nullptr || b == nullptr || scaling == nullptr)))
     return DW4_ERR_INVALID_ARG;
   DW4_TRY(check_matrix(x, ldx, num_rows, k));

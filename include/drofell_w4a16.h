@@ -668,7 +668,9 @@ int dw4_adapters_workspace_size(int num_rows, int num_adapters, int k, int n, in
  * dx [num_rows][k] (of the adapters alone; zeros in rows without one), da and db (shapes of a
  * and b; zeros for adapters without rows); each may be NULL, and lies apart from the inputs.
  * base's gradient is dout.
- * num_rows at least 1.  workspace: dw4_adapters_workspace_size bytes (backward 1). */
+ * num_rows at least 1.  Banks and batches for which a launch would have 2^32 threads are refused
+ * (some 2^29 columns of k + n over all adapters, or num_rows * max(k, n) of 2^39).
+ * workspace: dw4_adapters_workspace_size bytes (backward 1). */
 int dw4_adapters_backward(int dtype, int num_rows, int num_adapters, int k, int n, int rank,
                           const uint16_t* x, int64_t ldx, const uint16_t* dout, int64_t ldd,
                           const uint16_t* a, const uint16_t* b, const float* scaling,

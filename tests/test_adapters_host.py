@@ -397,3 +397,14 @@ def test_backward_workspaces_hold_what_is_written():
         # beside them: planes and packed operands, some 16 planes of 32 rows an adapter with rows
         positions = 32 * (rows // 32 + min(count + 1, rows))
         assert turned <= need <= turned + 4 * several * rank * (k + n) + positions * max(rank, 16) * (16 * 4 + 12) + 4096
+
+
+def test_gradients_beyond_a_launch_are_refused():
+    """A launch of 2^32 threads or more, which banks and batches within the other limits would need."""
+    size, out = _lib.load().dw4_adapters_workspace_size, ctypes.c_size_t(0)
+    for rows, count, k, n, rank in ((2000, 1024, 1 << 20, 64, 8), (2000, 512, 1 << 19, 1 << 19, 72), (1 << 24, 64, 1 << 20, 64, 8),
+                                    (1 << 24, 64, 64, 1 << 20, 8)):
+        assert size(rows, count, k, n, rank, 1, ctypes.byref(out), None) == UNSUP
+        assert size(rows, count, k, n, rank, 0, ctypes.byref(out), None) == OK
+        assert backward(rows=rows, count=count, k=k, n=n, rank=rank, ldx=k, ldg=n, lddx=k, wsb=1 << 62) == UNSUP
+    assert size(2000, 500, 1 << 19, 1 << 19, 8, 1, ctypes.byref(out), None) == OK

@@ -17,6 +17,8 @@ from __future__ import annotations
 import torch
 
 STEP = 2.0 ** -23
+# wide features: rows, k, n, rank, adapters, order of the rows' adapters
+WIDE = [(1, 4096, 64, 16, 1, "one"), (31, 4168, 1096, 8, 3, "mixed"), (65, 8200, 520, 72, 2, "runs"), (96, 64, 4360, 128, 3, "runs")]
 WORD = 0xFFFFFFFF
 
 
@@ -94,3 +96,16 @@ def low_rank(x, base, a, b, scaling, index, dout=None, mask=None, drop: int = 0)
         dx, edx = torch.where(mask, dx, 0.0), torch.where(mask, edx, 0.0)
     values, errors = (out, dx, da, db), (err, edx, eda, edb)
     return values, tuple(e + u * (v.abs() + e) + tiny for v, e in zip(values, errors))
+
+
+def whole_case(rows, k, n, rank, adapters, dtype, seed):
+    """(x, base, a, b, scaling, dout) of whole numbers, small enough that with a dropout of one half every sum
+    stays below 2^24 of its units in any order: float32 holds it exactly, two 16-bit parts hold h and dh (one
+    does not, where the features are wide), and results equal the formulas' rounded once."""
+    g = torch.Generator().manual_seed(seed)
+
+    def ints(most, *shape):
+        return torch.randint(-most, most + 1, shape, generator=g).to(dtype)
+
+    scaling = 2.0 ** -torch.randint(7, 10, (adapters,), generator=g).float()
+    return ints(31, rows, k), ints(100, rows, n), ints(3, adapters, rank, k), ints(1, adapters, n, rank), scaling, ints(63, rows, n)

@@ -408,3 +408,58 @@ def test_gradients_beyond_a_launch_are_refused():
         assert size(rows, count, k, n, rank, 0, ctypes.byref(out), None) == OK
         assert backward(rows=rows, count=count, k=k, n=n, rank=rank, ldx=k, ldg=n, lddx=k, wsb=1 << 62) == UNSUP
     assert size(2000, 500, 1 << 19, 1 << 19, 8, 1, ctypes.byref(out), None) == OK
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,k,n,rank,adapters,order", O.WIDE)
+def test_whole_numbers_tell_what_is_missing(rows, k, n, rank, adapters, order, dtype):
+    """The whole-number cases are exact, and show the last columns, a part of the reduced axis or the second part
+    of h or dh missing."""
+    x, base, a, b, s, dout = O.whole_case(rows, k, n, rank, adapters, dtype, 13)
+    index = torch.arange(rows) % adapters
+
+    def results(x=x, dout=dout, one_part=False):
+        """(out, db), (dx, da) with x, or dout, as the first products see them."""
+        out, dx = base.double().clone(), torch.zeros(rows, k).double()
+        da, db = torch.zeros(adapters, rank, k).double(), torch.zeros(adapters, n, rank).double()
+        for i in range(adapters):
+            t = index == i
+            f = 2 * float(s[i])
+            h, dh = f * (x[t].double() @ a[i].double().T), f * (dout[t].double() @ b[i].double())
+            if one_part:
+                h, dh = h.to(dtype).double(), dh.to(dtype).double()
+            out[t] += h @ b[i].double().T
+            db[i], dx[t], da[i] = whole[1][t].double().T @ h, dh @ a[i].double(), dh.T @ whole[0][t].double()
+        return (out, db), (dx, da)
+
+    whole = (x, dout)
+    want = results()
+    # exact: sums of absolute values in their units
+    for i in range(adapters):
+        h, dh = x.double().abs() @ a[i].double().abs().T, dout.double().abs() @ b[i].double().abs()
+        small = x.double() @ a[i].double().T, dout.double() @ b[i].double()
+        assert max(h.max(), dh.max()) < 2 ** 24 and max(v.abs().max() for v in small) < 2 ** 16
+        for sums in (small[0].abs() @ b[i].double().abs().T + 100 / s[i], dout.double().abs().T @ small[0].abs(),
+                     small[1].abs() @ a[i].double().abs(), small[1].abs().T @ x.double().abs()):
+            assert sums.max() < 2 ** 24
+    assert all(v.abs().max() < torch.finfo(torch.float16).max for pair in want for v in pair)
+
+    def differ(got, i):
+        return all(not torch.equal(g.to(dtype), w.to(dtype)) for g, w in zip(got[i], want[i]))
+
+    lost = torch.ones(k).to(dtype)
+    lost[-8:] = 0
+    assert differ(results(x=x * lost), 0)
+    lost = torch.ones(n).to(dtype)
+    lost[-8:] = 0
+    assert differ(results(dout=dout * lost), 1)
+    if k > 4000:
+        lost = torch.ones(k).to(dtype)
+        lost[256:320] = 0
+        assert differ(results(x=x * lost), 0)
+        assert differ(results(one_part=True), 0)
+    if n > 4000:
+        lost = torch.ones(n).to(dtype)
+        lost[256:320] = 0
+        assert differ(results(dout=dout * lost), 1)
+        assert differ(results(one_part=True), 1)

@@ -608,3 +608,21 @@ def test_gradients_of_adapters_with_and_without_shares(hip_device, dtype):
         want, err = case.want(grads=True)
         for name, g, w, e in zip(("out", "dx", "da", "db"), case.grads(), want, err):
             check(g, w, e, name)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("rows,k,n,rank,adapters,order", O.WIDE)
+def test_wide_features_exactly(hip_device, rows, k, n, rank, adapters, order, p, dtype):
+    """Whole numbers, whose sums float32 holds exactly: every part of the reduced axis, its last columns and
+    both parts of h and dh are in the results, to the bit."""
+    say(f"whole numbers, {rows} rows {k} -> {n}, rank {rank}, {adapters} adapters {order} p {p} {dtype}")
+    case = Case(hip_device, rows, k, n, rank, adapters, dtype, order, dropout=p, trainable=True, seed=13)
+    case.x, case.base, case.a, case.b, case.scaling, case.dout = O.whole_case(rows, k, n, rank, adapters, dtype, 13)
+    case.put()
+    want, _ = case.want(grads=True)
+    got = case.grads()
+    for name, g, w in zip(("out", "dx", "da", "db"), got, want):
+        assert torch.equal(g.cpu(), w.to(dtype)), name
+    with torch.no_grad():
+        assert torch.equal(case.run(), got[0])

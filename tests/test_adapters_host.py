@@ -4,6 +4,7 @@ published numbers."""
 from __future__ import annotations
 
 import ctypes
+import math
 from types import SimpleNamespace
 
 import pytest
@@ -463,3 +464,36 @@ def test_whole_numbers_tell_what_is_missing(rows, k, n, rank, adapters, order, d
         lost[256:320] = 0
         assert differ(results(dout=dout * lost), 1)
         assert differ(results(one_part=True), 1)
+
+
+def test_scalings_by_their_definitions():
+    """Each pair's frequency from wavelengths and from the places of the blend worked out by hand, apart from the
+    implementation."""
+    plain = [10000.0 ** (-i / 64) for i in range(64)]
+
+    def same(got, want):
+        assert len(got) == len(want) and all(abs(g / w - 1) < 1e-12 for g, w in zip(got, want))
+
+    same(rotary_frequencies(128, 10000.0)[0], plain)
+    same(rotary_frequencies(128, 10000.0, RotaryScaling("linear", 2.5))[0], [f / 2.5 for f in plain])
+    # the last of 64 pairs is divided by the factor: base' ^ (-126/128) = base ^ (-126/128) / factor
+    stretched = (10000.0 ** (126 / 128) * 8.0) ** (128 / 126)
+    same(rotary_frequencies(128, 10000.0, RotaryScaling("ntk", 8.0))[0], [stretched ** (-i / 64) for i in range(64)])
+    # by wavelength: below L / high as they are, above L / low divided, between them in turns
+    for length, low, high, factor in ((8192, 1.0, 4.0, 8.0), (4096, 0.5, 16.0, 32.0)):
+        want = []
+        for f in plain:
+            wave = 2 * math.pi / f
+            share = 1.0 if wave < length / high else 0.0 if wave > length / low else (length / wave - low) / (high - low)
+            want.append((1 - share) * f / factor + share * f)
+        assert 0 < sum(w not in (f, f / factor) for w, f in zip(want, plain)) < 30
+        same(rotary_frequencies(128, 10000.0, RotaryScaling("wavelength", factor, length, low=low, high=high))[0], want)
+    # by index: 64 ln(4096 / 64 pi) / ln 10000 = 20.9, 64 ln(4096 / 2 pi) / ln 10000 = 45.03: whole up to pair 20, divided from 46
+    # on, in 26 equal steps between
+    got, magnitude = rotary_frequencies(128, 10000.0, RotaryScaling("yarn", 8.0, 4096))
+    same(got, [f * (1 - min(max(i - 20, 0), 26) / 26 * (1 - 1 / 8)) for i, f in enumerate(plain)])
+    assert abs(magnitude - 1.2079441541679836) < 1e-15
+    # 16 of a head: 8 ln(1024 / 64 pi) / ln 500000 = 0.99, 8 ln(1024 / 2 pi) / ln 500000 = 3.1
+    got, magnitude = rotary_frequencies(16, 500000.0, RotaryScaling("yarn", 4.0, 1024, magnitude=0.5))
+    same(got, [500000.0 ** (-i / 8) * (1 - min(i, 4) / 4 * 0.75) for i in range(8)])
+    assert magnitude == 0.5

@@ -292,21 +292,11 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
   const bool alone = chunk.w < 0;
   float* share = o.share + (int64_t)max(chunk.w, 0) * o.width * p.r;
   uint16_t* grad = o.grad + (int64_t)ad * o.width * p.r;
-  auto first_parts = [&](int r, int col, float sum) {
-    float s = 0.f;
-#pragma unroll 1
-    for (int i = 0; i < chunk.z; ++i) {
-      const int from = order[i], pos = chunk.y + i;
-      uint32_t v = o.in[from * o.ld + k0 + col];
-      if constexpr (DROP) v &= philox.mask((k0 + col) >> 3, from, p.drop)[(col & 7) >> 1] >> (16 * (col & 1));
-      s += unpack16<BF>(v, 0) * unpack16<BF>(o.packs.col[(int64_t)(pos & ~7) * kR + r * 8 + (pos & 7)], 0);
-    }
-    return isfinite(s) ? sum : s;
-  };
   auto store = [&](int64_t at, f4 v) {
     if (alone) *(uint2*)(grad + at) = make_uint2(pack16<BF>(v[0], v[1]), pack16<BF>(v[2], v[3]));
     else *(f4*)(share + at) = v;
   };
+  bool odd = false;
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     __syncthreads();
@@ -321,9 +311,7 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += sums[(w * 16 + r + e) * kSumPitch + col];
       if (k0 + col < o.width && u * 16 + r < p.r) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (isnan(v[e])) v[e] = first_parts(u * 16 + r + e, col, v[e]);
+        odd = odd || isnan(v[0] + v[1] + v[2] + v[3]);
         store((int64_t)(k0 + col) * p.r + u * 16 + r, v);
       }
     } else {
@@ -331,12 +319,40 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
 #pragma unroll
       for (int w = 0; w < kOuterWaves; ++w) v += *(const f4*)(sums + (w * 16 + r) * kSumPitch + col);
       if (k0 + col < o.width && u * 16 + r < p.r) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (isnan(v[e])) v[e] = first_parts(u * 16 + r, col + e, v[e]);
+        odd = odd || isnan(v[0] + v[1] + v[2] + v[3]);
         store((int64_t)(u * 16 + r) * o.width + k0 + col, v);
       }
     }
+  }
+  if (!odd) return;
+  asm volatile("" ::: "memory");  // what the thread has stored is read as another type
+#pragma unroll 1
+  for (int i = 0; i < 4 * NT; ++i) {  // (the thread's places: once more behind the sums, whose registers are free now)
+    const int r = i / 4 * 16 + (COLS ? (threadIdx.x & 3) * 4 + i % 4 : threadIdx.x >> 4);
+    const int col = COLS ? threadIdx.x >> 2 : (threadIdx.x & 15) * 4 + i % 4;
+    if (k0 + col >= o.width || r >= p.r) continue;
+    const int64_t to = COLS ? (int64_t)(k0 + col) * p.r + r : (int64_t)r * o.width + k0 + col;
+    if (!isnan(alone ? unpack16<BF>(grad[to], 0) : share[to])) continue;
+    float s = 0.f;
+#pragma unroll 1
+    for (int t = 0; t < chunk.z && !isnan(s); t += 8) {  // eight positions' h side by side
+      u4 h = *(const u4*)(o.packs.col + (int64_t)(chunk.y + t) * kR + r * 8);
+      uint32_t v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = t + e < chunk.z ? o.in[order[t + e] * o.ld + k0 + col] : 0;
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) {
+        if (DROP && t + e < chunk.z)
+          v[0] &= philox.mask((k0 + col) >> 3, order[t + e], p.drop)[(col & 7) >> 1] >> (16 * (col & 1));
+        s += unpack16<BF>(v[0], 0) * unpack16<BF>(h[0], 0);
+#pragma unroll
+        for (int j = 0; j < 7; ++j) v[j] = v[j + 1];
+        h = u4{h[0] >> 16 | h[1] << 16, h[1] >> 16 | h[2] << 16, h[2] >> 16 | h[3] << 16, h[3] >> 16};
+      }
+    }
+    if (isfinite(s)) continue;
+    if (alone) grad[to] = (uint16_t)pack16<BF>(s, 0.f);
+    else share[to] = s;
   }
 }
 

@@ -20,8 +20,8 @@ constexpr int kAdapterMaxRows = 1 << 24;
 // The counts are bounds that the host knows: an adapter has several chunks from kChunkRows + 1 rows on.
 //
 // Measured against tiles of 64 positions (both products of a serving call, 4096 x 4096, rank 16): 256 rows of
-// 32 adapters 9.9 us against 12.1, 2048 rows of 8 18.4 against 24.5, 8192 of 8 51 against 73; only
-// rank 64 with all rows on one adapter had gained from 64 (4096 rows 58 against 65).
+// 32 adapters 9.9 us against 12.1, 2048 rows of 8 18.4 against 24.5, 8192 of 8 51 against 73.  Rank 64 with
+// all rows on one adapter is better off with 64 (4096 rows 58 against 65): one size serves all.
 constexpr int kTileRows = 32, kChunkRows = 512;
 struct AdapterLayout {
   int tiles, chunks, shares;
@@ -75,7 +75,7 @@ inline void place_col(AdapterPacks& p, const AdapterLayout& l, int r, void* at) 
 struct AdapterArgs {
   AdapterLayout l;
   bool bf16;
-  int rows, k, n, r, adapters;
+  int k, n, r, adapters;
   const int32_t* plan;
   const uint16_t* x;     // [rows][k]
   int64_t ldx;

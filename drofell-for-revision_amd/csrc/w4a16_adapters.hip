@@ -337,7 +337,8 @@ join_kernel(AdapterArgs p, const float* planes, int splits, AdapterPacks packs) 
 // first workgroup packs it by column: 5325 rows of rank 16 20.2 us that way, 18.7 by rows that a launch of
 // 4.1 had packed before; 1763 of rank 64 35.1, and 28.5 behind 5.1.
 // Bound by the output, read and written once as whole lines: 10175 rows of 4096 by rank 16 40 us for 169 MB,
-// 4.2 TB/s; rank 64 by 11008 is bound by B's way from the L2 to every tile (1763 rows 35 us for 91 MB).
+// 4.2 TB/s; rank 64 by 11008 by its reads of the L2, 241 MB for 91 (1763 rows 35 us): about 124 of planes, which
+// each of a tile's 17 workgroups sums anew, and 80 of B, which goes to every tile.
 // The first group's loads before the planes' sums take the registers of a wave (10175 rows 50.5 us for 40.2).
 template <bool BF, int NT>
 __global__ void __launch_bounds__(kThreads) expand_kernel(AdapterArgs p, int splits, AdapterPacks packs, int wide) {
@@ -560,8 +561,8 @@ void shrink_rank(const ShrinkArgs& a, int splits, hipStream_t stream) {
 template <bool BF, int NT>
 void expand_of(const AdapterArgs& a, int splits, const AdapterPacks& packs, hipStream_t stream) {
   const int groups = (a.n + 63) / 64;
-  // About four workgroups per CU of four waves each.  Half as many: 10175 rows against rank 16 76 us for 40;
-  // twice as many 39.6, but each sums the planes anew.
+  // About four workgroups per CU (of 256) of four waves each, by the bound of tiles (adapter_splits()).  Half as
+  // many: 10175 rows against rank 16 76 us for 40; twice as many 39.6, but each sums the planes anew.
   const int wide = std::max(1, std::min((groups + 3) / 4, 1024 / a.l.tiles));
   expand_kernel<BF, NT><<<(unsigned)a.l.tiles * wide, kThreads, 0, stream>>>(a, splits, packs, wide);
 }
@@ -578,6 +579,8 @@ void expand_rank(const AdapterArgs& a, int splits, const AdapterPacks& packs, hi
 int adapter_splits(const AdapterLayout& l, int width, int cus) {
   // About four workgroups per CU, parts of at least 64 values per wave, up to 16 planes.  Up to 8: 1 row of
   // 11008 by rank 16 7.1 us for 6.75 (both products), 2048 rows by rank 64 40.0 for 41.9; up to 4: 8.1 and 40.4.
+  // The bound of tiles counts one more for each adapter of the bank: in a bank of many hundred, of which few are
+  // used, there are fewer workgroups (1024 rows of 3 adapters 11.7 us in a bank of 8, 18 in one of 256, 40 in 1024).
   const int want = (4 * cus + l.tiles - 1) / l.tiles;
   return std::max(1, std::min({want, width / 256, kMaxSplits}));
 }

@@ -9,7 +9,9 @@
 // workgroup; dx comes from the same tile of x and its dropout mask.  The chunks' shares of
 // dA and dB are added up in order: no float atomics.
 //
-// Bound by memory: x, g and dx pass once, g a second time on its way to dh.  Chunks of 256 rows took longer
+// Bound by memory: x, g and dx pass once, g a second time on its way to dh, with two to four waves a SIMD at ranks up
+// to 32 and two at 64; rank 64 with dropout, and 128 with dx, hold operands and sums of the whole rank in one
+// wave's registers.  Chunks of 256 rows took longer
 // for their shares, chunks of 1024 left CUs idle; workgroups of eight waves were slower than of four.
 
 #include <hip/hip_runtime.h>
@@ -357,7 +359,7 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
 }
 
 // The first launch of a backward pass: A [r][k] turned to [k][r] and B [n][r] to [r][n], and g h^T.  5325 rows
-// of 4096 by rank 16 14.6 us for 51 MB (3.5 TB/s), 1763 of 11008 by rank 64 22.2 us for 63 MB (2.8 TB/s).
+// of 4096 by rank 16 14.3 us for 51 MB (3.5 TB/s), 1763 of 11008 by rank 64 22.0 us for 63 MB (2.9 TB/s).
 template <bool BF, int NT>
 __global__ void __launch_bounds__(kOuterThreads)
 first_kernel(AdapterArgs p, OuterArgs o, uint16_t* at, uint16_t* bt, int a_tiles, int b_tiles) {
@@ -382,8 +384,8 @@ first_kernel(AdapterArgs p, OuterArgs o, uint16_t* at, uint16_t* bt, int a_tiles
   const int cols = (o.width + 63) / 64;
   outer<BF, NT, false, false, true>(p, o, i / cols, i % cols * 64, lds);
 }
-// dh x^T and dx, of the same tiles of x.  5325 rows of 4096 by rank 16 with dropout 27.1 us for 96 MB
-// (3.5 TB/s), 1763 by rank 64 15.8 us for 41 MB (2.6 TB/s).
+// dh x^T and dx, of the same tiles of x.  5325 rows of 4096 by rank 16 with dropout 26.5 us for 96 MB
+// (3.6 TB/s), 1763 by rank 64 16.2 us for 41 MB (2.5 TB/s).
 template <bool BF, int NT, bool DX, bool DROP>
 __global__ void __launch_bounds__(kOuterThreads) outer_kernel(AdapterArgs p, OuterArgs o) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[kOuterLds];

@@ -67,7 +67,6 @@ dw4::AdapterArgs adapter_args(int dtype, int rows, int k, int n, int rank, int a
   dw4::AdapterArgs p = {};
   p.l = dw4::adapter_layout(rows, adapters);
   p.bf16 = dtype == DW4_BF16;
-  p.rows = rows;
   p.k = k;
   p.n = n;
   p.r = rank;

@@ -10,8 +10,8 @@
 //
 // Bound by memory: every element is read and written once.  A thread holds the sines and
 // cosines of eight pairs (four, interleaved) of a row and turns them in one head after the other.
-// Measured: 7907 rows of 32 + 32 heads of 128 (bf16) 52 us for 259 MB, 5.0 TB/s; 11678 rows of 32 + 8 heads into
-// the cache 63 us for 289 MB, 4.6 TB/s; a decode step of 48 rows 6.1 us, one launch.
+// Measured on several cards: 7907 rows of 32 + 32 heads of 128 (bf16) 49 to 52 us for 259 MB, 5.0 to 5.3 TB/s; 11678
+// rows of 32 + 8 heads into the cache 57 to 63 us for 289 MB, 4.6 to 5.0; a decode step of 48 rows 6.1 to 6.3, one launch.
 
 #include <hip/hip_runtime.h>
 

@@ -121,6 +121,7 @@ class LowRankAdapters(nn.Module):
         self.b = nn.Parameter(torch.zeros(num_adapters, out_features, rank, dtype=dtype, device=device),
                               requires_grad=trainable)
         self.register_buffer("scaling", torch.ones(num_adapters, dtype=torch.float32, device=device))
+        self._shapes = self.a.shape, self.b.shape, self.scaling.shape
 
     @property
     def dropout(self) -> float:
@@ -169,8 +170,7 @@ class LowRankAdapters(nn.Module):
             raise ValueError(f"x and base must be [..., {self.in_features}] and [..., {self.out_features}] of the same rows")
         if dtype not in _DTYPES or base.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
             raise TypeError("x, base and the adapters must be of one type, fp16 or bf16")
-        if a.shape != (self.num_adapters, self.rank, width) or scaling.shape != (self.num_adapters,) or \
-                b.shape != (self.num_adapters, self.out_features, self.rank):
+        if (a.shape, b.shape, scaling.shape) != self._shapes:
             raise ValueError(f"A, B and the scaling must keep the shapes of {self.num_adapters} adapters of rank {self.rank}")
         if base.device != device or a.device != device or b.device != device or scaling.device != device or \
                 rows.device != device:

@@ -15,8 +15,11 @@ import pytest
 import torch
 
 from gptq_synth import make_layer
+from hip_extends.marlin import MarlinDenseCache, MarlinTuningParams
 from hip_extends.w4a16 import CacheV2, TuningParams
 from operators.core.linear.adapters import AdaptedLinear, AdapterRows, CounterDropout, LowRankAdapters
+from operators.core.linear.real import Linear
+from operators.core.linear.real_marlin import MarlinQuantLinearMaker
 from operators.core.linear.real_quant import QuantLinearMaker
 from oracle import adapters as O
 
@@ -626,3 +629,78 @@ def test_wide_features_exactly(hip_device, rows, k, n, rank, adapters, order, p,
         assert torch.equal(g.cpu(), w.to(dtype)), name
     with torch.no_grad():
         assert torch.equal(case.run(), got[0])
+
+
+class Dense(Linear):
+    """A projection of its own kind, whose output it keeps."""
+
+    def __init__(self, weight):
+        torch.nn.Module.__init__(self)
+        self.weight, self.kept = torch.nn.Parameter(weight, requires_grad=False), None
+
+    def forward(self, x):
+        self.kept = x @ self.weight
+        return self.kept
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_adapters_on_other_projections(hip_device, dtype):
+    """A Marlin-path projection and one from outside the package, with and without gradients, in several
+    dimensions; what a projection or a hook keeps stays as it is."""
+    say(f"adapters on other projections {dtype}")
+    lay = make_layer(256, 128, 128, seed=6, symmetric=True)
+    maker = MarlinQuantLinearMaker(quantization_group_size=128, use_act_order=False)
+    with torch.device(hip_device):
+        marlin = maker.make_linear(256, 128, bias=False)
+    marlin.load_state_dict({"qweight": lay.qweight, "qzeros": lay.qzeros, "scales": lay.scales, "g_idx": lay.g_idx}, strict=False)
+    cache = MarlinDenseCache(hip_device)
+    maker.post_init(MarlinTuningParams(), cache)
+    cache.init_cache()
+    g = torch.Generator().manual_seed(8)
+    dense = Dense((torch.randn(256, 128, generator=g) / 16).to(hip_device, dtype))
+    seen = []
+    hooked = quant(hip_device, 256, 128, seed=4)
+    hooked.register_forward_hook(lambda module, args, y: seen.append(y))
+    for lin in (marlin, dense, hooked):
+        case = Case(hip_device, 48, 256, 128, 16, 3, dtype, trainable=True)
+        adapted = AdaptedLinear(lin, case.bank)
+        x = case.x.to(hip_device)
+        with torch.no_grad():
+            case.base = lin(x).cpu()
+            got = adapted(x, case.rows)
+            check(got, *case.want(), "out")
+            kept = dense.kept if lin is dense else seen[-1] if lin is hooked else None
+            assert kept is None or torch.equal(kept.cpu(), case.base)
+            assert torch.equal(adapted(x.view(6, 8, 256), case.rows), got.view(6, 8, 128))
+        leaf = x.clone().requires_grad_(True)
+        y = adapted(leaf, case.rows)
+        case.base = lin(leaf).detach().cpu()
+        want, errs = case.want(grads=True)
+        da, db = torch.autograd.grad(y, (case.bank.a, case.bank.b), case.dout.to(hip_device))
+        for name, t, w, e in (("out", y.detach(), want[0], errs[0]), ("da", da, want[2], errs[2]), ("db", db, want[3], errs[3])):
+            check(t, w, e, name)
+
+
+def test_two_captured_calls(hip_device):
+    """Two graphs of one bank, replayed in turn and over each other's inputs: their workspaces are their own."""
+    say("two captured calls")
+    cases = [Case(hip_device, rows, 256, 136, 16, 5, F16, seed=rows) for rows in (33, 120)]
+    cases[1].bank, cases[1].a, cases[1].b, cases[1].scaling = cases[0].bank, cases[0].a, cases[0].b, cases[0].scaling
+    held = []
+    for case in cases:
+        x, base = case.x.to(hip_device), case.base.to(hip_device)
+        case.bank(x, base, case.rows)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = case.bank(x, base, case.rows)
+        held.append((case, x, base, out, graph))
+    for i in range(4):
+        for case, x, base, out, graph in held if i % 2 else held[::-1]:
+            case.x = torch.randn(case.x.shape, generator=case.g).to(F16)
+            x.copy_(case.x)
+            graph.replay()
+        torch.cuda.synchronize()
+        for case, x, base, out, graph in held:
+            check(out, *case.want(), f"replay {i}")
+            assert torch.equal(out, case.bank(x, base, case.rows))

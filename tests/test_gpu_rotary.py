@@ -434,3 +434,34 @@ def test_turned_in_place_of_queries_with_a_gradient(hip_device):
     with pytest.raises(RuntimeError, match="leaf"):
         rotary.forward_cached(leaf, k, k, pos, pos, holder, output=leaf)
     assert torch.equal(rotary.forward(leaf.detach(), k, pos)[0], want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,rd,interleaved,rows", [(128, 128, False, 70), (80, 20, True, 9), (64, 64, False, 1)])
+def test_queries_of_a_merged_product_in_place(hip_device, hd, rd, interleaved, rows, dtype):
+    """The queries' part of merged rows turned where it stands, keys and values beside it unchanged; the gradients
+    of such parts."""
+    say(f"merged rows in place: {rows} rows, heads of {hd}, {rd} turning, interleaved {interleaved} {dtype}")
+    g = torch.Generator().manual_seed(rows)
+    heads, kvh = 4, 2
+    holder, pages = cache(hip_device, rows // 16 + 2, kvh, hd, 16, dtype, g)
+    rotary = RotaryEmbedding(hd, rd, interleaved=interleaved, device=hip_device)
+    merged = torch.randn(rows, (heads + 2 * kvh) * hd, generator=g).to(dtype)
+    pos = torch.randint(0, 9000, (rows,), generator=g)
+    dev = merged.to(hip_device)
+    q, k, v = (t.view(rows, -1, hd) for t in dev.split([heads * hd, kvh * hd, kvh * hd], 1))
+    want = rotary.forward(q, k, pos.to(hip_device))
+    assert rotary.forward_cached(q, k, v, pos.to(hip_device), torch.arange(rows, device=hip_device), holder, output=q) is q
+    check(q, *turned(merged[:, :heads * hd].reshape(rows, heads, hd), pos, rotary), "q")
+    assert torch.equal(q, want[0]) and torch.equal(dev[:, heads * hd:].cpu(), merged[:, heads * hd:])
+    got = holder.kv_tensor_from_slots_with_convert_with_create(torch.arange(rows, device=hip_device))
+    assert torch.equal(got[0], want[1]) and torch.equal(got[1], v)
+    leaf = merged.to(hip_device).requires_grad_(True)
+    parts = [t.view(rows, -1, hd) for t in leaf.split([heads * hd, kvh * hd, kvh * hd], 1)]
+    grads = torch.randn(merged.shape, generator=g).to(dtype)
+    dq, dk = (t.reshape(rows, -1, hd) for t in grads.split([heads * hd, kvh * hd, kvh * hd], 1)[:2])
+    given = [t.view(rows, -1, hd) for t in grads.to(hip_device).split([heads * hd, kvh * hd, kvh * hd], 1)]
+    (dx,) = torch.autograd.grad(rotary.forward(*parts[:2], pos.to(hip_device)), leaf, given[:2])
+    for name, x, first in (("dq", dq, 0), ("dk", dk, heads)):
+        check(dx[:, first * hd:(first + x.shape[1]) * hd].view(rows, -1, hd), *turned(x, pos, rotary, True), name)
+    assert not dx[:, (heads + kvh) * hd:].any()

@@ -271,6 +271,7 @@ __device__ __forceinline__ void outer(const AdapterArgs& p, const OuterArgs& o, 
   // stored it.
   if constexpr (DX) {
     if (odd_a) {
+      asm volatile("" ::: "memory");  // what the lane has stored is written over as another type
 #pragma unroll 1
       for (int i = 0; wave * kStep + i / 4 * kStride < chunk.z; ++i) {
         const int from = wave * kStep + i / 4 * kStride + i % 4 * 8 + line;
